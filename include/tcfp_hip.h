@@ -639,6 +639,98 @@ int tcfp_block_wgrad_presplit(const uint16_t* g_split_t, int split_lo, int64_t m
                               int64_t k_in, int block, float* dw, void* workspace,
                               size_t workspace_bytes, void* stream);
 
+/* ---- decoder operators (no reference counterpart) ------------------------ */
+
+/* Residual addition and root-mean-square norm of [rows, cols]:
+ *   s = x (+ residual), fp32;  rstd = 1 / sqrt(mean(s^2) + eps);
+ *   h = s rounded to residual's dtype;  y = s * rstd * weight.
+ * x and residual may differ in dtype and have row strides ldx / ldr (in
+ * elements); weight [cols]; h [rows, cols] contiguous (NULL: not written;
+ * without a residual h is x itself and must be NULL); rstd [rows]; y
+ * [rows, cols] contiguous in y_dtype.  y is formed from s before its rounding
+ * to h.  Any rows, cols >= 0; pointers aligned to their element. */
+int tcfp_rms_norm(const void* x, int x_dtype, int64_t ldx, const void* residual, int r_dtype,
+                  int64_t ldr, const void* weight, int w_dtype, int64_t rows, int64_t cols,
+                  float eps, void* h, void* y, int y_dtype, float* rstd, void* stream);
+
+/* The same with y quantised per (row, block of columns) as tcfp_block_quantize
+ * / tcfp_block_quantize_f32s quantise an fp32 y: q [rows, cols] codes, scales
+ * [cols / block, rows] int8 exponents (f32_scales == 0) or fp32 multipliers.
+ * block 32, 64 or 128, cols % block == 0; q 8-byte aligned. */
+int tcfp_rms_norm_quantize(const void* x, int x_dtype, int64_t ldx, const void* residual,
+                           int r_dtype, int64_t ldr, const void* weight, int w_dtype,
+                           int64_t rows, int64_t cols, float eps, int block, int fp8_fmt,
+                           int f32_scales, void* h, uint8_t* q, void* scales, float* rstd,
+                           void* stream);
+
+/* The gradients of either (the quantisation passes gradients through):
+ *   xh = h * rstd, g = grad_y * weight,
+ *   dx = rstd * (g - xh * mean(g * xh)) (+ grad_h), in h's dtype,
+ *   dw[c] = sum over rows of grad_y * xh, fp32, in one order fixed by the
+ *   sizes.
+ * grad_y, h, grad_h (NULL or h's dtype) and dx [rows, cols] contiguous; h is
+ * what the forward wrote (x without a residual).  dx is the gradient of both
+ * x and the residual.  dw may be NULL.  workspace: ..._workspace_bytes, any
+ * contents, 16-byte aligned. */
+size_t tcfp_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int tcfp_rms_norm_backward(const void* grad_y, int gy_dtype, const void* h, int h_dtype,
+                           const float* rstd, const void* weight, int w_dtype,
+                           const void* grad_h, int64_t rows, int64_t cols, void* dx, float* dw,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* A paged K/V cache holds, for K and for V, E4M3 codes
+ * [num_pages, kv_heads, page_size, dim] and one power-of-two exponent per
+XX: page * page_size + place in the page.  dim 64, 128 or 256; page_size a
+ * power of two from 16 to 1024; codes 16-byte aligned.
+ *
+ * Write: k, v [tokens, kv_heads, dim] (f32 or bf16, dim contiguous, token and
+ * head strides in elements, 16-byte aligned rows) quantised into the places
+ * slots[t]; a slot below 0 or past the pool leaves its token out.  Tokens of
+ * one call must have different slots. */
+int tcfp_kv_cache_write(const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                        const void* v, int64_t v_token_stride, int64_t v_head_stride, int dtype,
+                        int64_t tokens, int kv_heads, int dim, const int64_t* slots,
+                        int64_t num_pages, int page_size, uint8_t* k_codes, uint8_t* v_codes,
+                        int8_t* k_exps, int8_t* v_exps, void* stream);
+
+/* Read: k, v [tokens, kv_heads, dim] contiguous (f32: exact; bf16: exact but
+ * for values under bf16's smallest) of the places slots[t]; zeros for a slot
+ * outside the pool. */
+int tcfp_kv_cache_read(const uint8_t* k_codes, const uint8_t* v_codes, const int8_t* k_exps,
+                       const int8_t* v_exps, int64_t num_pages, int page_size, int kv_heads,
+                       int dim, const int64_t* slots, int64_t tokens, void* k, void* v,
+                       int dtype, void* stream);
+
+/* Attention of the new tokens of a batch over the paged cache.
+ *   q, out [tokens, heads, dim] bf16 (q: token and head strides in elements,
+ *   16-byte aligned rows; out contiguous); heads % kv_heads == 0, query head h
+ *   reads K/V head h / (heads / kv_heads).
+ *   query_start [batch + 1]: sequence b's new tokens are rows
+ *   query_start[b] ... query_start[b + 1] - 1 of q; seq_lens [batch]: its
+ *   tokens in the cache, the new ones (already written) last; page_table
+ *   [batch, table_width] (row stride table_stride): its pages in order.
+ * New token i of n in a sequence of len tokens stands at position
+ * p = len - n + i and sees the keys j < len with j <= p (causal) and
+ * j > p - window (window > 0).  Keys on a page outside the pool, or past the
+ * table, are not seen; a token that sees nothing gets zeros.
+ * out = softmax(scale * q K^T) V, scores, maximum and sums in fp32.
+ * max_query_len and max_seq_len bound the batch's lengths (they size the
+ * launch and the workspace; larger lengths are still answered rightly, only
+ * slower).  workspace: tcfp_paged_attention_workspace_bytes, any contents,
+ * 16-byte aligned.  Results do not depend on the launch's timing. */
+size_t tcfp_paged_attention_workspace_bytes(int64_t tokens, int heads, int kv_heads, int dim,
+                                            int64_t batch, int64_t max_query_len,
+                                            int64_t max_seq_len);
+int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                         const uint8_t* k_codes, const uint8_t* v_codes, const int8_t* k_exps,
+                         const int8_t* v_exps, int64_t num_pages, int page_size, int kv_heads,
+                         int dim, const int32_t* page_table, int64_t table_stride,
+                         int64_t table_width, const int32_t* seq_lens,
+                         const int32_t* query_start, int64_t batch, int64_t tokens, int heads,
+                         int64_t max_query_len, int64_t max_seq_len, float scale, int causal,
+                         int64_t window, void* out, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 /* ---- layout helpers ---------------------------------------------------- */
 
 /* dst[c, r] = src[r, c] for a [rows, cols] byte matrix (ld = cols / rows).

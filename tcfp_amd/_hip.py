@@ -143,6 +143,25 @@ _SIGNATURES = {
     "tcfp_block_wgrad_presplit_workspace_bytes": [_i64, _i64, _i64, _i32],
     "tcfp_quantize_batch_workspace_bytes": [_i32],
     "tcfp_quantize_batch": [_i32, ctypes.POINTER(QuantJob), _c_void_p, ctypes.c_size_t, _c_void_p],
+    "tcfp_rms_norm": [_c_void_p, _i32, _i64, _c_void_p, _i32, _i64, _c_void_p, _i32, _i64, _i64,
+                      ctypes.c_float, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p],
+    "tcfp_rms_norm_quantize": [_c_void_p, _i32, _i64, _c_void_p, _i32, _i64, _c_void_p, _i32,
+                               _i64, _i64, ctypes.c_float, _i32, _i32, _i32, _c_void_p,
+                               _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    "tcfp_rms_norm_backward_workspace_bytes": [_i64, _i64],
+    "tcfp_rms_norm_backward": [_c_void_p, _i32, _c_void_p, _i32, _c_void_p, _c_void_p, _i32,
+                               _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
+                               ctypes.c_size_t, _c_void_p],
+    "tcfp_kv_cache_write": [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i32, _i64, _i32, _i32,
+                            _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                            _c_void_p],
+    "tcfp_kv_cache_read": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _i32,
+                           _c_void_p, _i64, _c_void_p, _c_void_p, _i32, _c_void_p],
+    "tcfp_paged_attention_workspace_bytes": [_i64, _i32, _i32, _i32, _i64, _i64, _i64],
+    "tcfp_paged_attention": [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                             _i64, _i32, _i32, _i32, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+                             _i64, _i64, _i32, _i64, _i64, ctypes.c_float, _i32, _i64, _c_void_p,
+                             _c_void_p, ctypes.c_size_t, _c_void_p],
     "tcfp_gemm_set_tile_policy": [_i32],
     "tcfp_dual_quantize_set_candidates": [_i32],
     "tcfp_transpose_u8": [_c_void_p, _i64, _i64, _c_void_p, _c_void_p],
@@ -161,6 +180,8 @@ _RESTYPE = {
     "tcfp_block_wgrad_presplit_workspace_bytes": ctypes.c_size_t,
     "tcfp_wgrad_f32_workspace_bytes": ctypes.c_size_t,
     "tcfp_quantize_batch_workspace_bytes": ctypes.c_size_t,
+    "tcfp_rms_norm_backward_workspace_bytes": ctypes.c_size_t,
+    "tcfp_paged_attention_workspace_bytes": ctypes.c_size_t,
 }
 
 _lib = None

@@ -24,6 +24,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <optional>
@@ -756,6 +757,294 @@ Outs block_linear_backward(const Tensor& grad_2d, const OptT& act_fp8, const Opt
   return outs(dx, dw, db);
 }
 
+// ---- decoder operators -------------------------------------------------------
+
+// Rows of the last axis: a 2-D tensor's rows may be apart, anything else is
+// made contiguous.
+struct Rows {
+  Tensor t;
+  int64_t rows, cols, ld;
+};
+Rows rows_of(const Tensor& x, const char* name) {
+  if (x.dim() == 0) value_error(std::string(name) + " needs at least one dimension");
+  Rows r{x, 0, x.size(-1), 0};
+  const bool apart = x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= x.size(1);
+  if (!apart && !x.is_contiguous()) r.t = x.contiguous();
+  r.rows = r.cols ? r.t.numel() / r.cols : 0;
+  r.ld = apart ? r.t.stride(0) : r.cols;
+  return r;
+}
+
+struct NormIn {
+  Rows x, r;
+  Tensor w, h, rstd;
+  int xd, rd, wd;
+};
+NormIn norm_inputs(OnGpu& g, const Tensor& x, const Tensor& weight, const OptT& residual) {
+  g.add(x);
+  g.add(weight);
+  g.add(residual);
+  NormIn n;
+  n.x = rows_of(x, "x");
+  n.xd = in_dtype(x);
+  n.wd = in_dtype(weight);
+  n.rd = n.xd;
+  if (weight.dim() != 1 || weight.size(0) != n.x.cols)
+    value_error("weight must have shape (" + std::to_string(n.x.cols) + ",), got " +
+                shape_str(weight.sizes()));
+  n.w = weight.contiguous();
+  if (residual) {
+    if (residual->sizes() != x.sizes())
+      value_error("residual shape " + shape_str(residual->sizes()) + " != x shape " +
+                  shape_str(x.sizes()));
+    n.r = rows_of(*residual, "residual");
+    n.rd = in_dtype(*residual);
+    n.h = g.empty(x.sizes(), residual->scalar_type());
+  }
+  n.rstd = g.empty(x.sizes().slice(0, size_t(x.dim() - 1)), at::kFloat);
+  return n;
+}
+
+Outs rms_norm(const Tensor& x, const Tensor& weight, const OptT& residual, double eps,
+              at::ScalarType out_dtype) {
+  OnGpu g;
+  NormIn n = norm_inputs(g, x, weight, residual);
+  const c10::DeviceGuard guard(g.device());
+  const int yd = out_dtype_of(out_dtype);
+  Tensor y = g.empty(x.sizes(), out_dtype);
+  check(tcfp_rms_norm(ptr(n.x.t), n.xd, n.x.ld, ptr(n.r.t), n.rd, n.r.ld, ptr(n.w), n.wd, n.x.rows,
+                      n.x.cols, float(eps), ptr(n.h), ptr(y), yd, f32(n.rstd), g.stream()),
+        "rms_norm");
+  Tensor h = residual ? n.h : x;
+  return outs(y, h, n.rstd);
+}
+
+Outs rms_norm_quantize(const Tensor& x, const Tensor& weight, const OptT& residual, double eps,
+                       int64_t bs, at::ScalarType fp8, bool f32s) {
+  if (bs != 32 && bs != 64 && bs != 128)
+    value_error("block_size must be 32, 64, or 128, got " + std::to_string(bs));
+  const int fmt = fmt_of(fp8);
+  OnGpu g;
+  NormIn n = norm_inputs(g, x, weight, residual);
+  const c10::DeviceGuard guard(g.device());
+  if (n.x.cols % bs != 0)
+    value_error("the last dimension (" + std::to_string(n.x.cols) +
+                ") must be divisible by block_size (" + std::to_string(bs) + ")");
+  Tensor q = g.empty(x.sizes(), fp8);
+  Tensor s = g.empty({n.x.cols / bs, n.x.rows}, f32s ? at::kFloat : at::kChar);
+  check(tcfp_rms_norm_quantize(ptr(n.x.t), n.xd, n.x.ld, ptr(n.r.t), n.rd, n.r.ld, ptr(n.w), n.wd,
+                               n.x.rows, n.x.cols, float(eps), int(bs), fmt, f32s ? 1 : 0,
+                               ptr(n.h), bytes(q), ptr(s), f32(n.rstd), g.stream()),
+        "rms_norm_quantize");
+  Tensor h = residual ? n.h : x;
+  return outs(q, s, h, n.rstd);
+}
+
+Outs rms_norm_backward(const Tensor& grad_y, const Tensor& h, const Tensor& rstd,
+                       const Tensor& weight, const OptT& grad_h, bool need_dw) {
+  OnGpu g;
+  g.add(grad_y);
+  g.add(h);
+  g.add(rstd);
+  g.add(weight);
+  g.add(grad_h);
+  const c10::DeviceGuard guard(g.device());
+  if (h.dim() == 0) value_error("h needs at least one dimension");
+  const int64_t cols = h.size(-1), rows = cols ? h.numel() / cols : 0;
+  const int gd = in_dtype(grad_y), hd = in_dtype(h), wd = in_dtype(weight);
+  if (grad_y.sizes() != h.sizes())
+    value_error("grad_y shape " + shape_str(grad_y.sizes()) + " != h shape " +
+                shape_str(h.sizes()));
+  if (rstd.scalar_type() != at::kFloat || rstd.numel() != (cols ? rows : rstd.numel()))
+    value_error("rstd must hold a float32 for each of the " + std::to_string(rows) + " rows");
+  if (weight.dim() != 1 || weight.size(0) != cols)
+    value_error("weight must have shape (" + std::to_string(cols) + ",), got " +
+                shape_str(weight.sizes()));
+  Tensor gh;
+  if (grad_h) {
+    if (grad_h->sizes() != h.sizes())
+      value_error("grad_h shape " + shape_str(grad_h->sizes()) + " != h shape " +
+                  shape_str(h.sizes()));
+    if (grad_h->scalar_type() != h.scalar_type())
+      type_error(std::string("grad_h must have h's dtype ") + dtype_str(h.scalar_type()) +
+                 ", got " + dtype_str(grad_h->scalar_type()));
+    gh = grad_h->contiguous();
+  }
+  const Tensor gy = grad_y.contiguous(), hc = h.contiguous(), rs = rstd.contiguous(),
+               w = weight.contiguous();
+  Tensor dx = g.empty(h.sizes(), h.scalar_type()), dw, ws;
+  size_t nb = 0;
+  if (need_dw) {
+    dw = g.empty({cols}, at::kFloat);
+    nb = tcfp_rms_norm_backward_workspace_bytes(rows, cols);
+    ws = g.empty({int64_t(std::max<size_t>(nb, 16))}, at::kByte);
+  }
+  check(tcfp_rms_norm_backward(ptr(gy), gd, ptr(hc), hd, f32(rs), ptr(w), wd, ptr(gh), rows, cols,
+                               ptr(dx), f32(dw), ptr(ws), nb, g.stream()),
+        "rms_norm_backward");
+  return outs(dx, dw);
+}
+
+// The pool's tensors, as every cache op takes them.
+struct Cache {
+  int64_t pages, page_size;
+  int heads, dim;
+};
+Cache check_cache(OnGpu& g, const Tensor& kc, const Tensor& vc, const Tensor& ke,
+                  const Tensor& ve) {
+  g.add(kc);
+  g.add(vc);
+  g.add(ke);
+  g.add(ve);
+  for (const Tensor* t : {&kc, &vc})
+    if (t->scalar_type() != at::kFloat8_e4m3fn)
+      type_error(std::string("cache codes must be torch.float8_e4m3fn, got ") +
+                 dtype_str(t->scalar_type()));
+  for (const Tensor* t : {&ke, &ve})
+    if (t->scalar_type() != at::kChar)
+      type_error(std::string("cache exponents must be torch.int8, got ") +
+                 dtype_str(t->scalar_type()));
+  if (kc.dim() != 4 || vc.sizes() != kc.sizes())
+    value_error("cache codes must have one shape (pages, kv_heads, page_size, dim), got " +
+                shape_str(kc.sizes()) + " and " + shape_str(vc.sizes()));
+  const at::IntArrayRef rows = kc.sizes().slice(0, 3);
+  if (ke.sizes() != rows || ve.sizes() != rows)
+    value_error("cache exponents must have shape " + shape_str(rows) + ", got " +
+                shape_str(ke.sizes()) + " and " + shape_str(ve.sizes()));
+  for (const Tensor* t : {&kc, &vc, &ke, &ve})
+    if (!t->is_contiguous()) value_error("the cache's tensors must be contiguous");
+  const int64_t p = kc.size(2), d = kc.size(3);
+  if (d != 64 && d != 128 && d != 256)
+    value_error("the head dimension must be 64, 128 or 256, got " + std::to_string(d));
+  if (p < 16 || p > 1024 || (p & (p - 1)))
+    value_error("page_size must be a power of two from 16 to 1024, got " + std::to_string(p));
+  if (kc.size(1) < 1 || kc.size(1) > 65535)
+    value_error("the cache needs 1 to 65535 heads, got " + std::to_string(kc.size(1)));
+  return {kc.size(0), p, int(kc.size(1)), int(d)};
+}
+Tensor check_slots(const Tensor& slots, int64_t tokens) {
+  if (slots.scalar_type() != at::kLong)
+    type_error(std::string("slots must be torch.int64, got ") + dtype_str(slots.scalar_type()));
+  if (slots.dim() != 1 || (tokens >= 0 && slots.size(0) != tokens))
+    value_error("slots must have shape (" + (tokens >= 0 ? std::to_string(tokens) : "tokens") +
+                ",), got " + shape_str(slots.sizes()));
+  return slots.contiguous();
+}
+// [tokens, heads, dim] with its heads' rows whole and aligned.
+Tensor head_rows(const Tensor& x) {
+  const int64_t unit = 16 / x.element_size();
+  if (x.stride(2) == 1 && x.stride(0) % unit == 0 && x.stride(1) % unit == 0 && al16(x)) return x;
+  Tensor c = x.contiguous();
+  return al16(c) ? c : c.clone();
+}
+void check_heads(const Tensor& x, int64_t heads, int64_t dim, const char* name) {
+  if (x.dim() != 3 || (heads > 0 && x.size(1) != heads) || x.size(2) != dim)
+    value_error(std::string(name) + " must have shape (tokens, " +
+                (heads > 0 ? std::to_string(heads) : "heads") + ", " + std::to_string(dim) +
+                "), got " + shape_str(x.sizes()));
+}
+
+void kv_cache_write(const Tensor& k_, const Tensor& v_, const Tensor& kc, const Tensor& vc,
+                    const Tensor& ke, const Tensor& ve, const Tensor& slots_) {
+  OnGpu g;
+  g.add(k_);
+  g.add(v_);
+  const Cache c = check_cache(g, kc, vc, ke, ve);
+  g.add(slots_);
+  const c10::DeviceGuard guard(g.device());
+  check_heads(k_, c.heads, c.dim, "k");
+  check_heads(v_, c.heads, c.dim, "v");
+  const int dt = in_dtype(k_);
+  if (v_.scalar_type() != k_.scalar_type())
+    type_error(std::string("k and v must have one dtype, got ") + dtype_str(k_.scalar_type()) +
+               " and " + dtype_str(v_.scalar_type()));
+  if (v_.size(0) != k_.size(0))
+    value_error("k has " + std::to_string(k_.size(0)) + " tokens, v " +
+                std::to_string(v_.size(0)));
+  const Tensor slots = check_slots(slots_, k_.size(0));
+  const Tensor k = head_rows(k_), v = head_rows(v_);
+  check(tcfp_kv_cache_write(ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), dt,
+                            k.size(0), c.heads, c.dim, ptr<int64_t>(slots), c.pages,
+                            int(c.page_size), bytes(kc), bytes(vc), exps(ke), exps(ve),
+                            g.stream()),
+        "kv_cache_write");
+}
+
+Outs kv_cache_read(const Tensor& kc, const Tensor& vc, const Tensor& ke, const Tensor& ve,
+                   const Tensor& slots_, at::ScalarType out_dtype) {
+  OnGpu g;
+  const Cache c = check_cache(g, kc, vc, ke, ve);
+  g.add(slots_);
+  const c10::DeviceGuard guard(g.device());
+  const Tensor slots = check_slots(slots_, -1);
+  const int dt = out_dtype_of(out_dtype);
+  const int64_t n = slots.size(0);
+  Tensor k = g.empty({n, c.heads, c.dim}, out_dtype), v = g.empty({n, c.heads, c.dim}, out_dtype);
+  check(tcfp_kv_cache_read(bytes(kc), bytes(vc), exps(ke), exps(ve), c.pages, int(c.page_size),
+                           c.heads, c.dim, ptr<int64_t>(slots), n, ptr(k), ptr(v), dt,
+                           g.stream()),
+        "kv_cache_read");
+  return outs(k, v);
+}
+
+Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& ke,
+                       const Tensor& ve, const Tensor& table_, const Tensor& lens_,
+                       const Tensor& starts_, int64_t max_query_len,
+                       std::optional<int64_t> max_seq_len, std::optional<double> scale,
+                       bool causal, int64_t window) {
+  OnGpu g;
+  g.add(q_);
+  const Cache c = check_cache(g, kc, vc, ke, ve);
+  g.add(table_);
+  g.add(lens_);
+  g.add(starts_);
+  const c10::DeviceGuard guard(g.device());
+  if (q_.scalar_type() != at::kBFloat16)
+    type_error(std::string("q must be torch.bfloat16, got ") + dtype_str(q_.scalar_type()));
+  check_heads(q_, 0, c.dim, "q");
+  const int64_t tokens = q_.size(0), heads = q_.size(1);
+  if (heads < 1 || heads > 65535 || heads % c.heads != 0)
+    value_error("q's heads (" + std::to_string(heads) + ") must be a multiple of the cache's (" +
+                std::to_string(c.heads) + ")");
+  const std::pair<const char*, const Tensor*> ints[] = {
+      {"page_table", &table_}, {"seq_lens", &lens_}, {"query_start", &starts_}};
+  for (const auto& [name, t] : ints)
+    if (t->scalar_type() != at::kInt)
+      type_error(std::string(name) + " must be torch.int32, got " + dtype_str(t->scalar_type()));
+  if (table_.dim() != 2)
+    value_error("page_table must be 2-D (sequences, pages), got " + shape_str(table_.sizes()));
+  const int64_t batch = table_.size(0);
+  if (lens_.dim() != 1 || lens_.size(0) != batch)
+    value_error("seq_lens must have shape (" + std::to_string(batch) + ",), got " +
+                shape_str(lens_.sizes()));
+  if (starts_.dim() != 1 || starts_.size(0) != batch + 1)
+    value_error("query_start must have shape (" + std::to_string(batch + 1) + ",), got " +
+                shape_str(starts_.sizes()));
+  if (batch > 65535) value_error("at most 65535 sequences, got " + std::to_string(batch));
+  if (max_query_len < 0 || (max_seq_len && *max_seq_len < 0))
+    value_error("max_query_len and max_seq_len must not be negative");
+  if (window < 0) value_error("window must not be negative, got " + std::to_string(window));
+  if (tokens > 0 && batch == 0) value_error("q has tokens but there are no sequences");
+  const bool rows = table_.stride(1) == 1 && table_.stride(0) >= table_.size(1);
+  const Tensor q = head_rows(q_), lens = lens_.contiguous(), starts = starts_.contiguous(),
+               table = rows ? table_ : table_.contiguous();
+  const int64_t width = table.size(1);
+  const int64_t most = std::min(max_seq_len.value_or(width * c.page_size), width * c.page_size);
+  Tensor out = g.empty({tokens, heads, c.dim}, at::kBFloat16), ws;
+  const size_t nb = tcfp_paged_attention_workspace_bytes(tokens, int(heads), c.heads, c.dim, batch,
+                                                         max_query_len, most);
+  if (nb) ws = g.empty({int64_t(nb)}, at::kByte);
+  check(tcfp_paged_attention(ptr(q), q.stride(0), q.stride(1), bytes(kc), bytes(vc), exps(ke),
+                             exps(ve), c.pages, int(c.page_size), c.heads, c.dim,
+                             ptr<int32_t>(table), rows ? table.stride(0) : width, width,
+                             ptr<int32_t>(lens), ptr<int32_t>(starts), batch, tokens, int(heads),
+                             max_query_len, most,
+                             float(scale.value_or(1.0 / std::sqrt(double(c.dim)))), causal ? 1 : 0,
+                             window, ptr(out), ptr(ws), nb, g.stream()),
+        "paged_attention");
+  return out;
+}
+
 }  // namespace
 
 namespace pybind11::detail {
@@ -805,4 +1094,10 @@ PYBIND11_MODULE(_tcfp_host, m) {
   m.def("wgrad_f32", &wgrad_f32, NoGil());
   m.def("block_linear_forward", &block_linear_forward, NoGil());
   m.def("block_linear_backward", &block_linear_backward, NoGil());
+  m.def("rms_norm", &rms_norm, NoGil());
+  m.def("rms_norm_quantize", &rms_norm_quantize, NoGil());
+  m.def("rms_norm_backward", &rms_norm_backward, NoGil());
+  m.def("kv_cache_write", &kv_cache_write, NoGil());
+  m.def("kv_cache_read", &kv_cache_read, NoGil());
+  m.def("paged_attention", &paged_attention, NoGil());
 }
