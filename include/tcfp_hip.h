@@ -720,7 +720,7 @@ int tcfp_kv_cache_read(const uint8_t* k_codes, const uint8_t* v_codes, const int
  * 16-byte aligned.  Results do not depend on the launch's timing. */
 size_t tcfp_paged_attention_workspace_bytes(int64_t tokens, int heads, int kv_heads, int dim,
                                             int64_t batch, int64_t max_query_len,
-                                            int64_t max_seq_len);
+                                            int64_t max_seq_len, int64_t window);
 int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                          const uint8_t* k_codes, const uint8_t* v_codes, const int8_t* k_exps,
                          const int8_t* v_exps, int64_t num_pages, int page_size, int kv_heads,

@@ -157,7 +157,7 @@ _SIGNATURES = {
                             _c_void_p],
     "tcfp_kv_cache_read": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _i32,
                            _c_void_p, _i64, _c_void_p, _c_void_p, _i32, _c_void_p],
-    "tcfp_paged_attention_workspace_bytes": [_i64, _i32, _i32, _i32, _i64, _i64, _i64],
+    "tcfp_paged_attention_workspace_bytes": [_i64, _i32, _i32, _i32, _i64, _i64, _i64, _i64],
     "tcfp_paged_attention": [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                              _i64, _i32, _i32, _i32, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
                              _i64, _i64, _i32, _i64, _i64, ctypes.c_float, _i32, _i64, _c_void_p,

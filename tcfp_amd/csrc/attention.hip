@@ -5,6 +5,7 @@
 //   page_size]: the keys of one page and head are one contiguous run, so a
 //   tile of keys is read in whole lines whatever the number of heads.
 #include <algorithm>
+#include <cmath>
 
 #include "common.h"
 
@@ -132,6 +133,34 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(Pool pool, const i
 }
 
 // ---- attention ---------------------------------------------------------------
+//
+// The rows of a (sequence, K/V head) are its new tokens times the group of
+// query heads that share the head: row r is token r / group, head r % group
+// of the group.  A workgroup takes a tile of rows over a run of keys (a
+// split); rows whose keys are in one split are finished there, the others
+// leave (sum p v, max, sum p) for the combining kernel.
+//
+//   S^T = K Q^T      A = K codes, B = Q   keys down the registers, rows across lanes
+//   O^T += V^T P^T   A = V^T,     B = P^T
+// Transposed like this, a lane's S values are the P values that the second
+// product wants of it (the order of its keys is the same permutation on both
+// sides), a row's maximum and sum are over a lane's own registers and one or
+// two other lanes, and rescaling O is a multiplication by the lane's own factor.
+//
+// The first product runs on the codes as they are cached: q = hi + lo in E4M3
+// with one power-of-two scale a row is exact for bf16 values down to 2^-10 of
+// the row's largest (4 + 4 significant bits) and within 2^-18 of the largest
+// below that; the matrix instruction applies 2^e of a key as its block scale,
+// and two FP8 products cost what one bf16 product would, without converting K.  V is converted to bf16 with its
+// exponent (both exact) and P is rounded to bf16: 2^-9 of a weight.
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+
+constexpr int kMaxSplits = 64;
 
 struct Attend {
   const uint16_t* q;
@@ -140,95 +169,870 @@ struct Attend {
   const uint8_t* v_codes;
   const int8_t* k_exps;
   const int8_t* v_exps;
-  int64_t num_pages;
+  int num_pages;
   int page_bits;
   int kv_heads;
   const int32_t* table;
   int64_t table_stride;
-  int64_t table_keys;  // keys that a row of the table spans
+  int table_keys;  // keys that a row of the table spans
   const int32_t* seq_lens;
   const int32_t* starts;
-  int64_t batch;
-  int64_t tokens;
+  int batch;
+  int tokens;
   int heads;
-  int group;  // heads / kv_heads
-  float scale;
+  int group;        // heads / kv_heads
+  float c;          // |scale| * log2(e), 1 for a scale of 0
+  float q_mul;      // sign of the scale
   int causal;
-  int64_t window;
+  int window;       // 0: none
+  int tiles;        // row tiles of a (sequence, head) in the launch
+  int splits;       // of a row tile's keys
+  int chunk;        // keys of a split but the last
   uint16_t* out;
+  float* part;      // [splits][tokens * heads][dim]
+  float* part_ml;   // [splits][tokens * heads][2]: max (in units of s), sum
 };
 
-// One wave a (new token, head), 64 keys at a time: a lane scores a key, the
-// wave takes the running maximum and sum, then each lane gathers DIM / 64 of
-// the output's columns over the keys.
-template <int DIM>
-__global__ __launch_bounds__(64) void attend_row_kernel(Attend a) {
-  constexpr int C = DIM / 64;
-  __shared__ float qs[DIM];
-  const int64_t t = blockIdx.x;
-  const int head = blockIdx.y, kvh = head / a.group, lane = threadIdx.x;
-  int64_t lo = 0, hi = a.batch;  // the sequence of token t: starts[lo] <= t < starts[lo + 1]
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) / 2;
-    if (a.starts[mid] <= t) lo = mid;
-    else hi = mid;
+// The rows of sequence b.
+struct Seq {
+  int start, new_tokens, len, pos0, rows;
+};
+TCFP_DEV Seq sequence(const Attend& a, int b) {
+  Seq s;
+  s.start = min(max(a.starts[b], 0), a.tokens);
+  s.new_tokens = max(min(a.starts[b + 1], a.tokens) - s.start, 0);
+  const int total = a.seq_lens[b];
+  s.len = min(max(total, 0), a.table_keys);
+  s.pos0 = total - s.new_tokens;  // position of the first new token
+  s.rows = s.new_tokens * a.group;
+  return s;
+}
+// Keys that new token i sees: [lo, hi).
+TCFP_DEV int key_lo(const Attend& a, const Seq& s, int i) {
+  return a.window > 0 ? max(s.pos0 + i - a.window + 1, 0) : 0;
+}
+TCFP_DEV int key_hi(const Attend& a, const Seq& s, int i) {
+  return a.causal ? min(s.len, s.pos0 + i + 1) : s.len;
+}
+// Keys of a tile of rows [r0, r0 + n) and the splits that hold some.
+struct Keys {
+  int begin, end;  // begin is a multiple of 64
+  int live;
+};
+TCFP_DEV Keys keys_of(const Attend& a, const Seq& s, int r0, int n) {
+  Keys k;
+  k.begin = key_lo(a, s, r0 / a.group) & ~63;
+  k.end = key_hi(a, s, (min(r0 + n, s.rows) - 1) / a.group);
+  const int span = max(k.end - k.begin, 0);
+  k.live = min((span + a.chunk - 1) / a.chunk, a.splits);
+  return k;
+}
+
+// A lane's N runs of 32 values of a row of q (p, p + step, ...) as E4M3 hi + lo,
+// with one scale for the row, whose other values lanes +- 32 (LANES == 2) or
+// +- 16, 32 (LANES == 4) hold; the scale is returned as the biased exponent that
+// the matrix instructions take.  (Their scale of a lane belongs to a block of 32
+// columns that is not the one whose values the lane holds: one scale for the
+// row, and for K's row, leaves that without effect.)
+template <int N, int LANES>
+TCFP_DEV int split_q(const uint16_t* p, int step, float mul, v8i* hi, v8i* lo) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      float v[8];
+      load8(p + n * step + i, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = umax(m, absbits(v[j] * mul));
+    }
+  if constexpr (LANES == 4) m = umax(m, uint32_t(__shfl_xor(int(m), 16, 64)));
+  m = umax(m, uint32_t(__shfl_xor(int(m), 32, 64)));
+  const int e = block_exponent(__uint_as_float(m), kE4M3Max);
+  const float up = exp2i(-e) * mul;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      float v[8];
+      load8(p + n * step + i, v);
+#pragma unroll
+      for (int h = 0; h < 8; h += 4) {
+        float x[4], r[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = clampf(v[h + j] * up, kE4M3Max);
+        const uint32_t w = cvt4_fp8<TCFP_FP8_E4M3>(x[0], x[1], x[2], x[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = x[j] - e4m3_to_f32(w >> (8 * j));
+        hi[n][(i + h) / 4] = int(w);
+        lo[n][(i + h) / 4] = int(cvt4_fp8<TCFP_FP8_E4M3>(r[0], r[1], r[2], r[3]));
+      }
+    }
+  return e + 127;  // (255, the format's NaN, where the row holds an infinity)
+}
+
+// Two neighbouring codes (of bytes 0, 1 or 2, 3) times 2^e as bf16.
+template <bool HIGH>
+TCFP_DEV uint32_t deq2(uint32_t w, float scale) {
+  const v2bf r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HIGH);
+  return __builtin_bit_cast(uint32_t, r);
+}
+// The low / high halves of two words, one after the other.
+TCFP_DEV uint32_t lows(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+TCFP_DEV uint32_t highs(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// 2^e of the signed byte j of w, for the exponents that a cache is written with
+// (-126 ... 120).
+TCFP_DEV float exp_scale(uint32_t w, int j) {
+  return __uint_as_float(uint32_t(max(int(int8_t(w >> (8 * j))) + 127, 0)) << 23);
+}
+TCFP_DEV bool has_nan_code(uint32_t w) {
+  return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
+}
+// w with its NaN codes made zero.
+TCFP_DEV uint32_t without_nan(uint32_t w) {
+  const uint32_t t = (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
+  return w & ~(t * 255u);
+}
+TCFP_DEV v8bf as_bf(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(v8bf, make_uint4(a, b, c, d));
+}
+TCFP_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+TCFP_DEV int valid_page(const Attend& a, int p) { return p >= 0 && p < a.num_pages ? p : -1; }
+
+// Rows of q before the first and after the last sequence: zeros.
+TCFP_DEV void zero_rest(const Attend& a, int b, int kvh, const Seq& s, int dim) {
+  const int lo0 = b == 0 ? 0 : a.tokens, hi0 = b == 0 ? s.start : 0;
+  const int lo1 = b == a.batch - 1 ? s.start + s.new_tokens : a.tokens, hi1 = a.tokens;
+  const int words = a.group * dim / 2;
+  for (int part = 0; part < 2; ++part)
+    for (int t = part ? lo1 : lo0; t < (part ? hi1 : hi0); ++t) {
+      uint32_t* p = reinterpret_cast<uint32_t*>(
+          a.out + (int64_t(t) * a.heads + kvh * a.group) * dim);
+      for (int i = threadIdx.x; i < words; i += blockDim.x) p[i] = 0;
+    }
+}
+
+// ---- few rows: one token a sequence, a few drafts ----------------------------
+//
+// Bound by reading the cache.  A wave takes KT keys at a time straight into
+// registers, the next KT in flight; nothing of K or V passes through LDS.  The
+// four waves of a workgroup take turns over the split's keys and are joined at
+// its end.
+template <int D>
+struct FewShape {
+  static constexpr int KT = 32;                  // keys of a wave's step
+  static constexpr int KG = KT / 16;             // groups of 16 keys, each in one page
+  static constexpr int DS = D == 256 ? 2 : 1;    // 128-column steps of the first product
+  static constexpr int VW = D / 64;              // words of a lane's share of a V row
+  static constexpr int NI = D / 16;              // column tiles of the output
+};
+
+template <int D>
+struct FewTile {
+  using S = FewShape<D>;
+  uint4 k[S::KG][S::DS][2];
+  uint32_t v[S::KG][4][S::VW];
+  int ke[S::KG];
+  uint32_t ve[S::KG];
+  int page[S::KG];
+};
+
+constexpr int kSegKeys = 2048;  // keys whose pages are held in LDS at a time
+
+template <int D>
+TCFP_DEV void few_load(const Attend& a, int kvh, const int* pages, int seg, int seg_end,
+                       int key0, FewTile<D>& t) {
+  using S = FewShape<D>;
+  const int lane = threadIdx.x & 63, col = lane & 15, g4 = lane >> 4;
+#pragma unroll
+  for (int g = 0; g < S::KG; ++g) {
+    const int key = key0 + 16 * g;
+    const int page = key < seg_end ? __builtin_amdgcn_readfirstlane(
+                                         pages[(key >> a.page_bits) - (seg >> a.page_bits)])
+                                   : -1;
+    t.page[g] = page;
+    // (a missing page, or keys past the end, are read from page 0 -- the pool
+    // has pages -- and masked)
+    const int64_t at = ((int64_t(max(page, 0)) * a.kv_heads + kvh) << a.page_bits) +
+                       (key & ((1 << a.page_bits) - 1));
+    const uint8_t* kp = a.k_codes + (at + col) * D + (D == 64 ? (g4 & 1) * 32 : g4 * 32);
+#pragma unroll
+    for (int s = 0; s < S::DS; ++s) {
+      t.k[g][s][0] = *reinterpret_cast<const uint4*>(kp + s * 128);
+      t.k[g][s][1] = *reinterpret_cast<const uint4*>(kp + s * 128 + 16);
+    }
+    t.ke[g] = a.k_exps[at + col];
+    const uint8_t* vp = a.v_codes + (at + 4 * g4) * D + col * (D / 16);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (S::VW == 1) {
+        t.v[g][r][0] = *reinterpret_cast<const uint32_t*>(vp + r * D);
+      } else if constexpr (S::VW == 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(vp + r * D);
+        t.v[g][r][0] = w.x; t.v[g][r][1] = w.y;
+      } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(vp + r * D);
+        t.v[g][r][0] = w.x; t.v[g][r][1] = w.y; t.v[g][r][2] = w.z; t.v[g][r][3] = w.w;
+      }
+    }
+    t.ve[g] = *reinterpret_cast<const uint32_t*>(a.v_exps + at + 4 * g4);
   }
-  uint16_t* out = a.out + (t * a.heads + head) * DIM;
-  float o[C] = {}, top = -INFINITY, sum = 0.0f;
-  if (t >= a.starts[lo] && t < a.starts[lo + 1]) {
-    const int64_t len = min(int64_t(a.seq_lens[lo]), a.table_keys);
-    const int64_t pos = int64_t(a.seq_lens[lo]) - a.starts[lo + 1] + t;
-    const int64_t end = a.causal ? min(len, pos + 1) : len;
-    const int64_t begin = a.window > 0 ? max(pos - a.window + 1, int64_t(0)) : 0;
-    const int32_t* table = a.table + lo * a.table_stride;
-    for (int c = lane; c < DIM; c += 64)
-      qs[c] = bf16_to_f32(a.q[t * a.q_token + head * a.q_head + c]);
-    __syncthreads();
-    for (int64_t j0 = begin; j0 < end; j0 += 64) {
-      const int64_t j = j0 + lane;
-      int64_t at = -1;
-      float s = -INFINITY;
-      if (j < end) {
-        const int64_t page = table[j >> a.page_bits];
-        if (page >= 0 && page < a.num_pages)
-          at = ((page * a.kv_heads + kvh) << a.page_bits) + (j & ((1 << a.page_bits) - 1));
-      }
-      if (at >= 0) {
-        float d = 0.0f;
-        for (int c = 0; c < DIM; c += 4) {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(a.k_codes + at * DIM + c);
+}
+
+template <int D, int NT>
+struct FewState {
+  using S = FewShape<D>;
+  v8i qhi[NT][S::DS], qlo[NT][S::DS];  // D == 64: hi and lo side by side in qhi
+  int qe[NT];
+  int lo[NT], hi[NT];                  // keys that the lane's row sees
+  float m[NT], l[NT];
+  v4f o[NT][S::NI];
+};
+
+// One step over KT keys; MASKED: some row does not see all of them (or a page
+// is missing).  [all_lo, all_hi): keys that any row sees.
+template <int D, int NT, bool MASKED>
+TCFP_DEV void few_step(const Attend& a, FewState<D, NT>& st, FewTile<D>& t, int key0, int all_lo,
+                       int all_hi) {
+  using S = FewShape<D>;
+  const int lane = threadIdx.x & 63, g4 = lane >> 4;
+  uint32_t bad = 0;  // keys of the lane (4 g + r) with a NaN among the codes of V
+  if constexpr (MASKED) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) d += qs[c + i] * e4m3_to_f32(w >> (8 * i));
+    for (int g = 0; g < S::KG; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = key0 + 16 * g + 4 * g4 + r;
+        const bool dead = key < all_lo || key >= all_hi || t.page[g] < 0;
+        bool nan = false;
+#pragma unroll
+        for (int w = 0; w < S::VW; ++w) nan |= has_nan_code(t.v[g][r][w]);
+        // what no row sees counts as zero, whatever the page holds there; a NaN
+        // among keys that some rows see is moved to the key's score, so that it
+        // reaches the rows that see it and no other (0 * NaN in the product)
+        const uint64_t any = __ballot(nan && !dead);
+        if ((any >> (16 * g4)) & 0xFFFFu) bad |= 1u << (4 * g + r);
+#pragma unroll
+        for (int w = 0; w < S::VW; ++w) t.v[g][r][w] = dead ? 0u : without_nan(t.v[g][r][w]);
+        if (dead) t.ve[g] &= ~(0xFFu << (8 * r));
+      }
+  }
+  float p[NT][S::KG][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < S::KG; ++g) {
+      v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int d = 0; d < S::DS; ++d) {
+        v8i k;
+        k[0] = int(t.k[g][d][0].x); k[1] = int(t.k[g][d][0].y);
+        k[2] = int(t.k[g][d][0].z); k[3] = int(t.k[g][d][0].w);
+        k[4] = int(t.k[g][d][1].x); k[5] = int(t.k[g][d][1].y);
+        k[6] = int(t.k[g][d][1].z); k[7] = int(t.k[g][d][1].w);
+        s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, st.qhi[n][d], s, 0, 0, 0,
+                                                             t.ke[g] + 127, 0, st.qe[n]);
+        if constexpr (D != 64)
+          s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, st.qlo[n][d], s, 0, 0, 0,
+                                                               t.ke[g] + 127, 0, st.qe[n]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = s[r];
+        if constexpr (MASKED) {
+          const int key = key0 + 16 * g + 4 * g4 + r;
+          if ((bad >> (4 * g + r)) & 1u) x = __uint_as_float(0x7FC00000u);
+          if (key < st.lo[n] || key >= st.hi[n] || t.page[g] < 0) x = -INFINITY;
         }
-        s = ldexpf(d, a.k_exps[at]) * a.scale;
+        p[n][g][r] = x;
+        top = fmaxf(top, x);
       }
-      const float m = fmaxf(top, wave_max(s));
-      if (__ballot(at >= 0) == 0) continue;
-      const float p = at >= 0 ? expf(s - m) : 0.0f;
-      const float old = top == -INFINITY ? 0.0f : expf(top - m);
-      float ps = p;
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    top = fmaxf(top, st.m[n]);
+    if (__ballot(top > st.m[n])) {
+      const float f = top == st.m[n] ? 1.0f : exp2_fast((st.m[n] - top) * a.c);
+      st.m[n] = top;
+      st.l[n] *= f;
 #pragma unroll
-      for (int x = 32; x > 0; x >>= 1) ps += __shfl_xor(ps, x, 64);
-      sum = sum * old + ps;
-      top = m;
+      for (int i = 0; i < S::NI; ++i) st.o[n][i] *= f;
+    }
+    const float off = top == -INFINITY ? 0.0f : top * a.c;
 #pragma unroll
-      for (int c = 0; c < C; ++c) o[c] *= old;
-      const float pe = at >= 0 ? ldexpf(p, a.v_exps[at]) : 0.0f;
-      for (int x = 0; x < 64; ++x) {
-        const int64_t ax = __shfl(at, x, 64);
-        if (ax < 0) continue;
-        const float px = __shfl(pe, x, 64);
+    for (int g = 0; g < S::KG; ++g)
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-          o[c] += px * e4m3_to_f32(a.v_codes[ax * DIM + c * 64 + lane]);
+      for (int r = 0; r < 4; ++r) {
+        p[n][g][r] = exp2_fast(__builtin_fmaf(p[n][g][r], a.c, -off));
+        st.l[n] += p[n][g][r];
+      }
+  }
+#pragma unroll
+  for (int g = 0; g < S::KG; g += 2) {  // 32 keys of the second product
+    v8bf pf[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      pf[n] = as_bf(pack_bf16(p[n][g][0], p[n][g][1]), pack_bf16(p[n][g][2], p[n][g][3]),
+                    pack_bf16(p[n][g + 1][0], p[n][g + 1][1]),
+                    pack_bf16(p[n][g + 1][2], p[n][g + 1][3]));
+    float sc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sc[j] = exp_scale(t.ve[g + j / 4], j % 4);
+#pragma unroll
+    for (int w = 0; w < S::VW; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // two columns of the lane's share at a time
+        uint32_t x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          x[j] = h ? deq2<true>(t.v[g + j / 4][j % 4][w], sc[j])
+                   : deq2<false>(t.v[g + j / 4][j % 4][w], sc[j]);
+        const v8bf v0 = as_bf(lows(x[0], x[1]), lows(x[2], x[3]), lows(x[4], x[5]), lows(x[6], x[7]));
+        const v8bf v1 =
+            as_bf(highs(x[0], x[1]), highs(x[2], x[3]), highs(x[4], x[5]), highs(x[6], x[7]));
+        const int i = 4 * w + 2 * h;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          st.o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pf[n], st.o[n][i], 0, 0, 0);
+          st.o[n][i + 1] =
+              __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pf[n], st.o[n][i + 1], 0, 0, 0);
+        }
+      }
+  }
+}
+
+template <int D, int NT>
+__global__ __launch_bounds__(256, D == 256 && NT == 2 ? 1 : 2) void attend_few_kernel(Attend a) {
+  using S = FewShape<D>;
+  constexpr int RT = 16 * NT;
+  __shared__ int pages[kSegKeys / 16];
+  __shared__ float ml[4][RT][2];
+  __shared__ float4 xo[4][8][64];
+  const int b = blockIdx.z, kvh = blockIdx.y % a.kv_heads, split = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g4 = lane >> 4;
+  const Seq seq = sequence(a, b);
+  if (split == 0 && int(blockIdx.y) < a.kv_heads) zero_rest(a, b, kvh, seq, D);
+  const int32_t* table = a.table + int64_t(b) * a.table_stride;
+  for (int r0 = int(blockIdx.y / a.kv_heads) * RT; r0 < seq.rows; r0 += a.tiles * RT) {
+    const Keys keys = keys_of(a, seq, r0, RT);
+    if (split >= max(keys.live, 1)) continue;
+    const int k0 = keys.begin + split * a.chunk;
+    const int k1 = split == a.splits - 1 ? keys.end : min(keys.end, k0 + a.chunk);
+    FewState<D, NT> st;
+    int lo_max = 0, hi_min = INT32_MAX;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = min(r0 + 16 * n + col, seq.rows - 1), i = r / a.group, h = r - i * a.group;
+      const uint16_t* q = a.q + int64_t(seq.start + i) * a.q_token +
+                          int64_t(kvh * a.group + h) * a.q_head;
+      st.qe[n] = split_q<S::DS, 4>(q + (D == 64 ? (g4 & 1) * 32 : g4 * 32), 128, a.q_mul,
+                                   st.qhi[n], st.qlo[n]);
+      if (D == 64 && g4 >= 2) st.qhi[n][0] = st.qlo[n][0];
+      st.lo[n] = key_lo(a, seq, i);
+      st.hi[n] = key_hi(a, seq, i);
+      st.m[n] = -INFINITY;
+      st.l[n] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < S::NI; ++x) st.o[n][x] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const int last = min(r0 + RT, seq.rows) - 1;
+    lo_max = key_lo(a, seq, last / a.group);
+    hi_min = key_hi(a, seq, r0 / a.group);
+    const int all_lo = key_lo(a, seq, r0 / a.group);
+    for (int seg = k0; seg < k1; seg += kSegKeys) {
+      const int seg_end = min(seg + kSegKeys, k1);
+      __syncthreads();
+      {
+        const int first = seg >> a.page_bits, n = ((seg_end - 1) >> a.page_bits) - first + 1;
+        for (int i = threadIdx.x; i < n; i += 256) pages[i] = valid_page(a, table[first + i]);
+      }
+      __syncthreads();
+      FewTile<D> cur, nxt;
+      int key = seg + wave * S::KT;
+      if (key < seg_end) few_load<D>(a, kvh, pages, seg, seg_end, key, cur);
+      for (; key < seg_end; key += 4 * S::KT) {
+        const int next = key + 4 * S::KT;
+        if (next < seg_end) few_load<D>(a, kvh, pages, seg, seg_end, next, nxt);
+        bool hole = false;
+#pragma unroll
+        for (int g = 0; g < S::KG; ++g) hole |= cur.page[g] < 0;
+        if (hole || key < lo_max || key + S::KT > hi_min)
+          few_step<D, NT, true>(a, st, cur, key, all_lo, keys.end);
+        else
+          few_step<D, NT, false>(a, st, cur, key, all_lo, keys.end);
+        cur = nxt;
+      }
+    }
+    // ---- the four waves joined ----
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float l = st.l[n];
+      l += __shfl_xor(l, 16, 64);
+      l += __shfl_xor(l, 32, 64);
+      if (g4 == 0) {
+        ml[wave][16 * n + col][0] = st.m[n];
+        ml[wave][16 * n + col][1] = l;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][16 * n + col][0]);
+      const float f = st.m[n] == top ? 1.0f : exp2_fast((st.m[n] - top) * a.c);
+#pragma unroll
+      for (int i0 = 0; i0 < S::NI; i0 += 8) {
+        constexpr int IB = S::NI < 8 ? S::NI : 8;
+#pragma unroll
+        for (int i = 0; i < IB; ++i) {
+          const v4f o = st.o[n][i0 + i] * f;
+          xo[wave][i][lane] = make_float4(o[0], o[1], o[2], o[3]);
+        }
+        __syncthreads();
+        // thread: columns i0 + 2 i2, + 1 of a lane's four rows of O^T
+        const int i2 = threadIdx.x >> 6;
+        if (2 * i2 < IB) {
+          float s[2][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float4 t = xo[0][2 * i2 + j][lane];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) {
+              const float4 u = xo[w][2 * i2 + j][lane];
+              t.x += u.x; t.y += u.y; t.z += u.z; t.w += u.w;
+            }
+            s[j][0] = t.x; s[j][1] = t.y; s[j][2] = t.z; s[j][3] = t.w;
+          }
+          float lsum = 0.0f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float mw = ml[w][16 * n + col][0];
+            lsum += ml[w][16 * n + col][1] *
+                    (mw == top ? 1.0f : exp2_fast((mw - top) * a.c));
+          }
+          const int r = r0 + 16 * n + col;
+          if (r < seq.rows) {
+            const int i = r / a.group, h = r - i * a.group;
+            const int64_t row = int64_t(seq.start + i) * a.heads + kvh * a.group + h;
+            if (keys.live <= 1) {
+              const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                *reinterpret_cast<uint32_t*>(a.out + row * D + (4 * g4 + x) * (D / 16) + i0 +
+                                             2 * i2) = pack_bf16(s[0][x] * inv, s[1][x] * inv);
+            } else {
+              const int64_t at = int64_t(split) * a.tokens * a.heads + row;
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                *reinterpret_cast<float2*>(a.part + at * D + (4 * g4 + x) * (D / 16) + i0 +
+                                           2 * i2) = make_float2(s[0][x], s[1][x]);
+              if (i0 == 0 && i2 == 0 && g4 == 0) {
+                a.part_ml[2 * at] = top;
+                a.part_ml[2 * at + 1] = lsum;
+              }
+            }
+          }
+        }
+        __syncthreads();
       }
     }
   }
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const float v = sum == 0.0f ? 0.0f : o[c] / sum;
-    out[c * 64 + lane] = f32_to_bf16_rne(v);
+}
+
+// ---- many rows: prompts ------------------------------------------------------
+//
+// Bound by the matrix and vector units together.  A workgroup's four waves
+// hold 32 rows each; per 64 keys K goes to LDS as codes and V as bf16,
+// transposed and in the order of keys that P has in its registers (both
+// buffered twice, the next 64 keys loaded into registers meanwhile), so every
+// operand is read with 16-byte LDS reads.  16-byte chunks of a line are
+// permuted by the row, which spreads eight rows' reads over the banks.
+constexpr int kManyRows = 128, kManyKeys = 64;
+
+template <int D>
+struct ManyShape {
+  static constexpr int DW = D / 64;            // words of a thread's share of a row
+  static constexpr int KB = kManyKeys * D;     // bytes of K
+  static constexpr int VB = kManyKeys * D * 2; // bytes of V
+  static constexpr int BUF = KB + VB + 64;     // and 64 scale bytes
+  static constexpr int DS = D / 64;            // 64-column steps of the first product
+  static constexpr int DT = D / 32;            // 32-row tiles of O^T
+};
+
+// byte offset of 16-byte chunk c of K row `row`
+template <int D>
+TCFP_DEV int k_at(int row, int c) {
+  if constexpr (D == 64) return row * D + ((c ^ ((row >> 1) & 3)) << 4);
+  else return row * D + ((c ^ (row & 7)) << 4);
+}
+// and of V^T row (column of V) d: 8 chunks of 8 keys
+TCFP_DEV int v_at(int d, int c) { return d * 128 + ((c ^ ((d ^ (d >> 3) ^ (d >> 6)) & 7)) << 4); }
+
+template <int D>
+struct ManyLoad {
+  uint32_t k[4][ManyShape<D>::DW], v[4][ManyShape<D>::DW];
+  uint32_t ke, ve;
+  int page;
+};
+
+template <int N>
+TCFP_DEV void load_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 t = *reinterpret_cast<const uint2*>(p);
+    w[0] = t.x; w[1] = t.y;
+  } else {
+    const uint4 t = *reinterpret_cast<const uint4*>(p);
+    w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
   }
+}
+template <int N>
+TCFP_DEV void store_lds(uint8_t* p, const uint32_t* w) {
+  if constexpr (N == 1) *reinterpret_cast<uint32_t*>(p) = w[0];
+  else if constexpr (N == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Thread: keys 4 kg ... 4 kg + 3 of the 64, bytes dg * D / 16 ... of their rows.
+template <int D>
+TCFP_DEV void many_load(const Attend& a, int kvh, int key0, int page, ManyLoad<D>& t) {
+  const int kg = threadIdx.x >> 4, dg = threadIdx.x & 15;
+  const int key = key0 + 4 * kg;
+  t.page = page;
+  const int64_t at = ((int64_t(max(page, 0)) * a.kv_heads + kvh) << a.page_bits) +
+                     (key & ((1 << a.page_bits) - 1));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    load_words<ManyShape<D>::DW>(a.k_codes + (at + j) * D + dg * (D / 16), t.k[j]);
+    load_words<ManyShape<D>::DW>(a.v_codes + (at + j) * D + dg * (D / 16), t.v[j]);
+  }
+  t.ke = *reinterpret_cast<const uint32_t*>(a.k_exps + at);
+  t.ve = *reinterpret_cast<const uint32_t*>(a.v_exps + at);
+}
+
+// The loaded keys into a buffer.  masked: some row of the workgroup does not
+// see all of them; what no row sees counts as zero, and a NaN among the codes
+// of V becomes a NaN scale of the key (so that it reaches the rows that see
+// the key and no other).
+template <int D>
+TCFP_DEV void many_store(uint8_t* buf, ManyLoad<D>& t, int key0, bool masked, int all_lo,
+                         int all_hi) {
+  using S = ManyShape<D>;
+  const int kg = threadIdx.x >> 4, dg = threadIdx.x & 15;
+  // 127 added to each byte
+  uint32_t scales = ((t.ke & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) ^ (t.ke & 0x80808080u);
+  if (masked) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int key = key0 + 4 * kg + j;
+      const bool dead = key < all_lo || key >= all_hi || t.page < 0;
+      bool nan = false;
+#pragma unroll
+      for (int w = 0; w < S::DW; ++w) nan |= has_nan_code(t.v[j][w]);
+      const uint64_t any = __ballot(nan && !dead);
+      if ((any >> (lane & 48)) & 0xFFFFu) scales |= 0xFFu << (8 * j);
+#pragma unroll
+      for (int w = 0; w < S::DW; ++w) t.v[j][w] = dead ? 0u : without_nan(t.v[j][w]);
+      if (dead) t.ve &= ~(0xFFu << (8 * j));
+    }
+    if (t.page < 0) scales = 0;  // no page: nobody sees these four keys
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int byte = dg * (D / 16);
+    store_lds<S::DW>(buf + k_at<D>(4 * kg + j, byte >> 4) + (byte & 15), t.k[j]);
+  }
+  uint8_t* vt = buf + S::KB;
+  const int c = (kg >> 2) * 2 + (kg & 1), sub = ((kg >> 1) & 1) * 8;
+  float sc[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sc[j] = exp_scale(t.ve, j);
+#pragma unroll
+  for (int w = 0; w < S::DW; ++w)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[j] = h ? deq2<true>(t.v[j][w], sc[j]) : deq2<false>(t.v[j][w], sc[j]);
+      const int d = dg * (D / 16) + 4 * w + 2 * h;
+      *reinterpret_cast<uint2*>(vt + v_at(d, c) + sub) =
+          make_uint2(lows(x[0], x[1]), lows(x[2], x[3]));
+      *reinterpret_cast<uint2*>(vt + v_at(d + 1, c) + sub) =
+          make_uint2(highs(x[0], x[1]), highs(x[2], x[3]));
+    }
+  if (dg == 0) *reinterpret_cast<uint32_t*>(buf + S::KB + S::VB + 4 * kg) = scales;
+}
+
+TCFP_DEV float other_half(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return (threadIdx.x & 32) ? __uint_as_float(r[0]) : __uint_as_float(r[1]);
+}
+
+template <int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Attend a) {
+  using S = ManyShape<D>;
+  __shared__ uint4 lds4[2 * S::BUF / 16];
+  uint8_t* const lds = reinterpret_cast<uint8_t*>(lds4);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  // Workgroups go round the 8 XCDs in turn: each XCD takes a contiguous run of
+  // (sequence, head, split, tile), whose tiles read the same keys from its L2.
+  const uint32_t total = gridDim.x, per = total / 8, rest = total % 8;
+  const uint32_t xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
+  uint32_t id = xcd * per + min(xcd, rest) + nth;
+  // the last tiles, which see the most keys, first
+  const int tile = a.tiles - 1 - int(id % uint32_t(a.tiles));
+  id /= uint32_t(a.tiles);
+  const int split = int(id % uint32_t(a.splits));
+  id /= uint32_t(a.splits);
+  const int kvh = int(id % uint32_t(a.kv_heads)), b = int(id / uint32_t(a.kv_heads));
+  const Seq seq = sequence(a, b);
+  if (split == 0 && tile == 0) zero_rest(a, b, kvh, seq, D);
+  const int32_t* table = a.table + int64_t(b) * a.table_stride;
+  const int kg = threadIdx.x >> 4;
+  for (int r0 = tile * kManyRows; r0 < seq.rows; r0 += a.tiles * kManyRows) {
+    const Keys keys = keys_of(a, seq, r0, kManyRows);
+    if (split >= max(keys.live, 1)) continue;
+    const int k0 = keys.begin + split * a.chunk;
+    const int k1 = split == a.splits - 1 ? keys.end : min(keys.end, k0 + a.chunk);
+    // rows of the tile, of the wave and of the lane; rows past the last repeat it
+    const int last = min(r0 + kManyRows, seq.rows) - 1;
+    const int row = min(r0 + 32 * wave + col, last), tok = row / a.group,
+              head = row - tok * a.group;
+    const int lo = key_lo(a, seq, tok), hi = key_hi(a, seq, tok);
+    const int wfirst = min(r0 + 32 * wave, last) / a.group,
+              wlast = min(r0 + 32 * wave + 31, last) / a.group;
+    const int all_lo = key_lo(a, seq, r0 / a.group), all_lo_max = key_lo(a, seq, last / a.group),
+              all_hi_min = key_hi(a, seq, r0 / a.group);
+    const int w_lo = key_lo(a, seq, wfirst), w_lo_max = key_lo(a, seq, wlast),
+              w_hi_min = key_hi(a, seq, wfirst), w_hi = key_hi(a, seq, wlast);
+    const bool idle = r0 + 32 * wave > last;
+    v8i qhi[S::DS], qlo[S::DS];
+    const int qe = split_q<S::DS, 2>(a.q + int64_t(seq.start + tok) * a.q_token +
+                                         int64_t(kvh * a.group + head) * a.q_head + half * 32,
+                                     64, a.q_mul, qhi, qlo);
+    v16f o[S::DT];
+#pragma unroll
+    for (int i = 0; i < S::DT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    if (k0 < k1) {
+      // a missing page anywhere in the run: every step looks for it
+      bool hole = false;
+      for (int p = (k0 >> a.page_bits) + int(threadIdx.x); p <= (k1 - 1) >> a.page_bits; p += 256)
+        hole |= valid_page(a, table[p]) < 0;
+      const bool holes = __syncthreads_or(hole);
+      const int last_page = (k1 - 1) >> a.page_bits;
+      auto page_at = [&](int key) {
+        return valid_page(a, table[min((key + 4 * kg) >> a.page_bits, last_page)]);
+      };
+      auto is_masked = [&](int key) {
+        return holes || key < all_lo_max || key + kManyKeys > all_hi_min;
+      };
+      ManyLoad<D> t;
+      many_load<D>(a, kvh, k0, page_at(k0), t);
+      int page = page_at(k0 + kManyKeys);
+      many_store<D>(lds, t, k0, is_masked(k0), all_lo, keys.end);
+      int cur = 0;
+      for (int key = k0; key < k1; key += kManyKeys) {
+        const bool more = key + kManyKeys < k1;
+        if (more) {
+          many_load<D>(a, kvh, key + kManyKeys, page, t);
+          page = page_at(key + 2 * kManyKeys);
+        }
+        __syncthreads();  // this step's buffer is written, the other one read
+        const uint8_t* buf = lds + cur * S::BUF;
+        if (!idle && key < w_hi && key + kManyKeys > w_lo) {
+          float p[2][16];
+          float top = -INFINITY;
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            const int krow = 32 * kt + col;
+            const int ks = buf[S::KB + S::VB + krow];
+            v16f s = {};
+#pragma unroll
+            for (int d = 0; d < S::DS; ++d) {
+              const uint4 x = *reinterpret_cast<const uint4*>(buf + k_at<D>(krow, 4 * d + 2 * half));
+              const uint4 y =
+                  *reinterpret_cast<const uint4*>(buf + k_at<D>(krow, 4 * d + 2 * half + 1));
+              v8i k;
+              k[0] = int(x.x); k[1] = int(x.y); k[2] = int(x.z); k[3] = int(x.w);
+              k[4] = int(y.x); k[5] = int(y.y); k[6] = int(y.z); k[7] = int(y.w);
+              s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, qhi[d], s, 0, 0, 0, ks, 0, qe);
+              s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, qlo[d], s, 0, 0, 0, ks, 0, qe);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) p[kt][j] = s[j];
+          }
+          if (holes || key < w_lo_max || key + kManyKeys > w_hi_min) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const bool gone =
+                    holes && *reinterpret_cast<const uint32_t*>(
+                                 buf + S::KB + S::VB + 32 * kt + 8 * g + 4 * half) == 0;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const int kk = key + 32 * kt + 8 * g + 4 * half + r;
+                  if (gone || kk < lo || kk >= hi) p[kt][4 * g + r] = -INFINITY;
+                }
+              }
+          }
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, p[kt][j]);
+          top = fmaxf(top, other_half(top));
+          top = fmaxf(top, m);
+          if (__ballot(top > m)) {
+            const float f = top == m ? 1.0f : exp2_fast((m - top) * a.c);
+            m = top;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < S::DT; ++i) o[i] *= f;
+          }
+          const float off = top == -INFINITY ? 0.0f : top * a.c;
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              p[kt][j] = exp2_fast(__builtin_fmaf(p[kt][j], a.c, -off));
+              l += p[kt][j];
+            }
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const float* x = p[s >> 1] + 8 * (s & 1);
+            const v8bf pf = as_bf(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]),
+                                  pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+#pragma unroll
+            for (int i = 0; i < S::DT; ++i) {
+              const uint4 w = *reinterpret_cast<const uint4*>(
+                  buf + S::KB + v_at(32 * i + col, 2 * s + half));
+              o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf(w.x, w.y, w.z, w.w), pf, o[i],
+                                                             0, 0, 0);
+            }
+          }
+        }
+        cur ^= 1;
+        if (more)
+          many_store<D>(lds + cur * S::BUF, t, key + kManyKeys, is_masked(key + kManyKeys), all_lo,
+                        keys.end);
+      }
+      __syncthreads();  // (the next tile writes the buffers again)
+    }
+    l += other_half(l);
+    if (r0 + 32 * wave + col <= last) {
+      const int64_t at = int64_t(seq.start + tok) * a.heads + kvh * a.group + head;
+      if (keys.live <= 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < S::DT; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint2*>(a.out + at * D + 32 * i + 8 * g + 4 * half) =
+                make_uint2(pack_bf16(o[i][4 * g] * inv, o[i][4 * g + 1] * inv),
+                           pack_bf16(o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv));
+      } else {
+        const int64_t pa = int64_t(split) * a.tokens * a.heads + at;
+#pragma unroll
+        for (int i = 0; i < S::DT; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float4*>(a.part + pa * D + 32 * i + 8 * g + 4 * half) =
+                make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+        if (half == 0) {
+          a.part_ml[2 * pa] = m;
+          a.part_ml[2 * pa + 1] = l;
+        }
+      }
+    }
+  }
+}
+
+// A wave a row whose keys were split: the splits' sums, brought to the largest
+// maximum and added in order.
+template <int D>
+__global__ __launch_bounds__(256) void attend_join_kernel(Attend a, int tile_rows) {
+  constexpr int C = D / 64;
+  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = int64_t(a.tokens) * a.heads;
+  if (row >= rows) return;
+  const int t = int(row / a.heads), h = int(row - int64_t(t) * a.heads);
+  int lo = 0, hi = a.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (a.starts[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  const Seq seq = sequence(a, lo);
+  if (t < seq.start || t >= seq.start + seq.new_tokens) return;
+  const int r = (t - seq.start) * a.group + h % a.group;
+  const Keys keys = keys_of(a, seq, r / tile_rows * tile_rows, tile_rows);
+  if (keys.live <= 1) return;
+  float m = -INFINITY, l = 0.0f;
+  if (lane < keys.live) {
+    m = a.part_ml[2 * (lane * rows + row)];
+    l = a.part_ml[2 * (lane * rows + row) + 1];
+  }
+  const float top = wave_max(m);
+  const float f = m == top ? 1.0f : exp2_fast((m - top) * a.c);
+  float sum = l * f;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
+  float o[C] = {};
+  for (int s = 0; s < keys.live; ++s) {
+    const float fs = __shfl(f, s, 64);
+    const float* p = a.part + (s * rows + row) * D + lane * C;
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] += fs * p[c];
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int c = 0; c < C; ++c) a.out[row * D + lane * C + c] = f32_to_bf16_rne(o[c] * inv);
+}
+
+// How the batch is laid over the card, from the bounds of its lengths.
+struct Launch {
+  int few_tiles;  // 16-row tiles a workgroup of the few-rows kernel takes; 0: many rows
+  int tile_rows, tiles, splits, chunk;
+};
+Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
+            int64_t max_query_len, int64_t max_seq_len, int64_t window) {
+  Launch p;
+  const int64_t group = heads / kv_heads;
+  const int64_t most = std::max<int64_t>(std::min(max_query_len, tokens), 1) * group;
+  p.few_tiles = most <= 16 ? 1 : most <= 32 ? 2 : 0;
+  p.tile_rows = p.few_tiles ? 16 * p.few_tiles : kManyRows;
+  p.tiles = int((most + p.tile_rows - 1) / p.tile_rows);
+  // workgroups without splitting: at most one tile a sequence is part full
+  const int64_t full = std::min<int64_t>(p.tiles * batch, tokens * group / p.tile_rows + batch);
+  const int64_t wgs = std::max<int64_t>(full * kv_heads, 1);
+  int64_t keys = std::clamp<int64_t>(max_seq_len, 1, int64_t(1) << 30);
+  if (window > 0) keys = std::min(keys, window + max_query_len + 64);
+  const int64_t unit = 256;
+  const int64_t want = p.few_tiles ? 2048 : 512;
+  const int64_t splits = std::clamp<int64_t>((want + wgs - 1) / wgs, 1, kMaxSplits);
+  const int64_t per = (keys + splits - 1) / splits;
+  const int64_t chunk = std::max<int64_t>((per + unit - 1) / unit * unit, unit);
+  p.chunk = int(std::min<int64_t>(chunk, int64_t(1) << 30));
+  p.splits = int(std::clamp<int64_t>((keys + 63 + p.chunk - 1) / p.chunk, 1, kMaxSplits));
+  return p;
+}
+
+size_t workspace_of(const Launch& p, int64_t tokens, int heads, int dim) {
+  if (p.splits <= 1) return 0;
+  return size_t(p.splits) * size_t(tokens) * size_t(heads) * size_t(dim + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -303,10 +1107,11 @@ int tcfp_kv_cache_read(const uint8_t* k_codes, const uint8_t* v_codes, const int
 
 size_t tcfp_paged_attention_workspace_bytes(int64_t tokens, int heads, int kv_heads, int dim,
                                             int64_t batch, int64_t max_query_len,
-                                            int64_t max_seq_len) {
-  (void)tokens, (void)heads, (void)kv_heads, (void)dim, (void)batch;
-  (void)max_query_len, (void)max_seq_len;
-  return 0;
+                                            int64_t max_seq_len, int64_t window) {
+  if (tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  return workspace_of(
+      plan(tokens, heads, kv_heads, dim, batch, max_query_len, max_seq_len, window), tokens, heads,
+      dim);
 }
 
 int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -323,24 +1128,82 @@ int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     return TCFP_ERR_SHAPE;
   if (heads <= 0 || heads > 65535 || heads % kv_heads != 0) return TCFP_ERR_SHAPE;
   if (table_width < 0 || table_stride < table_width || max_query_len < 0 || max_seq_len < 0 ||
-      window < 0)
+      window < 0 || tokens * (heads / kv_heads) > INT32_MAX / 2)
     return TCFP_ERR_SHAPE;
   if (!aligned16(q) || !aligned16(out) || !aligned16(k_codes) || !aligned16(v_codes) ||
-      q_token_stride % 8 || q_head_stride % 8)
+      q_token_stride % 8 || q_head_stride % 8 || (reinterpret_cast<uintptr_t>(k_exps) & 3u) ||
+      (reinterpret_cast<uintptr_t>(v_exps) & 3u))
     return TCFP_ERR_ALIGN;
   if (tokens == 0) return TCFP_OK;
   if (batch == 0) return TCFP_ERR_SHAPE;
-  (void)workspace, (void)workspace_bytes;
-  const Attend a{static_cast<const uint16_t*>(q), q_token_stride, q_head_stride, k_codes, v_codes,
-                 k_exps, v_exps, num_pages, log2i(page_size), kv_heads, page_table, table_stride,
-                 table_width * page_size, seq_lens, query_start, batch, tokens, heads,
-                 heads / kv_heads, scale, causal, window, static_cast<uint16_t*>(out)};
+  const Launch p =
+      plan(tokens, heads, kv_heads, dim, batch, max_query_len, max_seq_len, window);
+  const size_t need = workspace_of(p, tokens, heads, dim);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return TCFP_ERR_WORKSPACE;
+  Attend a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.k_codes = k_codes;
+  a.v_codes = v_codes;
+  a.k_exps = k_exps;
+  a.v_exps = v_exps;
+  a.num_pages = int(num_pages);
+  a.page_bits = log2i(page_size);
+  a.kv_heads = kv_heads;
+  a.table = page_table;
+  a.table_stride = table_stride;
+  // (a pool without pages holds no key; positions stay clear of 2^31)
+  a.table_keys = num_pages == 0 ? 0 : int(std::min<int64_t>(table_width * page_size, 1 << 30));
+  a.seq_lens = seq_lens;
+  a.starts = query_start;
+  a.batch = int(batch);
+  a.tokens = int(tokens);
+  a.heads = heads;
+  a.group = heads / kv_heads;
+  a.c = scale == 0.0f ? 1.0f : std::abs(scale) * 1.44269504088896340736f;
+  a.q_mul = scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f;
+  a.causal = causal != 0;
+  a.window = int(std::min<int64_t>(window, 1 << 30));
+  a.tiles = p.tiles;
+  a.splits = p.splits;
+  a.chunk = p.chunk;
+  a.out = static_cast<uint16_t*>(out);
+  a.part = static_cast<float*>(workspace);
+  a.part_ml = a.part + size_t(p.splits) * size_t(tokens) * size_t(heads) * size_t(dim);
   const auto st = static_cast<hipStream_t>(stream);
-  if (!grid_x_fits(tokens, 64)) return TCFP_ERR_SHAPE;
-  const dim3 grid{unsigned(tokens), unsigned(heads)};
-  if (dim == 64) attend_row_kernel<64><<<grid, 64, 0, st>>>(a);
-  else if (dim == 128) attend_row_kernel<128><<<grid, 64, 0, st>>>(a);
-  else attend_row_kernel<256><<<grid, 64, 0, st>>>(a);
+#define TCFP_BY_DIM(CALL)         \
+  do {                            \
+    if (dim == 64) CALL(64);      \
+    else if (dim == 128) CALL(128); \
+    else CALL(256);               \
+  } while (0)
+  if (p.few_tiles) {
+    if (int64_t(kv_heads) * p.tiles > 65535) return TCFP_ERR_SHAPE;
+    const dim3 grid(unsigned(p.splits), unsigned(kv_heads * p.tiles), unsigned(batch));
+#define TCFP_FEW(D)                                                       \
+  do {                                                                    \
+    if (p.few_tiles == 1) attend_few_kernel<D, 1><<<grid, 256, 0, st>>>(a); \
+    else attend_few_kernel<D, 2><<<grid, 256, 0, st>>>(a);                \
+  } while (0)
+    TCFP_BY_DIM(TCFP_FEW);
+#undef TCFP_FEW
+  } else {
+    const int64_t wgs = int64_t(p.tiles) * p.splits * kv_heads * batch;
+    if (wgs > INT32_MAX || !grid_x_fits(wgs, 256)) return TCFP_ERR_SHAPE;
+#define TCFP_MANY(D) attend_many_kernel<D><<<unsigned(wgs), 256, 0, st>>>(a)
+    TCFP_BY_DIM(TCFP_MANY);
+#undef TCFP_MANY
+  }
+  if (p.splits > 1) {
+    const int64_t blocks = (tokens * heads + 3) / 4;
+    if (!grid_x_fits(blocks, 256)) return TCFP_ERR_SHAPE;
+#define TCFP_JOIN(D) attend_join_kernel<D><<<unsigned(blocks), 256, 0, st>>>(a, p.tile_rows)
+    TCFP_BY_DIM(TCFP_JOIN);
+#undef TCFP_JOIN
+  }
+#undef TCFP_BY_DIM
   return launch_status();
 }
 

@@ -1032,7 +1032,7 @@ Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
   const int64_t most = std::min(max_seq_len.value_or(width * c.page_size), width * c.page_size);
   Tensor out = g.empty({tokens, heads, c.dim}, at::kBFloat16), ws;
   const size_t nb = tcfp_paged_attention_workspace_bytes(tokens, int(heads), c.heads, c.dim, batch,
-                                                         max_query_len, most);
+                                                         max_query_len, most, window);
   if (nb) ws = g.empty({int64_t(nb)}, at::kByte);
   check(tcfp_paged_attention(ptr(q), q.stride(0), q.stride(1), bytes(kc), bytes(vc), exps(ke),
                              exps(ve), c.pages, int(c.page_size), c.heads, c.dim,
