@@ -759,6 +759,12 @@ Outs block_linear_backward(const Tensor& grad_2d, const OptT& act_fp8, const Opt
 
 // ---- decoder operators -------------------------------------------------------
 
+// Contiguous and 16-byte aligned.
+Tensor whole(const Tensor& x) {
+  Tensor c = x.contiguous();
+  return al16(c) ? c : c.clone();
+}
+
 // Rows of the last axis: a 2-D tensor's rows may be apart, anything else is
 // made contiguous.
 struct Rows {
@@ -768,8 +774,11 @@ struct Rows {
 Rows rows_of(const Tensor& x, const char* name) {
   if (x.dim() == 0) value_error(std::string(name) + " needs at least one dimension");
   Rows r{x, 0, x.size(-1), 0};
-  const bool apart = x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= x.size(1);
-  if (!apart && !x.is_contiguous()) r.t = x.contiguous();
+  // (rows that 16-byte loads do not take are copied, so that the result does
+  // not depend on where they lie)
+  const bool apart = x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= x.size(1) && al16(x) &&
+                     x.stride(0) * x.element_size() % 16 == 0;
+  if (!apart) r.t = whole(x);
   r.rows = r.cols ? r.t.numel() / r.cols : 0;
   r.ld = apart ? r.t.stride(0) : r.cols;
   return r;
@@ -792,7 +801,7 @@ NormIn norm_inputs(OnGpu& g, const Tensor& x, const Tensor& weight, const OptT& 
   if (weight.dim() != 1 || weight.size(0) != n.x.cols)
     value_error("weight must have shape (" + std::to_string(n.x.cols) + ",), got " +
                 shape_str(weight.sizes()));
-  n.w = weight.contiguous();
+  n.w = whole(weight);
   if (residual) {
     if (residual->sizes() != x.sizes())
       value_error("residual shape " + shape_str(residual->sizes()) + " != x shape " +
@@ -868,10 +877,9 @@ Outs rms_norm_backward(const Tensor& grad_y, const Tensor& h, const Tensor& rstd
     if (grad_h->scalar_type() != h.scalar_type())
       type_error(std::string("grad_h must have h's dtype ") + dtype_str(h.scalar_type()) +
                  ", got " + dtype_str(grad_h->scalar_type()));
-    gh = grad_h->contiguous();
+    gh = whole(*grad_h);
   }
-  const Tensor gy = grad_y.contiguous(), hc = h.contiguous(), rs = rstd.contiguous(),
-               w = weight.contiguous();
+  const Tensor gy = whole(grad_y), hc = whole(h), rs = rstd.contiguous(), w = whole(weight);
   Tensor dx = g.empty(h.sizes(), h.scalar_type()), dw, ws;
   size_t nb = 0;
   if (need_dw) {
@@ -934,8 +942,7 @@ Tensor check_slots(const Tensor& slots, int64_t tokens) {
 Tensor head_rows(const Tensor& x) {
   const int64_t unit = 16 / x.element_size();
   if (x.stride(2) == 1 && x.stride(0) % unit == 0 && x.stride(1) % unit == 0 && al16(x)) return x;
-  Tensor c = x.contiguous();
-  return al16(c) ? c : c.clone();
+  return whole(x);
 }
 void check_heads(const Tensor& x, int64_t heads, int64_t dim, const char* name) {
   if (x.dim() != 3 || (heads > 0 && x.size(1) != heads) || x.size(2) != dim)

@@ -52,8 +52,6 @@ TCFP_DEV void scale_of(float amax, float fmax, float& mul, float& inv) {
   inv = __fdiv_rn(1.0f, mul);
 }
 
-enum { kPlain = 0, kExps = 1, kF32Scales = 2 };
-
 struct Norm {
   const void* x;
   const void* r;
@@ -63,7 +61,7 @@ struct Norm {
   int64_t rows;
   int64_t cols;
   float eps;
-  int block, fmt;
+  int block, fmt, f32_scales;
   void* h;
   void* y;
   uint8_t* q;
@@ -74,7 +72,7 @@ struct Norm {
 // One workgroup a row, any width and alignment: the row is read twice, the
 // second time from L2.  Blocks of the quantised output are groups of 32
 // consecutive threads, an element each, stepping over a block's columns.
-template <int MODE>
+template <bool QUANT>
 __global__ __launch_bounds__(kThreads) void norm_any_kernel(Norm a) {
   __shared__ float red[kThreads / 64];
   const int64_t row = blockIdx.x;
@@ -92,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void norm_any_kernel(Norm a) {
   ss = block_sum<kThreads>(ss, red);
   const float rstd = 1.0f / sqrtf(ss / float(a.cols) + a.eps);
   if (threadIdx.x == 0) a.rstd[row] = rstd;
-  if constexpr (MODE == kPlain) {
+  if constexpr (!QUANT) {
     for (int64_t c = threadIdx.x; c < a.cols; c += kThreads)
       store1(a.y, a.y_dtype, row * a.cols + c, sum_at(c) * rstd * load1(a.w, a.w_dtype, c));
   } else {
@@ -108,7 +106,7 @@ __global__ __launch_bounds__(kThreads) void norm_any_kernel(Norm a) {
       for (int o = 16; o > 0; o >>= 1) m = umax(m, uint32_t(__shfl_xor(int(m), o, 32)));
       float mul, inv = 0.0f;
       int e = 0;
-      if constexpr (MODE == kF32Scales) {
+      if (a.f32_scales) {
         scale_of(__uint_as_float(m), fmax, mul, inv);
       } else {
         e = block_exponent(__uint_as_float(m), fmax);
@@ -121,11 +119,259 @@ __global__ __launch_bounds__(kThreads) void norm_any_kernel(Norm a) {
             uint8_t(a.fmt == TCFP_FP8_E5M2 ? f32_to_e5m2(v) : f32_to_e4m3(v));
       }
       if (lane == 0) {
-        if constexpr (MODE == kF32Scales) static_cast<float*>(a.scales)[kb * a.rows + row] = inv;
+        if (a.f32_scales) static_cast<float*>(a.scales)[kb * a.rows + row] = inv;
         else static_cast<int8_t*>(a.scales)[kb * a.rows + row] = int8_t(e);
       }
     }
   }
+}
+
+// ---- rows held in registers --------------------------------------------------
+//
+// Bound by HBM: each input is read and each output written once.  T threads
+// hold a row, C vectors of 8 neighbouring elements each (vector i of thread t
+// at column 8 (t + i T)), so a block's maximum is over 4, 8 or 16 neighbouring
+// lanes.  A workgroup walks `run` neighbouring rows with the next row's loads
+// in flight; block scales, whose neighbours in memory are neighbouring rows,
+// are gathered in LDS and written as runs of `run` values.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<uint16_t> {
+  uint4 a;
+  TCFP_DEV void load(const uint16_t* p) { a = *reinterpret_cast<const uint4*>(p); }
+  TCFP_DEV void zero() { a = make_uint4(0, 0, 0, 0); }
+  TCFP_DEV void get(float* v) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+};
+template <>
+struct Raw8<float> {
+  float4 a, b;
+  TCFP_DEV void load(const float* p) {
+    a = reinterpret_cast<const float4*>(p)[0];
+    b = reinterpret_cast<const float4*>(p)[1];
+  }
+  TCFP_DEV void zero() { a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+  TCFP_DEV void get(float* v) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+};
+TCFP_DEV uint32_t pack_bf16(float a, float b) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  const bf2 r = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, r);
+}
+TCFP_DEV void store8(uint16_t* p, const float* v) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]),
+                                            pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+TCFP_DEV void store8(float* p, const float* v) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+TCFP_DEV void load8_any(const void* p, int dtype, int64_t i, float* v) {
+  if (dtype == TCFP_DTYPE_BF16) {
+    Raw8<uint16_t> r;
+    r.load(static_cast<const uint16_t*>(p) + i);
+    r.get(v);
+  } else {
+    Raw8<float> r;
+    r.load(static_cast<const float*>(p) + i);
+    r.get(v);
+  }
+}
+
+constexpr int kWaveCols = 2048;      // widest row of a wave
+constexpr int kWaveColsBack = 1024;  // and in the backward
+constexpr int kRun = 16;  // rows of a workgroup at most
+
+// Sum over the T threads of a row, to each of them.  T > 64: through `red`,
+// whose use alternates between two arrays by row, one barrier a row.
+template <int T, int W>
+TCFP_DEV float row_sum(float v, float (*red)[W], int parity) {
+  v = wave_sum(v);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) red[parity][threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[parity][0];
+#pragma unroll
+    for (int i = 1; i < T / 64; ++i) v += red[parity][i];
+  }
+  return v;
+}
+
+template <typename XT, typename RT, bool QUANT, int T, int C>
+__global__ __launch_bounds__(kThreads) void norm_rows_kernel(Norm a, int run) {
+  constexpr int G = kThreads / T;  // rows at a time
+  constexpr int NB = QUANT ? T * C / 4 : 1;
+  __shared__ float red[2][kThreads / 64];
+  __shared__ uint32_t sc[NB * kRun];
+  const int t = threadIdx.x % T, g = threadIdx.x / T;
+  const int64_t row0 = int64_t(blockIdx.x) * run;
+  const int nvec = int(a.cols / 8);
+  const XT* x = static_cast<const XT*>(a.x);
+  const RT* r = static_cast<const RT*>(a.r);
+  float w[C][8];
+  Raw8<XT> nx[C];
+  Raw8<RT> nr[C];
+  auto fetch = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int v = t + i * T;
+      if (v < nvec && row < a.rows) {
+        nx[i].load(x + row * a.ldx + v * 8);
+        if (r) nr[i].load(r + row * a.ldr + v * 8);
+      } else {
+        nx[i].zero();
+        nr[i].zero();
+      }
+    }
+  };
+  fetch(row0 + g);
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+    if (t + i * T < nvec) {
+      load8_any(a.w, a.w_dtype, (t + i * T) * 8, w[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[i][j] = 0.0f;
+    }
+  for (int k = 0; k < run; k += G) {
+    const int64_t row = row0 + k + g;
+    const bool live = row < a.rows;
+    float s[C][8];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      nx[i].get(s[i]);
+      if (r) {
+        float rv[8];
+        nr[i].get(rv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[i][j] += rv[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(s[i][j], s[i][j], ss);
+    }
+    if (k + G < run) fetch(row + G);
+    if (a.h && live) {
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+        if (t + i * T < nvec)
+          store8(static_cast<RT*>(a.h) + row * a.cols + (t + i * T) * 8, s[i]);
+    }
+    ss = row_sum<T>(ss, red, (k / G) & 1);
+    const float rstd = 1.0f / sqrtf(ss / float(a.cols) + a.eps);
+    if (t == 0 && live) a.rstd[row] = rstd;
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[i][j] = s[i][j] * rstd * w[i][j];
+    if constexpr (!QUANT) {
+      if (live) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          if (t + i * T >= nvec) continue;
+          const int64_t at = row * a.cols + (t + i * T) * 8;
+          if (a.y_dtype == TCFP_DTYPE_BF16) store8(static_cast<uint16_t*>(a.y) + at, s[i]);
+          else store8(static_cast<float*>(a.y) + at, s[i]);
+        }
+      }
+    } else {
+      const float fmax = fp8_max(a.fmt);
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = umax(m, absbits(s[i][j]));
+        if (a.block == 32) m = seg_umax<4>(m);
+        else if (a.block == 64) m = seg_umax<8>(m);
+        else m = seg_umax<16>(m);
+        float mul;
+        uint32_t code;
+        if (a.f32_scales) {
+          float inv;
+          scale_of(__uint_as_float(m), fmax, mul, inv);
+          code = __float_as_uint(inv);
+        } else {
+          const int e = block_exponent(__uint_as_float(m), fmax);
+          mul = exp2i(-e);
+          code = uint32_t(e);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[i][j] = clampf(s[i][j] * mul, fmax);
+        uint2 q;
+        if (a.fmt == TCFP_FP8_E5M2)
+          q = make_uint2(cvt4_fp8<TCFP_FP8_E5M2>(s[i][0], s[i][1], s[i][2], s[i][3]),
+                         cvt4_fp8<TCFP_FP8_E5M2>(s[i][4], s[i][5], s[i][6], s[i][7]));
+        else
+          q = make_uint2(cvt4_fp8<TCFP_FP8_E4M3>(s[i][0], s[i][1], s[i][2], s[i][3]),
+                         cvt4_fp8<TCFP_FP8_E4M3>(s[i][4], s[i][5], s[i][6], s[i][7]));
+        const int v = t + i * T;
+        if (v < nvec) {
+          if (live) *reinterpret_cast<uint2*>(a.q + row * a.cols + v * 8) = q;
+          if ((v * 8) % a.block == 0) sc[(v * 8 / a.block) * kRun + k + g] = code;
+        }
+      }
+    }
+  }
+  if constexpr (QUANT) {
+    __syncthreads();
+    const int n = int(a.cols / a.block) * run;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const int kb = i / run, k = i - kb * run;
+      if (row0 + k >= a.rows) continue;
+      const int64_t at = kb * a.rows + row0 + k;
+      const uint32_t code = sc[kb * kRun + k];
+      if (a.f32_scales) static_cast<uint32_t*>(a.scales)[at] = code;
+      else static_cast<int8_t*>(a.scales)[at] = int8_t(code);
+    }
+  }
+}
+
+// Threads and vectors of a row: a wave a row where the rows alone fill the
+// card, else the row over a workgroup; 0: the kernel for any row.
+struct RowShape {
+  int t, c;
+};
+RowShape row_shape(int64_t rows, int64_t cols, int64_t wave_cols) {
+  if (cols % 8 != 0 || cols > kThreads * 64) return {0, 0};
+  const int64_t nvec = cols / 8;
+  const int t = rows >= 1024 && cols <= wave_cols ? 64 : nvec <= 64 ? 64 : kThreads;
+  int c = 1;
+  while (int64_t(t) * c < nvec) c *= 2;
+  return {t, c};
+}
+bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+int64_t size_of(int dtype) { return dtype == TCFP_DTYPE_BF16 ? 2 : 4; }
+
+template <typename XT, typename RT, bool QUANT>
+int norm_rows_launch(const Norm& a, RowShape s, hipStream_t st) {
+  const int g = kThreads / s.t;
+  // rows of a workgroup: at least two workgroups a CU
+  const int64_t fill = a.rows / 512;
+  int run = g;
+  while (run * 2 <= kRun && run * 2 <= fill) run *= 2;
+  const unsigned blocks = unsigned((a.rows + run - 1) / run);
+#define TCFP_NR(T, C) norm_rows_kernel<XT, RT, QUANT, T, C><<<blocks, kThreads, 0, st>>>(a, run)
+#define TCFP_NR_C(T)                  \
+  do {                                \
+    if (s.c == 1) TCFP_NR(T, 1);      \
+    else if (s.c == 2) TCFP_NR(T, 2); \
+    else if (s.c == 4) TCFP_NR(T, 4); \
+    else TCFP_NR(T, 8);               \
+  } while (0)
+  if (s.t == 64) TCFP_NR_C(64); else TCFP_NR_C(kThreads);
+#undef TCFP_NR_C
+#undef TCFP_NR
+  return launch_status();
 }
 
 struct NormBack {
@@ -172,16 +418,159 @@ __global__ __launch_bounds__(kThreads) void norm_dw_any_kernel(NormBack a, int64
   a.part[int64_t(blockIdx.y) * a.cols + c] = s;
 }
 
-__global__ __launch_bounds__(kThreads) void norm_dw_sum_kernel(const float* part, int64_t parts,
-                                                               int64_t cols, float* dw) {
-  const int64_t c = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  if (c >= cols) return;
-  float s = 0.0f;
-  for (int64_t p = 0; p < parts; ++p) s += part[p * cols + c];
-  dw[c] = s;
+// ---- the backward with rows in registers -------------------------------------
+//
+// Bound by HBM like the forward.  Workgroups take every gridDim.x-th group of
+// rows, the next rows' loads in flight; a thread's columns are the same in all
+// its rows, so it sums its share of dw in registers, the workgroup leaves one
+// partial row and a second launch adds the partials.
+template <typename GT, typename HT, int T, int C>
+__global__ __launch_bounds__(T > kThreads ? T : kThreads) void norm_back_rows_kernel(NormBack a) {
+  constexpr int W = T > kThreads ? T : kThreads;  // threads of a workgroup
+  constexpr int G = W / T;
+  __shared__ float red[2][W / 64];
+  __shared__ float4 dws[G > 1 ? (G - 1) * T * C * 2 : 1];
+  const int t = threadIdx.x % T, g = threadIdx.x / T;
+  const int nvec = int(a.cols / 8);
+  const GT* gy = static_cast<const GT*>(a.gy);
+  const HT* h = static_cast<const HT*>(a.h);
+  const HT* gh = static_cast<const HT*>(a.gh);
+  float w[C][8], dw[C][8];
+  Raw8<GT> ng[C];
+  Raw8<HT> nh[C], na[C];
+  float nrs = 0.0f;
+  auto fetch = [&](int64_t row) {
+    const bool live = row < a.rows;
+    nrs = live ? a.rstd[row] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int v = t + i * T;
+      if (v < nvec && live) {
+        const int64_t at = row * a.cols + v * 8;
+        ng[i].load(gy + at);
+        nh[i].load(h + at);
+        if (gh) na[i].load(gh + at);
+      } else {
+        ng[i].zero();
+        nh[i].zero();
+        na[i].zero();
+      }
+    }
+  };
+  fetch(int64_t(blockIdx.x) * G + g);
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[i][j] = dw[i][j] = 0.0f;
+    if (t + i * T < nvec) load8_any(a.w, a.w_dtype, (t + i * T) * 8, w[i]);
+  }
+  const float inv_n = 1.0f / float(a.cols);
+  int parity = 0;
+  for (int64_t row0 = int64_t(blockIdx.x) * G; row0 < a.rows; row0 += int64_t(gridDim.x) * G) {
+    const int64_t row = row0 + g;
+    const float rs = nrs;
+    float gg[C][8], xh[C][8], add[C][8];
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      ng[i].get(gg[i]);
+      nh[i].get(xh[i]);
+      if (gh) na[i].get(add[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        xh[i][j] *= rs;
+        dw[i][j] = __builtin_fmaf(gg[i][j], xh[i][j], dw[i][j]);
+        gg[i][j] *= w[i][j];
+        s = __builtin_fmaf(gg[i][j], xh[i][j], s);
+      }
+    }
+    fetch(row + int64_t(gridDim.x) * G);
+    s = row_sum<T>(s, red, parity) * inv_n;
+    parity ^= 1;
+    if (row < a.rows) {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const int v = t + i * T;
+        if (v >= nvec) continue;
+        float d[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          d[j] = rs * (gg[i][j] - xh[i][j] * s);
+          if (gh) d[j] += add[i][j];
+        }
+        store8(static_cast<HT*>(a.dx) + row * a.cols + v * 8, d);
+      }
+    }
+  }
+  if (!a.part) return;
+  if constexpr (G > 1) {
+    if (g > 0) {
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          dws[(((g - 1) * C + i) * 2 + j) * T + t] =
+              make_float4(dw[i][4 * j], dw[i][4 * j + 1], dw[i][4 * j + 2], dw[i][4 * j + 3]);
+    }
+    __syncthreads();
+    if (g > 0) return;
+    for (int x = 0; x < G - 1; ++x)
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float4 o = dws[((x * C + i) * 2 + j) * T + t];
+          dw[i][4 * j] += o.x; dw[i][4 * j + 1] += o.y;
+          dw[i][4 * j + 2] += o.z; dw[i][4 * j + 3] += o.w;
+        }
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+    if (t + i * T < nvec)
+      store8(a.part + int64_t(blockIdx.x) * a.cols + (t + i * T) * 8, dw[i]);
 }
 
-constexpr int64_t kMaxParts = 256;
+template <typename GT, typename HT>
+void norm_back_launch(const NormBack& a, RowShape s, unsigned blocks, hipStream_t st) {
+#define TCFP_NB(T, C) \
+  norm_back_rows_kernel<GT, HT, T, C><<<blocks, (T) > kThreads ? (T) : kThreads, 0, st>>>(a)
+  if (s.t == 64) {
+    if (s.c == 1) TCFP_NB(64, 1);
+    else TCFP_NB(64, 2);
+  } else {
+    if (s.c == 1) TCFP_NB(kThreads, 1);
+    else if (s.c == 2) TCFP_NB(kThreads, 2);
+    else if (s.c == 4) TCFP_NB(kThreads, 4);
+    else TCFP_NB(2 * kThreads, 4);  // (eight vectors a thread would spill)
+  }
+#undef TCFP_NB
+}
+
+// dw from the partial rows: a workgroup 16 columns, its threads 16 partials at
+// a time, then the 16 sums in order.
+__global__ __launch_bounds__(kThreads) void norm_dw_sum_kernel(const float* part, int parts,
+                                                               int64_t cols, float* dw) {
+  __shared__ float s[16][17];
+  const int c = threadIdx.x & 15, p0 = threadIdx.x >> 4;
+  const int64_t col = int64_t(blockIdx.x) * 16 + c;
+  float v = 0.0f;
+  if (col < cols) {
+#pragma unroll 8
+    for (int p = p0; p < parts; p += 16) v += part[int64_t(p) * cols + col];
+  }
+  s[p0][c] = v;
+  __syncthreads();
+  if (p0 == 0 && col < cols) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += s[i][c];
+    dw[col] = v;
+  }
+}
+
+constexpr int64_t kMaxParts = 512;  // two workgroups a CU
+
+// Partial rows of dw: at least four rows each.
+int64_t parts_of(int64_t rows) { return std::clamp<int64_t>(rows / 4, 1, kMaxParts); }
 
 int norm_checks(const Norm& a, bool quantised) {
   if (a.rows < 0 || a.cols < 0 || a.rows > INT32_MAX || a.cols > INT32_MAX) return TCFP_ERR_SHAPE;
@@ -201,11 +590,24 @@ int norm_checks(const Norm& a, bool quantised) {
   return TCFP_OK;
 }
 
-template <int MODE>
+template <bool QUANT>
 int norm_launch(const Norm& a, hipStream_t st) {
-  const int rc = norm_checks(a, MODE != kPlain);
+  const int rc = norm_checks(a, QUANT);
   if (rc != TCFP_OK || a.rows == 0 || a.cols == 0) return rc;
-  norm_any_kernel<MODE><<<unsigned(a.rows), kThreads, 0, st>>>(a);
+  const RowShape s = row_shape(a.rows, a.cols, kWaveCols);
+  const int64_t xs = size_of(a.x_dtype), rs = size_of(a.r_dtype);
+  const bool vec = aligned(a.x, 16) && a.ldx * xs % 16 == 0 && aligned(a.w, 16) &&
+                   (!a.r || (aligned(a.r, 16) && a.ldr * rs % 16 == 0)) && aligned(a.h, 16) &&
+                   aligned(a.y, 16);
+  if (s.t && vec) {
+    const bool xb = a.x_dtype == TCFP_DTYPE_BF16;
+    const bool rb = a.r ? a.r_dtype == TCFP_DTYPE_BF16 : xb;
+    if (xb) return rb ? norm_rows_launch<uint16_t, uint16_t, QUANT>(a, s, st)
+                      : norm_rows_launch<uint16_t, float, QUANT>(a, s, st);
+    return rb ? norm_rows_launch<float, uint16_t, QUANT>(a, s, st)
+              : norm_rows_launch<float, float, QUANT>(a, s, st);
+  }
+  norm_any_kernel<QUANT><<<unsigned(a.rows), kThreads, 0, st>>>(a);
   return launch_status();
 }
 
@@ -217,8 +619,8 @@ int tcfp_rms_norm(const void* x, int x_dtype, int64_t ldx, const void* residual,
                   int64_t ldr, const void* weight, int w_dtype, int64_t rows, int64_t cols,
                   float eps, void* h, void* y, int y_dtype, float* rstd, void* stream) {
   const Norm a{x, residual, weight, ldx, ldr, x_dtype, r_dtype, w_dtype, y_dtype, rows, cols,
-               eps, 0, 0, h, y, nullptr, nullptr, rstd};
-  return norm_launch<kPlain>(a, static_cast<hipStream_t>(stream));
+               eps, 0, 0, 0, h, y, nullptr, nullptr, rstd};
+  return norm_launch<false>(a, static_cast<hipStream_t>(stream));
 }
 
 int tcfp_rms_norm_quantize(const void* x, int x_dtype, int64_t ldx, const void* residual,
@@ -227,14 +629,13 @@ int tcfp_rms_norm_quantize(const void* x, int x_dtype, int64_t ldx, const void* 
                            int f32_scales, void* h, uint8_t* q, void* scales, float* rstd,
                            void* stream) {
   const Norm a{x, residual, weight, ldx, ldr, x_dtype, r_dtype, w_dtype, 0, rows, cols,
-               eps, block, fp8_fmt, h, nullptr, q, scales, rstd};
-  const auto st = static_cast<hipStream_t>(stream);
-  return f32_scales ? norm_launch<kF32Scales>(a, st) : norm_launch<kExps>(a, st);
+               eps, block, fp8_fmt, f32_scales != 0, h, nullptr, q, scales, rstd};
+  return norm_launch<true>(a, static_cast<hipStream_t>(stream));
 }
 
 size_t tcfp_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return size_t(std::min(rows, kMaxParts)) * size_t(cols) * sizeof(float);
+  return size_t(parts_of(rows)) * size_t(cols) * sizeof(float);
 }
 
 int tcfp_rms_norm_backward(const void* grad_y, int gy_dtype, const void* h, int h_dtype,
@@ -246,20 +647,34 @@ int tcfp_rms_norm_backward(const void* grad_y, int gy_dtype, const void* h, int 
   if (!dtype_ok(gy_dtype) || !dtype_ok(h_dtype) || !dtype_ok(w_dtype)) return TCFP_ERR_DTYPE;
   if (cols == 0 || (rows == 0 && !dw)) return TCFP_OK;
   const auto st = static_cast<hipStream_t>(stream);
-  const unsigned cg = unsigned((cols + kThreads - 1) / kThreads);
-  if (dw && workspace_bytes < tcfp_rms_norm_backward_workspace_bytes(rows, cols))
+  if (dw && rows > 0 && workspace_bytes < tcfp_rms_norm_backward_workspace_bytes(rows, cols))
     return TCFP_ERR_WORKSPACE;
-  const NormBack a{grad_y, h, rstd, weight, grad_h, gy_dtype, h_dtype, w_dtype, rows, cols,
-                   dx, static_cast<float*>(workspace)};
-  if (rows > 0) norm_dx_any_kernel<<<unsigned(rows), kThreads, 0, st>>>(a);
-  if (dw) {
-    const int64_t parts = std::min(rows, kMaxParts);
-    if (rows > 0) {
-      const int64_t per = (rows + parts - 1) / parts;
-      norm_dw_any_kernel<<<dim3(cg, unsigned(parts)), kThreads, 0, st>>>(a, per);
+  const int64_t parts = rows > 0 ? parts_of(rows) : 0;
+  // (one partial row is dw itself)
+  NormBack a{grad_y, h, rstd, weight, grad_h, gy_dtype, h_dtype, w_dtype, rows, cols, dx,
+             !dw ? nullptr : parts == 1 ? dw : static_cast<float*>(workspace)};
+  if (rows > 0) {
+    const RowShape s = row_shape(rows, cols, kWaveColsBack);
+    const bool vec = aligned(grad_y, 16) && aligned(h, 16) && aligned(weight, 16) &&
+                     aligned(grad_h, 16) && aligned(dx, 16) && aligned(a.part, 16);
+    if (s.t && vec) {
+      const unsigned blocks = unsigned(
+          dw ? parts : std::min<int64_t>((rows * s.t + kThreads - 1) / kThreads, 4 * kMaxParts));
+      const bool gb = gy_dtype == TCFP_DTYPE_BF16, hb = h_dtype == TCFP_DTYPE_BF16;
+      if (gb && hb) norm_back_launch<uint16_t, uint16_t>(a, s, blocks, st);
+      else if (gb) norm_back_launch<uint16_t, float>(a, s, blocks, st);
+      else if (hb) norm_back_launch<float, uint16_t>(a, s, blocks, st);
+      else norm_back_launch<float, float>(a, s, blocks, st);
+    } else {
+      norm_dx_any_kernel<<<unsigned(rows), kThreads, 0, st>>>(a);
+      if (dw)
+        norm_dw_any_kernel<<<dim3(unsigned((cols + kThreads - 1) / kThreads), unsigned(parts)),
+                             kThreads, 0, st>>>(a, (rows + parts - 1) / parts);
     }
-    norm_dw_sum_kernel<<<cg, kThreads, 0, st>>>(a.part, parts, cols, dw);
   }
+  if (dw && parts != 1)
+    norm_dw_sum_kernel<<<unsigned((cols + 15) / 16), kThreads, 0, st>>>(a.part, int(parts), cols,
+                                                                        dw);
   return launch_status();
 }
 
