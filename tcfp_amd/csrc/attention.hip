@@ -1026,7 +1026,7 @@ Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
   const int64_t per = (keys + splits - 1) / splits;
   const int64_t chunk = std::max<int64_t>((per + unit - 1) / unit * unit, unit);
   p.chunk = int(std::min<int64_t>(chunk, int64_t(1) << 30));
-  p.splits = int(std::clamp<int64_t>((keys + 63 + p.chunk - 1) / p.chunk, 1, kMaxSplits));
+  p.splits = int(std::clamp<int64_t>((keys + p.chunk - 1) / p.chunk, 1, kMaxSplits));
   return p;
 }
 
