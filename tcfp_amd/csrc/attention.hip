@@ -188,6 +188,7 @@ struct Attend {
   int tiles;        // row tiles of a (sequence, head) in the launch
   int splits;       // of a row tile's keys
   int chunk;        // keys of a split but the last
+  int sets;         // (sequence, K/V head, split)s of the many-rows launches
   uint16_t* out;
   float* part;      // [splits][tokens * heads][dim]
   float* part_ml;   // [splits][tokens * heads][2]: max (in units of s), sum
@@ -643,6 +644,30 @@ __global__ __launch_bounds__(256, D == 256 && NT == 2 ? 1 : 2) void attend_few_k
   }
 }
 
+// Workgroups go round the 8 XCDs in turn.  The row tiles of a (sequence, head,
+// split) read the same keys: they go to one XCD, whose L2 then serves them, the
+// last tiles, which see the most keys, first; where there are fewer than eight
+// such sets their tiles are dealt over all XCDs.  False: nothing to do.
+TCFP_DEV bool place(const Attend& a, int& tile, int& split, int& kvh, int& b) {
+  const uint32_t tiles = uint32_t(a.tiles);
+  uint32_t set, t;
+  if (a.sets >= 8) {
+    const uint32_t nth = blockIdx.x / 8;
+    set = nth / tiles * 8 + blockIdx.x % 8;
+    t = nth % tiles;
+  } else {
+    set = blockIdx.x / tiles;
+    t = blockIdx.x % tiles;
+  }
+  if (set >= uint32_t(a.sets)) return false;
+  tile = a.tiles - 1 - int(t);
+  split = int(set % uint32_t(a.splits));
+  set /= uint32_t(a.splits);
+  kvh = int(set % uint32_t(a.kv_heads));
+  b = int(set / uint32_t(a.kv_heads));
+  return true;
+}
+
 // ---- many rows: prompts ------------------------------------------------------
 //
 // Bound by the matrix and vector units together.  A workgroup's four waves
@@ -703,6 +728,7 @@ template <int D>
 TCFP_DEV void many_load(const Attend& a, int kvh, int key0, int page, ManyLoad<D>& t) {
   const int kg = threadIdx.x >> 4, dg = threadIdx.x & 15;
   const int key = key0 + 4 * kg;
+  page = valid_page(a, page);
   t.page = page;
   const int64_t at = ((int64_t(max(page, 0)) * a.kv_heads + kvh) << a.page_bits) +
                      (key & ((1 << a.page_bits) - 1));
@@ -782,17 +808,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
   __shared__ uint4 lds4[2 * S::BUF / 16];
   uint8_t* const lds = reinterpret_cast<uint8_t*>(lds4);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
-  // Workgroups go round the 8 XCDs in turn: each XCD takes a contiguous run of
-  // (sequence, head, split, tile), whose tiles read the same keys from its L2.
-  const uint32_t total = gridDim.x, per = total / 8, rest = total % 8;
-  const uint32_t xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
-  uint32_t id = xcd * per + min(xcd, rest) + nth;
-  // the last tiles, which see the most keys, first
-  const int tile = a.tiles - 1 - int(id % uint32_t(a.tiles));
-  id /= uint32_t(a.tiles);
-  const int split = int(id % uint32_t(a.splits));
-  id /= uint32_t(a.splits);
-  const int kvh = int(id % uint32_t(a.kv_heads)), b = int(id / uint32_t(a.kv_heads));
+  int tile, split, kvh, b;
+  if (!place(a, tile, split, kvh, b)) return;
   const Seq seq = sequence(a, b);
   if (split == 0 && tile == 0) zero_rest(a, b, kvh, seq, D);
   const int32_t* table = a.table + int64_t(b) * a.table_stride;
@@ -833,7 +850,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
       const bool holes = __syncthreads_or(hole);
       const int last_page = (k1 - 1) >> a.page_bits;
       auto page_at = [&](int key) {
-        return valid_page(a, table[min((key + 4 * kg) >> a.page_bits, last_page)]);
+        return table[min((key + 4 * kg) >> a.page_bits, last_page)];
       };
       auto is_masked = [&](int key) {
         return holes || key < all_lo_max || key + kManyKeys > all_hi_min;
@@ -959,6 +976,293 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
   }
 }
 
+// ---- many rows, eight waves --------------------------------------------------
+//
+// As above with 256 rows a workgroup, so that each key is fetched, converted
+// and written to LDS for twice the rows, and 128 keys between two barriers, so
+// that the two waves of a SIMD drift apart and one's products run beside the
+// other's softmax.  The codes of K need no work: each wave copies the 8 or 16
+// rows it stages straight into LDS.  Keys staged by a wave lie in one page, so
+// their addresses are the wave's own.
+constexpr int kWideRows = 256;
+
+template <int D>
+struct WideShape {
+  static constexpr int DS = D / 64, DT = D / 32;
+  static constexpr int DG = D / 4;                      // threads across a row of codes
+  static constexpr int KW = 256 / DG;                   // keys a wave stages of a 64-key step
+  static constexpr int TU = D == 128 ? 2 : 1;           // steps that a thread stages
+  static constexpr int KB = kManyKeys * D;              // bytes of K
+  static constexpr int VB = kManyKeys * D * 2;          // and of V
+  static constexpr int BUF = 2 * (KB + VB + kManyKeys); // two steps with their scales
+};
+
+// byte offset of chunk c (8 keys) of column d of V
+TCFP_DEV int vp_at(int d, int c) { return d * 128 + ((c ^ ((d ^ ((d >> 3) & 3)) & 7)) << 4); }
+
+// 16 bytes from base + off of each lane into LDS at lds + 16 * lane (base and
+// lds the wave's); done when vmcnt has counted it.
+TCFP_DEV void copy_to_lds(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+
+struct WideLoad {
+  uint32_t v[4], ke, ve;
+  int page;
+};
+
+template <int D>
+__global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
+  using S = WideShape<D>;
+  __shared__ uint4 lds4[2 * S::BUF / 16];
+  uint8_t* const lds = reinterpret_cast<uint8_t*>(lds4);
+  const uint32_t lds_at =
+      uint32_t(uintptr_t((__attribute__((address_space(3))) uint8_t*)(lds4)));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
+            col = lane & 31, half = lane >> 5;
+  int tile, split, kvh, b;
+  if (!place(a, tile, split, kvh, b)) return;
+  const Seq seq = sequence(a, b);
+  if (split == 0 && tile == 0) zero_rest(a, b, kvh, seq, D);
+  const int32_t* table = a.table + int64_t(b) * a.table_stride;
+  // The wave stages keys 16 k16 + ... of a step: of K the rows kwave ... of
+  // those 16, 16 bytes a lane (the chunk that belongs at the lane's place), of
+  // V the thread's four keys 4 kg ..., one word of their rows each.  (The two or
+  // four groups of four keys of a wave are dealt so that each half of it writes
+  // both halves of the 16-byte chunks of V.)
+  const int k16 = D == 128 ? wave >> 1 : wave & 3, kwave = D == 128 ? 8 * (wave & 1) : 0;
+  const int krow_l = lane / (D / 16), kch = lane % (D / 16);
+  const uint32_t koff =
+      uint32_t(krow_l * D + ((kch ^ (D == 64 ? (krow_l >> 1) & 3 : krow_l & 7)) << 4));
+  const int x4 = lane >> 4;
+  const int kg = 4 * k16 + (D == 128 ? (wave & 1) + 2 * (x4 & 1) : ((x4 & 1) << 1) + (x4 >> 1));
+  const int dg = (lane & 15) + (D == 128 ? (x4 >> 1) * 16 : 0);
+  const uint64_t row_lanes = D == 128 ? 0x0000FFFF0000FFFFull << (16 * (x4 & 1))
+                                      : 0xFFFFull << (16 * x4);
+  const int voff = (kg & 3) * 4 * D + dg * 4;
+  const int vchunk = (kg >> 2) * 2 + (kg & 1), sub = ((kg >> 1) & 1) * 8;
+  for (int r0 = tile * kWideRows; r0 < seq.rows; r0 += a.tiles * kWideRows) {
+    const Keys keys = keys_of(a, seq, r0, kWideRows);
+    if (split >= max(keys.live, 1)) continue;
+    const int k0 = keys.begin + split * a.chunk;
+    const int k1 = split == a.splits - 1 ? keys.end : min(keys.end, k0 + a.chunk);
+    const int last = min(r0 + kWideRows, seq.rows) - 1;
+    const int row = min(r0 + 32 * wave + col, last), tok = row / a.group,
+              head = row - tok * a.group;
+    const int lo = key_lo(a, seq, tok), hi = key_hi(a, seq, tok);
+    const int wfirst = min(r0 + 32 * wave, last) / a.group,
+              wlast = min(r0 + 32 * wave + 31, last) / a.group;
+    const int all_lo = key_lo(a, seq, r0 / a.group), all_lo_max = key_lo(a, seq, last / a.group),
+              all_hi_min = key_hi(a, seq, r0 / a.group);
+    const int w_lo = key_lo(a, seq, wfirst), w_lo_max = key_lo(a, seq, wlast),
+              w_hi_min = key_hi(a, seq, wfirst), w_hi = key_hi(a, seq, wlast);
+    const bool idle = r0 + 32 * wave > last;
+    v8i qhi[S::DS], qlo[S::DS];
+    const int qe = split_q<S::DS, 2>(a.q + int64_t(seq.start + tok) * a.q_token +
+                                         int64_t(kvh * a.group + head) * a.q_head + half * 32,
+                                     64, a.q_mul, qhi, qlo);
+    v16f o[S::DT];
+#pragma unroll
+    for (int i = 0; i < S::DT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    if (k0 < k1) {
+      const int last_page = (k1 - 1) >> a.page_bits;
+      bool hole = false;
+      for (int p = (k0 >> a.page_bits) + int(threadIdx.x); p <= last_page; p += 512)
+        hole |= valid_page(a, table[p]) < 0;
+      const bool holes = __syncthreads_or(hole);
+      auto is_masked = [&](int key) {
+        return holes || key < all_lo_max || key + kManyKeys > all_hi_min;
+      };
+      // the page of the wave's keys of a step (as read; made scalar at its use)
+      auto page_of = [&](int key) { return table[min((key + 16 * k16) >> a.page_bits, last_page)]; };
+      auto step_of = [&](int i) { return D == 128 ? i : wave >> 2; };
+      WideLoad t[S::TU];
+      int page[S::TU];
+      // keys of the steps at key0 on their way: K to LDS, V to registers
+      auto fetch = [&](int key0, uint32_t buf) {
+#pragma unroll
+        for (int i = 0; i < S::TU; ++i) {
+          const int u = step_of(i), key = key0 + u * kManyKeys;
+          const int pg = __builtin_amdgcn_readfirstlane(valid_page(a, page[i]));
+          t[i].page = pg;
+          const int64_t at = ((int64_t(max(pg, 0)) * a.kv_heads + kvh) << a.page_bits) +
+                             ((key + 16 * k16) & ((1 << a.page_bits) - 1));
+          copy_to_lds(a.k_codes + (at + kwave) * D, koff,
+                      buf + uint32_t(u * S::KB + (16 * k16 + kwave) * D));
+          const uint8_t* v = a.v_codes + at * D + voff;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) t[i].v[j] = *reinterpret_cast<const uint32_t*>(v + j * D);
+          t[i].ke = *reinterpret_cast<const uint32_t*>(a.k_exps + at + (kg & 3) * 4);
+          t[i].ve = *reinterpret_cast<const uint32_t*>(a.v_exps + at + (kg & 3) * 4);
+          page[i] = page_of(key + 2 * kManyKeys);
+        }
+      };
+      // what fetch() brought, complete in the buffer but for a barrier
+      auto settle = [&](int key0, uint8_t* buf) {
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+#pragma unroll
+        for (int i = 0; i < S::TU; ++i) {
+          const int u = step_of(i), key = key0 + u * kManyKeys;
+          uint32_t scales = ((t[i].ke & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) ^ (t[i].ke & 0x80808080u);
+          if (is_masked(key)) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int kk = key + 4 * kg + j;
+              const bool dead = kk < all_lo || kk >= keys.end || t[i].page < 0;
+              const uint64_t any = __ballot(has_nan_code(t[i].v[j]) && !dead);
+              if (any & row_lanes) scales |= 0xFFu << (8 * j);
+              t[i].v[j] = dead ? 0u : without_nan(t[i].v[j]);
+              if (dead) t[i].ve &= ~(0xFFu << (8 * j));
+            }
+            if (t[i].page < 0) scales = 0;
+          }
+          float sc[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[j] = exp_scale(t[i].ve, j);
+          uint8_t* vb = buf + 2 * S::KB + u * S::VB + sub;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              x[j] = h ? deq2<true>(t[i].v[j], sc[j]) : deq2<false>(t[i].v[j], sc[j]);
+            *reinterpret_cast<uint2*>(vb + vp_at(dg * 4 + 2 * h, vchunk)) =
+                make_uint2(lows(x[0], x[1]), lows(x[2], x[3]));
+            *reinterpret_cast<uint2*>(vb + vp_at(dg * 4 + 2 * h + 1, vchunk)) =
+                make_uint2(highs(x[0], x[1]), highs(x[2], x[3]));
+          }
+          if (dg == 0)
+            *reinterpret_cast<uint32_t*>(buf + 2 * (S::KB + S::VB) + u * kManyKeys + 4 * kg) = scales;
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < S::TU; ++i) page[i] = page_of(k0 + step_of(i) * kManyKeys);
+      fetch(k0, lds_at);
+      settle(k0, lds);
+      int cur = 0;
+      for (int key0 = k0; key0 < k1; key0 += 2 * kManyKeys) {
+        const bool more = key0 + 2 * kManyKeys < k1;
+        __syncthreads();  // this buffer is written, the other one read
+        if (more) fetch(key0 + 2 * kManyKeys, lds_at + uint32_t((cur ^ 1) * S::BUF));
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+          const int key = key0 + u * kManyKeys;
+          if (idle || key >= w_hi || key + kManyKeys <= w_lo || key >= k1) continue;
+          const uint8_t* buf = lds + cur * S::BUF + u * S::KB;
+          const uint8_t* vb = lds + cur * S::BUF + 2 * S::KB + u * S::VB;
+          const uint8_t* sb = lds + cur * S::BUF + 2 * (S::KB + S::VB) + u * kManyKeys;
+          __builtin_amdgcn_s_setprio(1);
+          v16f s[2];
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            const int krow = 32 * kt + col;
+            const int ks = sb[krow];
+            s[kt] = v16f{};
+#pragma unroll
+            for (int d = 0; d < S::DS; ++d) {
+              const uint4 x = *reinterpret_cast<const uint4*>(buf + k_at<D>(krow, 4 * d + 2 * half));
+              const uint4 y =
+                  *reinterpret_cast<const uint4*>(buf + k_at<D>(krow, 4 * d + 2 * half + 1));
+              v8i k;
+              k[0] = int(x.x); k[1] = int(x.y); k[2] = int(x.z); k[3] = int(x.w);
+              k[4] = int(y.x); k[5] = int(y.y); k[6] = int(y.z); k[7] = int(y.w);
+              s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, qhi[d], s[kt], 0, 0, 0, ks,
+                                                                      0, qe);
+              s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, qlo[d], s[kt], 0, 0, 0, ks,
+                                                                      0, qe);
+            }
+          }
+          __builtin_amdgcn_s_setprio(0);
+          if (holes || key < w_lo_max || key + kManyKeys > w_hi_min) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const bool gone = holes && *reinterpret_cast<const uint32_t*>(
+                                               sb + 32 * kt + 8 * g + 4 * half) == 0;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const int kk = key + 32 * kt + 8 * g + 4 * half + r;
+                  if (gone || kk < lo || kk >= hi) s[kt][4 * g + r] = -INFINITY;
+                }
+              }
+          }
+          float top = s[0][0];
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) top = fmaxf(top, s[kt][x]);
+          top = fmaxf(top, other_half(top));
+          top = fmaxf(top, m);
+          if (__ballot(top > m)) {
+            const float f = top == m ? 1.0f : exp2_fast((m - top) * a.c);
+            m = top;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < S::DT; ++i) o[i] *= f;
+          }
+          const float off = top == -INFINITY ? 0.0f : top * a.c;
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              s[kt][x] = exp2_fast(__builtin_fmaf(s[kt][x], a.c, -off));
+              l += s[kt][x];
+            }
+
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const v16f& e = s[x >> 1];
+            const int z = 8 * (x & 1);
+            const v8bf p = as_bf(pack_bf16(e[z], e[z + 1]), pack_bf16(e[z + 2], e[z + 3]),
+                         pack_bf16(e[z + 4], e[z + 5]), pack_bf16(e[z + 6], e[z + 7]));
+#pragma unroll
+            for (int i = 0; i < S::DT; ++i) {
+              const uint4 w = *reinterpret_cast<const uint4*>(vb + vp_at(col, 2 * x + half) + 4096 * i);
+              o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf(w.x, w.y, w.z, w.w), p, o[i],
+                                                             0, 0, 0);
+            }
+          }
+        }
+        cur ^= 1;
+        if (more) settle(key0 + 2 * kManyKeys, lds + cur * S::BUF);
+      }
+      __syncthreads();  // (the next tile writes the buffers again)
+    }
+    l += other_half(l);
+    if (r0 + 32 * wave + col <= last) {
+      const int64_t at = int64_t(seq.start + tok) * a.heads + kvh * a.group + head;
+      if (keys.live <= 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < S::DT; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint2*>(a.out + at * D + 32 * i + 8 * g + 4 * half) =
+                make_uint2(pack_bf16(o[i][4 * g] * inv, o[i][4 * g + 1] * inv),
+                           pack_bf16(o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv));
+      } else {
+        const int64_t pa = int64_t(split) * a.tokens * a.heads + at;
+#pragma unroll
+        for (int i = 0; i < S::DT; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float4*>(a.part + pa * D + 32 * i + 8 * g + 4 * half) =
+                make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+        if (half == 0) {
+          a.part_ml[2 * pa] = m;
+          a.part_ml[2 * pa + 1] = l;
+        }
+      }
+    }
+  }
+}
+
+
 // A wave a row whose keys were split: the splits' sums, brought to the largest
 // maximum and added in order.
 template <int D>
@@ -1005,6 +1309,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(Attend a, int tile_row
 // How the batch is laid over the card, from the bounds of its lengths.
 struct Launch {
   int few_tiles;  // 16-row tiles a workgroup of the few-rows kernel takes; 0: many rows
+  bool wide;      // 256 rows a workgroup
   int tile_rows, tiles, splits, chunk;
 };
 Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
@@ -1013,7 +1318,8 @@ Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
   const int64_t group = heads / kv_heads;
   const int64_t most = std::max<int64_t>(std::min(max_query_len, tokens), 1) * group;
   p.few_tiles = most <= 16 ? 1 : most <= 32 ? 2 : 0;
-  p.tile_rows = p.few_tiles ? 16 * p.few_tiles : kManyRows;
+  p.wide = most > 128 && dim <= 128;
+  p.tile_rows = p.few_tiles ? 16 * p.few_tiles : p.wide ? kWideRows : kManyRows;
   p.tiles = int((most + p.tile_rows - 1) / p.tile_rows);
   // workgroups without splitting: at most one tile a sequence is part full
   const int64_t full = std::min<int64_t>(p.tiles * batch, tokens * group / p.tile_rows + batch);
@@ -1021,7 +1327,7 @@ Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
   int64_t keys = std::clamp<int64_t>(max_seq_len, 1, int64_t(1) << 30);
   if (window > 0) keys = std::min(keys, window + max_query_len + 64);
   const int64_t unit = 256;
-  const int64_t want = p.few_tiles ? 2048 : 512;
+  const int64_t want = p.few_tiles ? 2048 : p.wide ? 256 : 512;
   const int64_t splits = std::clamp<int64_t>((want + wgs - 1) / wgs, 1, kMaxSplits);
   const int64_t per = (keys + splits - 1) / splits;
   const int64_t chunk = std::max<int64_t>((per + unit - 1) / unit * unit, unit);
@@ -1190,10 +1496,14 @@ int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     TCFP_BY_DIM(TCFP_FEW);
 #undef TCFP_FEW
   } else {
-    const int64_t wgs = int64_t(p.tiles) * p.splits * kv_heads * batch;
-    if (wgs > INT32_MAX || !grid_x_fits(wgs, 256)) return TCFP_ERR_SHAPE;
+    const int64_t sets = int64_t(p.splits) * kv_heads * batch;
+    const int64_t wgs = p.tiles * (sets >= 8 ? (sets + 7) / 8 * 8 : sets);
+    a.sets = int(std::min<int64_t>(sets, INT32_MAX));
+    if (wgs > INT32_MAX || !grid_x_fits(wgs, 512)) return TCFP_ERR_SHAPE;
 #define TCFP_MANY(D) attend_many_kernel<D><<<unsigned(wgs), 256, 0, st>>>(a)
-    TCFP_BY_DIM(TCFP_MANY);
+    if (p.wide && dim == 64) attend_wide_kernel<64><<<unsigned(wgs), 512, 0, st>>>(a);
+    else if (p.wide) attend_wide_kernel<128><<<unsigned(wgs), 512, 0, st>>>(a);
+    else TCFP_BY_DIM(TCFP_MANY);
 #undef TCFP_MANY
   }
   if (p.splits > 1) {
