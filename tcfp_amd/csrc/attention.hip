@@ -189,6 +189,8 @@ struct Attend {
   int splits;       // of a row tile's keys
   int chunk;        // keys of a split but the last
   int sets;         // (sequence, K/V head, split)s of the many-rows launches
+  int workers;      // workgroups of the few-rows launch
+  int whole;        // their items are not divided
   uint16_t* out;
   float* part;      // [splits][tokens * heads][dim]
   float* part_ml;   // [splits][tokens * heads][2]: max (in units of s), sum
@@ -235,7 +237,7 @@ TCFP_DEV Keys keys_of(const Attend& a, const Seq& s, int r0, int n) {
 // the matrix instructions take.  (Their scale of a lane belongs to a block of 32
 // columns that is not the one whose values the lane holds: one scale for the
 // row, and for K's row, leaves that without effect.)
-template <int N, int LANES>
+template <int N, int LANES, int APART>
 TCFP_DEV int split_q(const uint16_t* p, int step, float mul, v8i* hi, v8i* lo) {
   uint32_t m = 0;
 #pragma unroll
@@ -243,25 +245,25 @@ TCFP_DEV int split_q(const uint16_t* p, int step, float mul, v8i* hi, v8i* lo) {
 #pragma unroll
     for (int i = 0; i < 32; i += 8) {
       float v[8];
-      load8(p + n * step + i, v);
+      load8(p + n * step + (i & 8) + (i >> 4) * APART, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = umax(m, absbits(v[j] * mul));
+      for (int j = 0; j < 8; ++j) m = umax(m, absbits(v[j]));
     }
   if constexpr (LANES == 4) m = umax(m, uint32_t(__shfl_xor(int(m), 16, 64)));
   m = umax(m, uint32_t(__shfl_xor(int(m), 32, 64)));
   const int e = block_exponent(__uint_as_float(m), kE4M3Max);
-  const float up = exp2i(-e) * mul;
+  const float up = exp2i(-e) * mul;  // (no value passes 448 but where the row's scale is NaN)
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int i = 0; i < 32; i += 8) {
       float v[8];
-      load8(p + n * step + i, v);
+      load8(p + n * step + (i & 8) + (i >> 4) * APART, v);
 #pragma unroll
       for (int h = 0; h < 8; h += 4) {
         float x[4], r[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = clampf(v[h + j] * up, kE4M3Max);
+        for (int j = 0; j < 4; ++j) x[j] = v[h + j] * up;
         const uint32_t w = cvt4_fp8<TCFP_FP8_E4M3>(x[0], x[1], x[2], x[3]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) r[j] = x[j] - e4m3_to_f32(w >> (8 * j));
@@ -302,17 +304,15 @@ TCFP_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 TCFP_DEV int valid_page(const Attend& a, int p) { return p >= 0 && p < a.num_pages ? p : -1; }
 
-// Rows of q before the first and after the last sequence: zeros.
-TCFP_DEV void zero_rest(const Attend& a, int b, int kvh, const Seq& s, int dim) {
-  const int lo0 = b == 0 ? 0 : a.tokens, hi0 = b == 0 ? s.start : 0;
-  const int lo1 = b == a.batch - 1 ? s.start + s.new_tokens : a.tokens, hi1 = a.tokens;
-  const int words = a.group * dim / 2;
-  for (int part = 0; part < 2; ++part)
-    for (int t = part ? lo1 : lo0; t < (part ? hi1 : hi0); ++t) {
-      uint32_t* p = reinterpret_cast<uint32_t*>(
-          a.out + (int64_t(t) * a.heads + kvh * a.group) * dim);
-      for (int i = threadIdx.x; i < words; i += blockDim.x) p[i] = 0;
-    }
+// Rows of q before the first (lead) and from behind the last sequence (tail):
+// zeros, for `heads` heads from head `first`.
+TCFP_DEV void zero_rest(const Attend& a, int lead, int tail, int first, int heads, int dim) {
+  const int words = heads * dim / 2, rest = max(a.tokens - max(tail, lead), 0);
+  for (int i = 0; i < lead + rest; ++i) {
+    const int t = i < lead ? i : max(tail, lead) + i - lead;
+    uint32_t* p = reinterpret_cast<uint32_t*>(a.out + (int64_t(t) * a.heads + first) * dim);
+    for (int x = threadIdx.x; x < words; x += blockDim.x) p[x] = 0;
+  }
 }
 
 // ---- few rows: one token a sequence, a few drafts ----------------------------
@@ -342,43 +342,60 @@ struct FewTile {
 
 constexpr int kSegKeys = 2048;  // keys whose pages are held in LDS at a time
 
+// A value that is the same in every lane, as the wave's own.
+TCFP_DEV int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+TCFP_DEV int64_t scalar(int64_t v) {
+  return int64_t(uint64_t(uint32_t(scalar(int(uint64_t(v) >> 32)))) << 32 |
+                 uint32_t(scalar(int(uint32_t(uint64_t(v))))));
+}
+
+template <int N>
+TCFP_DEV void load_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 t = *reinterpret_cast<const uint2*>(p);
+    w[0] = t.x; w[1] = t.y;
+  } else {
+    const uint4 t = *reinterpret_cast<const uint4*>(p);
+    w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
+  }
+}
+// Lane offsets of a group of 16 keys: its share of a key of K, of four keys of
+// V, of their exponents.
+struct FewLane {
+  uint32_t k, v, ke, ve;
+};
+template <int D>
+TCFP_DEV FewLane few_lane(int lane) {
+  const uint32_t col = lane & 15, g4 = lane >> 4;
+  return {col * D + (D == 64 ? (g4 & 1) * 16 : g4 * 16), 4 * g4 * D + col * (D / 16), col, 4 * g4};
+}
+
 template <int D>
 TCFP_DEV void few_load(const Attend& a, int kvh, const int* pages, int seg, int seg_end,
-                       int key0, FewTile<D>& t) {
+                       int key0, const FewLane& off, FewTile<D>& t) {
   using S = FewShape<D>;
-  const int lane = threadIdx.x & 63, col = lane & 15, g4 = lane >> 4;
 #pragma unroll
   for (int g = 0; g < S::KG; ++g) {
     const int key = key0 + 16 * g;
-    const int page = key < seg_end ? __builtin_amdgcn_readfirstlane(
-                                         pages[(key >> a.page_bits) - (seg >> a.page_bits)])
-                                   : -1;
-    t.page[g] = page;
-    // (a missing page, or keys past the end, are read from page 0 -- the pool
-    // has pages -- and masked)
-    const int64_t at = ((int64_t(max(page, 0)) * a.kv_heads + kvh) << a.page_bits) +
+    // (past the end: the last page's entry, masked)
+    const int held = scalar(pages[(min(key, seg_end - 1) >> a.page_bits) - (seg >> a.page_bits)]);
+    t.page[g] = key < seg_end ? held : -1;
+    // (a missing page is read from page 0 -- the pool has pages -- and masked)
+    const int64_t at = ((int64_t(max(held, 0)) * a.kv_heads + kvh) << a.page_bits) +
                        (key & ((1 << a.page_bits) - 1));
-    const uint8_t* kp = a.k_codes + (at + col) * D + (D == 64 ? (g4 & 1) * 32 : g4 * 32);
+    const uint8_t* kp = a.k_codes + at * D;
 #pragma unroll
     for (int s = 0; s < S::DS; ++s) {
-      t.k[g][s][0] = *reinterpret_cast<const uint4*>(kp + s * 128);
-      t.k[g][s][1] = *reinterpret_cast<const uint4*>(kp + s * 128 + 16);
+      t.k[g][s][0] = *reinterpret_cast<const uint4*>(kp + off.k + s * 128);
+      t.k[g][s][1] = *reinterpret_cast<const uint4*>(kp + off.k + s * 128 + (D == 64 ? 32 : 64));
     }
-    t.ke[g] = a.k_exps[at + col];
-    const uint8_t* vp = a.v_codes + (at + 4 * g4) * D + col * (D / 16);
+    t.ke[g] = (a.k_exps + at)[off.ke];
+    const uint8_t* vp = a.v_codes + at * D;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if constexpr (S::VW == 1) {
-        t.v[g][r][0] = *reinterpret_cast<const uint32_t*>(vp + r * D);
-      } else if constexpr (S::VW == 2) {
-        const uint2 w = *reinterpret_cast<const uint2*>(vp + r * D);
-        t.v[g][r][0] = w.x; t.v[g][r][1] = w.y;
-      } else {
-        const uint4 w = *reinterpret_cast<const uint4*>(vp + r * D);
-        t.v[g][r][0] = w.x; t.v[g][r][1] = w.y; t.v[g][r][2] = w.z; t.v[g][r][3] = w.w;
-      }
-    }
-    t.ve[g] = *reinterpret_cast<const uint32_t*>(a.v_exps + at + 4 * g4);
+    for (int r = 0; r < 4; ++r) load_words<S::VW>(vp + off.v + r * D, t.v[g][r]);
+    t.ve[g] = *reinterpret_cast<const uint32_t*>(a.v_exps + at + off.ve);
   }
 }
 
@@ -392,15 +409,15 @@ struct FewState {
   v4f o[NT][S::NI];
 };
 
-// One step over KT keys; MASKED: some row does not see all of them (or a page
+// One step over KT keys; masked: some row does not see all of them (or a page
 // is missing).  [all_lo, all_hi): keys that any row sees.
-template <int D, int NT, bool MASKED>
-TCFP_DEV void few_step(const Attend& a, FewState<D, NT>& st, FewTile<D>& t, int key0, int all_lo,
-                       int all_hi) {
+template <int D, int NT, bool masked>
+TCFP_DEV void few_step(const Attend& a, FewState<D, NT>& st, FewTile<D>& t, int key0,
+                       int all_lo, int all_hi) {
   using S = FewShape<D>;
   const int lane = threadIdx.x & 63, g4 = lane >> 4;
   uint32_t bad = 0;  // keys of the lane (4 g + r) with a NaN among the codes of V
-  if constexpr (MASKED) {
+  if (masked) {
 #pragma unroll
     for (int g = 0; g < S::KG; ++g)
 #pragma unroll
@@ -441,17 +458,22 @@ TCFP_DEV void few_step(const Attend& a, FewState<D, NT>& st, FewTile<D>& t, int 
                                                                t.ke[g] + 127, 0, st.qe[n]);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float x = s[r];
-        if constexpr (MASKED) {
-          const int key = key0 + 16 * g + 4 * g4 + r;
-          if ((bad >> (4 * g + r)) & 1u) x = __uint_as_float(0x7FC00000u);
-          if (key < st.lo[n] || key >= st.hi[n] || t.page[g] < 0) x = -INFINITY;
-        }
-        p[n][g][r] = x;
-        top = fmaxf(top, x);
-      }
+      for (int r = 0; r < 4; ++r) p[n][g][r] = s[r];
     }
+    if (masked) {
+#pragma unroll
+      for (int g = 0; g < S::KG; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = key0 + 16 * g + 4 * g4 + r;
+          if ((bad >> (4 * g + r)) & 1u) p[n][g][r] = __uint_as_float(0x7FC00000u);
+          if (key < st.lo[n] || key >= st.hi[n] || t.page[g] < 0) p[n][g][r] = -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < S::KG; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, p[n][g][r]);
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     top = fmaxf(top, st.m[n]);
@@ -505,6 +527,150 @@ TCFP_DEV void few_step(const Attend& a, FewState<D, NT>& st, FewTile<D>& t, int 
   }
 }
 
+// The value of a lane (its number the same in every lane).
+TCFP_DEV int of_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+TCFP_DEV int64_t of_lane(int64_t v, int lane) {
+  return int64_t(uint64_t(uint32_t(of_lane(int(uint64_t(v) >> 32), lane))) << 32 |
+                 uint32_t(of_lane(int(uint32_t(uint64_t(v))), lane)));
+}
+
+// The few-rows launch cuts the batch's keys into equal runs, whatever the
+// lengths: an item is a (sequence, row tile, head), its keys count in units of
+// kUnit, and workgroup w takes the units [w q, (w + 1) q) of all items in order
+// (q from the lengths, which are on the device: every workgroup adds them up).
+// An item within one workgroup is finished there; of the others each part goes
+// to a place of its own, 2 w for a workgroup's first part and 2 w + 1 for an item
+// that only starts in it, and the joining launch adds an item's parts in order.
+// With `whole` an item is one unit and nothing is joined.
+constexpr int kUnit = 128;
+
+// Items of sequence b: units of each, and how many there are.
+TCFP_DEV int units_of(const Attend& a, const Seq& s) {
+  if (a.whole) return 1;
+  const int begin = key_lo(a, s, 0) & ~63, end = key_hi(a, s, s.new_tokens - 1);
+  return max((end - begin + kUnit - 1) / kUnit, 1);
+}
+TCFP_DEV int items_of(const Attend& a, const Seq& s, int tile_rows) {
+  return (s.rows + tile_rows - 1) / tile_rows * a.kv_heads;
+}
+
+// a / b of non-negative numbers, by the 32-bit division where that does.
+TCFP_DEV int64_t divide(int64_t a, int64_t b) {
+  if (uint64_t(a | b) >> 32) return a / b;
+  return uint32_t(a) / uint32_t(b);
+}
+
+// Units of a workgroup of the launch: two at least, as a part costs a quarter of
+// the time of its keys.
+TCFP_DEV int64_t share_of(const Attend& a, int64_t total) {
+  return max(divide(total + a.workers - 1, a.workers), int64_t(a.whole ? 1 : 2));
+}
+
+// A sequence, the units before it and those of the whole batch.
+struct Found {
+  int b;
+  Seq seq;
+  int64_t before, total;
+  int lead, tail;  // rows of q before the first sequence, and up to the last one's end
+};
+struct FindLds {
+  int64_t wave[4], before;
+  Seq seq;
+  int b;
+};
+
+// The sequence for which pick(seq, units before it, its units, all units) holds
+// -- for one at most -- sought by a workgroup of 256 with 256 sequences at a
+// time, or by each wave for itself where there are at most 64; false: none.
+template <typename Pick>
+TCFP_DEV bool find(const Attend& a, int tile_rows, FindLds& lds, Pick pick, Found& f) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (a.batch == 1) {
+    f.seq = sequence(a, 0);
+    const int64_t n =
+        f.seq.rows > 0 ? int64_t(units_of(a, f.seq)) * items_of(a, f.seq, tile_rows) : 0;
+    f.b = 0;
+    f.before = 0;
+    f.total = n;
+    f.lead = f.seq.start;
+    f.tail = f.seq.start + f.seq.new_tokens;
+    return pick(f.seq, 0, n, n);
+  }
+  if (a.batch <= 64) {
+    Seq s{};
+    int64_t n = 0;
+    if (lane < a.batch) {
+      s = sequence(a, lane);
+      if (s.rows > 0) n = int64_t(units_of(a, s)) * items_of(a, s, tile_rows);
+    }
+    int64_t upto = n;
+    for (int x = 1; x < a.batch; x <<= 1) {
+      const int64_t y = __shfl_up(upto, x, 64);
+      if (lane >= x) upto += y;
+    }
+    f.total = of_lane(upto, a.batch - 1);
+    f.lead = scalar(s.start);  // (of the first lane)
+    f.tail = of_lane(s.start + s.new_tokens, a.batch - 1);
+    const uint64_t here = __ballot(lane < a.batch && pick(s, upto - n, n, f.total));
+    if (!here) return false;
+    f.b = __builtin_ctzll(here);
+    f.before = of_lane(upto - n, f.b);
+    f.seq = {of_lane(s.start, f.b), of_lane(s.new_tokens, f.b), of_lane(s.len, f.b),
+             of_lane(s.pos0, f.b), of_lane(s.rows, f.b)};
+    return true;
+  }
+  Seq s{};
+  int64_t n = 0, upto = 0, chunk = 0;  // units of the thread's sequence, of the wave's up to it, of the 256
+  auto scan = [&](int b0) {
+    const int b = b0 + int(threadIdx.x);
+    s = Seq{};
+    n = 0;
+    if (b < a.batch) {
+      s = sequence(a, b);
+      if (s.rows > 0) n = int64_t(units_of(a, s)) * items_of(a, s, tile_rows);
+    }
+    upto = n;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+      const int64_t y = __shfl_up(upto, x, 64);
+      if (lane >= x) upto += y;
+    }
+    if (lane == 63) lds.wave[wave] = upto;
+    __syncthreads();
+    chunk = lds.wave[0] + lds.wave[1] + lds.wave[2] + lds.wave[3];
+    for (int w = 0; w < wave; ++w) upto += lds.wave[w];
+    __syncthreads();
+  };
+  const Seq end = sequence(a, a.batch - 1);
+  f.lead = sequence(a, 0).start;
+  f.tail = end.start + end.new_tokens;
+  f.total = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 256) {
+    scan(b0);
+    f.total += chunk;
+  }
+  f.total = scalar(f.total);
+  int64_t start = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 256) {
+    if (a.batch > 256) scan(b0);
+    const bool here = b0 + int(threadIdx.x) < a.batch && pick(s, start + upto - n, n, f.total);
+    if (here) {
+      lds.b = b0 + int(threadIdx.x);
+      lds.seq = s;
+      lds.before = start + upto - n;
+    }
+    if (__syncthreads_or(here)) {
+      f.b = scalar(lds.b);
+      f.before = scalar(lds.before);
+      f.seq = {scalar(lds.seq.start), scalar(lds.seq.new_tokens), scalar(lds.seq.len),
+               scalar(lds.seq.pos0), scalar(lds.seq.rows)};
+      return true;
+    }
+    start += chunk;
+  }
+  return false;
+}
+
 template <int D, int NT>
 __global__ __launch_bounds__(256, D == 256 && NT == 2 ? 1 : 2) void attend_few_kernel(Attend a) {
   using S = FewShape<D>;
@@ -512,16 +678,46 @@ __global__ __launch_bounds__(256, D == 256 && NT == 2 ? 1 : 2) void attend_few_k
   __shared__ int pages[kSegKeys / 16];
   __shared__ float ml[4][RT][2];
   __shared__ float4 xo[4][8][64];
-  const int b = blockIdx.z, kvh = blockIdx.y % a.kv_heads, split = blockIdx.x;
+  __shared__ FindLds fl;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g4 = lane >> 4;
-  const Seq seq = sequence(a, b);
-  if (split == 0 && int(blockIdx.y) < a.kv_heads) zero_rest(a, b, kvh, seq, D);
-  const int32_t* table = a.table + int64_t(b) * a.table_stride;
-  for (int r0 = int(blockIdx.y / a.kv_heads) * RT; r0 < seq.rows; r0 += a.tiles * RT) {
-    const Keys keys = keys_of(a, seq, r0, RT);
-    if (split >= max(keys.live, 1)) continue;
-    const int k0 = keys.begin + split * a.chunk;
-    const int k1 = split == a.splits - 1 ? keys.end : min(keys.end, k0 + a.chunk);
+  const FewLane off = few_lane<D>(lane);
+  Found f;
+  const bool any = find(
+      a, RT, fl,
+      [&](const Seq&, int64_t first, int64_t n, int64_t total) {
+        const int64_t u = int64_t(blockIdx.x) * share_of(a, total);
+        return n > 0 && u >= first && u < first + n;
+      },
+      f);
+  if (blockIdx.x == 0) zero_rest(a, f.lead, f.tail, 0, a.heads, D);
+  if (!any) return;
+  const int64_t share = share_of(a, f.total);
+  int64_t u = int64_t(blockIdx.x) * share, before = f.before;
+  const int64_t u1 = min(u + share, f.total);
+  int b = f.b;
+  Seq seq = f.seq;
+  while (u < u1) {
+    const int units = units_of(a, seq), items = items_of(a, seq, RT);
+    if (seq.rows <= 0 || u - before >= int64_t(units) * items) {  // on to the next sequence
+      if (seq.rows > 0) before += int64_t(units) * items;
+      seq = sequence(a, ++b);
+      continue;
+    }
+    const int item = int(divide(u - before, units)), part = int(u - before - int64_t(item) * units);
+    const int count = int(min(int64_t(units - part), u1 - u));
+    const bool all = count == units;
+    const int64_t place = 2 * int64_t(blockIdx.x) + (part == 0 ? 1 : 0);
+    u += count;
+    const int kvh = item % a.kv_heads, r0 = item / a.kv_heads * RT;
+    const int32_t* table = a.table + int64_t(b) * a.table_stride;
+    const int first = key_lo(a, seq, 0) & ~63, end = key_hi(a, seq, seq.new_tokens - 1);
+    const int k0 = first + part * kUnit;
+    const int k1 = a.whole ? end : min(end, k0 + count * kUnit);
+    // (the first pages, on their way while q is split)
+    const int page0 = k0 >> a.page_bits;
+    int held = -1;
+    if (k0 < k1 && page0 + int(threadIdx.x) <= (min(k1, k0 + kSegKeys) - 1) >> a.page_bits)
+      held = table[page0 + threadIdx.x];
     FewState<D, NT> st;
     int lo_max = 0, hi_min = INT32_MAX;
 #pragma unroll
@@ -529,7 +725,7 @@ __global__ __launch_bounds__(256, D == 256 && NT == 2 ? 1 : 2) void attend_few_k
       const int r = min(r0 + 16 * n + col, seq.rows - 1), i = r / a.group, h = r - i * a.group;
       const uint16_t* q = a.q + int64_t(seq.start + i) * a.q_token +
                           int64_t(kvh * a.group + h) * a.q_head;
-      st.qe[n] = split_q<S::DS, 4>(q + (D == 64 ? (g4 & 1) * 32 : g4 * 32), 128, a.q_mul,
+      st.qe[n] = split_q<S::DS, 4, D == 64 ? 32 : 64>(q + (D == 64 ? (g4 & 1) * 16 : g4 * 16), 128, a.q_mul,
                                    st.qhi[n], st.qlo[n]);
       if (D == 64 && g4 >= 2) st.qhi[n][0] = st.qlo[n][0];
       st.lo[n] = key_lo(a, seq, i);
@@ -542,28 +738,31 @@ __global__ __launch_bounds__(256, D == 256 && NT == 2 ? 1 : 2) void attend_few_k
     const int last = min(r0 + RT, seq.rows) - 1;
     lo_max = key_lo(a, seq, last / a.group);
     hi_min = key_hi(a, seq, r0 / a.group);
-    const int all_lo = key_lo(a, seq, r0 / a.group);
+    const int all_lo = key_lo(a, seq, r0 / a.group), all_hi = key_hi(a, seq, last / a.group);
     for (int seg = k0; seg < k1; seg += kSegKeys) {
       const int seg_end = min(seg + kSegKeys, k1);
       __syncthreads();
       {
-        const int first = seg >> a.page_bits, n = ((seg_end - 1) >> a.page_bits) - first + 1;
-        for (int i = threadIdx.x; i < n; i += 256) pages[i] = valid_page(a, table[first + i]);
+        const int page = (seg >> a.page_bits) + int(threadIdx.x);
+        if (page <= (seg_end - 1) >> a.page_bits)  // (128 at most)
+          pages[threadIdx.x] = valid_page(a, seg == k0 ? held : table[page]);
       }
       __syncthreads();
-      FewTile<D> cur, nxt;
       int key = seg + wave * S::KT;
-      if (key < seg_end) few_load<D>(a, kvh, pages, seg, seg_end, key, cur);
+      if (key >= seg_end) continue;  // (barriers: at the top of the loop only)
+      FewTile<D> cur, nxt;
+      few_load<D>(a, kvh, pages, seg, seg_end, key, off, cur);
       for (; key < seg_end; key += 4 * S::KT) {
-        const int next = key + 4 * S::KT;
-        if (next < seg_end) few_load<D>(a, kvh, pages, seg, seg_end, next, nxt);
+        // (the last step loads its own keys again, from L2)
+        const int next = key + 4 * S::KT < seg_end ? key + 4 * S::KT : key;
+        few_load<D>(a, kvh, pages, seg, seg_end, next, off, nxt);
         bool hole = false;
 #pragma unroll
         for (int g = 0; g < S::KG; ++g) hole |= cur.page[g] < 0;
         if (hole || key < lo_max || key + S::KT > hi_min)
-          few_step<D, NT, true>(a, st, cur, key, all_lo, keys.end);
+          few_step<D, NT, true>(a, st, cur, key, all_lo, all_hi);
         else
-          few_step<D, NT, false>(a, st, cur, key, all_lo, keys.end);
+          few_step<D, NT, false>(a, st, cur, key, all_lo, all_hi);
         cur = nxt;
       }
     }
@@ -619,14 +818,14 @@ __global__ __launch_bounds__(256, D == 256 && NT == 2 ? 1 : 2) void attend_few_k
           if (r < seq.rows) {
             const int i = r / a.group, h = r - i * a.group;
             const int64_t row = int64_t(seq.start + i) * a.heads + kvh * a.group + h;
-            if (keys.live <= 1) {
+            if (all) {
               const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
 #pragma unroll
               for (int x = 0; x < 4; ++x)
                 *reinterpret_cast<uint32_t*>(a.out + row * D + (4 * g4 + x) * (D / 16) + i0 +
                                              2 * i2) = pack_bf16(s[0][x] * inv, s[1][x] * inv);
             } else {
-              const int64_t at = int64_t(split) * a.tokens * a.heads + row;
+              const int64_t at = place * RT + 16 * n + col;
 #pragma unroll
               for (int x = 0; x < 4; ++x)
                 *reinterpret_cast<float2*>(a.part + at * D + (4 * g4 + x) * (D / 16) + i0 +
@@ -704,18 +903,6 @@ struct ManyLoad {
   int page;
 };
 
-template <int N>
-TCFP_DEV void load_words(const uint8_t* p, uint32_t* w) {
-  if constexpr (N == 1) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  } else if constexpr (N == 2) {
-    const uint2 t = *reinterpret_cast<const uint2*>(p);
-    w[0] = t.x; w[1] = t.y;
-  } else {
-    const uint4 t = *reinterpret_cast<const uint4*>(p);
-    w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
-  }
-}
 template <int N>
 TCFP_DEV void store_lds(uint8_t* p, const uint32_t* w) {
   if constexpr (N == 1) *reinterpret_cast<uint32_t*>(p) = w[0];
@@ -811,7 +998,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
   int tile, split, kvh, b;
   if (!place(a, tile, split, kvh, b)) return;
   const Seq seq = sequence(a, b);
-  if (split == 0 && tile == 0) zero_rest(a, b, kvh, seq, D);
+  if (split == 0 && tile == 0)
+    zero_rest(a, b == 0 ? seq.start : 0,
+              b == a.batch - 1 ? seq.start + seq.new_tokens : a.tokens, kvh * a.group, a.group, D);
   const int32_t* table = a.table + int64_t(b) * a.table_stride;
   const int kg = threadIdx.x >> 4;
   for (int r0 = tile * kManyRows; r0 < seq.rows; r0 += a.tiles * kManyRows) {
@@ -832,7 +1021,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
               w_hi_min = key_hi(a, seq, wfirst), w_hi = key_hi(a, seq, wlast);
     const bool idle = r0 + 32 * wave > last;
     v8i qhi[S::DS], qlo[S::DS];
-    const int qe = split_q<S::DS, 2>(a.q + int64_t(seq.start + tok) * a.q_token +
+    const int qe = split_q<S::DS, 2, 16>(a.q + int64_t(seq.start + tok) * a.q_token +
                                          int64_t(kvh * a.group + head) * a.q_head + half * 32,
                                      64, a.q_mul, qhi, qlo);
     v16f o[S::DT];
@@ -1023,7 +1212,9 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
   int tile, split, kvh, b;
   if (!place(a, tile, split, kvh, b)) return;
   const Seq seq = sequence(a, b);
-  if (split == 0 && tile == 0) zero_rest(a, b, kvh, seq, D);
+  if (split == 0 && tile == 0)
+    zero_rest(a, b == 0 ? seq.start : 0,
+              b == a.batch - 1 ? seq.start + seq.new_tokens : a.tokens, kvh * a.group, a.group, D);
   const int32_t* table = a.table + int64_t(b) * a.table_stride;
   // The wave stages keys 16 k16 + ... of a step: of K the rows kwave ... of
   // those 16, 16 bytes a lane (the chunk that belongs at the lane's place), of
@@ -1058,7 +1249,7 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
               w_hi_min = key_hi(a, seq, wfirst), w_hi = key_hi(a, seq, wlast);
     const bool idle = r0 + 32 * wave > last;
     v8i qhi[S::DS], qlo[S::DS];
-    const int qe = split_q<S::DS, 2>(a.q + int64_t(seq.start + tok) * a.q_token +
+    const int qe = split_q<S::DS, 2, 16>(a.q + int64_t(seq.start + tok) * a.q_token +
                                          int64_t(kvh * a.group + head) * a.q_head + half * 32,
                                      64, a.q_mul, qhi, qlo);
     v16f o[S::DT];
@@ -1263,6 +1454,80 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
 }
 
 
+// A workgroup a row: the parts of its item, if it has several.  Each wave takes
+// every fourth part with a running maximum, then the waves are joined in order.
+template <int D>
+__global__ __launch_bounds__(256) void attend_few_join_kernel(Attend a, int tile_rows) {
+  constexpr int C = D / 64;
+  __shared__ FindLds fl;
+  __shared__ float ml[4][2];
+  __shared__ float xo[4][D];
+  const int t = int(blockIdx.x / a.heads), h = int(blockIdx.x - unsigned(t) * a.heads);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Found at;
+  const bool any = find(
+      a, tile_rows, fl,
+      [&](const Seq& s, int64_t, int64_t, int64_t) {
+        return t >= s.start && t < s.start + s.new_tokens;
+      },
+      at);
+  if (!any) return;
+  const int64_t share = share_of(a, at.total);
+  const int r = (t - at.seq.start) * a.group + h % a.group, units = units_of(a, at.seq);
+  const int64_t first =
+      at.before + int64_t(r / tile_rows * a.kv_heads + h / a.group) * units;  // the item's first unit
+  const int w0 = int(divide(first, share)), w1 = int(divide(first + units - 1, share));
+  if (w0 == w1) return;
+  float m = -INFINITY, l = 0.0f, o[C] = {};
+  constexpr int N = 4;  // parts of a wave in flight
+  for (int w = w0 + wave; w <= w1; w += 4 * N) {
+    float pm[N], pl[N], po[N][C];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = min(w + 4 * i, w1);
+      const int64_t p = (2 * int64_t(x) + (x == w0 ? 1 : 0)) * tile_rows + r % tile_rows;
+      pm[i] = a.part_ml[2 * p];
+      pl[i] = a.part_ml[2 * p + 1];
+#pragma unroll
+      for (int c = 0; c < C; ++c) po[i][c] = a.part[p * D + lane * C + c];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (w + 4 * i > w1) continue;
+      const float top = fmaxf(m, pm[i]);
+      const float f = m == top ? 1.0f : exp2_fast((m - top) * a.c);
+      const float g = pm[i] == top ? 1.0f : exp2_fast((pm[i] - top) * a.c);
+      m = top;
+      l = l * f + pl[i] * g;
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] = o[c] * f + po[i][c] * g;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) xo[wave][lane * C + c] = o[c];
+  if (lane == 0) {
+    ml[wave][0] = m;
+    ml[wave][1] = l;
+  }
+  __syncthreads();
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][0]);
+  float sum = 0.0f, f[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = ml[w][0] == top ? 1.0f : exp2_fast((ml[w][0] - top) * a.c);
+    sum += ml[w][1] * f[w];
+  }
+  if (threadIdx.x < D) {
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v += xo[w][threadIdx.x] * f[w];
+    a.out[(int64_t(t) * a.heads + h) * D + threadIdx.x] =
+        f32_to_bf16_rne(sum == 0.0f ? 0.0f : v / sum);
+  }
+}
+
 // A wave a row whose keys were split: the splits' sums, brought to the largest
 // maximum and added in order.
 template <int D>
@@ -1311,34 +1576,47 @@ struct Launch {
   int few_tiles;  // 16-row tiles a workgroup of the few-rows kernel takes; 0: many rows
   bool wide;      // 256 rows a workgroup
   int tile_rows, tiles, splits, chunk;
+  int workers;    // few rows: workgroups
+  bool whole;     // few rows: one workgroup an item
 };
 Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
             int64_t max_query_len, int64_t max_seq_len, int64_t window) {
-  Launch p;
+  Launch p{};
   const int64_t group = heads / kv_heads;
   const int64_t most = std::max<int64_t>(std::min(max_query_len, tokens), 1) * group;
   p.few_tiles = most <= 16 ? 1 : most <= 32 ? 2 : 0;
   p.wide = most > 128 && dim <= 128;
   p.tile_rows = p.few_tiles ? 16 * p.few_tiles : p.wide ? kWideRows : kManyRows;
   p.tiles = int((most + p.tile_rows - 1) / p.tile_rows);
+  int64_t keys = std::clamp<int64_t>(max_seq_len, 1, int64_t(1) << 30);
+  if (window > 0) keys = std::min(keys, window + max_query_len + 64);
+  if (p.few_tiles) {
+    // two workgroups a CU (one of the widest), fewer where there is less to do
+    const int64_t items = batch * kv_heads;
+    p.whole = keys <= 2 * kUnit;
+    const int64_t units = p.whole ? items : items * ((keys + kUnit - 1) / kUnit + 1);
+    p.workers = int(std::min<int64_t>(units, dim == 256 && p.few_tiles == 2 ? 256 : 512));
+    p.splits = p.whole ? 1 : 2;
+    return p;
+  }
   // workgroups without splitting: at most one tile a sequence is part full
   const int64_t full = std::min<int64_t>(p.tiles * batch, tokens * group / p.tile_rows + batch);
   const int64_t wgs = std::max<int64_t>(full * kv_heads, 1);
-  int64_t keys = std::clamp<int64_t>(max_seq_len, 1, int64_t(1) << 30);
-  if (window > 0) keys = std::min(keys, window + max_query_len + 64);
-  const int64_t unit = 256;
-  const int64_t want = p.few_tiles ? 2048 : p.wide ? 256 : 512;
+  const int64_t unit = 256, want = p.wide ? 256 : 512;
   const int64_t splits = std::clamp<int64_t>((want + wgs - 1) / wgs, 1, kMaxSplits);
   const int64_t per = (keys + splits - 1) / splits;
-  const int64_t chunk = std::max<int64_t>((per + unit - 1) / unit * unit, unit);
-  p.chunk = int(std::min<int64_t>(chunk, int64_t(1) << 30));
+  p.chunk = int(std::max<int64_t>((per + unit - 1) / unit * unit, unit));
   p.splits = int(std::clamp<int64_t>((keys + p.chunk - 1) / p.chunk, 1, kMaxSplits));
   return p;
 }
 
-size_t workspace_of(const Launch& p, int64_t tokens, int heads, int dim) {
+// Rows that parts are kept of.
+int64_t part_rows(const Launch& p, int64_t tokens, int heads) {
   if (p.splits <= 1) return 0;
-  return size_t(p.splits) * size_t(tokens) * size_t(heads) * size_t(dim + 2) * sizeof(float);
+  return p.few_tiles ? 2 * int64_t(p.workers) * p.tile_rows : p.splits * tokens * heads;
+}
+size_t workspace_of(const Launch& p, int64_t tokens, int heads, int dim) {
+  return size_t(part_rows(p, tokens, heads)) * size_t(dim + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -1477,7 +1755,9 @@ int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
   a.chunk = p.chunk;
   a.out = static_cast<uint16_t*>(out);
   a.part = static_cast<float*>(workspace);
-  a.part_ml = a.part + size_t(p.splits) * size_t(tokens) * size_t(heads) * size_t(dim);
+  a.part_ml = a.part + part_rows(p, tokens, heads) * dim;
+  a.workers = p.workers;
+  a.whole = p.whole;
   const auto st = static_cast<hipStream_t>(stream);
 #define TCFP_BY_DIM(CALL)         \
   do {                            \
@@ -1486,12 +1766,10 @@ int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     else CALL(256);               \
   } while (0)
   if (p.few_tiles) {
-    if (int64_t(kv_heads) * p.tiles > 65535) return TCFP_ERR_SHAPE;
-    const dim3 grid(unsigned(p.splits), unsigned(kv_heads * p.tiles), unsigned(batch));
 #define TCFP_FEW(D)                                                       \
   do {                                                                    \
-    if (p.few_tiles == 1) attend_few_kernel<D, 1><<<grid, 256, 0, st>>>(a); \
-    else attend_few_kernel<D, 2><<<grid, 256, 0, st>>>(a);                \
+    if (p.few_tiles == 1) attend_few_kernel<D, 1><<<p.workers, 256, 0, st>>>(a); \
+    else attend_few_kernel<D, 2><<<p.workers, 256, 0, st>>>(a);                \
   } while (0)
     TCFP_BY_DIM(TCFP_FEW);
 #undef TCFP_FEW
@@ -1506,7 +1784,13 @@ int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     else TCFP_BY_DIM(TCFP_MANY);
 #undef TCFP_MANY
   }
-  if (p.splits > 1) {
+  if (p.splits > 1 && p.few_tiles) {
+    if (!grid_x_fits(tokens * heads, 256)) return TCFP_ERR_SHAPE;
+#define TCFP_JOIN(D) \
+  attend_few_join_kernel<D><<<unsigned(tokens * heads), 256, 0, st>>>(a, p.tile_rows)
+    TCFP_BY_DIM(TCFP_JOIN);
+#undef TCFP_JOIN
+  } else if (p.splits > 1) {
     const int64_t blocks = (tokens * heads + 3) / 4;
     if (!grid_x_fits(blocks, 256)) return TCFP_ERR_SHAPE;
 #define TCFP_JOIN(D) attend_join_kernel<D><<<unsigned(blocks), 256, 0, st>>>(a, p.tile_rows)

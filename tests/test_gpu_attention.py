@@ -242,6 +242,32 @@ def test_lengths(dev, lens, heads, kv_heads):
     b.check(b.attend())
 
 
+@pytest.mark.parametrize("sequences", [2, 63, 65, 300, 520])
+def test_many_sequences(dev, sequences):
+    """More sequences than a wave or a workgroup looks at in one go, some
+    without new tokens, their keys cut into runs that span sequences."""
+    print(f"[attend] {sequences} sequences", flush=True)
+    for new in (1, 3):
+        lens = [(new if b % 7 else 0, 1 + (b * 37) % 290) for b in range(sequences)]
+        lens = [(n, max(n, total)) for n, total in lens]
+        b = Batch(dev, lens, 4, 2, 64, 16, seed=14)
+        b.check(b.attend())
+        b.check(b.attend(max_seq_len=40))
+    lens = [(40, 40 + b % 11) if b % 5 else (1, 9) for b in range(min(sequences, 100))]
+    b = Batch(dev, lens, 4, 2, 64, 16, seed=15)
+    b.check(b.attend())
+
+
+def test_long_sequences(dev):
+    """Keys cut into more runs than the card has places for, and a window."""
+    for lens, heads in (([(1, 40000)], 4), ([(2, 30000), (1, 5), (1, 9000)], 8),
+                        ([(70, 20000)], 2)):
+        print(f"[attend] {lens}", flush=True)
+        b = Batch(dev, lens, heads, 1, 64, 64, seed=16)
+        b.check(b.attend())
+        b.check(b.attend(window=7000), window=7000)
+
+
 @pytest.mark.parametrize("page", [16, 32, 128, 256, 1024])
 def test_page_sizes(dev, page):
     b = Batch(dev, [(1, 5), (1, 700), (1, 1500)], 8, 2, 64, page, seed=3)
