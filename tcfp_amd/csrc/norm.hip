@@ -131,15 +131,27 @@ __global__ __launch_bounds__(kThreads) void norm_any_kernel(Norm a) {
 // Bound by HBM: each input is read and each output written once.  T threads
 // hold a row, C vectors of 8 neighbouring elements each (vector i of thread t
 // at column 8 (t + i T)), so a block's maximum is over 4, 8 or 16 neighbouring
-// lanes.  A workgroup walks `run` neighbouring rows with the next row's loads
-// in flight; block scales, whose neighbours in memory are neighbouring rows,
-// are gathered in LDS and written as runs of `run` values.
+// lanes.  One row for each T threads of the launch: thousands of small
+// workgroups keep more loads in flight than few that walk rows with the next
+// row prefetched (8192 x 4096 bf16 + residual: 47.6 us against 51 / 60 / 63 at
+// 2 / 8 / 16 rows a workgroup).
+// (NT: with the non-temporal hint)
+template <bool NT>
+TCFP_DEV uint4 load16(const void* p) {
+  typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+  const v4u* q = static_cast<const v4u*>(p);
+  const v4u t = NT ? __builtin_nontemporal_load(q) : *q;
+  return make_uint4(t.x, t.y, t.z, t.w);
+}
 template <typename T>
 struct Raw8;
 template <>
 struct Raw8<uint16_t> {
   uint4 a;
-  TCFP_DEV void load(const uint16_t* p) { a = *reinterpret_cast<const uint4*>(p); }
+  template <bool NT = false>
+  TCFP_DEV void load(const uint16_t* p) {
+    a = load16<NT>(p);
+  }
   TCFP_DEV void zero() { a = make_uint4(0, 0, 0, 0); }
   TCFP_DEV void get(float* v) const {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
@@ -153,9 +165,10 @@ struct Raw8<uint16_t> {
 template <>
 struct Raw8<float> {
   float4 a, b;
+  template <bool NT = false>
   TCFP_DEV void load(const float* p) {
-    a = reinterpret_cast<const float4*>(p)[0];
-    b = reinterpret_cast<const float4*>(p)[1];
+    a = __builtin_bit_cast(float4, load16<NT>(p));
+    b = __builtin_bit_cast(float4, load16<NT>(p + 4));
   }
   TCFP_DEV void zero() { a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
   TCFP_DEV void get(float* v) const {
@@ -168,13 +181,22 @@ TCFP_DEV uint32_t pack_bf16(float a, float b) {
   const bf2 r = {(__bf16)a, (__bf16)b};
   return __builtin_bit_cast(uint32_t, r);
 }
-TCFP_DEV void store8(uint16_t* p, const float* v) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]),
-                                            pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+template <bool NT>
+TCFP_DEV void store16(void* p, uint4 v) {
+  typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+  const v4u t = {v.x, v.y, v.z, v.w};
+  if constexpr (NT) __builtin_nontemporal_store(t, static_cast<v4u*>(p));
+  else *static_cast<v4u*>(p) = t;
 }
+template <bool NT = false>
+TCFP_DEV void store8(uint16_t* p, const float* v) {
+  store16<NT>(p, make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
+                            pack_bf16(v[6], v[7])));
+}
+template <bool NT = false>
 TCFP_DEV void store8(float* p, const float* v) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  store16<NT>(p, __builtin_bit_cast(uint4, make_float4(v[0], v[1], v[2], v[3])));
+  store16<NT>(p + 4, __builtin_bit_cast(uint4, make_float4(v[4], v[5], v[6], v[7])));
 }
 TCFP_DEV void load8_any(const void* p, int dtype, int64_t i, float* v) {
   if (dtype == TCFP_DTYPE_BF16) {
@@ -188,188 +210,184 @@ TCFP_DEV void load8_any(const void* p, int dtype, int64_t i, float* v) {
   }
 }
 
-constexpr int kWaveCols = 2048;      // widest row of a wave
-constexpr int kWaveColsBack = 1024;  // and in the backward
-constexpr int kRun = 16;  // rows of a workgroup at most
+// Threads of a workgroup whose rows take T of them.
+constexpr int wg_of(int t) { return t > kThreads ? t : kThreads; }
 
-// Sum over the T threads of a row, to each of them.  T > 64: through `red`,
-// whose use alternates between two arrays by row, one barrier a row.
-template <int T, int W>
-TCFP_DEV float row_sum(float v, float (*red)[W], int parity) {
+// Sum over the T threads of a row, to each of them, through `red` (a float per
+// wave of the workgroup) where a row is more than a wave.
+template <int T>
+TCFP_DEV float row_sum(float v, float* red) {
   v = wave_sum(v);
   if constexpr (T > 64) {
-    if ((threadIdx.x & 63) == 0) red[parity][threadIdx.x >> 6] = v;
+    const int first = threadIdx.x / T * (T / 64);
+    red[threadIdx.x >> 6] = v;  // (every lane of the wave the same)
     __syncthreads();
-    v = red[parity][0];
+    v = red[first];
 #pragma unroll
-    for (int i = 1; i < T / 64; ++i) v += red[parity][i];
+    for (int i = 1; i < T / 64; ++i) v += red[first + i];
   }
   return v;
 }
 
-template <typename XT, typename RT, bool QUANT, int T, int C>
-__global__ __launch_bounds__(kThreads) void norm_rows_kernel(Norm a, int run) {
-  constexpr int G = kThreads / T;  // rows at a time
-  constexpr int NB = QUANT ? T * C / 4 : 1;
-  __shared__ float red[2][kThreads / 64];
-  __shared__ uint32_t sc[NB * kRun];
+template <typename XT, typename RT, bool QUANT, bool NT, int T, int C>
+__global__ __launch_bounds__(wg_of(T)) void norm_rows_kernel(Norm a) {
+  constexpr int G = wg_of(T) / T;  // rows of a workgroup
+  __shared__ float red[wg_of(T) / 64];
+  __shared__ uint32_t sc[QUANT ? G * T * C / 4 : 1];  // scales of its blocks of 32 columns or more
   const int t = threadIdx.x % T, g = threadIdx.x / T;
-  const int64_t row0 = int64_t(blockIdx.x) * run;
+  const int64_t row = int64_t(blockIdx.x) * G + g;
+  const bool live = row < a.rows;
   const int nvec = int(a.cols / 8);
   const XT* x = static_cast<const XT*>(a.x);
   const RT* r = static_cast<const RT*>(a.r);
-  float w[C][8];
   Raw8<XT> nx[C];
   Raw8<RT> nr[C];
-  auto fetch = [&](int64_t row) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int v = t + i * T;
-      if (v < nvec && row < a.rows) {
-        nx[i].load(x + row * a.ldx + v * 8);
-        if (r) nr[i].load(r + row * a.ldr + v * 8);
-      } else {
-        nx[i].zero();
-        nr[i].zero();
-      }
+  for (int i = 0; i < C; ++i) {
+    const int v = t + i * T;
+    nx[i].zero();
+    nr[i].zero();
+    if (v < nvec && live) {
+      nx[i].template load<NT>(x + row * a.ldx + v * 8);
+      if (r) nr[i].template load<NT>(r + row * a.ldr + v * 8);
     }
-  };
-  fetch(row0 + g);
+  }
+  float w[C][8] = {};
 #pragma unroll
   for (int i = 0; i < C; ++i)
-    if (t + i * T < nvec) {
-      load8_any(a.w, a.w_dtype, (t + i * T) * 8, w[i]);
-    } else {
+    if (t + i * T < nvec) load8_any(a.w, a.w_dtype, (t + i * T) * 8, w[i]);
+  float s[C][8];
+  float ss = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[i][j] = 0.0f;
+  for (int i = 0; i < C; ++i) {
+    nx[i].get(s[i]);
+    if (r) {
+      float rv[8];
+      nr[i].get(rv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[i][j] += rv[j];
     }
-  for (int k = 0; k < run; k += G) {
-    const int64_t row = row0 + k + g;
-    const bool live = row < a.rows;
-    float s[C][8];
-    float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      nx[i].get(s[i]);
-      if (r) {
-        float rv[8];
-        nr[i].get(rv);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[i][j] += rv[j];
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(s[i][j], s[i][j], ss);
-    }
-    if (k + G < run) fetch(row + G);
-    if (a.h && live) {
-#pragma unroll
-      for (int i = 0; i < C; ++i)
-        if (t + i * T < nvec)
-          store8(static_cast<RT*>(a.h) + row * a.cols + (t + i * T) * 8, s[i]);
-    }
-    ss = row_sum<T>(ss, red, (k / G) & 1);
-    const float rstd = 1.0f / sqrtf(ss / float(a.cols) + a.eps);
-    if (t == 0 && live) a.rstd[row] = rstd;
+    for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(s[i][j], s[i][j], ss);
+  }
+  if (a.h && live) {
+    // (not read again before the layer between is done: non-temporal, which
+    // leaves the L2 to the rest: 48.5 us against 50.8 at 8192 x 4096, 7.9
+    // against 9.0 at 4096 x 1024)
 #pragma unroll
     for (int i = 0; i < C; ++i)
+      if (t + i * T < nvec)
+        store8<true>(static_cast<RT*>(a.h) + row * a.cols + (t + i * T) * 8, s[i]);
+  }
+  ss = row_sum<T>(ss, red);
+  const float rstd = 1.0f / sqrtf(ss / float(a.cols) + a.eps);
+  if (t == 0 && live) a.rstd[row] = rstd;
+  const float fmax = fp8_max(a.fmt);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[i][j] = s[i][j] * rstd * w[i][j];
+  for (int i = 0; i < C; ++i) {
+    const int v = t + i * T;
+    const bool mine = live && v < nvec;
+    const int64_t at = row * a.cols + v * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[i][j] = s[i][j] * rstd * w[i][j];
     if constexpr (!QUANT) {
-      if (live) {
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-          if (t + i * T >= nvec) continue;
-          const int64_t at = row * a.cols + (t + i * T) * 8;
-          if (a.y_dtype == TCFP_DTYPE_BF16) store8(static_cast<uint16_t*>(a.y) + at, s[i]);
-          else store8(static_cast<float*>(a.y) + at, s[i]);
-        }
-      }
+      if (!mine) continue;
+      if (a.y_dtype == TCFP_DTYPE_BF16) store8(static_cast<uint16_t*>(a.y) + at, s[i]);
+      else store8(static_cast<float*>(a.y) + at, s[i]);
     } else {
-      const float fmax = fp8_max(a.fmt);
+      uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = umax(m, absbits(s[i][j]));
-        if (a.block == 32) m = seg_umax<4>(m);
-        else if (a.block == 64) m = seg_umax<8>(m);
-        else m = seg_umax<16>(m);
-        float mul;
-        uint32_t code;
-        if (a.f32_scales) {
-          float inv;
-          scale_of(__uint_as_float(m), fmax, mul, inv);
-          code = __float_as_uint(inv);
-        } else {
-          const int e = block_exponent(__uint_as_float(m), fmax);
-          mul = exp2i(-e);
-          code = uint32_t(e);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[i][j] = clampf(s[i][j] * mul, fmax);
-        uint2 q;
-        if (a.fmt == TCFP_FP8_E5M2)
-          q = make_uint2(cvt4_fp8<TCFP_FP8_E5M2>(s[i][0], s[i][1], s[i][2], s[i][3]),
-                         cvt4_fp8<TCFP_FP8_E5M2>(s[i][4], s[i][5], s[i][6], s[i][7]));
-        else
-          q = make_uint2(cvt4_fp8<TCFP_FP8_E4M3>(s[i][0], s[i][1], s[i][2], s[i][3]),
-                         cvt4_fp8<TCFP_FP8_E4M3>(s[i][4], s[i][5], s[i][6], s[i][7]));
-        const int v = t + i * T;
-        if (v < nvec) {
-          if (live) *reinterpret_cast<uint2*>(a.q + row * a.cols + v * 8) = q;
-          if ((v * 8) % a.block == 0) sc[(v * 8 / a.block) * kRun + k + g] = code;
-        }
+      for (int j = 0; j < 8; ++j) m = umax(m, absbits(s[i][j]));
+      if (a.block == 32) m = seg_umax<4>(m);
+      else if (a.block == 64) m = seg_umax<8>(m);
+      else m = seg_umax<16>(m);
+      float mul, inv = 0.0f;
+      int e = 0;
+      if (a.f32_scales) {
+        scale_of(__uint_as_float(m), fmax, mul, inv);
+      } else {
+        e = block_exponent(__uint_as_float(m), fmax);
+        mul = exp2i(-e);
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[i][j] = clampf(s[i][j] * mul, fmax);
+      uint2 q;
+      if (a.fmt == TCFP_FP8_E5M2)
+        q = make_uint2(cvt4_fp8<TCFP_FP8_E5M2>(s[i][0], s[i][1], s[i][2], s[i][3]),
+                       cvt4_fp8<TCFP_FP8_E5M2>(s[i][4], s[i][5], s[i][6], s[i][7]));
+      else
+        q = make_uint2(cvt4_fp8<TCFP_FP8_E4M3>(s[i][0], s[i][1], s[i][2], s[i][3]),
+                       cvt4_fp8<TCFP_FP8_E4M3>(s[i][4], s[i][5], s[i][6], s[i][7]));
+      if (!mine) continue;
+      *reinterpret_cast<uint2*>(a.q + at) = q;
+      if ((v * 8) % a.block == 0)
+        sc[v * 8 / a.block * G + g] = a.f32_scales ? __float_as_uint(inv) : uint32_t(e);
     }
   }
   if constexpr (QUANT) {
+    // the scales, gathered: written by whole waves (47.6 us against 52.9 at
+    // 8192 x 4096 where the lanes that found them write them)
     __syncthreads();
-    const int n = int(a.cols / a.block) * run;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int kb = i / run, k = i - kb * run;
-      if (row0 + k >= a.rows) continue;
-      const int64_t at = kb * a.rows + row0 + k;
-      const uint32_t code = sc[kb * kRun + k];
-      if (a.f32_scales) static_cast<uint32_t*>(a.scales)[at] = code;
-      else static_cast<int8_t*>(a.scales)[at] = int8_t(code);
+    const int64_t row0 = int64_t(blockIdx.x) * G;
+    for (int i = threadIdx.x; i < int(a.cols / a.block) * G; i += wg_of(T)) {
+      if (row0 + i % G >= a.rows) continue;
+      const int64_t at = int64_t(i / G) * a.rows + row0 + i % G;
+      if (a.f32_scales) static_cast<uint32_t*>(a.scales)[at] = sc[i];
+      else static_cast<int8_t*>(a.scales)[at] = int8_t(sc[i]);
     }
   }
 }
 
-// Threads and vectors of a row: a wave a row where the rows alone fill the
-// card, else the row over a workgroup; 0: the kernel for any row.
+// Threads and vectors of a row: two vectors a thread where the rows fill the
+// card, one where there are few (latency); t == 0: the kernel for any row.
 struct RowShape {
   int t, c;
 };
-RowShape row_shape(int64_t rows, int64_t cols, int64_t wave_cols) {
-  if (cols % 8 != 0 || cols > kThreads * 64) return {0, 0};
+RowShape row_shape(int64_t rows, int64_t cols) {
+  if (cols % 8 != 0 || cols > 1024 * 16) return {0, 0};
   const int64_t nvec = cols / 8;
-  const int t = rows >= 1024 && cols <= wave_cols ? 64 : nvec <= 64 ? 64 : kThreads;
-  int c = 1;
-  while (int64_t(t) * c < nvec) c *= 2;
-  return {t, c};
+  int t = 64;
+  if (rows >= 1024) {
+    while (t * 2 < nvec) t *= 2;
+  } else {
+    while (t < nvec && t < 1024) t *= 2;
+  }
+  return {t, t < nvec ? 2 : 1};
 }
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 int64_t size_of(int dtype) { return dtype == TCFP_DTYPE_BF16 ? 2 : 4; }
 
+// Inputs of more than half the 256 MiB cache behind the L2s are read with the
+// non-temporal hint (8192 x 4096 bf16 + residual: forward 50.0 us against 52.9,
+// backward 52.4 against 57.0); smaller ones, which their producer may have left
+// there, are not (8192 x 1024: 13.3 us against 14.8 with it, 16.7 against 18.6).
+constexpr int64_t kStreamBytes = 96ll << 20;
+
+#define TCFP_ROWS(CALL)                              \
+  do {                                               \
+    const bool one = s.c == 1;                       \
+    if (s.t == 64 && one) CALL(64, 1);               \
+    else if (s.t == 64) CALL(64, 2);                 \
+    else if (s.t == 128 && one) CALL(128, 1);        \
+    else if (s.t == 128) CALL(128, 2);               \
+    else if (s.t == 256 && one) CALL(256, 1);        \
+    else if (s.t == 256) CALL(256, 2);               \
+    else if (s.t == 512 && one) CALL(512, 1);        \
+    else if (s.t == 512) CALL(512, 2);               \
+    else if (one) CALL(1024, 1);                     \
+    else CALL(1024, 2);                              \
+  } while (0)
+
 template <typename XT, typename RT, bool QUANT>
 int norm_rows_launch(const Norm& a, RowShape s, hipStream_t st) {
-  const int g = kThreads / s.t;
-  // rows of a workgroup: at least two workgroups a CU
-  const int64_t fill = a.rows / 512;
-  int run = g;
-  while (run * 2 <= kRun && run * 2 <= fill) run *= 2;
-  const unsigned blocks = unsigned((a.rows + run - 1) / run);
-#define TCFP_NR(T, C) norm_rows_kernel<XT, RT, QUANT, T, C><<<blocks, kThreads, 0, st>>>(a, run)
-#define TCFP_NR_C(T)                  \
-  do {                                \
-    if (s.c == 1) TCFP_NR(T, 1);      \
-    else if (s.c == 2) TCFP_NR(T, 2); \
-    else if (s.c == 4) TCFP_NR(T, 4); \
-    else TCFP_NR(T, 8);               \
-  } while (0)
-  if (s.t == 64) TCFP_NR_C(64); else TCFP_NR_C(kThreads);
-#undef TCFP_NR_C
+  const int g = wg_of(s.t) / s.t;
+  const unsigned blocks = unsigned((a.rows + g - 1) / g);
+  const int64_t in = a.rows * a.cols * (size_of(a.x_dtype) + (a.r ? size_of(a.r_dtype) : 0));
+#define TCFP_NR(T, C) norm_rows_kernel<XT, RT, QUANT, false, T, C><<<blocks, wg_of(T), 0, st>>>(a)
+#define TCFP_NR_NT(T, C) norm_rows_kernel<XT, RT, QUANT, true, T, C><<<blocks, wg_of(T), 0, st>>>(a)
+  if (in > kStreamBytes) TCFP_ROWS(TCFP_NR_NT);
+  else TCFP_ROWS(TCFP_NR);
+#undef TCFP_NR_NT
 #undef TCFP_NR
   return launch_status();
 }
@@ -424,11 +442,10 @@ __global__ __launch_bounds__(kThreads) void norm_dw_any_kernel(NormBack a, int64
 // rows, the next rows' loads in flight; a thread's columns are the same in all
 // its rows, so it sums its share of dw in registers, the workgroup leaves one
 // partial row and a second launch adds the partials.
-template <typename GT, typename HT, int T, int C>
-__global__ __launch_bounds__(T > kThreads ? T : kThreads) void norm_back_rows_kernel(NormBack a) {
-  constexpr int W = T > kThreads ? T : kThreads;  // threads of a workgroup
-  constexpr int G = W / T;
-  __shared__ float red[2][W / 64];
+template <typename GT, typename HT, bool NT, int T, int C>
+__global__ __launch_bounds__(wg_of(T)) void norm_back_rows_kernel(NormBack a) {
+  constexpr int G = wg_of(T) / T;
+  __shared__ float red[2][wg_of(T) / 64];
   __shared__ float4 dws[G > 1 ? (G - 1) * T * C * 2 : 1];
   const int t = threadIdx.x % T, g = threadIdx.x / T;
   const int nvec = int(a.cols / 8);
@@ -447,9 +464,9 @@ __global__ __launch_bounds__(T > kThreads ? T : kThreads) void norm_back_rows_ke
       const int v = t + i * T;
       if (v < nvec && live) {
         const int64_t at = row * a.cols + v * 8;
-        ng[i].load(gy + at);
-        nh[i].load(h + at);
-        if (gh) na[i].load(gh + at);
+        ng[i].template load<NT>(gy + at);
+        nh[i].template load<NT>(h + at);
+        if (gh) na[i].template load<NT>(gh + at);
       } else {
         ng[i].zero();
         nh[i].zero();
@@ -485,7 +502,7 @@ __global__ __launch_bounds__(T > kThreads ? T : kThreads) void norm_back_rows_ke
       }
     }
     fetch(row + int64_t(gridDim.x) * G);
-    s = row_sum<T>(s, red, parity) * inv_n;
+    s = row_sum<T>(s, red[parity]) * inv_n;  // (one barrier a row: two arrays in turn)
     parity ^= 1;
     if (row < a.rows) {
 #pragma unroll
@@ -530,47 +547,56 @@ __global__ __launch_bounds__(T > kThreads ? T : kThreads) void norm_back_rows_ke
       store8(a.part + int64_t(blockIdx.x) * a.cols + (t + i * T) * 8, dw[i]);
 }
 
-template <typename GT, typename HT>
+// The backward holds three inputs, dw and w of a row: two vectors for each of
+// 1024 threads would spill.
+RowShape back_shape(int64_t rows, int64_t cols) {
+  const RowShape s = row_shape(rows, cols);
+  return s.t == 1024 && s.c == 2 ? RowShape{512, 4} : s;
+}
+
+template <typename GT, typename HT, bool NT>
 void norm_back_launch(const NormBack& a, RowShape s, unsigned blocks, hipStream_t st) {
-#define TCFP_NB(T, C) \
-  norm_back_rows_kernel<GT, HT, T, C><<<blocks, (T) > kThreads ? (T) : kThreads, 0, st>>>(a)
-  if (s.t == 64) {
-    if (s.c == 1) TCFP_NB(64, 1);
-    else TCFP_NB(64, 2);
-  } else {
-    if (s.c == 1) TCFP_NB(kThreads, 1);
-    else if (s.c == 2) TCFP_NB(kThreads, 2);
-    else if (s.c == 4) TCFP_NB(kThreads, 4);
-    else TCFP_NB(2 * kThreads, 4);  // (eight vectors a thread would spill)
-  }
+#define TCFP_NB(T, C) norm_back_rows_kernel<GT, HT, NT, T, C><<<blocks, wg_of(T), 0, st>>>(a)
+#define TCFP_NB_SMALL(T, C) TCFP_NB(T, (T) == 1024 ? 1 : (C))
+  if (s.c == 4) TCFP_NB(512, 4);
+  else TCFP_ROWS(TCFP_NB_SMALL);
+#undef TCFP_NB_SMALL
 #undef TCFP_NB
 }
 
-// dw from the partial rows: a workgroup 16 columns, its threads 16 partials at
-// a time, then the 16 sums in order.
-__global__ __launch_bounds__(kThreads) void norm_dw_sum_kernel(const float* part, int parts,
-                                                               int64_t cols, float* dw) {
-  __shared__ float s[16][17];
+// dw from the partial rows: a workgroup 16 columns, its threads 64 partials at a
+// time (a few loads in a row each: what is left is latency), then the lanes' and
+// the waves' sums in order.
+constexpr int kSumThreads = 1024;
+__global__ __launch_bounds__(kSumThreads) void norm_dw_sum_kernel(const float* part, int parts,
+                                                                  int64_t cols, float* dw) {
+  __shared__ float s[kSumThreads / 64][16];
   const int c = threadIdx.x & 15, p0 = threadIdx.x >> 4;
   const int64_t col = int64_t(blockIdx.x) * 16 + c;
   float v = 0.0f;
   if (col < cols) {
-#pragma unroll 8
-    for (int p = p0; p < parts; p += 16) v += part[int64_t(p) * cols + col];
+#pragma unroll 4
+    for (int p = p0; p < parts; p += kSumThreads / 16) v += part[int64_t(p) * cols + col];
   }
-  s[p0][c] = v;
+  v += __shfl_xor(v, 16, 64);
+  v += __shfl_xor(v, 32, 64);
+  if ((threadIdx.x & 63) < 16) s[threadIdx.x >> 6][c] = v;
   __syncthreads();
-  if (p0 == 0 && col < cols) {
+  if (threadIdx.x < 16 && col < cols) {
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += s[i][c];
+    for (int i = 1; i < kSumThreads / 64; ++i) v += s[i][c];
     dw[col] = v;
   }
 }
 
-constexpr int64_t kMaxParts = 512;  // two workgroups a CU
-
-// Partial rows of dw: at least four rows each.
-int64_t parts_of(int64_t rows) { return std::clamp<int64_t>(rows / 4, 1, kMaxParts); }
+// Workgroups of the backward, each a partial row of dw: as many as a CU holds
+// of them at a time (three of 256 threads, one of 512 or 1024; a part of a
+// second round costs as much as a whole one: 8192 x 8192 bf16 115 us with 256,
+// 140 with 384), fewer where there are few rows, at least two each.
+int64_t parts_of(int64_t rows, int64_t cols) {
+  const RowShape s = back_shape(rows, cols);
+  return std::clamp<int64_t>(rows / 2, 1, s.t > 256 ? 256 : rows <= 4096 ? 512 : 768);
+}
 
 int norm_checks(const Norm& a, bool quantised) {
   if (a.rows < 0 || a.cols < 0 || a.rows > INT32_MAX || a.cols > INT32_MAX) return TCFP_ERR_SHAPE;
@@ -578,7 +604,7 @@ int norm_checks(const Norm& a, bool quantised) {
   if (!dtype_ok(a.x_dtype) || !dtype_ok(a.w_dtype) || (a.r && !dtype_ok(a.r_dtype)))
     return TCFP_ERR_DTYPE;
   if (a.h && !a.r) return TCFP_ERR_SHAPE;
-  if (!grid_x_fits(a.rows, kThreads)) return TCFP_ERR_SHAPE;
+  if (!grid_x_fits(a.rows, 1024)) return TCFP_ERR_SHAPE;
   if (quantised) {
     if (a.block != 32 && a.block != 64 && a.block != 128) return TCFP_ERR_SHAPE;
     if (a.cols % a.block != 0) return TCFP_ERR_SHAPE;
@@ -594,7 +620,7 @@ template <bool QUANT>
 int norm_launch(const Norm& a, hipStream_t st) {
   const int rc = norm_checks(a, QUANT);
   if (rc != TCFP_OK || a.rows == 0 || a.cols == 0) return rc;
-  const RowShape s = row_shape(a.rows, a.cols, kWaveCols);
+  const RowShape s = row_shape(a.rows, a.cols);
   const int64_t xs = size_of(a.x_dtype), rs = size_of(a.r_dtype);
   const bool vec = aligned(a.x, 16) && a.ldx * xs % 16 == 0 && aligned(a.w, 16) &&
                    (!a.r || (aligned(a.r, 16) && a.ldr * rs % 16 == 0)) && aligned(a.h, 16) &&
@@ -635,7 +661,7 @@ int tcfp_rms_norm_quantize(const void* x, int x_dtype, int64_t ldx, const void* 
 
 size_t tcfp_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return size_t(parts_of(rows)) * size_t(cols) * sizeof(float);
+  return size_t(parts_of(rows, cols)) * size_t(cols) * sizeof(float);
 }
 
 int tcfp_rms_norm_backward(const void* grad_y, int gy_dtype, const void* h, int h_dtype,
@@ -649,22 +675,30 @@ int tcfp_rms_norm_backward(const void* grad_y, int gy_dtype, const void* h, int 
   const auto st = static_cast<hipStream_t>(stream);
   if (dw && rows > 0 && workspace_bytes < tcfp_rms_norm_backward_workspace_bytes(rows, cols))
     return TCFP_ERR_WORKSPACE;
-  const int64_t parts = rows > 0 ? parts_of(rows) : 0;
+  const int64_t parts = rows > 0 ? parts_of(rows, cols) : 0;
   // (one partial row is dw itself)
   NormBack a{grad_y, h, rstd, weight, grad_h, gy_dtype, h_dtype, w_dtype, rows, cols, dx,
              !dw ? nullptr : parts == 1 ? dw : static_cast<float*>(workspace)};
   if (rows > 0) {
-    const RowShape s = row_shape(rows, cols, kWaveColsBack);
+    const RowShape s = back_shape(rows, cols);
     const bool vec = aligned(grad_y, 16) && aligned(h, 16) && aligned(weight, 16) &&
                      aligned(grad_h, 16) && aligned(dx, 16) && aligned(a.part, 16);
     if (s.t && vec) {
       const unsigned blocks = unsigned(
-          dw ? parts : std::min<int64_t>((rows * s.t + kThreads - 1) / kThreads, 4 * kMaxParts));
+          dw ? parts : std::min<int64_t>((rows * s.t + wg_of(s.t) - 1) / wg_of(s.t), 2048));
       const bool gb = gy_dtype == TCFP_DTYPE_BF16, hb = h_dtype == TCFP_DTYPE_BF16;
-      if (gb && hb) norm_back_launch<uint16_t, uint16_t>(a, s, blocks, st);
-      else if (gb) norm_back_launch<uint16_t, float>(a, s, blocks, st);
-      else if (hb) norm_back_launch<float, uint16_t>(a, s, blocks, st);
-      else norm_back_launch<float, float>(a, s, blocks, st);
+      const bool nt = rows * cols * (size_of(gy_dtype) + (grad_h ? 2 : 1) * size_of(h_dtype)) >
+                      kStreamBytes;
+#define TCFP_NB_TYPES(NT)                                                          \
+  do {                                                                             \
+    if (gb && hb) norm_back_launch<uint16_t, uint16_t, NT>(a, s, blocks, st);      \
+    else if (gb) norm_back_launch<uint16_t, float, NT>(a, s, blocks, st);          \
+    else if (hb) norm_back_launch<float, uint16_t, NT>(a, s, blocks, st);          \
+    else norm_back_launch<float, float, NT>(a, s, blocks, st);                     \
+  } while (0)
+      if (nt) TCFP_NB_TYPES(true);
+      else TCFP_NB_TYPES(false);
+#undef TCFP_NB_TYPES
     } else {
       norm_dx_any_kernel<<<unsigned(rows), kThreads, 0, st>>>(a);
       if (dw)
@@ -673,7 +707,7 @@ int tcfp_rms_norm_backward(const void* grad_y, int gy_dtype, const void* h, int 
     }
   }
   if (dw && parts != 1)
-    norm_dw_sum_kernel<<<unsigned((cols + 15) / 16), kThreads, 0, st>>>(a.part, int(parts), cols,
+    norm_dw_sum_kernel<<<unsigned((cols + 15) / 16), kSumThreads, 0, st>>>(a.part, int(parts), cols,
                                                                         dw);
   return launch_status();
 }
