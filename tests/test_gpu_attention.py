@@ -378,6 +378,46 @@ def test_nan_in_masked_places(dev):
             assert torch.equal(got[:first], ref[:first])
 
 
+@pytest.mark.parametrize("dim,window", [(64, 0), (64, 300), (128, 0), (128, 300)])
+def test_nan_and_missing_pages_among_many_rows(dev, dim, window):
+    """The same two among more rows than a small tile has, in front of long
+    contexts (the eight-wave kernel)."""
+    nq, total, page = 200, 1000, 16
+    b = Batch(dev, [(nq, total), (150, 700)], 4, 2, dim, page, seed=17)
+    want = b.attend(window=window)
+    b.check(want, window=window)
+    for which in (0, 1):
+        for at in (total - 150, 500, 3):
+            codes = b.pool[which].view(torch.uint8)
+            slot = int(b.slots[0][at])
+            keep = codes[slot // page, :, slot % page].clone()
+            codes[slot // page, 0, slot % page, 7] = 0x7F
+            got = b.attend(window=window)
+            codes[slot // page, :, slot % page] = keep
+            pos = torch.arange(total - nq, total, device=dev)
+            sees = pos >= at
+            if window:
+                sees &= pos < at + window
+            assert torch.equal(got[:nq][~sees], want[:nq][~sees])
+            assert torch.equal(got[:, 2:], want[:, 2:]) and torch.equal(got[nq:], want[nq:])
+            assert got[:nq][sees][:, :2, 7].float().isnan().all()
+    b.table[0, :40] = -1  # the first 640 keys
+    got = b.attend(window=window)
+    assert torch.equal(got[nq:], want[nq:])
+    k, v = _values(b.pool)
+    seen = _mask(nq, total, True, window, dev)[:, 640:]
+    for h in range(4):
+        kh, vh = (t[b.slots[0][640:], h // 2] for t in (k, v))
+        _check(got[:nq, h], b.q[:nq, h], kh, vh, seen, dim**-0.5)
+    b.table[0, 50] = 10**6  # and a hole inside
+    got = b.attend(window=window)
+    keep = torch.ones(total - 640, dtype=torch.bool, device=dev)
+    keep[160:176] = False
+    for h in range(4):
+        kh, vh = (t[b.slots[0][640:], h // 2] for t in (k, v))
+        _check(got[:nq, h], b.q[:nq, h], kh, vh, seen & keep, dim**-0.5)
+
+
 def test_strides(dev):
     """Queries as a slice of the QKV projection, the page table as a slice."""
     b = Batch(dev, MIXED + DECODE, 6, 2, 64, 16, seed=10)
