@@ -10,8 +10,12 @@ autograd Functions.  ``import tcfp`` (the sibling ``tcfp`` package) binds
 this package under the reference's import name.  All device work runs in
 hand-written HIP kernels (``libtcfp_hip.so``, C ABI in
 ``include/tcfp_hip.h``).
+
+``tcfp_amd.norm`` (residual + RMS norm with FP8 output) and
+``tcfp_amd.attention`` (an 8-bit paged K/V cache and attention over it) are the
+operators between the linear layers of a decoder; the reference has neither.
 """
-from . import core, cuda_ext, kernels, nn  # noqa: F401
+from . import attention, core, cuda_ext, kernels, nn, norm  # noqa: F401
 from .core import (  # noqa: F401
     ErrorFeedbackState,
     FP8Config,

@@ -33,12 +33,17 @@ import torch.autograd.forward_ad as fwAD
 import torch.nn as nn
 import torch.nn.functional as F
 
+from types import SimpleNamespace
+
 from .. import kernels as K
+from .. import norm as N
 from ..core import DEFAULT_BLOCK_SIZE, ErrorFeedbackState, TCFPMode
 
 __all__ = [
     "TCFPLinear",
     "TCFPMLP",
+    "TCFPNormLinear",
+    "TCFPRMSNorm",
     "convert_to_tcfp",
     "fuse_tcfp_mlp",
     "set_block_dgrad",
@@ -46,6 +51,7 @@ __all__ = [
     "_TCFP12TensorCoreFunction",
     "_TCFP12BlockScaledFunction",
     "_TCFP12FusedMLPFunction",
+    "_TCFP12NormLinearFunction",
 ]
 
 
@@ -586,6 +592,174 @@ class TCFPLinear(nn.Module):
         if self._bf16_fallback:
             parts.append("bf16_fallback=True")
         return ", ".join(parts)
+
+
+class _RMSNormFunction(torch.autograd.Function):
+    """``norm.rms_norm`` as an autograd node (no reference counterpart):
+    ``(y, h)`` with a residual, ``y`` without."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, out_dtype):
+        y, h, rstd = N.rms_norm(x, weight, residual, eps=eps, out_dtype=out_dtype)
+        ctx.set_materialize_grads(False)
+        ctx.x_dtype = x.dtype
+        ctx.has_residual = residual is not None
+        ctx.save_for_backward(h, rstd, weight)
+        return (y, h) if ctx.has_residual else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_y, grad_h=None):
+        h, rstd, weight = ctx.saved_tensors
+        dx, dw = _norm_backward(ctx, grad_y, grad_h, h, rstd, weight, ctx.needs_input_grad[:3])
+        return (*dx, dw, None, None)
+
+
+def _norm_backward(ctx, grad_y, grad_h, h, rstd, weight, needs):
+    """Gradients ``((x, residual), weight)`` of a norm whose output's gradient is
+    ``grad_y`` and whose sum's is ``grad_h`` (either may be None)."""
+    need_x, need_r, need_w = needs
+    if grad_y is None:  # only the sum was used
+        g = grad_h
+        dw = torch.zeros_like(weight) if need_w else None
+    else:
+        if grad_y.dtype not in (torch.float32, torch.bfloat16):
+            grad_y = grad_y.float()
+        g, dw = N.rms_norm_backward(grad_y, h, rstd, weight, grad_h, need_weight_grad=need_w)
+        dw = dw.to(weight.dtype) if need_w else None
+    dx = g.to(ctx.x_dtype) if need_x and g is not None else None
+    return (dx, g if need_r and ctx.has_residual else None), dw
+
+
+class TCFPRMSNorm(nn.Module):
+    """Root-mean-square norm over the last axis with an optional residual
+    addition in front, on the HIP kernels of ``tcfp_amd.norm`` (no reference
+    counterpart).
+
+    ``norm(x)`` returns the normalised tensor in ``x``'s dtype;
+    ``norm(x, residual)`` returns it and the sum ``x + residual`` in the
+    residual's dtype, which the next residual addition takes.
+    """
+
+    def __init__(self, dim: int, eps: float = 1e-6, *, device=None, dtype=None) -> None:
+        super().__init__()
+        self.dim, self.eps = dim, eps
+        self.weight = nn.Parameter(torch.ones(dim, device=device, dtype=dtype))
+
+    @torch.compiler.disable
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        x, residual, weight = _for_inference(x, residual, self.weight)
+        return _RMSNormFunction.apply(x, residual, weight, self.eps, x.dtype)
+
+    def extra_repr(self) -> str:
+        return f"{self.dim}, eps={self.eps}"
+
+
+class _TCFP12NormLinearFunction(torch.autograd.Function):
+    """Residual addition + RMS norm + block-scaled TCFP linear as one autograd
+    node (no reference counterpart): the norm writes the E4M3 codes and
+    exponents that the dual GEMM reads, so the normalised activations are never
+    stored, forward or backward (the weight gradient reads the codes, as the
+    block-scaled layer's does).  Equal to ``_TCFP12BlockScaledFunction`` on the
+    norm's fp32 output."""
+
+    @staticmethod
+    def forward(  # noqa: PLR0913
+        ctx, x, residual, norm_weight, weight, bias, eps, bs, error_state, param_name, abd, srr,
+        update_ef,
+    ):
+        w = weight if weight.is_contiguous() else weight.contiguous()
+        x2d = _flatten(x)
+        r2d = None if residual is None else _flatten(residual)
+        w_hi, w_lo, sh, sl = K.fused_dual_quantize_fp8(
+            w, bs, _ef_buffer(error_state, param_name, weight), stochastic_lo=srr,
+            update_ef=update_ef)
+        q, e, h, rstd = N.rms_norm_quantize(x2d, norm_weight, r2d, eps=eps, block_size=bs)
+        out = K.fused_block_scaled_dual_gemm_forward(q, w_hi, w_lo, e, sh, sl, bs, bias=bias)
+
+        ctx.set_materialize_grads(False)
+        ctx.x_dtype = x.dtype
+        ctx.has_residual = residual is not None
+        ctx.has_bias = bias is not None
+        ctx.bs, ctx.abd, ctx.shape = bs, abd, x.shape
+        ctx.fp8_dgrad = _BLOCK_DGRAD == "fp8"
+        ctx.bf16_wgrad = _BLOCK_WGRAD == "bf16"
+        need_y, need_dw = any(ctx.needs_input_grad[:3]), ctx.needs_input_grad[3]
+        w_lo, sl = (None, None) if abd else (w_lo, sl)
+        if not need_y:
+            w_hi = w_lo = sh = sl = None
+        elif ctx.fp8_dgrad:
+            w_hi, w_lo, sh, sl = K.block_requant_t(w_hi, w_lo, sh, sl, bs)
+        ctx.save_for_backward(q if need_dw else None, e if need_dw else None, w_hi, w_lo, sh, sl,
+                              h if need_y else None, rstd if need_y else None, norm_weight)
+        out = out.reshape(*x.shape[:-1], out.shape[-1])
+        return (out, h.reshape(x.shape)) if ctx.has_residual else out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out, grad_h=None):
+        *saved, h, rstd, norm_weight = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        need_y = any(needs[:3])
+        dy = dw = db = None
+        if grad_out is not None:
+            # the block-scaled layer's backward, for the norm's output
+            layer = SimpleNamespace(
+                saved_tensors=saved, needs_input_grad=(need_y, needs[3], needs[4]),
+                hp_grad_weight=False, input_shape=(grad_out.numel() // grad_out.shape[-1], ctx.shape[-1]),
+                dx_dtype=_grad_dtype(h) if need_y else torch.float32, has_bias=ctx.has_bias,
+                bs=ctx.bs, abd=ctx.abd, fp8_dgrad=ctx.fp8_dgrad, bf16_wgrad=ctx.bf16_wgrad)
+            dy, dw, db = _TCFP12BlockScaledFunction.backward(layer, grad_out)[:3]
+        dx = dr = dn = None
+        if need_y:
+            g_h = None if grad_h is None else _flatten(grad_h)
+            (dx, dr), dn = _norm_backward(ctx, dy, g_h, h, rstd, norm_weight, needs[:3])
+            dx = None if dx is None else dx.reshape(ctx.shape)
+            dr = None if dr is None else dr.reshape(ctx.shape)
+        return (dx, dr, dn, dw, db) + (None,) * 7
+
+
+class TCFPNormLinear(TCFPLinear):
+    """``TCFPRMSNorm`` followed by a block-scaled ``TCFPLinear``, the norm's
+    output quantised where it is computed (no reference counterpart).
+
+    ``layer(x)`` is the linear layer on the normalised ``x``; ``layer(x,
+    residual)`` returns it for ``x + residual``, and that sum in the residual's
+    dtype.  Constructor arguments as ``TCFPLinear``; ``scale_block_size`` (64 by
+    default) is required, since a per-tensor scale would need the norm of every
+    row first.  ``hp_grad_weight`` and warm-up or fallback calls take the norm's
+    output in fp32 through the plain layer.
+    """
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, *,
+                 eps: float = 1e-6, scale_block_size: int = 64, use_tensor_cores: bool = True,
+                 **kw) -> None:
+        if scale_block_size is None:
+            raise ValueError("TCFPNormLinear needs block scales (scale_block_size 32, 64 or 128)")
+        super().__init__(in_features, out_features, bias, scale_block_size=scale_block_size,
+                         use_tensor_cores=use_tensor_cores, **kw)
+        self.eps = eps
+        self.norm_weight = nn.Parameter(torch.ones(in_features, device=self.weight.device,
+                                                   dtype=self.weight.dtype))
+
+    @torch.compiler.disable
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        if self._bf16_fallback or self._warmup_remaining > 0 or self.hp_grad_weight:
+            y = _RMSNormFunction.apply(x, residual, self.norm_weight, self.eps, torch.float32)
+            y, h = (y, None) if residual is None else y
+            if self._bf16_fallback or self._warmup_remaining > 0:
+                y = y.to(self.weight.dtype)
+            out = super().forward(y)
+            return out if residual is None else (out, h)
+        update_ef = self._ef_update_flag()
+        x, residual, norm_weight, weight, bias = _for_inference(
+            x, residual, self.norm_weight, self.weight, self.bias)
+        return _TCFP12NormLinearFunction.apply(
+            x, residual, norm_weight, weight, bias, self.eps, self.scale_block_size,
+            self._error_state, self._param_name, self.abd, self.srr, update_ef)
+
+    def extra_repr(self) -> str:
+        return super().extra_repr() + f", eps={self.eps}"
 
 
 class _TCFP12FusedMLPFunction(torch.autograd.Function):
