@@ -75,7 +75,9 @@ struct Strided {
   int64_t token[2], head[2];
 };
 
-// DIM / 8 lanes a (token, head), 8 values each; blockIdx.y: K or V.
+// DIM / 8 lanes a (token, head), 8 values each; blockIdx.y: K or V.  Bound by HBM:
+// 8000 tokens of 8 heads of 128 in fp32 15.7 us (5.2 TB/s), 30011 tokens read
+// into bf16 40.6 us (4.6 TB/s); 64 tokens 2.7 us, a launch and two latencies.
 template <typename T, int DIM>
 __global__ __launch_bounds__(kThreads) void cache_write_kernel(Strided x, Pool pool,
                                                                const int64_t* slots,
@@ -136,9 +138,9 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(Pool pool, const i
 //
 // The rows of a (sequence, K/V head) are its new tokens times the group of
 // query heads that share the head: row r is token r / group, head r % group
-// of the group.  A workgroup takes a tile of rows over a run of keys (a
-// split); rows whose keys are in one split are finished there, the others
-// leave (sum p v, max, sum p) for the combining kernel.
+// of the group.  A workgroup takes a tile of rows over a run of keys; rows whose
+// keys are all in one run are finished there, the others leave (sum p v, max,
+// sum p) for a joining launch, which adds the runs in order.
 //
 //   S^T = K Q^T      A = K codes, B = Q   keys down the registers, rows across lanes
 //   O^T += V^T P^T   A = V^T,     B = P^T
@@ -151,8 +153,10 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(Pool pool, const i
 // with one power-of-two scale a row is exact for bf16 values down to 2^-10 of
 // the row's largest (4 + 4 significant bits) and within 2^-18 of the largest
 // below that; the matrix instruction applies 2^e of a key as its block scale,
-// and two FP8 products cost what one bf16 product would, without converting K.  V is converted to bf16 with its
-// exponent (both exact) and P is rounded to bf16: 2^-9 of a weight.
+// and two FP8 products cost what one bf16 product would, without converting K.
+// V is converted to bf16 with its exponent (both exact) and P is rounded to
+// bf16: 2^-9 of a weight, where the result's own rounding to bf16 is 2^-9 too.
+// Scores, maxima and sums are fp32; the sum is of P before its rounding.
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -318,10 +322,13 @@ TCFP_DEV void zero_rest(const Attend& a, int lead, int tail, int first, int head
 
 // ---- few rows: one token a sequence, a few drafts ----------------------------
 //
-// Bound by reading the cache.  A wave takes KT keys at a time straight into
-// registers, the next KT in flight; nothing of K or V passes through LDS.  The
-// four waves of a workgroup take turns over the split's keys and are joined at
-// its end.
+// Bound by reading the cache: 64 sequences of up to 8192 tokens, 32 / 8 heads of
+// 128, 135 us with the joining launch (5.15 TB/s of codes and exponents), heads
+// of 64 78 us, heads of 256 (16 / 8) 248 us (5.6 TB/s); one sequence of 127
+// tokens 5.3 us, a chain of latencies: lengths, page table, keys, the waves'
+// join.  A wave takes KT keys at a time straight into registers, the next KT in
+// flight; nothing of K or V passes through LDS.  The four waves of a workgroup
+// take turns over its run of keys and are joined at its end.
 template <int D>
 struct FewShape {
   static constexpr int KT = 32;                  // keys of a wave's step
@@ -673,7 +680,7 @@ TCFP_DEV bool find(const Attend& a, int tile_rows, FindLds& lds, Pick pick, Foun
 }
 
 template <int D, int NT>
-__global__ __launch_bounds__(256, D == 256 && NT == 2 ? 1 : 2) void attend_few_kernel(Attend a) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Attend a) {
   using S = FewShape<D>;
   constexpr int RT = 16 * NT;
   __shared__ int pages[kSegKeys / 16];
@@ -873,8 +880,10 @@ TCFP_DEV bool place(const Attend& a, int& tile, int& split, int& kvh, int& b) {
 
 // ---- many rows: prompts ------------------------------------------------------
 //
-// Bound by the matrix and vector units together.  A workgroup's four waves
-// hold 32 rows each; per 64 keys K goes to LDS as codes and V as bf16,
+// Bound by the matrix and vector units together and by what passes between
+// them: with the exponentials taken out a 2048-token chunk over 14336 tokens
+// (32 / 8 heads of 128) goes from 553 us to 485, without its second product to
+// 532, without moving keys to 414.  A workgroup's four waves hold 32 rows each; per 64 keys K goes to LDS as codes and V as bf16,
 // transposed and in the order of keys that P has in its registers (both
 // buffered twice, the next 64 keys loaded into registers meanwhile), so every
 // operand is read with 16-byte LDS reads.  16-byte chunks of a line are
@@ -1171,7 +1180,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
 
 // ---- many rows, eight waves --------------------------------------------------
 //
-// As above with 256 rows a workgroup, so that each key is fetched, converted
+// As above (the same chunk: 493 us, 1046 TFLOP/s counting 4 flops a visible
+// key, head and column, where a bf16 product of the library reaches 1245; heads
+// of 64 317 us) with 256 rows a workgroup, so that each key is fetched, converted
 // and written to LDS for twice the rows, and 128 keys between two barriers, so
 // that the two waves of a SIMD drift apart and one's products run beside the
 // other's softmax.  The codes of K need no work: each wave copies the 8 or 16
@@ -1350,6 +1361,7 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
           const uint8_t* buf = lds + cur * S::BUF + u * S::KB;
           const uint8_t* vb = lds + cur * S::BUF + 2 * S::KB + u * S::VB;
           const uint8_t* sb = lds + cur * S::BUF + 2 * (S::KB + S::VB) + u * kManyKeys;
+          // (a wave at its products goes first: 498 -> 493 us)
           __builtin_amdgcn_s_setprio(1);
           v16f s[2];
 #pragma unroll
@@ -1594,11 +1606,13 @@ Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
   if (p.few_tiles) {
     p.tile_rows = 16 * p.few_tiles;
     p.tiles = 1;
-    // two workgroups a CU (one of the widest), fewer where there is less to do
+    // two workgroups a CU, one for heads of 256, which need twice the registers
+    // (64 sequences of up to 8192 tokens, 16 / 8 heads of 256: 449 us with spills
+    // at two, 248 us at one), fewer where there is less to do
     const int64_t items = batch * kv_heads;
     p.whole = keys <= 2 * kUnit;
     const int64_t units = p.whole ? items : items * ((keys + kUnit - 1) / kUnit + 1);
-    p.workers = int(std::min<int64_t>(units, dim == 256 && p.few_tiles == 2 ? 256 : 512));
+    p.workers = int(std::min<int64_t>(units, dim == 256 ? 256 : 512));
     p.splits = p.whole ? 1 : 2;
     return p;
   }

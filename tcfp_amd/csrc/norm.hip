@@ -134,7 +134,8 @@ __global__ __launch_bounds__(kThreads) void norm_any_kernel(Norm a) {
 // lanes.  One row for each T threads of the launch: thousands of small
 // workgroups keep more loads in flight than few that walk rows with the next
 // row prefetched (8192 x 4096 bf16 + residual: 47.6 us against 51 / 60 / 63 at
-// 2 / 8 / 16 rows a workgroup).
+// 2 / 8 / 16 rows a workgroup).  Now 47.0 us there (5.0 TB/s), 161 us at 65536 x
+// 2048 (5.8 TB/s), 2.8 us for a single row of 4096 (a launch and two latencies).
 // (NT: with the non-temporal hint)
 template <bool NT>
 TCFP_DEV uint4 load16(const void* p) {
@@ -325,8 +326,7 @@ __global__ __launch_bounds__(wg_of(T)) void norm_rows_kernel(Norm a) {
     }
   }
   if constexpr (QUANT) {
-    // the scales, gathered: written by whole waves (47.6 us against 52.9 at
-    // 8192 x 4096 where the lanes that found them write them)
+    // the scales, gathered, so that whole waves write them
     __syncthreads();
     const int64_t row0 = int64_t(blockIdx.x) * G;
     for (int i = threadIdx.x; i < int(a.cols / a.block) * G; i += wg_of(T)) {
@@ -382,6 +382,7 @@ template <typename XT, typename RT, bool QUANT>
 int norm_rows_launch(const Norm& a, RowShape s, hipStream_t st) {
   const int g = wg_of(s.t) / s.t;
   const unsigned blocks = unsigned((a.rows + g - 1) / g);
+  if (!grid_x_fits(blocks, wg_of(s.t))) return TCFP_ERR_SHAPE;
   const int64_t in = a.rows * a.cols * (size_of(a.x_dtype) + (a.r ? size_of(a.r_dtype) : 0));
 #define TCFP_NR(T, C) norm_rows_kernel<XT, RT, QUANT, false, T, C><<<blocks, wg_of(T), 0, st>>>(a)
 #define TCFP_NR_NT(T, C) norm_rows_kernel<XT, RT, QUANT, true, T, C><<<blocks, wg_of(T), 0, st>>>(a)
@@ -438,10 +439,13 @@ __global__ __launch_bounds__(kThreads) void norm_dw_any_kernel(NormBack a, int64
 
 // ---- the backward with rows in registers -------------------------------------
 //
-// Bound by HBM like the forward.  Workgroups take every gridDim.x-th group of
-// rows, the next rows' loads in flight; a thread's columns are the same in all
-// its rows, so it sums its share of dw in registers, the workgroup leaves one
-// partial row and a second launch adds the partials.
+// Bound by HBM like the forward (8192 x 4096 bf16 with the residual's gradient:
+// 53 us with the joining launch, 5.1 TB/s; 65536 x 2048 5.8 TB/s), at a thousand
+// rows by latency (1000 x 1056 fp32 8.5 us: two launches of 5.4 and 2.7).
+// Workgroups take every gridDim.x-th group of rows, the next rows' loads in
+// flight; a thread's columns are the same in all its rows, so it sums its share
+// of dw in registers, the workgroup leaves one partial row and a second launch
+// adds the partials, in an order that the sizes fix.
 template <typename GT, typename HT, bool NT, int T, int C>
 __global__ __launch_bounds__(wg_of(T)) void norm_back_rows_kernel(NormBack a) {
   constexpr int G = wg_of(T) / T;
@@ -604,7 +608,6 @@ int norm_checks(const Norm& a, bool quantised) {
   if (!dtype_ok(a.x_dtype) || !dtype_ok(a.w_dtype) || (a.r && !dtype_ok(a.r_dtype)))
     return TCFP_ERR_DTYPE;
   if (a.h && !a.r) return TCFP_ERR_SHAPE;
-  if (!grid_x_fits(a.rows, 1024)) return TCFP_ERR_SHAPE;
   if (quantised) {
     if (a.block != 32 && a.block != 64 && a.block != 128) return TCFP_ERR_SHAPE;
     if (a.cols % a.block != 0) return TCFP_ERR_SHAPE;
@@ -633,6 +636,7 @@ int norm_launch(const Norm& a, hipStream_t st) {
     return rb ? norm_rows_launch<float, uint16_t, QUANT>(a, s, st)
               : norm_rows_launch<float, float, QUANT>(a, s, st);
   }
+  if (!grid_x_fits(a.rows, kThreads)) return TCFP_ERR_SHAPE;
   norm_any_kernel<QUANT><<<unsigned(a.rows), kThreads, 0, st>>>(a);
   return launch_status();
 }
@@ -669,7 +673,6 @@ int tcfp_rms_norm_backward(const void* grad_y, int gy_dtype, const void* h, int 
                            const void* grad_h, int64_t rows, int64_t cols, void* dx, float* dw,
                            void* workspace, size_t workspace_bytes, void* stream) {
   if (rows < 0 || cols < 0 || rows > INT32_MAX || cols > INT32_MAX) return TCFP_ERR_SHAPE;
-  if (!grid_x_fits(rows, kThreads)) return TCFP_ERR_SHAPE;
   if (!dtype_ok(gy_dtype) || !dtype_ok(h_dtype) || !dtype_ok(w_dtype)) return TCFP_ERR_DTYPE;
   if (cols == 0 || (rows == 0 && !dw)) return TCFP_OK;
   const auto st = static_cast<hipStream_t>(stream);
@@ -700,6 +703,7 @@ int tcfp_rms_norm_backward(const void* grad_y, int gy_dtype, const void* h, int 
       else TCFP_NB_TYPES(false);
 #undef TCFP_NB_TYPES
     } else {
+      if (!grid_x_fits(rows, kThreads)) return TCFP_ERR_SHAPE;
       norm_dx_any_kernel<<<unsigned(rows), kThreads, 0, st>>>(a);
       if (dw)
         norm_dw_any_kernel<<<dim3(unsigned((cols + kThreads - 1) / kThreads), unsigned(parts)),
