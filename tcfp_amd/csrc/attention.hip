@@ -863,8 +863,10 @@ TCFP_DEV bool place(const Attend& a, int& tile, int& split, int& kvh, int& b) {
   uint32_t set, t;
   if (a.sets >= 8) {
     const uint32_t nth = blockIdx.x / 8, sets = (uint32_t(a.sets) + 7) / 8;
-    set = (a.tiles_first ? nth % sets : nth / tiles) * 8 + blockIdx.x % 8;
     t = a.tiles_first ? nth / sets : nth % tiles;
+    // (in turn, from another one each time: an XCD deals its workgroups over its
+    // four shader engines in turn too, and a long sequence would keep to one)
+    set = (a.tiles_first ? (nth + t) % sets : nth / tiles) * 8 + blockIdx.x % 8;
   } else {
     set = blockIdx.x / tiles;
     t = blockIdx.x % tiles;
@@ -1627,7 +1629,7 @@ Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
   // prompt (one of 2048 tokens, 32 / 8 heads of 128: 66.6 us against 76.2; four
   // of up to 500: 25.7 against 29.6; 2048 over 14336: 553 against 493).
   p.wide = dim <= 128 && most > kWideRows &&
-           (keys >= 2 * max_query_len || workgroups(kWideRows) >= 1024);
+           (keys >= 2 * max_query_len || workgroups(kWideRows) >= 512);
   p.tile_rows = p.wide ? kWideRows : kManyRows;
   p.tiles = int((most + p.tile_rows - 1) / p.tile_rows);
   // split where a CU in two or more would have nothing to do, into runs of at
