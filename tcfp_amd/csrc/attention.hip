@@ -885,11 +885,12 @@ TCFP_DEV bool place(const Attend& a, int& tile, int& split, int& kvh, int& b) {
 // Bound by the matrix and vector units together and by what passes between
 // them: with the exponentials taken out a 2048-token chunk over 14336 tokens
 // (32 / 8 heads of 128) goes from 553 us to 485, without its second product to
-// 532, without moving keys to 414.  A workgroup's four waves hold 32 rows each; per 64 keys K goes to LDS as codes and V as bf16,
-// transposed and in the order of keys that P has in its registers (both
-// buffered twice, the next 64 keys loaded into registers meanwhile), so every
-// operand is read with 16-byte LDS reads.  16-byte chunks of a line are
-// permuted by the row, which spreads eight rows' reads over the banks.
+// 532, without moving keys to 414.  A workgroup's four waves hold 32 rows each;
+// per 64 keys K goes to LDS as codes and V as bf16, transposed and in the order
+// of keys that P has in its registers (both buffered twice, the next 64 keys
+// loaded into registers meanwhile), so every operand is read with 16-byte LDS
+// reads.  16-byte chunks of a line are permuted by the row, which spreads eight
+// rows' reads over the banks.
 constexpr int kManyRows = 128, kManyKeys = 64;
 
 template <int D>
@@ -1632,13 +1633,22 @@ Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
            (keys >= 2 * max_query_len || workgroups(kWideRows) >= 512);
   p.tile_rows = p.wide ? kWideRows : kManyRows;
   p.tiles = int((most + p.tile_rows - 1) / p.tile_rows);
-  // split where a CU in two or more would have nothing to do, into runs of at
-  // least 256 keys: writing and joining the parts costs about as much (four
-  // prompts of up to 500 tokens, 187 workgroups: 59.6 us in two runs, 29.6 whole)
-  const int64_t want = p.wide ? 256 : 512;
-  const int64_t splits = std::clamp<int64_t>(want / workgroups(p.tile_rows), 1, kMaxSplits);
-  const int64_t per = (keys + splits - 1) / splits;
-  p.chunk = int(std::max<int64_t>((per + 255) / 256 * 256, 256));
+  // Splits of the keys, as many as there is room for at most, by what they are
+  // about to take: a workgroup's pass over its keys, 0.21 ns a key and column (64
+  // keys of 64, 128 and 256 columns: 1.1, 1.75 and 3.6 us); writing and joining
+  // the parts, 3 TB/s; another launch, 5 us.  (A causal prompt of 1000 tokens, 32
+  // / 8 heads of 128: 36.3 us whole, 47.8 in two; 64 tokens over 4000: 105 whole,
+  // 28.7 in 12 runs, 34.8 in 32; 512 over 4096, 8 / 2 heads of 256: 61.7 in 8 runs,
+  // which fill the card once, 79.0 in 16.)
+  const int64_t room = (p.wide || dim == 256 ? 256 : 512) / workgroups(p.tile_rows);
+  const double pass = 0.21 * double(keys) * dim, part = double(tokens) * heads * dim * 8 / 3000;
+  int64_t splits = 1;
+  double least = pass;
+  for (int64_t n = 2; n <= std::min<int64_t>(room, kMaxSplits); ++n) {
+    const double t = pass / double(n) + part * double(n) + 5000;
+    if (t < least) least = t, splits = n;
+  }
+  p.chunk = int(((keys + splits - 1) / splits + 127) / 128 * 128);
   p.splits = int(std::clamp<int64_t>((keys + p.chunk - 1) / p.chunk, 1, kMaxSplits));
   return p;
 }
