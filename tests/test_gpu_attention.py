@@ -268,6 +268,29 @@ def test_long_sequences(dev):
         b.check(b.attend(window=7000), window=7000)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads", [(3, 3), (6, 2), (16, 2)])
+@pytest.mark.parametrize("window", [0, 900])
+def test_prompts_whose_keys_are_split(dev, dim, heads, kv_heads, window):
+    """Long contexts in front of few tiles of rows, beside sequences that do
+    not reach the second run of keys and rows that a hole leaves with none of
+    a run."""
+    lens = [(90, 6000), (40, 40), (1, 3000), (57, 4097)]
+    print(f"[attend] split {dim} {heads} {kv_heads} {window}", flush=True)
+    b = Batch(dev, lens, heads, kv_heads, dim, 32, seed=18)
+    b.check(b.attend(window=window), window=window)
+    b.check(b.attend(causal=False, window=window), False, window)
+    b.table[0, 10:160] = -1  # keys 320 ... 5119
+    got = b.attend(window=window)
+    k, v = _values(b.pool)
+    seen = _mask(90, 6000, True, window, dev)
+    seen[:, 320:5120] = False
+    group = heads // kv_heads
+    for h in range(heads):
+        kh, vh = (t[b.slots[0], h // group] for t in (k, v))
+        _check(got[:90, h], b.q[:90, h], kh, vh, seen, dim**-0.5)
+
+
 @pytest.mark.parametrize("page", [16, 32, 128, 256, 1024])
 def test_page_sizes(dev, page):
     b = Batch(dev, [(1, 5), (1, 700), (1, 1500)], 8, 2, 64, page, seed=3)
