@@ -258,6 +258,18 @@ def test_many_sequences(dev, sequences):
     b.check(b.attend())
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(6, 2), (5, 1), (8, 8)])
+@pytest.mark.parametrize("sequences", [60, 250])
+def test_many_rows_of_split_items(dev, heads, kv_heads, sequences):
+    """So many rows that one wave each joins their parts, in numbers of heads
+    that fill its workgroups and that do not."""
+    print(f"[attend] {sequences} x {heads}", flush=True)
+    new = 4 if sequences == 60 else 1
+    lens = [(new if b % 9 else 0, 300 + (b * 53) % 700) for b in range(sequences)]
+    b = Batch(dev, lens, heads, kv_heads, 128, 16, seed=19)
+    b.check(b.attend())
+
+
 def test_long_sequences(dev):
     """Keys cut into more runs than the card has places for, and a window."""
     for lens, heads in (([(1, 40000)], 4), ([(2, 30000), (1, 5), (1, 9000)], 8),
