@@ -680,8 +680,9 @@ int tcfp_rms_norm_backward(const void* grad_y, int gy_dtype, const void* h, int 
 
 /* A paged K/V cache holds, for K and for V, E4M3 codes
  * [num_pages, kv_heads, page_size, dim] and one power-of-two exponent per
-XX: page * page_size + place in the page.  dim 64, 128 or 256; page_size a
- * power of two from 16 to 1024; codes 16-byte aligned.
+ * token and head, exps [num_pages, kv_heads, page_size]: value = code * 2^exp.
+ * A slot is page * page_size + place in the page.  dim 64, 128 or 256;
+ * page_size a power of two from 16 to 1024; codes 16-byte aligned.
  *
  * Write: k, v [tokens, kv_heads, dim] (f32 or bf16, dim contiguous, token and
  * head strides in elements, 16-byte aligned rows) quantised into the places

@@ -59,8 +59,8 @@ def kv_cache_read(
     out_dtype: torch.dtype = torch.bfloat16,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """``(k, v)`` [tokens, kv_heads, dim] of the cache's ``slots`` (int64), in
-    fp32 or bf16 (both hold a cached value exactly); zeros where a slot is
-    outside the pool."""
+    fp32 or bf16 (both hold a cached value exactly, bf16 but for values under
+    its smallest); zeros where a slot is outside the pool."""
     return _hip.host().kv_cache_read(k_codes, v_codes, k_exps, v_exps, slots, out_dtype)
 
 
