@@ -1191,6 +1191,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
 // other's softmax.  The codes of K need no work: each wave copies the 8 or 16
 // rows it stages straight into LDS.  Keys staged by a wave lie in one page, so
 // their addresses are the wave's own.
+//
+// KS == 2: 128 rows a workgroup; of the 128 keys each wave takes 64, four waves
+// the even steps and four the odd ones, and the two sums of a row are joined
+// through LDS at the end.  A wave alone on its SIMD takes 1.05 us a step (heads of
+// 64), products and softmax in turn: a prompt of few tiles is as slow as its
+// longest chain of steps, which this halves.
 constexpr int kWideRows = 256;
 
 template <int D>
@@ -1218,9 +1224,10 @@ struct WideLoad {
   int page;
 };
 
-template <int D>
+template <int D, int KS>
 __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
   using S = WideShape<D>;
+  constexpr int RT = kWideRows / KS;
   __shared__ uint4 lds4[2 * S::BUF / 16];
   uint8_t* const lds = reinterpret_cast<uint8_t*>(lds4);
   const uint32_t lds_at =
@@ -1233,6 +1240,7 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
   if (split == 0 && tile == 0)
     zero_rest(a, b == 0 ? seq.start : 0,
               b == a.batch - 1 ? seq.start + seq.new_tokens : a.tokens, kvh * a.group, a.group, D);
+  const int mine = wave % (8 / KS);  // the wave's 32 rows of the tile
   const int32_t* table = a.table + int64_t(b) * a.table_stride;
   // The wave stages keys 16 k16 + ... of a step: of K the rows kwave ... of
   // those 16, 16 bytes a lane (the chunk that belongs at the lane's place), of
@@ -1250,22 +1258,22 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
                                       : 0xFFFFull << (16 * x4);
   const int voff = (kg & 3) * 4 * D + dg * 4;
   const int vchunk = (kg >> 2) * 2 + (kg & 1), sub = ((kg >> 1) & 1) * 8;
-  for (int r0 = tile * kWideRows; r0 < seq.rows; r0 += a.tiles * kWideRows) {
-    const Keys keys = keys_of(a, seq, r0, kWideRows);
+  for (int r0 = tile * RT; r0 < seq.rows; r0 += a.tiles * RT) {
+    const Keys keys = keys_of(a, seq, r0, RT);
     if (split >= max(keys.live, 1)) continue;
     const int k0 = keys.begin + split * a.chunk;
     const int k1 = split == a.splits - 1 ? keys.end : min(keys.end, k0 + a.chunk);
-    const int last = min(r0 + kWideRows, seq.rows) - 1;
-    const int row = min(r0 + 32 * wave + col, last), tok = row / a.group,
+    const int last = min(r0 + RT, seq.rows) - 1;
+    const int row = min(r0 + 32 * mine + col, last), tok = row / a.group,
               head = row - tok * a.group;
     const int lo = key_lo(a, seq, tok), hi = key_hi(a, seq, tok);
-    const int wfirst = min(r0 + 32 * wave, last) / a.group,
-              wlast = min(r0 + 32 * wave + 31, last) / a.group;
+    const int wfirst = min(r0 + 32 * mine, last) / a.group,
+              wlast = min(r0 + 32 * mine + 31, last) / a.group;
     const int all_lo = key_lo(a, seq, r0 / a.group), all_lo_max = key_lo(a, seq, last / a.group),
               all_hi_min = key_hi(a, seq, r0 / a.group);
     const int w_lo = key_lo(a, seq, wfirst), w_lo_max = key_lo(a, seq, wlast),
               w_hi_min = key_hi(a, seq, wfirst), w_hi = key_hi(a, seq, wlast);
-    const bool idle = r0 + 32 * wave > last;
+    const bool idle = r0 + 32 * mine > last;
     v8i qhi[S::DS], qlo[S::DS];
     const int qe = split_q<S::DS, 2, 16>(a.q + int64_t(seq.start + tok) * a.q_token +
                                          int64_t(kvh * a.group + head) * a.q_head + half * 32,
@@ -1358,7 +1366,7 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
         __syncthreads();  // this buffer is written, the other one read
         if (more) fetch(key0 + 2 * kManyKeys, lds_at + uint32_t((cur ^ 1) * S::BUF));
 #pragma unroll 1
-        for (int u = 0; u < 2; ++u) {
+        for (int u = wave / (8 / KS); u < 2; u += KS) {
           const int key = key0 + u * kManyKeys;
           if (idle || key >= w_hi || key + kManyKeys <= w_lo || key >= k1) continue;
           const uint8_t* buf = lds + cur * S::BUF + u * S::KB;
@@ -1442,9 +1450,32 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
         if (more) settle(key0 + 2 * kManyKeys, lds + cur * S::BUF);
       }
       __syncthreads();  // (the next tile writes the buffers again)
+      if constexpr (KS == 2) {
+        // the rows' sums over the odd steps, from the upper waves to the lower
+        constexpr int N = 16 * S::DT;
+        static_assert(4 * (N + 2) * 64 * 4 <= 2 * S::BUF, "the sums fit where the keys were");
+        float* const x = reinterpret_cast<float*>(lds) + mine * (N + 2) * 64 + lane;
+        if (wave >= 4) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) x[64 * i] = o[i / 16][i % 16];
+          x[64 * N] = m;
+          x[64 * N + 64] = l;
+        }
+        __syncthreads();
+        if (wave < 4) {
+          const float om = x[64 * N], top = fmaxf(m, om);
+          const float f = m == top ? 1.0f : exp2_fast((m - top) * a.c);
+          const float g = om == top ? 1.0f : exp2_fast((om - top) * a.c);
+          m = top;
+          l = l * f + x[64 * N + 64] * g;
+#pragma unroll
+          for (int i = 0; i < N; ++i) o[i / 16][i % 16] = o[i / 16][i % 16] * f + x[64 * i] * g;
+        }
+        __syncthreads();
+      }
     }
     l += other_half(l);
-    if (r0 + 32 * wave + col <= last) {
+    if (wave < 8 / KS && r0 + 32 * mine + col <= last) {
       const int64_t at = int64_t(seq.start + tok) * a.heads + kvh * a.group + head;
       if (keys.live <= 1) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1604,6 +1635,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(Attend a, int tile_row
 struct Launch {
   int few_tiles;  // 16-row tiles a workgroup of the few-rows kernel takes; 0: many rows
   bool wide;      // 256 rows a workgroup
+  bool paired;    // 128 rows of eight waves
   int tile_rows, tiles, splits, chunk;
   int workers;    // few rows: workgroups
   bool whole;     // few rows: one workgroup an item
@@ -1641,6 +1673,14 @@ Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
   // of up to 500: 25.7 against 29.6; 2048 over 14336: 553 against 493).
   p.wide = dim <= 128 && most > kWideRows &&
            (keys >= 2 * max_query_len || workgroups(kWideRows) >= 512);
+  // Eight waves on 128 rows, which halves the chain of a tile's steps, where
+  // there are tiles for a good part of the CUs and for no CU two, and the longest
+  // is not short (one prompt of 1000 tokens, 16 heads of 64: 24.7 -> 19.7 us; of
+  // 2048, 8 / 2 heads of 128: 47.1 -> 38.7; six of up to 1000, 16 heads of 64, 480
+  // tiles: 32.8 against 40.0; 600 over 300, 4 heads of 128, 20 tiles: 21.3 against
+  // 23.1, as fewer runs fill the card; 256, 32 / 8 heads of 128: 14.8 against 15.7).
+  const int64_t tiles = workgroups(kManyRows);
+  p.paired = !p.wide && dim <= 128 && keys >= 512 && tiles > 64 && tiles <= 256;
   p.tile_rows = p.wide ? kWideRows : kManyRows;
   p.tiles = int((most + p.tile_rows - 1) / p.tile_rows);
   // Splits of the keys, as many as there is room for at most, by what they are
@@ -1650,7 +1690,7 @@ Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
   // / 8 heads of 128: 36.3 us whole, 47.8 in two; 64 tokens over 4000: 105 whole,
   // 28.7 in 12 runs, 34.8 in 32; 512 over 4096, 8 / 2 heads of 256: 61.7 in 8 runs,
   // which fill the card once, 79.0 in 16.)
-  const int64_t room = (p.wide || dim == 256 ? 256 : 512) / workgroups(p.tile_rows);
+  const int64_t room = (p.wide || p.paired || dim == 256 ? 256 : 512) / workgroups(p.tile_rows);
   const double pass = 0.21 * double(keys) * dim, part = double(tokens) * heads * dim * 8 / 3000;
   int64_t splits = 1;
   double least = pass;
@@ -1834,8 +1874,10 @@ int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     a.tiles_first = (sets + 7) / 8 * std::min<int64_t>(p.chunk, max_seq_len) * dim * 2 <= 2 << 20;
     if (wgs > INT32_MAX || !grid_x_fits(wgs, 512)) return TCFP_ERR_SHAPE;
 #define TCFP_MANY(D) attend_many_kernel<D><<<unsigned(wgs), 256, 0, st>>>(a)
-    if (p.wide && dim == 64) attend_wide_kernel<64><<<unsigned(wgs), 512, 0, st>>>(a);
-    else if (p.wide) attend_wide_kernel<128><<<unsigned(wgs), 512, 0, st>>>(a);
+    if (p.wide && dim == 64) attend_wide_kernel<64, 1><<<unsigned(wgs), 512, 0, st>>>(a);
+    else if (p.wide) attend_wide_kernel<128, 1><<<unsigned(wgs), 512, 0, st>>>(a);
+    else if (p.paired && dim == 64) attend_wide_kernel<64, 2><<<unsigned(wgs), 512, 0, st>>>(a);
+    else if (p.paired) attend_wide_kernel<128, 2><<<unsigned(wgs), 512, 0, st>>>(a);
     else TCFP_BY_DIM(TCFP_MANY);
 #undef TCFP_MANY
   }

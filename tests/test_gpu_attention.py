@@ -303,6 +303,50 @@ def test_prompts_whose_keys_are_split(dev, dim, heads, kv_heads, window):
         _check(got[:90, h], b.q[:90, h], kh, vh, seen, dim**-0.5)
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("lens,heads,kv_heads", [([(1100, 1100)], 8, 8), ([(900, 1000)], 32, 8),
+                                                 ([(700, 700), (0, 30), (1, 40), (511, 513)], 9, 9)])
+def test_long_prompts_of_few_tiles(dev, dim, page, lens, heads, kv_heads):
+    """Tiles whose steps two groups of waves share, with a window, a hole and
+    keys that only one of the groups sees."""
+    print(f"[attend] {lens} {heads} {kv_heads} {dim}", flush=True)
+    b = Batch(dev, lens, heads, kv_heads, dim, page, seed=20)
+    b.check(b.attend())
+    for window in (1, 65, 600):
+        b.check(b.attend(window=window), window=window)
+    b.check(b.attend(causal=False), False)
+    n, total = lens[0]
+    hole = slice(64 // page, 448 // page)
+    b.table[0, hole] = -1
+    got = b.attend()
+    k, v = _values(b.pool)
+    seen = _mask(n, total, True, 0, dev)
+    seen[:, 64:448] = False
+    for h in range(heads):
+        kh, vh = (t[b.slots[0], h // (heads // kv_heads)] for t in (k, v))
+        _check(got[:n, h], b.q[:n, h], kh, vh, seen, dim**-0.5)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_nan_in_long_prompts_of_few_tiles(dev, dim):
+    """A NaN of a cached key or value reaches the rows and heads that see it
+    and no other."""
+    n, page = 700, 16
+    b = Batch(dev, [(n, n)], 24, 12, dim, page, seed=21)
+    want = b.attend()
+    b.check(want)
+    for which in (0, 1):
+        for at in (650, 130, 3):
+            codes = b.pool[which].view(torch.uint8)
+            slot = int(b.slots[0][at])
+            keep = codes[slot // page, :, slot % page].clone()
+            codes[slot // page, 0, slot % page, 7] = 0x7F
+            got = b.attend()
+            codes[slot // page, :, slot % page] = keep
+            assert torch.equal(got[:at], want[:at]) and torch.equal(got[:, 2:], want[:, 2:])
+            assert got[at:, :2, 7].float().isnan().all()
+
+
 @pytest.mark.parametrize("page", [16, 32, 128, 256, 1024])
 def test_page_sizes(dev, page):
     b = Batch(dev, [(1, 5), (1, 700), (1, 1500)], 8, 2, 64, page, seed=3)
