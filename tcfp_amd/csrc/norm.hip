@@ -378,6 +378,18 @@ constexpr int64_t kStreamBytes = 96ll << 20;
     else CALL(1024, 2);                              \
   } while (0)
 
+// Those that inputs past kStreamBytes come in: a vector a thread only where rows
+// are short (of 1023 rows at most, 8192 wide at most, none is that large).
+#define TCFP_ROWS_STREAM(CALL, WIDEST)               \
+  do {                                               \
+    if (s.t == 64 && s.c == 1) CALL(64, 1);          \
+    else if (s.t == 64) CALL(64, 2);                 \
+    else if (s.t == 128) CALL(128, 2);               \
+    else if (s.t == 256) CALL(256, 2);               \
+    else if (s.t == 512 && s.c == 2) CALL(512, 2);   \
+    else WIDEST;                                     \
+  } while (0)
+
 template <typename XT, typename RT, bool QUANT>
 int norm_rows_launch(const Norm& a, RowShape s, hipStream_t st) {
   const int g = wg_of(s.t) / s.t;
@@ -386,7 +398,7 @@ int norm_rows_launch(const Norm& a, RowShape s, hipStream_t st) {
   const int64_t in = a.rows * a.cols * (size_of(a.x_dtype) + (a.r ? size_of(a.r_dtype) : 0));
 #define TCFP_NR(T, C) norm_rows_kernel<XT, RT, QUANT, false, T, C><<<blocks, wg_of(T), 0, st>>>(a)
 #define TCFP_NR_NT(T, C) norm_rows_kernel<XT, RT, QUANT, true, T, C><<<blocks, wg_of(T), 0, st>>>(a)
-  if (in > kStreamBytes) TCFP_ROWS(TCFP_NR_NT);
+  if (in > kStreamBytes) TCFP_ROWS_STREAM(TCFP_NR_NT, TCFP_NR_NT(1024, 2));
   else TCFP_ROWS(TCFP_NR);
 #undef TCFP_NR_NT
 #undef TCFP_NR
@@ -562,7 +574,8 @@ template <typename GT, typename HT, bool NT>
 void norm_back_launch(const NormBack& a, RowShape s, unsigned blocks, hipStream_t st) {
 #define TCFP_NB(T, C) norm_back_rows_kernel<GT, HT, NT, T, C><<<blocks, wg_of(T), 0, st>>>(a)
 #define TCFP_NB_SMALL(T, C) TCFP_NB(T, (T) == 1024 ? 1 : (C))
-  if (s.c == 4) TCFP_NB(512, 4);
+  if constexpr (NT) TCFP_ROWS_STREAM(TCFP_NB, TCFP_NB(512, 4));
+  else if (s.c == 4) TCFP_NB(512, 4);
   else TCFP_ROWS(TCFP_NB_SMALL);
 #undef TCFP_NB_SMALL
 #undef TCFP_NB

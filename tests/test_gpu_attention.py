@@ -270,6 +270,16 @@ def test_many_rows_of_split_items(dev, heads, kv_heads, sequences):
     b.check(b.attend())
 
 
+def test_heads_of_256_in_few_and_many_rows(dev):
+    """More than 16 rows of an item, and more than 1024 rows of split items."""
+    for lens, heads, kv_heads in (([(1, 700), (1, 3), (1, 2050)], 24, 1), ([(5, 900)], 20, 4),
+                                  ([(2, 600 + 7 * i) for i in range(70)], 8, 2)):
+        print(f"[attend] 256 {len(lens)} {heads} {kv_heads}", flush=True)
+        b = Batch(dev, lens, heads, kv_heads, 256, 16, seed=22)
+        b.check(b.attend())
+        b.check(b.attend(window=100), window=100)
+
+
 def test_long_sequences(dev):
     """Keys cut into more runs than the card has places for, and a window."""
     for lens, heads in (([(1, 40000)], 4), ([(2, 30000), (1, 5), (1, 9000)], 8),

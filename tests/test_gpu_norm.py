@@ -170,6 +170,73 @@ def test_backward(dev, m, d, ht, gt, add):
     assert none is None and torch.equal(dx2, dx)
 
 
+# Widths of every number of threads a row may have, two vectors a thread (one at
+# 512), in more than 1024 rows: so few that the input may be cached, and so many
+# that it is read past the caches.
+WIDE = [512, 1024, 1056, 2080, 4096, 8192, 16384]
+
+
+def _large(dev, d, many, bytes_each, seed):
+    m = (100 << 20) // (d * bytes_each) + 7 if many else 1100
+    g = torch.Generator(dev).manual_seed(seed)
+    return m, lambda dt: torch.randn(m, d, generator=g, device=dev).to(dt)
+
+
+@pytest.mark.parametrize("d", WIDE)
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("xt,rt", [(F32, None), (BF16, None), (F32, F32), (BF16, BF16),
+                                   (F32, BF16), (BF16, F32)])
+def test_many_rows(dev, d, many, xt, rt):
+    each = sum({F32: 4, BF16: 2}[t] for t in (xt, rt) if t is not None)
+    m, rand = _large(dev, d, many, each, 7)
+    print(f"[norm] {m} x {d} {xt} {rt}", flush=True)
+    x, r = rand(xt), None if rt is None else rand(rt)
+    w = 1 + 0.1 * torch.randn(d, device=dev)
+    y, h, rs = norm.rms_norm(x, w, r, eps=EPS, out_dtype=F32)
+    _, rstd, exact = _exact(x, r, w)
+    assert ((rs.double() - rstd).abs() <= 2e-6 * rstd).all()
+    assert ((y.double() - exact).abs() <= 2e-6 * exact.abs() + 1e-37).all()
+    if r is not None:
+        assert torch.equal(h, (x.float() + r.float()).to(rt))
+    del exact
+    for bs, sf in ((32, "exponent"), (32, "fp32")):
+        q, sc, hq, rq = norm.rms_norm_quantize(x, w, r, eps=EPS, block_size=bs, scale_format=sf)
+        q0, sc0 = K.block_quantize_fp8(y, bs, E4M3, scale_format=sf)
+        assert torch.equal(_bits(q), _bits(q0)) and torch.equal(sc, sc0)
+        assert torch.equal(rq, rs) and torch.equal(hq, h)
+
+
+@pytest.mark.parametrize("m,d", [s for s in SIZES if s[1] % 32 == 0])
+@pytest.mark.parametrize("xt,rt", [(BF16, F32), (F32, F32), (BF16, None)])
+def test_codes_of_other_types(dev, m, d, xt, rt):
+    test_codes_are_the_block_quantisation_of_the_norm(dev, m, d, xt, rt)
+
+
+@pytest.mark.parametrize("d", WIDE)
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("ht,gt", [(F32, F32), (BF16, BF16), (F32, BF16), (BF16, F32)])
+def test_backward_of_many_rows(dev, d, many, ht, gt):
+    size = {F32: 4, BF16: 2}
+    m, rand = _large(dev, d, many, size[gt] + 2 * size[ht], 8)
+    print(f"[norm] backward {m} x {d} {ht} {gt}", flush=True)
+    h, gy, gh = rand(ht), rand(gt), rand(ht)
+    w = 1 + 0.1 * torch.randn(d, device=dev)
+    _, _, rs = norm.rms_norm(h, w, eps=EPS)
+    dx, dw = norm.rms_norm_backward(gy, h, rs, w, gh)
+    rd = rs.double()[:, None]
+    gd, xh = gy.double(), h.double() * rd
+    dwe, mag = (gd * xh).sum(0), (gd * xh).abs().sum(0)
+    # chains of at most 512 additions on the way to a sum of m rows
+    assert ((dw.double() - dwe).abs() <= 512 * 2**-24 * mag + 1e-37).all()
+    gg = gd * w.double()
+    exact = rd * (gg - xh * (gg * xh).mean(1, keepdim=True)) + gh.double()
+    far = rd * (gg.abs() + xh.abs() * (gg * xh).abs().mean(1, keepdim=True)) + gh.double().abs()
+    tol = 4e-6 * far + (2**-8 * exact.abs() if ht == BF16 else 0)
+    assert ((dx.double() - exact).abs() <= tol + 1e-37).all()
+    again = norm.rms_norm_backward(gy, h, rs, w, gh)
+    assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
+
+
 def test_backward_against_differences(dev):
     """Central differences of the formula in 64 bits, step 1e-5: exact to some
     1e-9; the fp32 gradient to 1e-5 of its largest value."""
