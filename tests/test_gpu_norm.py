@@ -206,8 +206,8 @@ def test_many_rows(dev, d, many, xt, rt):
         assert torch.equal(rq, rs) and torch.equal(hq, h)
 
 
-@pytest.mark.parametrize("m,d", [s for s in SIZES if s[1] % 32 == 0])
-@pytest.mark.parametrize("xt,rt", [(BF16, F32), (F32, F32), (BF16, None)])
+@pytest.mark.parametrize("m,d", [*(s for s in SIZES if s[1] % 32 == 0), (40, 1024)])
+@pytest.mark.parametrize("xt,rt", [(BF16, F32), (F32, F32), (BF16, None), (F32, BF16)])
 def test_codes_of_other_types(dev, m, d, xt, rt):
     test_codes_are_the_block_quantisation_of_the_norm(dev, m, d, xt, rt)
 
@@ -235,6 +235,11 @@ def test_backward_of_many_rows(dev, d, many, ht, gt):
     assert ((dx.double() - exact).abs() <= tol + 1e-37).all()
     again = norm.rms_norm_backward(gy, h, rs, w, gh)
     assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
+
+
+def test_backward_of_1030_rows(dev):
+    """Two vectors a thread of 512, from inputs that may be cached."""
+    test_backward(dev, 1030, 5120, F32, F32, True)
 
 
 def test_backward_against_differences(dev):
