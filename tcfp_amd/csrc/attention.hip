@@ -323,7 +323,7 @@ TCFP_DEV void zero_rest(const Attend& a, int lead, int tail, int first, int head
 // ---- few rows: one token a sequence, a few drafts ----------------------------
 //
 // Bound by reading the cache: 64 sequences of up to 8192 tokens, 32 / 8 heads of
-// 128, 135 us with the joining launch (5.15 TB/s of codes and exponents), heads
+// 128, 132 us with the joining launch (5.26 TB/s of codes and exponents), heads
 // of 64 78 us, heads of 256 (16 / 8) 248 us (5.6 TB/s); one sequence of 127
 // tokens 5.3 us, a chain of latencies: lengths, page table, keys, the waves'
 // join.  A wave takes KT keys at a time straight into registers, the next KT in
