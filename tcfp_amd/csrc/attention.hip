@@ -891,6 +891,10 @@ TCFP_DEV bool place(const Attend& a, int& tile, int& split, int& kvh, int& b) {
 // loaded into registers meanwhile), so every operand is read with 16-byte LDS
 // reads.  16-byte chunks of a line are permuted by the row, which spreads eight
 // rows' reads over the banks.
+//
+// KS == 2, for heads of 256: 64 rows a workgroup, two waves with half of a step's
+// keys each, their sums joined at the end.  A step of these heads takes a wave
+// alone on its SIMD 3.3 us; short prompts are as slow as their longest tile.
 constexpr int kManyRows = 128, kManyKeys = 64;
 
 template <int D>
@@ -1005,12 +1009,40 @@ TCFP_DEV float other_half(float x) {
   return (threadIdx.x & 32) ? __uint_as_float(r[0]) : __uint_as_float(r[1]);
 }
 
-template <int D>
+// The rows' sums over the keys of the upper half of a workgroup's waves, of which
+// RW hold a row each, added to those of the lower half, through LDS.
+template <int DT, int RW, int BYTES>
+TCFP_DEV void join_halves(const Attend& a, uint8_t* lds, int wave, int lane, v16f* o, float& m,
+                          float& l) {
+  constexpr int N = 16 * DT;
+  static_assert(RW * (N + 2) * 64 * 4 <= BYTES, "the sums fit where the keys were");
+  float* const x = reinterpret_cast<float*>(lds) + wave % RW * (N + 2) * 64 + lane;
+  if (wave >= RW) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[64 * i] = o[i / 16][i % 16];
+    x[64 * N] = m;
+    x[64 * N + 64] = l;
+  }
+  __syncthreads();
+  if (wave < RW) {
+    const float om = x[64 * N], top = fmaxf(m, om);
+    const float f = m == top ? 1.0f : exp2_fast((m - top) * a.c);
+    const float g = om == top ? 1.0f : exp2_fast((om - top) * a.c);
+    m = top;
+    l = l * f + x[64 * N + 64] * g;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i / 16][i % 16] = o[i / 16][i % 16] * f + x[64 * i] * g;
+  }
+  __syncthreads();
+}
+
+template <int D, int KS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Attend a) {
   using S = ManyShape<D>;
+  constexpr int RT = kManyRows / KS, KT = 2 / KS;  // rows, and a wave's 32-key tiles of a step
   __shared__ uint4 lds4[2 * S::BUF / 16];
   uint8_t* const lds = reinterpret_cast<uint8_t*>(lds4);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = scalar(int(threadIdx.x >> 6)), col = lane & 31, half = lane >> 5;
   int tile, split, kvh, b;
   if (!place(a, tile, split, kvh, b)) return;
   const Seq seq = sequence(a, b);
@@ -1019,23 +1051,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
               b == a.batch - 1 ? seq.start + seq.new_tokens : a.tokens, kvh * a.group, a.group, D);
   const int32_t* table = a.table + int64_t(b) * a.table_stride;
   const int kg = threadIdx.x >> 4;
-  for (int r0 = tile * kManyRows; r0 < seq.rows; r0 += a.tiles * kManyRows) {
-    const Keys keys = keys_of(a, seq, r0, kManyRows);
+  const int mine = wave % (4 / KS), kfirst = KS == 1 ? 0 : wave / 2;
+  for (int r0 = tile * RT; r0 < seq.rows; r0 += a.tiles * RT) {
+    const Keys keys = keys_of(a, seq, r0, RT);
     if (split >= max(keys.live, 1)) continue;
     const int k0 = keys.begin + split * a.chunk;
     const int k1 = split == a.splits - 1 ? keys.end : min(keys.end, k0 + a.chunk);
     // rows of the tile, of the wave and of the lane; rows past the last repeat it
-    const int last = min(r0 + kManyRows, seq.rows) - 1;
-    const int row = min(r0 + 32 * wave + col, last), tok = row / a.group,
+    const int last = min(r0 + RT, seq.rows) - 1;
+    const int row = min(r0 + 32 * mine + col, last), tok = row / a.group,
               head = row - tok * a.group;
     const int lo = key_lo(a, seq, tok), hi = key_hi(a, seq, tok);
-    const int wfirst = min(r0 + 32 * wave, last) / a.group,
-              wlast = min(r0 + 32 * wave + 31, last) / a.group;
+    const int wfirst = min(r0 + 32 * mine, last) / a.group,
+              wlast = min(r0 + 32 * mine + 31, last) / a.group;
     const int all_lo = key_lo(a, seq, r0 / a.group), all_lo_max = key_lo(a, seq, last / a.group),
               all_hi_min = key_hi(a, seq, r0 / a.group);
     const int w_lo = key_lo(a, seq, wfirst), w_lo_max = key_lo(a, seq, wlast),
               w_hi_min = key_hi(a, seq, wfirst), w_hi = key_hi(a, seq, wlast);
-    const bool idle = r0 + 32 * wave > last;
+    const bool idle = r0 + 32 * mine > last;
     v8i qhi[S::DS], qlo[S::DS];
     const int qe = split_q<S::DS, 2, 16>(a.q + int64_t(seq.start + tok) * a.q_token +
                                          int64_t(kvh * a.group + head) * a.q_head + half * 32,
@@ -1074,11 +1107,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
         __syncthreads();  // this step's buffer is written, the other one read
         const uint8_t* buf = lds + cur * S::BUF;
         if (!idle && key < w_hi && key + kManyKeys > w_lo) {
-          float p[2][16];
+          float p[KT][16];
           float top = -INFINITY;
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt) {
-            const int krow = 32 * kt + col;
+          for (int kt = 0; kt < KT; ++kt) {
+            const int krow = 32 * (kfirst + kt) + col;
             const int ks = buf[S::KB + S::VB + krow];
             v16f s = {};
 #pragma unroll
@@ -1097,21 +1130,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
           }
           if (holes || key < w_lo_max || key + kManyKeys > w_hi_min) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
                 const bool gone =
                     holes && *reinterpret_cast<const uint32_t*>(
-                                 buf + S::KB + S::VB + 32 * kt + 8 * g + 4 * half) == 0;
+                                 buf + S::KB + S::VB + 32 * (kfirst + kt) + 8 * g + 4 * half) == 0;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                  const int kk = key + 32 * kt + 8 * g + 4 * half + r;
+                  const int kk = key + 32 * (kfirst + kt) + 8 * g + 4 * half + r;
                   if (gone || kk < lo || kk >= hi) p[kt][4 * g + r] = -INFINITY;
                 }
               }
           }
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt)
+          for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int j = 0; j < 16; ++j) top = fmaxf(top, p[kt][j]);
           top = fmaxf(top, other_half(top));
@@ -1125,21 +1158,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
           }
           const float off = top == -INFINITY ? 0.0f : top * a.c;
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt)
+          for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               p[kt][j] = exp2_fast(__builtin_fmaf(p[kt][j], a.c, -off));
               l += p[kt][j];
             }
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
+          for (int s = 0; s < 2 * KT; ++s) {
             const float* x = p[s >> 1] + 8 * (s & 1);
             const v8bf pf = as_bf(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]),
                                   pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
 #pragma unroll
             for (int i = 0; i < S::DT; ++i) {
               const uint4 w = *reinterpret_cast<const uint4*>(
-                  buf + S::KB + v_at(32 * i + col, 2 * s + half));
+                  buf + S::KB + v_at(32 * i + col, 2 * (2 * kfirst + s) + half));
               o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf(w.x, w.y, w.z, w.w), pf, o[i],
                                                              0, 0, 0);
             }
@@ -1151,9 +1184,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
                         keys.end);
       }
       __syncthreads();  // (the next tile writes the buffers again)
+      if constexpr (KS == 2) join_halves<S::DT, 2, 2 * S::BUF>(a, lds, wave, lane, o, m, l);
     }
     l += other_half(l);
-    if (r0 + 32 * wave + col <= last) {
+    if (wave < 4 / KS && r0 + 32 * mine + col <= last) {
       const int64_t at = int64_t(seq.start + tok) * a.heads + kvh * a.group + head;
       if (keys.live <= 1) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1450,29 +1484,7 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
         if (more) settle(key0 + 2 * kManyKeys, lds + cur * S::BUF);
       }
       __syncthreads();  // (the next tile writes the buffers again)
-      if constexpr (KS == 2) {
-        // the rows' sums over the odd steps, from the upper waves to the lower
-        constexpr int N = 16 * S::DT;
-        static_assert(4 * (N + 2) * 64 * 4 <= 2 * S::BUF, "the sums fit where the keys were");
-        float* const x = reinterpret_cast<float*>(lds) + mine * (N + 2) * 64 + lane;
-        if (wave >= 4) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) x[64 * i] = o[i / 16][i % 16];
-          x[64 * N] = m;
-          x[64 * N + 64] = l;
-        }
-        __syncthreads();
-        if (wave < 4) {
-          const float om = x[64 * N], top = fmaxf(m, om);
-          const float f = m == top ? 1.0f : exp2_fast((m - top) * a.c);
-          const float g = om == top ? 1.0f : exp2_fast((om - top) * a.c);
-          m = top;
-          l = l * f + x[64 * N + 64] * g;
-#pragma unroll
-          for (int i = 0; i < N; ++i) o[i / 16][i % 16] = o[i / 16][i % 16] * f + x[64 * i] * g;
-        }
-        __syncthreads();
-      }
+      if constexpr (KS == 2) join_halves<S::DT, 4, 2 * S::BUF>(a, lds, wave, lane, o, m, l);
     }
     l += other_half(l);
     if (wave < 8 / KS && r0 + 32 * mine + col <= last) {
@@ -1635,7 +1647,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(Attend a, int tile_row
 struct Launch {
   int few_tiles;  // 16-row tiles a workgroup of the few-rows kernel takes; 0: many rows
   bool wide;      // 256 rows a workgroup
-  bool paired;    // 128 rows of eight waves
+  bool paired;    // 128 rows of eight waves, 64 of four for heads of 256
   int tile_rows, tiles, splits, chunk;
   int workers;    // few rows: workgroups
   bool whole;     // few rows: one workgroup an item
@@ -1680,8 +1692,15 @@ Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
   // tiles: 32.8 against 40.0; 600 over 300, 4 heads of 128, 20 tiles: 21.3 against
   // 23.1, as fewer runs fill the card; 256, 32 / 8 heads of 128: 14.8 against 15.7).
   const int64_t tiles = workgroups(kManyRows);
-  p.paired = !p.wide && dim <= 128 && keys >= 512 && tiles > 64 && tiles <= 256;
+  p.paired = !p.wide && keys >= 512 && tiles > 64 && tiles <= 256;
   p.tile_rows = p.wide ? kWideRows : kManyRows;
+  if (dim == 256) {
+    // (64 rows of four waves, each with half of a step's keys; 100 tokens, 8 heads:
+    // 20.7 -> 16.2 us, 777 over 100, 6 / 2 heads: 64.1 -> 53.6; a long context is
+    // better split: 426 over 1218, 3 heads on one: 37.5 against 50.7)
+    p.paired = keys <= 1536 && workgroups(kManyRows / 2) <= 256;
+    if (p.paired) p.tile_rows = kManyRows / 2;
+  }
   p.tiles = int((most + p.tile_rows - 1) / p.tile_rows);
   // Splits of the keys, as many as there is room for at most, by what they are
   // about to take: a workgroup's pass over its keys, 0.21 ns a key and column (64
@@ -1873,11 +1892,12 @@ int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     // (half of an XCD's 4 MiB)
     a.tiles_first = (sets + 7) / 8 * std::min<int64_t>(p.chunk, max_seq_len) * dim * 2 <= 2 << 20;
     if (wgs > INT32_MAX || !grid_x_fits(wgs, 512)) return TCFP_ERR_SHAPE;
-#define TCFP_MANY(D) attend_many_kernel<D><<<unsigned(wgs), 256, 0, st>>>(a)
+#define TCFP_MANY(D) attend_many_kernel<D, 1><<<unsigned(wgs), 256, 0, st>>>(a)
     if (p.wide && dim == 64) attend_wide_kernel<64, 1><<<unsigned(wgs), 512, 0, st>>>(a);
     else if (p.wide) attend_wide_kernel<128, 1><<<unsigned(wgs), 512, 0, st>>>(a);
     else if (p.paired && dim == 64) attend_wide_kernel<64, 2><<<unsigned(wgs), 512, 0, st>>>(a);
-    else if (p.paired) attend_wide_kernel<128, 2><<<unsigned(wgs), 512, 0, st>>>(a);
+    else if (p.paired && dim == 128) attend_wide_kernel<128, 2><<<unsigned(wgs), 512, 0, st>>>(a);
+    else if (p.paired) attend_many_kernel<256, 2><<<unsigned(wgs), 256, 0, st>>>(a);
     else TCFP_BY_DIM(TCFP_MANY);
 #undef TCFP_MANY
   }
