@@ -1248,9 +1248,14 @@ struct WideShape {
 TCFP_DEV int vp_at(int d, int c) { return d * 128 + ((c ^ ((d ^ ((d >> 3) & 3)) & 7)) << 4); }
 
 // 16 bytes from base + off of each lane into LDS at lds + 16 * lane (base and
-// lds the wave's); done when vmcnt has counted it.
+// lds the wave's); done when vmcnt has counted it.  (A copy into LDS needs one
+// wait state behind the instruction that writes m0; the compiler, which sees to
+// that for instructions of its own, does not look into the assembly.)
 TCFP_DEV void copy_to_lds(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(lds) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(base), "{m0}"(lds)
+               : "memory");
 }
 
 struct WideLoad {
