@@ -97,6 +97,8 @@ TCFP_DEV v8i make_frag(uint4 lo, uint4 hi) {
 // does not know these writes do not alias the LDS reads of the other
 // buffer and would otherwise drain all loads before every LDS read.  Wait
 // counts for the DMA are therefore explicit (s_waitcnt before the barrier).
+// So is the wait state (s_nop) that a DMA needs behind the write of m0, which
+// the compiler adds for instructions of its own only.
 //
 // Stage layout (BM + 2*BN rows of 128 bytes): activation rows, then slot-0
 // weight rows, then slot-1 weight rows.  The eight 16-byte chunks of a row
@@ -129,7 +131,7 @@ TCFP_DEV v4i make_rsrc(const void* base, uint32_t bytes) {
 
 // 64 lanes x 16 bytes from rsrc + voff + soff into LDS [lds, lds + 1024).
 TCFP_DEV void dma16(v4i rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
-  asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds"
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
                :
                : "v"(voff), "s"(rsrc), "s"(soff), "{m0}"(lds)
                : "memory");
@@ -138,7 +140,7 @@ TCFP_DEV void dma16(v4i rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
 // dma16 with the non-temporal hint (data read once: kept out of the way of
 // the operands in L2 and the Infinity Cache).
 TCFP_DEV void dma16_nt(v4i rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
-  asm volatile("buffer_load_dwordx4 %0, %1, %2 offen nt lds"
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen nt lds"
                :
                : "v"(voff), "s"(rsrc), "s"(soff), "{m0}"(lds)
                : "memory");
@@ -147,7 +149,7 @@ TCFP_DEV void dma16_nt(v4i rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
 // One byte per lane from rsrc + voff + soff, zero-extended, into the 32-bit
 // LDS word lds + 4 * lane.
 TCFP_DEV void dma1(v4i rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
-  asm volatile("buffer_load_ubyte %0, %1, %2 offen lds"
+  asm volatile("s_nop 0\n\tbuffer_load_ubyte %0, %1, %2 offen lds"
                :
                : "v"(voff), "s"(rsrc), "s"(soff), "{m0}"(lds)
                : "memory");
@@ -156,7 +158,7 @@ TCFP_DEV void dma1(v4i rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
 // 16 bytes from a per-lane global address into LDS at lds + 16 * lane
 // (lds wave-uniform); counted by vmcnt like dma16.
 TCFP_DEV void gdma16(const void* src, uint32_t lds) {
-  asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(lds) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(lds) : "memory");
 }
 
 template <typename OutT>

@@ -92,7 +92,7 @@ def test_the_check_itself():
     assert short_waits(dis(copy, "buffer_load_dword v1, s[4:7], 0 offen")) == (1, [])
 
 
-@pytest.mark.parametrize("kernel", ["attend_wide_kernel"])
+@pytest.mark.parametrize("kernel", ["attend_wide_kernel", "gemm_nt_dma_kernel"])
 def test_copies_into_lds_keep_their_wait_states(kernel, tmp_path):
     text = next(t for t in _code_objects(tmp_path) if kernel in t)
     copies, short = short_waits(text)
