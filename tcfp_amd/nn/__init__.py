@@ -615,9 +615,14 @@ class _RMSNormFunction(torch.autograd.Function):
         return (*dx, dw, None, None)
 
 
-def _norm_backward(ctx, grad_y, grad_h, h, rstd, weight, needs):
+def _norm_backward(ctx, grad_y, grad_h, h, rstd, weight, needs, shape=None):
     """Gradients ``((x, residual), weight)`` of a norm whose output's gradient is
-    ``grad_y`` and whose sum's is ``grad_h`` (either may be None)."""
+    ``grad_y`` and whose sum's is ``grad_h`` (either may be None); ``shape``: the
+    input's, where ``h`` was flattened.
+
+    x and the residual get the same tensor object, and a sum's gradient that is
+    handed on is the object that came: a leaf keeps a gradient that nothing else
+    refers to, and two views of one storage would each look like that."""
     need_x, need_r, need_w = needs
     if grad_y is None:  # only the sum was used
         g = grad_h
@@ -625,8 +630,12 @@ def _norm_backward(ctx, grad_y, grad_h, h, rstd, weight, needs):
     else:
         if grad_y.dtype not in (torch.float32, torch.bfloat16):
             grad_y = grad_y.float()
+        if shape is not None and grad_h is not None:
+            grad_h = grad_h.reshape(h.shape)
         g, dw = N.rms_norm_backward(grad_y, h, rstd, weight, grad_h, need_weight_grad=need_w)
         dw = dw.to(weight.dtype) if need_w else None
+        if shape is not None:
+            g = g.reshape(shape)
     dx = g.to(ctx.x_dtype) if need_x and g is not None else None
     return (dx, g if need_r and ctx.has_residual else None), dw
 
@@ -712,10 +721,8 @@ class _TCFP12NormLinearFunction(torch.autograd.Function):
             dy, dw, db = _TCFP12BlockScaledFunction.backward(layer, grad_out)[:3]
         dx = dr = dn = None
         if need_y:
-            g_h = None if grad_h is None else _flatten(grad_h)
-            (dx, dr), dn = _norm_backward(ctx, dy, g_h, h, rstd, norm_weight, needs[:3])
-            dx = None if dx is None else dx.reshape(ctx.shape)
-            dr = None if dr is None else dr.reshape(ctx.shape)
+            (dx, dr), dn = _norm_backward(ctx, dy, grad_h, h, rstd, norm_weight, needs[:3],
+                                          ctx.shape)
         return (dx, dr, dn, dw, db) + (None,) * 7
 
 
