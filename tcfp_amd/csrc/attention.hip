@@ -165,6 +165,7 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 constexpr int kMaxSplits = 64;
+constexpr int64_t kMostKeys = 1 << 30;  // positions stay clear of 2^31
 
 struct Attend {
   const uint16_t* q;
@@ -1660,9 +1661,13 @@ struct Launch {
 Launch plan(int64_t tokens, int heads, int kv_heads, int dim, int64_t batch,
             int64_t max_query_len, int64_t max_seq_len, int64_t window) {
   Launch p{};
+  // (a window past every position is none, a bound past every length no bound;
+  // sums of larger ones would overflow)
+  window = std::min(window, kMostKeys);
+  max_query_len = std::min(max_query_len, kMostKeys);
   const int64_t group = heads / kv_heads;
   const int64_t most = std::max<int64_t>(std::min(max_query_len, tokens), 1) * group;
-  int64_t keys = std::clamp<int64_t>(max_seq_len, 1, int64_t(1) << 30);
+  int64_t keys = std::clamp<int64_t>(max_seq_len, 1, kMostKeys);
   if (window > 0) keys = std::min(keys, window + max_query_len + 64);
   p.few_tiles = most <= 16 ? 1 : most <= 32 ? 2 : 0;
   if (p.few_tiles) {
@@ -1855,8 +1860,8 @@ int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
   a.kv_heads = kv_heads;
   a.table = page_table;
   a.table_stride = table_stride;
-  // (a pool without pages holds no key; positions stay clear of 2^31)
-  a.table_keys = num_pages == 0 ? 0 : int(std::min<int64_t>(table_width * page_size, 1 << 30));
+  // (a pool without pages holds no key)
+  a.table_keys = num_pages == 0 ? 0 : int(std::min<int64_t>(table_width * page_size, kMostKeys));
   a.seq_lens = seq_lens;
   a.starts = query_start;
   a.batch = int(batch);
@@ -1866,7 +1871,7 @@ int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
   a.c = scale == 0.0f ? 1.0f : std::abs(scale) * 1.44269504088896340736f;
   a.q_mul = scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f;
   a.causal = causal != 0;
-  a.window = int(std::min<int64_t>(window, 1 << 30));
+  a.window = int(std::min<int64_t>(window, kMostKeys));
   a.tiles = p.tiles;
   a.splits = p.splits;
   a.chunk = p.chunk;
