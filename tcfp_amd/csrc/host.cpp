@@ -765,6 +765,11 @@ Tensor whole(const Tensor& x) {
   return al16(c) ? c : c.clone();
 }
 
+// Rows of the last axis, whether they have columns or not.
+int64_t row_count(const Tensor& x) {
+  return c10::multiply_integers(x.sizes().slice(0, size_t(x.dim() - 1)));
+}
+
 // Rows of the last axis: a 2-D tensor's rows may be apart, anything else is
 // made contiguous.
 struct Rows {
@@ -779,7 +784,7 @@ Rows rows_of(const Tensor& x, const char* name) {
   const bool apart = x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= x.size(1) && al16(x) &&
                      x.stride(0) * x.element_size() % 16 == 0;
   if (!apart) r.t = whole(x);
-  r.rows = r.cols ? r.t.numel() / r.cols : 0;
+  r.rows = row_count(x);
   r.ld = apart ? r.t.stride(0) : r.cols;
   return r;
 }
@@ -859,12 +864,12 @@ Outs rms_norm_backward(const Tensor& grad_y, const Tensor& h, const Tensor& rstd
   g.add(grad_h);
   const c10::DeviceGuard guard(g.device());
   if (h.dim() == 0) value_error("h needs at least one dimension");
-  const int64_t cols = h.size(-1), rows = cols ? h.numel() / cols : 0;
+  const int64_t cols = h.size(-1), rows = row_count(h);
   const int gd = in_dtype(grad_y), hd = in_dtype(h), wd = in_dtype(weight);
   if (grad_y.sizes() != h.sizes())
     value_error("grad_y shape " + shape_str(grad_y.sizes()) + " != h shape " +
                 shape_str(h.sizes()));
-  if (rstd.scalar_type() != at::kFloat || rstd.numel() != (cols ? rows : rstd.numel()))
+  if (rstd.scalar_type() != at::kFloat || rstd.numel() != rows)
     value_error("rstd must hold a float32 for each of the " + std::to_string(rows) + " rows");
   if (weight.dim() != 1 || weight.size(0) != cols)
     value_error("weight must have shape (" + std::to_string(cols) + ",), got " +

@@ -635,7 +635,7 @@ int norm_checks(const Norm& a, bool quantised) {
 template <bool QUANT>
 int norm_launch(const Norm& a, hipStream_t st) {
   const int rc = norm_checks(a, QUANT);
-  if (rc != TCFP_OK || a.rows == 0 || a.cols == 0) return rc;
+  if (rc != TCFP_OK || a.rows == 0) return rc;  // (rows without columns have their rstd, NaN)
   const RowShape s = row_shape(a.rows, a.cols);
   const int64_t xs = size_of(a.x_dtype), rs = size_of(a.r_dtype);
   const bool vec = aligned(a.x, 16) && a.ldx * xs % 16 == 0 && aligned(a.w, 16) &&
