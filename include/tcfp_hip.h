@@ -713,7 +713,8 @@ int tcfp_kv_cache_read(const uint8_t* k_codes, const uint8_t* v_codes, const int
  * New token i of n in a sequence of len tokens stands at position
  * p = len - n + i and sees the keys j < len with j <= p (causal) and
  * j > p - window (window > 0).  Keys on a page outside the pool, or past the
- * table, are not seen; a token that sees nothing gets zeros.
+ * table, are not seen; a token that sees nothing gets zeros.  A NaN code of a
+ * key reaches the tokens that see it, one of a value its own column of them.
  * out = softmax(scale * q K^T) V, scores, maximum and sums in fp32.
  * max_query_len and max_seq_len bound the batch's lengths (they size the
  * launch and the workspace; larger lengths are still answered rightly, only

@@ -96,7 +96,9 @@ def paged_attention(
     ``causal`` it sees all keys of the sequence, within the window behind it.
     Keys on a page outside the pool (-1: given up because no window reaches
     it) are not seen; a token that sees nothing, and one that belongs to no
-    sequence, gets zeros.  ``scale`` is ``dim ** -0.5`` by default.
+    sequence, gets zeros.  A NaN in a cached key reaches the tokens that see it,
+    one in a cached value its own column of them, and neither anything else.
+    ``scale`` is ``dim ** -0.5`` by default.
 
     ``max_query_len`` and ``max_seq_len`` (by default what the table spans)
     bound the batch's lengths and size the launch.

@@ -295,20 +295,53 @@ TCFP_DEV uint32_t highs(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b
 TCFP_DEV float exp_scale(uint32_t w, int j) {
   return __uint_as_float(uint32_t(max(int(int8_t(w >> (8 * j))) + 127, 0)) << 23);
 }
-TCFP_DEV bool has_nan_code(uint32_t w) {
-  return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
+// Bit 7 of the bytes of w that are NaN codes.
+TCFP_DEV uint32_t nan_bytes(uint32_t w) {
+  return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
 }
 // w with its NaN codes made zero.
-TCFP_DEV uint32_t without_nan(uint32_t w) {
-  const uint32_t t = (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
-  return w & ~(t * 255u);
-}
+TCFP_DEV uint32_t without_nan(uint32_t w) { return w & ~((nan_bytes(w) >> 7) * 255u); }
 TCFP_DEV v8bf as_bf(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __builtin_bit_cast(v8bf, make_uint4(a, b, c, d));
 }
 TCFP_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 TCFP_DEV int valid_page(const Attend& a, int p) { return p >= 0 && p < a.num_pages ? p : -1; }
+
+// NaN codes of V.  A row takes sum p v over all keys of a step, with p = 0 for the
+// keys that it does not see, so a NaN must not stand in a step whose keys some row
+// does not see (0 * NaN).  There it counts as zero, the step's keys are noted, and
+// mark_nan makes the columns NaN afterwards, for the rows that see the key.  (A
+// workgroup's notes, in LDS, are of all it does: a row's own bounds say which of
+// their keys it sees.)
+struct NanKeys {
+  int begin, end;  // none: end <= begin
+};
+TCFP_DEV void note_nan(NanKeys* nans, int key0, int keys) {
+  atomicMin(&nans->begin, key0);
+  atomicMax(&nans->end, key0 + keys);
+}
+// Calls mark(w, nan_bytes) for the lane's words of V (word w is codes w * STRIDE + at
+// ...) that hold a NaN of a key in [n.begin, n.end) and [lo, hi).
+template <int D, int WORDS, int STRIDE, typename Mark>
+TCFP_DEV void mark_nan(const Attend& a, const int32_t* table, int kvh, NanKeys n, int lo, int hi,
+                       int at, Mark mark) {
+  const int end = min(n.end, hi);
+#pragma unroll 1
+  for (int key = max(n.begin, lo); key < end; ++key) {
+    const int page = valid_page(a, table[key >> a.page_bits]);
+    if (page < 0) continue;
+    const uint8_t* v = a.v_codes +
+                       ((((int64_t(page) * a.kv_heads + kvh) << a.page_bits) +
+                         (key & ((1 << a.page_bits) - 1))) * D + at);
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      const uint32_t x = *reinterpret_cast<const uint32_t*>(v + w * STRIDE);
+      if (nan_bytes(x)) mark(w, nan_bytes(x));
+    }
+  }
+}
+TCFP_DEV bool byte_of(uint32_t nans, int byte) { return (nans >> (8 * byte + 7)) & 1u; }
 
 // Rows of q before the first (lead) and from behind the last sequence (tail):
 // zeros, for `heads` heads from head `first`.
@@ -422,10 +455,10 @@ struct FewState {
 // is missing).  [all_lo, all_hi): keys that any row sees.
 template <int D, int NT, bool masked>
 TCFP_DEV void few_step(const Attend& a, FewState<D, NT>& st, FewTile<D>& t, int key0,
-                       int all_lo, int all_hi) {
+                       int all_lo, int all_hi, NanKeys* nans) {
   using S = FewShape<D>;
   const int lane = threadIdx.x & 63, g4 = lane >> 4;
-  uint32_t bad = 0;  // keys of the lane (4 g + r) with a NaN among the codes of V
+  bool nan = false;
   if (masked) {
 #pragma unroll
     for (int g = 0; g < S::KG; ++g)
@@ -433,16 +466,15 @@ TCFP_DEV void few_step(const Attend& a, FewState<D, NT>& st, FewTile<D>& t, int 
       for (int r = 0; r < 4; ++r) {
         const int key = key0 + 16 * g + 4 * g4 + r;
         const bool dead = key < all_lo || key >= all_hi || t.page[g] < 0;
-        bool nan = false;
+        // what no row sees counts as zero, whatever the page holds there
+        uint32_t codes = 0;
 #pragma unroll
-        for (int w = 0; w < S::VW; ++w) nan |= has_nan_code(t.v[g][r][w]);
-        // what no row sees counts as zero, whatever the page holds there; a NaN
-        // among keys that some rows see is moved to the key's score, so that it
-        // reaches the rows that see it and no other (0 * NaN in the product)
-        const uint64_t any = __ballot(nan && !dead);
-        if ((any >> (16 * g4)) & 0xFFFFu) bad |= 1u << (4 * g + r);
-#pragma unroll
-        for (int w = 0; w < S::VW; ++w) t.v[g][r][w] = dead ? 0u : without_nan(t.v[g][r][w]);
+        for (int w = 0; w < S::VW; ++w) {
+          if (dead) t.v[g][r][w] = 0;
+          codes |= nan_bytes(t.v[g][r][w]);
+          t.v[g][r][w] = without_nan(t.v[g][r][w]);
+        }
+        nan |= codes != 0;
         if (dead) t.ve[g] &= ~(0xFFu << (8 * r));
       }
   }
@@ -475,7 +507,6 @@ TCFP_DEV void few_step(const Attend& a, FewState<D, NT>& st, FewTile<D>& t, int 
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int key = key0 + 16 * g + 4 * g4 + r;
-          if ((bad >> (4 * g + r)) & 1u) p[n][g][r] = __uint_as_float(0x7FC00000u);
           if (key < st.lo[n] || key >= st.hi[n] || t.page[g] < 0) p[n][g][r] = -INFINITY;
         }
     }
@@ -534,6 +565,7 @@ TCFP_DEV void few_step(const Attend& a, FewState<D, NT>& st, FewTile<D>& t, int 
         }
       }
   }
+  if (masked && nan) note_nan(nans, key0, S::KT);
 }
 
 // The value of a lane (its number the same in every lane).
@@ -688,6 +720,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
   __shared__ float ml[4][RT][2];
   __shared__ float4 xo[4][8][64];
   __shared__ FindLds fl;
+  __shared__ NanKeys nans;
+  if (threadIdx.x == 0) nans = {INT32_MAX, 0};  // (a barrier follows before any step)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g4 = lane >> 4;
   const FewLane off = few_lane<D>(lane);
   Found f;
@@ -769,9 +803,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
 #pragma unroll
         for (int g = 0; g < S::KG; ++g) hole |= cur.page[g] < 0;
         if (hole || key < lo_max || key + S::KT > hi_min)
-          few_step<D, NT, true>(a, st, cur, key, all_lo, all_hi);
+          few_step<D, NT, true>(a, st, cur, key, all_lo, all_hi, &nans);
         else
-          few_step<D, NT, false>(a, st, cur, key, all_lo, all_hi);
+          few_step<D, NT, false>(a, st, cur, key, all_lo, all_hi, &nans);
         cur = nxt;
       }
     }
@@ -787,6 +821,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
       }
     }
     __syncthreads();
+    if (nans.begin < nans.end) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        mark_nan<D, 4 * S::VW, 4>(a, table, kvh, nans, st.lo[n], st.hi[n], 4 * g4 * (D / 16),
+                                  [&](int w, uint32_t x) {
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+                                      if (byte_of(x, j))
+                                        st.o[n][4 * (w % S::VW) + j][w / S::VW] = NAN;
+                                  });
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float top = -INFINITY;
@@ -950,31 +995,30 @@ TCFP_DEV void many_load(const Attend& a, int kvh, int key0, int page, ManyLoad<D
 }
 
 // The loaded keys into a buffer.  masked: some row of the workgroup does not
-// see all of them; what no row sees counts as zero, and a NaN among the codes
-// of V becomes a NaN scale of the key (so that it reaches the rows that see
-// the key and no other).
+// see all of them; what no row sees counts as zero, and so does a NaN among the
+// codes of V, which is noted.
 template <int D>
 TCFP_DEV void many_store(uint8_t* buf, ManyLoad<D>& t, int key0, bool masked, int all_lo,
-                         int all_hi) {
+                         int all_hi, NanKeys* nans) {
   using S = ManyShape<D>;
   const int kg = threadIdx.x >> 4, dg = threadIdx.x & 15;
   // 127 added to each byte
   uint32_t scales = ((t.ke & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) ^ (t.ke & 0x80808080u);
   if (masked) {
-    const int lane = threadIdx.x & 63;
+    bool nan = false;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int key = key0 + 4 * kg + j;
       const bool dead = key < all_lo || key >= all_hi || t.page < 0;
-      bool nan = false;
 #pragma unroll
-      for (int w = 0; w < S::DW; ++w) nan |= has_nan_code(t.v[j][w]);
-      const uint64_t any = __ballot(nan && !dead);
-      if ((any >> (lane & 48)) & 0xFFFFu) scales |= 0xFFu << (8 * j);
-#pragma unroll
-      for (int w = 0; w < S::DW; ++w) t.v[j][w] = dead ? 0u : without_nan(t.v[j][w]);
+      for (int w = 0; w < S::DW; ++w) {
+        if (dead) t.v[j][w] = 0;
+        nan |= nan_bytes(t.v[j][w]) != 0;
+        t.v[j][w] = without_nan(t.v[j][w]);
+      }
       if (dead) t.ve &= ~(0xFFu << (8 * j));
     }
+    if (nan) note_nan(nans, key0, kManyKeys);
     if (t.page < 0) scales = 0;  // no page: nobody sees these four keys
   }
 #pragma unroll
@@ -1037,11 +1081,25 @@ TCFP_DEV void join_halves(const Attend& a, uint8_t* lds, int wave, int lane, v16
   __syncthreads();
 }
 
+// mark_nan for a lane's columns of O^T, 8 g + 4 half ... of every 32.
+template <int D>
+TCFP_DEV void mark_nan_rows(const Attend& a, const int32_t* table, int kvh, const NanKeys& nans,
+                            int lo, int hi, int half, v16f* o) {
+  if (nans.begin >= nans.end) return;
+  mark_nan<D, D / 8, 8>(a, table, kvh, nans, lo, hi, 4 * half, [&](int w, uint32_t x) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (byte_of(x, r)) o[w / 4][4 * (w % 4) + r] = NAN;
+  });
+}
+
 template <int D, int KS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Attend a) {
   using S = ManyShape<D>;
   constexpr int RT = kManyRows / KS, KT = 2 / KS;  // rows, and a wave's 32-key tiles of a step
   __shared__ uint4 lds4[2 * S::BUF / 16];
+  __shared__ NanKeys nans;
+  if (threadIdx.x == 0) nans = {INT32_MAX, 0};  // (a barrier follows before any step)
   uint8_t* const lds = reinterpret_cast<uint8_t*>(lds4);
   const int lane = threadIdx.x & 63, wave = scalar(int(threadIdx.x >> 6)), col = lane & 31, half = lane >> 5;
   int tile, split, kvh, b;
@@ -1097,7 +1155,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
       ManyLoad<D> t;
       many_load<D>(a, kvh, k0, page_at(k0), t);
       int page = page_at(k0 + kManyKeys);
-      many_store<D>(lds, t, k0, is_masked(k0), all_lo, keys.end);
+      many_store<D>(lds, t, k0, is_masked(k0), all_lo, keys.end, &nans);
       int cur = 0;
       for (int key = k0; key < k1; key += kManyKeys) {
         const bool more = key + kManyKeys < k1;
@@ -1182,10 +1240,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
         cur ^= 1;
         if (more)
           many_store<D>(lds + cur * S::BUF, t, key + kManyKeys, is_masked(key + kManyKeys), all_lo,
-                        keys.end);
+                        keys.end, &nans);
       }
       __syncthreads();  // (the next tile writes the buffers again)
       if constexpr (KS == 2) join_halves<S::DT, 2, 2 * S::BUF>(a, lds, wave, lane, o, m, l);
+      mark_nan_rows<D>(a, table, kvh, nans, lo, hi, half, o);
     }
     l += other_half(l);
     if (wave < 4 / KS && r0 + 32 * mine + col <= last) {
@@ -1269,6 +1328,8 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
   using S = WideShape<D>;
   constexpr int RT = kWideRows / KS;
   __shared__ uint4 lds4[2 * S::BUF / 16];
+  __shared__ NanKeys nans;
+  if (threadIdx.x == 0) nans = {INT32_MAX, 0};  // (a barrier follows before any step)
   uint8_t* const lds = reinterpret_cast<uint8_t*>(lds4);
   const uint32_t lds_at =
       uint32_t(uintptr_t((__attribute__((address_space(3))) uint8_t*)(lds4)));
@@ -1294,8 +1355,6 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
   const int x4 = lane >> 4;
   const int kg = 4 * k16 + (D == 128 ? (wave & 1) + 2 * (x4 & 1) : ((x4 & 1) << 1) + (x4 >> 1));
   const int dg = (lane & 15) + (D == 128 ? (x4 >> 1) * 16 : 0);
-  const uint64_t row_lanes = D == 128 ? 0x0000FFFF0000FFFFull << (16 * (x4 & 1))
-                                      : 0xFFFFull << (16 * x4);
   const int voff = (kg & 3) * 4 * D + dg * 4;
   const int vchunk = (kg >> 2) * 2 + (kg & 1), sub = ((kg >> 1) & 1) * 8;
   for (int r0 = tile * RT; r0 < seq.rows; r0 += a.tiles * RT) {
@@ -1366,15 +1425,17 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
           const int u = step_of(i), key = key0 + u * kManyKeys;
           uint32_t scales = ((t[i].ke & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) ^ (t[i].ke & 0x80808080u);
           if (is_masked(key)) {
+            bool nan = false;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int kk = key + 4 * kg + j;
               const bool dead = kk < all_lo || kk >= keys.end || t[i].page < 0;
-              const uint64_t any = __ballot(has_nan_code(t[i].v[j]) && !dead);
-              if (any & row_lanes) scales |= 0xFFu << (8 * j);
-              t[i].v[j] = dead ? 0u : without_nan(t[i].v[j]);
+              if (dead) t[i].v[j] = 0;
+              nan |= nan_bytes(t[i].v[j]) != 0;
+              t[i].v[j] = without_nan(t[i].v[j]);
               if (dead) t[i].ve &= ~(0xFFu << (8 * j));
             }
+            if (nan) note_nan(&nans, key, kManyKeys);
             if (t[i].page < 0) scales = 0;
           }
           float sc[4];
@@ -1491,6 +1552,7 @@ __global__ __launch_bounds__(512, 2) void attend_wide_kernel(Attend a) {
       }
       __syncthreads();  // (the next tile writes the buffers again)
       if constexpr (KS == 2) join_halves<S::DT, 4, 2 * S::BUF>(a, lds, wave, lane, o, m, l);
+      mark_nan_rows<D>(a, table, kvh, nans, lo, hi, half, o);
     }
     l += other_half(l);
     if (wave < 8 / KS && r0 + 32 * mine + col <= last) {

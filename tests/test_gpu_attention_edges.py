@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tcfp_amd import attention as A
-from test_gpu_attention import DECODE, MIXED, Batch
+from test_gpu_attention import DECODE, MIXED, Batch, _mask, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -41,6 +41,78 @@ FORMS = {
     "wide": ([(200, 1000), (150, 700)], 4, 2),
     "split": ([(90, 6000), (40, 40), (57, 4097)], 3, 3),
 }
+
+
+def _expected_nan(b, bad, causal, window, rows):
+    """[rows, heads, dim]: which outputs see a NaN; bad [slots, kv_heads, dim]."""
+    out = torch.zeros(rows, b.heads, b.dim, dtype=torch.bool, device=bad.device)
+    for s, (n, total) in enumerate(b.lens):
+        if n:
+            seen = _mask(n, total, causal, window, bad.device)
+            for x in b.holes.get(s, ()):
+                seen[:, x] = False
+            hit = torch.stack([seen.float() @ bad[b.slots[s], h].float()
+                               for h in range(bad.shape[1])], 1) > 0
+            out[b.at[s]:b.at[s + 1]] = hit.repeat_interleave(b.group, 1)
+    return out
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 150), (False, 0), (False, 40)])
+def test_nan_in_a_column_of_v(dev, dim, form, causal, window):
+    """A NaN in one column of a cached value reaches that column of the rows that
+    see it: no other column, no other row, whatever the launch."""
+    lens, heads, kv_heads = FORMS[form]
+    print(f"[attend] nan {form} {dim} {causal} {window}", flush=True)
+    page = 16
+    b = Batch(dev, lens, heads, kv_heads, dim, page, seed=24)
+    b.holes = {}
+    kw = dict(causal=causal, window=window)
+    clean = b.attend(**kw)
+    g = torch.Generator().manual_seed(25)
+    codes = b.pool[1].view(torch.uint8)
+    kept = codes.clone()
+    for tries in range(3):
+        codes.copy_(kept)
+        for s, (n, total) in enumerate(lens):
+            # near the ends of what is seen, and anywhere
+            spots = [total - 1, max(total - n, 0), max(total - n - window, 0)]
+            spots += torch.randint(0, max(total, 1), (2,), generator=g).tolist()
+            for j in spots[tries:tries + 3]:
+                if j < total:
+                    slot = int(b.slots[s][j])
+                    h = int(torch.randint(0, kv_heads, (), generator=g))
+                    d = int(torch.randint(0, dim, (), generator=g))
+                    codes[slot // page, h, slot % page, d] = 0x7F if j % 2 else 0xFF
+        bad = _values(b.pool)[1].isnan()
+        got = b.attend(**kw)
+        want = _expected_nan(b, bad, causal, window, got.shape[0])
+        assert torch.equal(got.isnan(), want)
+        assert torch.equal(got[~want], clean[~want])
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", ["few-one", "prompts", "paired", "wide", "split"])
+def test_nan_in_a_column_of_v_beside_a_hole(dev, dim, form):
+    """The same where pages are missing, so that every step is looked at."""
+    lens, heads, kv_heads = FORMS[form]
+    print(f"[attend] nan and hole {form} {dim}", flush=True)
+    page = 16
+    b = Batch(dev, lens, heads, kv_heads, dim, page, seed=26)
+    b.table[0, 3:6] = -1
+    b.holes = {0: [slice(48, 96)]}
+    clean = b.attend()
+    codes = b.pool[1].view(torch.uint8)
+    for j, d in ((0, 3), (47, 60), (60, 10), (96, dim - 1), (lens[0][1] // 2, 33),
+                 (lens[0][1] - 1, 0)):
+        slot = int(b.slots[0][j])
+        codes[slot // page, kv_heads - 1, slot % page, d] = 0x7F
+    bad = _values(b.pool)[1].isnan()
+    got = b.attend()
+    want = _expected_nan(b, bad, True, 0, got.shape[0])
+    assert torch.equal(got.isnan(), want) and want.any()
+    assert torch.equal(got[~want], clean[~want])
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
