@@ -102,12 +102,33 @@ def paged_attention(
 
     ``max_query_len`` and ``max_seq_len`` (by default what the table spans)
     bound the batch's lengths and size the launch.
+
+    For serving: there is no backward pass.  Where ``q`` requires a gradient the
+    result does too, and a backward pass that reaches it raises
+    ``NotImplementedError``.
     """
-    return _hip.host().paged_attention(q, k_codes, v_codes, k_exps, v_exps, page_table, seq_lens,
-                                       query_start, int(max_query_len),
-                                       None if max_seq_len is None else int(max_seq_len),
-                                       None if scale is None else float(scale), bool(causal),
-                                       int(window))
+    out = _hip.host().paged_attention(q, k_codes, v_codes, k_exps, v_exps, page_table, seq_lens,
+                                      query_start, int(max_query_len),
+                                      None if max_seq_len is None else int(max_seq_len),
+                                      None if scale is None else float(scale), bool(causal),
+                                      int(window))
+    if torch.is_grad_enabled() and q.requires_grad:
+        return _NoBackward.apply(q, out)
+    return out
+
+
+class _NoBackward(torch.autograd.Function):
+    """Ties ``paged_attention``'s result to its ``q``, so that a gradient is not
+    lost without a word."""
+
+    @staticmethod
+    def forward(ctx, q, out):
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise NotImplementedError("paged_attention has no backward pass (the cache holds "
+                                  "quantised keys and values, for serving)")
 
 
 @dataclass

@@ -143,3 +143,21 @@ def test_scale_of_zero(dev, dim, form):
     b = Batch(dev, lens, heads, kv_heads, dim, 16, seed=28)
     b.check(b.attend(scale=0.0), scale=0.0)
     b.check(b.attend(scale=0.0, window=50), scale=0.0, window=50)
+
+
+def test_a_gradient_is_refused_and_not_lost(dev):
+    """There is no backward pass: the result stays in the graph, and the pass that
+    reaches it raises."""
+    b = Batch(dev, [(3, 20)], 4, 2, 64, 16, seed=29)
+    want = b.attend()
+    assert not want.requires_grad
+    b.q = b.q.clone().requires_grad_(True)
+    got = b.attend()
+    assert got.requires_grad and torch.equal(got.detach(), want)
+    with pytest.raises(NotImplementedError, match="no backward"):
+        got.float().sum().backward()
+    with torch.no_grad():
+        got = b.attend()
+        assert not got.requires_grad and torch.equal(got, want)
+    with torch.inference_mode():
+        assert torch.equal(b.attend(), want)
