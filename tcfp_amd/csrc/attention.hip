@@ -1610,7 +1610,11 @@ __global__ __launch_bounds__(256) void attend_few_join_kernel(Attend a, int tile
   const int r = (t - at.seq.start) * a.group + h % a.group, units = units_of(a, at.seq);
   const int64_t first =
       at.before + int64_t(r / tile_rows * a.kv_heads + h / a.group) * units;  // the item's first unit
-  const int w0 = int(divide(first, share)), w1 = int(divide(first + units - 1, share));
+  // (bounded: sequences whose rows overlap, which no batch has, would be found as a
+  // mixture of several, and their parts nowhere)
+  const int64_t most = a.workers - 1;
+  const int w0 = int(min(divide(first, share), most)),
+            w1 = int(min(divide(first + units - 1, share), most));
   if (w0 == w1) return;
   float m = -INFINITY, l = 0.0f, o[C] = {};
   constexpr int N = 4;  // parts of a wave in flight

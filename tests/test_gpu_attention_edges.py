@@ -161,3 +161,19 @@ def test_a_gradient_is_refused_and_not_lost(dev):
         assert not got.requires_grad and torch.equal(got, want)
     with torch.inference_mode():
         assert torch.equal(b.attend(), want)
+
+
+@pytest.mark.parametrize("sequences", [3, 70, 300])
+def test_sequences_whose_rows_overlap(dev, sequences):
+    """Starts that go back: no batch of the operator, but nothing is read or
+    written out of place for them, and the batches after it are as ever."""
+    print(f"[attend] overlap {sequences}", flush=True)
+    lens = [(4, 300 + (b * 53) % 700) for b in range(sequences)]
+    b = Batch(dev, lens, 4, 2, 64, 16, seed=30)
+    want = b.attend()
+    b.check(want)
+    kept = b.starts.clone()
+    b.starts = torch.where(torch.arange(sequences + 1, device=dev) % 3 == 1, kept + 7, kept)
+    assert b.attend().shape == want.shape
+    b.starts = kept
+    assert torch.equal(b.attend(), want)
