@@ -71,6 +71,9 @@ class Decoder(nn.Module):
                 nn.init.normal_(m.weight, std=0.02)
 
     def forward(self, idx):
+        if idx.shape[1] > self.pos.num_embeddings:
+            raise ValueError(f"{idx.shape[1]} tokens, the model has {self.pos.num_embeddings} "
+                             "positions")
         h = self.tok(idx)
         x = self.pos(torch.arange(idx.shape[1], device=idx.device)).expand_as(h)
         for layer in self.layers:
@@ -103,6 +106,12 @@ class Server:
         token, one sequence after another."""
         model, dev = self.model, self.model.tok.weight.device
         starts = [self.cache.length(s) for s in seqs]
+        # (an index that a table does not have would end the process on the GPU)
+        room = model.pos.num_embeddings
+        if any(a + len(t) > room for a, t in zip(starts, tokens)):
+            raise ValueError(f"a sequence would pass the model's {room} positions")
+        if any(not 0 <= t < model.tok.num_embeddings for ts in tokens for t in ts):
+            raise ValueError(f"tokens must lie in [0, {model.tok.num_embeddings})")
         batch = self.cache.extend(seqs, [len(t) for t in tokens])
         idx = torch.tensor([t for ts in tokens for t in ts], device=dev)
         pos = torch.tensor([a + i for a, t in zip(starts, tokens) for i in range(len(t))],
@@ -124,7 +133,11 @@ class Server:
         return y.float() @ model.tok.weight.t()
 
     def generate(self, prompts: list[list[int]], count: int) -> list[list[int]]:
-        """The likeliest ``count`` tokens after each prompt."""
+        """The likeliest ``count`` tokens after each prompt (of a token or more)."""
+        if not all(prompts):
+            raise ValueError("a prompt needs a token")
+        if count < 1:
+            return [[] for _ in prompts]
         seqs = [self.cache.open() for _ in prompts]
         try:
             logits = self.step(seqs, prompts)
