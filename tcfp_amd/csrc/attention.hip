@@ -322,7 +322,8 @@ TCFP_DEV void note_nan(NanKeys* nans, int key0, int keys) {
   atomicMax(&nans->end, key0 + keys);
 }
 // Calls mark(w, nan_bytes) for the lane's words of V (word w is codes w * STRIDE + at
-// ...) that hold a NaN of a key in [n.begin, n.end) and [lo, hi).
+// ...) that hold a NaN of a key in [n.begin, n.end) and [lo, hi), one key after
+// another: a cache that holds NaN is no case to be fast at.
 template <int D, int WORDS, int STRIDE, typename Mark>
 TCFP_DEV void mark_nan(const Attend& a, const int32_t* table, int kvh, NanKeys n, int lo, int hi,
                        int at, Mark mark) {
@@ -358,7 +359,7 @@ TCFP_DEV void zero_rest(const Attend& a, int lead, int tail, int first, int head
 //
 // Bound by reading the cache: 64 sequences of up to 8192 tokens, 32 / 8 heads of
 // 128, 132 us with the joining launch (5.26 TB/s of codes and exponents), heads
-// of 64 78 us, heads of 256 (16 / 8) 248 us (5.6 TB/s); one sequence of 127
+// of 64 75 us, heads of 256 (16 / 8) 248 us (5.6 TB/s); one sequence of 127
 // tokens 5.3 us, a chain of latencies: lengths, page table, keys, the waves'
 // join.  A wave takes KT keys at a time straight into registers, the next KT in
 // flight; nothing of K or V passes through LDS.  The four waves of a workgroup
@@ -929,9 +930,12 @@ TCFP_DEV bool place(const Attend& a, int& tile, int& split, int& kvh, int& b) {
 // ---- many rows: prompts ------------------------------------------------------
 //
 // Bound by the matrix and vector units together and by what passes between
-// them: with the exponentials taken out a 2048-token chunk over 14336 tokens
-// (32 / 8 heads of 128) goes from 553 us to 485, without its second product to
-// 532, without moving keys to 414.  A workgroup's four waves hold 32 rows each;
+// them.  (A 2048-token chunk over 14336 tokens, 32 / 8 heads of 128, which the
+// eight-wave kernel takes, ran 553 us here, 485 with the exponentials taken out, 532
+// without its second product, 414 without moving keys.)  One prompt of 2048 tokens,
+// 32 / 8 heads of 128: 67 us; six ragged ones of up to 1000, 16 heads of 64: 30 us,
+// vector units 56% and matrix units 16% busy.  A workgroup's four waves hold 32 rows
+// each;
 // per 64 keys K goes to LDS as codes and V as bf16, transposed and in the order
 // of keys that P has in its registers (both buffered twice, the next 64 keys
 // loaded into registers meanwhile), so every operand is read with 16-byte LDS
@@ -1277,9 +1281,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_many_kernel(Atte
 
 // ---- many rows, eight waves --------------------------------------------------
 //
-// As above (the same chunk: 493 us, 1046 TFLOP/s counting 4 flops a visible
+// As above (that chunk: 493-500 us, 1031-1046 TFLOP/s counting 4 flops a visible
 // key, head and column, where a bf16 product of the library reaches 1245; heads
-// of 64 317 us) with 256 rows a workgroup, so that each key is fetched, converted
+// of 64 319-321 us) with 256 rows a workgroup, so that each key is fetched, converted
 // and written to LDS for twice the rows, and 128 keys between two barriers, so
 // that the two waves of a SIMD drift apart and one's products run beside the
 // other's softmax.  The codes of K need no work: each wave copies the 8 or 16

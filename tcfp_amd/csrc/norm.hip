@@ -340,6 +340,7 @@ __global__ __launch_bounds__(wg_of(T)) void norm_rows_kernel(Norm a) {
 
 // Threads and vectors of a row: two vectors a thread where the rows fill the
 // card, one where there are few (latency); t == 0: the kernel for any row.
+constexpr int64_t kManyRows = 1024;
 struct RowShape {
   int t, c;
 };
@@ -347,7 +348,7 @@ RowShape row_shape(int64_t rows, int64_t cols) {
   if (cols % 8 != 0 || cols > 1024 * 16) return {0, 0};
   const int64_t nvec = cols / 8;
   int t = 64;
-  if (rows >= 1024) {
+  if (rows >= kManyRows) {
     while (t * 2 < nvec) t *= 2;
   } else {
     while (t < nvec && t < 1024) t *= 2;
@@ -357,10 +358,11 @@ RowShape row_shape(int64_t rows, int64_t cols) {
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 int64_t size_of(int dtype) { return dtype == TCFP_DTYPE_BF16 ? 2 : 4; }
 
-// Inputs of more than half the 256 MiB cache behind the L2s are read with the
-// non-temporal hint (8192 x 4096 bf16 + residual: forward 50.0 us against 52.9,
-// backward 52.4 against 57.0); smaller ones, which their producer may have left
-// there, are not (8192 x 1024: 13.3 us against 14.8 with it, 16.7 against 18.6).
+// Inputs of more than 96 MiB, three eighths of the cache behind the L2s, are read
+// with the non-temporal hint (8192 x 4096 bf16 + residual, 128 MiB: forward 50.0 us
+// against 52.9; backward, 192 MiB, 52.4 against 57.0); smaller ones, which their
+// producer may have left there, are not (8192 x 1024: 13.3 us against 14.8 with it,
+// 16.7 against 18.6).
 constexpr int64_t kStreamBytes = 96ll << 20;
 
 #define TCFP_ROWS(CALL)                              \
@@ -379,7 +381,9 @@ constexpr int64_t kStreamBytes = 96ll << 20;
   } while (0)
 
 // Those that inputs past kStreamBytes come in: a vector a thread only where rows
-// are short (of 1023 rows at most, 8192 wide at most, none is that large).
+// are short (with fewer than kManyRows rows, 8192 wide at most, 12 bytes a column at
+// most, none is that large).
+static_assert((kManyRows - 1) * 8192 * 12 <= kStreamBytes, "no one-vector form is streamed");
 #define TCFP_ROWS_STREAM(CALL, WIDEST)               \
   do {                                               \
     if (s.t == 64 && s.c == 1) CALL(64, 1);          \
@@ -453,7 +457,7 @@ __global__ __launch_bounds__(kThreads) void norm_dw_any_kernel(NormBack a, int64
 //
 // Bound by HBM like the forward (8192 x 4096 bf16 with the residual's gradient:
 // 53 us with the joining launch, 5.1 TB/s; 65536 x 2048 5.8 TB/s), at a thousand
-// rows by latency (1000 x 1056 fp32 8.5 us: two launches of 5.4 and 2.7).
+// rows by latency (1000 x 1056 fp32 9.1 us: two dependent launches of 5.5 and 3.4).
 // Workgroups take every gridDim.x-th group of rows, the next rows' loads in
 // flight; a thread's columns are the same in all its rows, so it sums its share
 // of dw in registers, the workgroup leaves one partial row and a second launch

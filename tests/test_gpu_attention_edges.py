@@ -177,3 +177,23 @@ def test_sequences_whose_rows_overlap(dev, sequences):
     assert b.attend().shape == want.shape
     b.starts = kept
     assert torch.equal(b.attend(), want)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_queries_that_are_not_finite(dev, dim, form, value):
+    """NaN in every column of that token and head (an infinite score less the
+    largest is NaN), the bits of the others as ever."""
+    lens, heads, kv_heads = FORMS[form]
+    print(f"[attend] q {value} {form} {dim}", flush=True)
+    b = Batch(dev, lens, heads, kv_heads, dim, 16, seed=31)
+    clean = b.attend()
+    bad = torch.zeros(b.q.shape[0], heads, dtype=torch.bool, device=dev)
+    for s, (n, _) in enumerate(lens):
+        if n:
+            bad[b.at[s] + n // 2, s % heads] = True
+    b.q[..., 5] = torch.where(bad, torch.tensor(value, dtype=b.q.dtype, device=dev), b.q[..., 5])
+    got = b.attend()
+    assert got[bad].isnan().all()
+    assert torch.equal(got[~bad], clean[~bad])
