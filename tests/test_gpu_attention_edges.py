@@ -197,3 +197,33 @@ def test_queries_that_are_not_finite(dev, dim, form, value):
     got = b.attend()
     assert got[bad].isnan().all()
     assert torch.equal(got[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_scores_of_hundreds(dev, dim, form):
+    """A scale of 1.  Beside the two roundings to bf16 (2^-8 of sum p |v| and of the
+    result) a score is off by what its products lose: the matrix instruction keeps
+    no bit under 2^-13 of the largest of eight, so seven lose up to 2^-13 of it
+    each, of either sign: for products of random size some 2^-17 of sum |q k| (one
+    standard deviation of dim / 8 such groups), 2^-14 asked.  A weight changes by
+    that of itself, and so does the sum they are divided by."""
+    lens, heads, kv_heads = FORMS[form]
+    print(f"[attend] scale 1 {form} {dim}", flush=True)
+    b = Batch(dev, lens, heads, kv_heads, dim, 16, seed=32, q_size=3.0)
+    got = b.attend(scale=1.0).double()
+    k, v = _values(b.pool)
+    for s, (n, total) in enumerate(lens):
+        if not n:
+            continue
+        seen = _mask(n, total, True, 0, dev)
+        for h in range(heads):
+            q = b.q[b.at[s]:b.at[s + 1], h].double()
+            kh, vh = (t[b.slots[s], h // b.group] for t in (k, v))
+            score = (q @ kh.t()).masked_fill(~seen, float("-inf"))
+            p = torch.softmax(score, 1)
+            want, size = p @ vh, p @ vh.abs()
+            lost = 2**-14 * (q.abs() @ kh.abs().t()).masked_fill(~seen, 0).amax(1, keepdim=True)
+            err = (got[b.at[s]:b.at[s + 1], h] - want).abs()
+            # (1e-30: weights under fp32's smallest, as in the other tests)
+            assert (err <= 2**-8 * (size + want.abs()) + 2 * lost * size + 1e-30).all()
