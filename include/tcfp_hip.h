@@ -715,7 +715,9 @@ int tcfp_kv_cache_read(const uint8_t* k_codes, const uint8_t* v_codes, const int
  * j > p - window (window > 0).  Keys on a page outside the pool, or past the
  * table, are not seen; a token that sees nothing gets zeros.  A NaN code of a
  * key reaches the tokens that see it, one of a value its own column of them.
- * out = softmax(scale * q K^T) V, scores, maximum and sums in fp32.
+ * out = softmax(scale * q K^T) V, scores, maximum and sums in fp32 (of eight
+ * neighbouring products of a score nothing under 2^-13 of the largest is kept),
+ * weights rounded to bf16 before the second product.
  * max_query_len and max_seq_len bound the batch's lengths (they size the
  * launch and the workspace; larger lengths are still answered rightly, only
  * slower).  workspace: tcfp_paged_attention_workspace_bytes, any contents,
