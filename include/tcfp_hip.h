@@ -735,6 +735,104 @@ int tcfp_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
                          int64_t window, void* out, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/* ---- a decoder's training step (no reference counterpart) --------------- */
+
+/* Rotary positions: pair i < rotary / 2 of every head of q [tokens, q_heads,
+ * dim] and k [tokens, k_heads, dim] (f32 or bf16; dim contiguous, token and head
+ * strides in elements) turned by angle = positions[t] * freqs[i] radians,
+ *   (a, b) -> amplitude * (a cos - b sin, a sin + b cos),
+ * or by -angle (inverse != 0), which is the gradient.  Pairs are columns
+ * (2 i, 2 i + 1) with interleaved != 0, (i, i + rotary / 2) without; columns from
+ * `rotary` on are copied.  The angle is formed in f64 and reduced by whole turns
+ * before it is rounded.  Outputs contiguous, not the inputs; either of q and k
+ * may have no heads.  rotary even, 2 to 4096; any strides and alignment (16-byte
+ * vectors throughout are faster). */
+int tcfp_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
+                const void* k, int64_t k_token_stride, int64_t k_head_stride, int k_heads,
+                int dtype, int64_t tokens, int dim, const int64_t* positions,
+                const double* freqs, int rotary, int interleaved, float amplitude, int inverse,
+                void* q_out, void* k_out, void* stream);
+
+/* Attention within packed sequences.
+ *   q, out [tokens, heads, dim], k, v [keys, kv_heads, dim] bf16 (inputs: dim
+ *   contiguous, token and head strides in elements, multiples of 8, 16-byte
+ *   aligned; out contiguous); heads % kv_heads == 0, query head h reads K/V head
+ *   h / (heads / kv_heads); dim 64, 128 or 256.
+ *   Sequence b has the rows q_starts[b] ... q_starts[b + 1] - 1 of q and
+ *   k_starts[b] ... of k and v ([batch + 1] each, not decreasing; the same array
+ *   where a sequence attends to itself).
+ * Query i of n stands at position p = (the sequence's keys) - n + i and sees the
+ * keys j <= p (causal) with j > p - window (window > 0).  A query that sees
+ * nothing, and one outside the sequences, gets zeros.
+ * out = softmax(scale * q K^T) V with scores, maxima and sums in f32, the weights
+ * rounded to bf16 before the second product.  lse [heads, tokens] f32 (may be
+ * NULL): log2 of the sum of 2^(score * log2 e), +inf for a query that sees
+ * nothing; not written for one outside the sequences.
+ * max_len bounds the sequences' queries and sizes the launch (longer ones are
+ * still answered rightly, only slower).  What is not finite stays within its
+ * sequence.  No workspace; results do not depend on the launch's timing. */
+int tcfp_packed_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                          const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                          const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                          const int32_t* q_starts, const int32_t* k_starts, int64_t batch,
+                          int64_t tokens, int64_t keys, int heads, int kv_heads, int dim,
+                          int64_t max_len, float scale, int causal, int64_t window, void* out,
+                          float* lse, void* stream);
+
+/* Its gradients: dq [tokens, heads, dim], dk and dv [keys, kv_heads, dim] bf16,
+ * contiguous, from grad_out (strided like q), the inputs, and out and lse as the
+ * forward wrote them.  The gradients of a K/V head are summed in f32 over the
+ * query heads that share it, in an order that the sizes fix; rows outside the
+ * sequences get zeros.  dS is rounded to bf16 before the products it goes into.
+ * max_key_len bounds the sequences' keys.  workspace:
+ * ..._workspace_bytes, any contents, 16-byte aligned. */
+size_t tcfp_packed_attention_backward_workspace_bytes(int64_t tokens, int64_t keys, int64_t batch,
+                                                      int64_t max_key_len, int heads,
+                                                      int kv_heads, int dim);
+int tcfp_packed_attention_backward(
+    const void* grad_out, int64_t go_token_stride, int64_t go_head_stride, const void* q,
+    int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+    int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+    const void* out, const float* lse, const int32_t* q_starts, const int32_t* k_starts,
+    int64_t batch, int64_t tokens, int64_t keys, int heads, int kv_heads, int dim,
+    int64_t max_len, int64_t max_key_len, float scale, int causal, int64_t window, void* dq,
+    void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Softmax cross entropy of a linear head, without storing its logits z = hidden
+ * weight^T: losses[t] = log sum exp z[t] - z[t][targets[t]].
+ *   hidden [tokens, dim], weight [vocab, dim] bf16, rows ldh / ldw apart
+ *   (multiples of 8, 16-byte aligned), dim % 8 == 0.
+ * A token whose target is `ignore` has loss 0; one whose target is neither that
+ * nor a class has loss NaN.  lse [tokens] f32: log sum exp z.  total (may be
+ * NULL): [0] the sum of the losses, or (mean != 0) their mean over the tokens that
+ * are not ignored (NaN if all are), [1] the number of those; summed in f64 in an
+ * order that the sizes fix.  workspace: ..._workspace_bytes, any contents, 16-byte
+ * aligned. */
+size_t tcfp_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t vocab);
+int tcfp_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+                              const int64_t* targets, int64_t ignore, int64_t tokens,
+                              int64_t vocab, int64_t dim, float* losses, float* lse, int mean,
+                              float* total, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* Its gradients: g[t] = (softmax(z[t]) - onehot(targets[t])) * grad[t * grad_step]
+ * (/ *count, if count is not NULL), 0 for an ignored token;
+ *   grad_hidden = g weight, grad_weight = g^T hidden,
+ * bf16, contiguous, either may be NULL.  grad_step is 1 (a gradient a token) or 0
+ * (one for all, of a sum, or with count of a mean).  z is formed again, for a run
+ * of classes at a time whose g, rounded to bf16, takes at most 256 MiB of the
+ * workspace; sums are f32.  hidden is read for ignored tokens too: a value that is
+ * not finite there reaches grad_weight. */
+size_t tcfp_linear_cross_entropy_backward_workspace_bytes(int64_t tokens, int64_t vocab,
+                                                          int64_t dim, int need_hidden,
+                                                          int need_weight);
+int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const void* weight,
+                                       int64_t ldw, const int64_t* targets, int64_t ignore,
+                                       const float* lse, const float* grad, int64_t grad_step,
+                                       const float* count, int64_t tokens, int64_t vocab,
+                                       int64_t dim, void* grad_hidden, void* grad_weight,
+                                       void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- layout helpers ---------------------------------------------------- */
 
 /* dst[c, r] = src[r, c] for a [rows, cols] byte matrix (ld = cols / rows).

@@ -11,8 +11,8 @@ tile policy, the HIP library handle) is shared between the two names.
 import sys
 
 import tcfp_amd as _pkg
-from tcfp_amd import attention, core, cuda_ext, kernels, nn, norm  # noqa: F401
+from tcfp_amd import attention, core, cuda_ext, kernels, loss, nn, norm, rotary  # noqa: F401
 
-for _name in ("attention", "core", "cuda_ext", "kernels", "nn", "norm"):
+for _name in ("attention", "core", "cuda_ext", "kernels", "loss", "nn", "norm", "rotary"):
     sys.modules[f"{__name__}.{_name}"] = getattr(_pkg, _name)
 sys.modules[__name__] = _pkg

@@ -11,11 +11,13 @@ this package under the reference's import name.  All device work runs in
 hand-written HIP kernels (``libtcfp_hip.so``, C ABI in
 ``include/tcfp_hip.h``).
 
-``tcfp_amd.norm`` (residual + RMS norm with FP8 output) and
-``tcfp_amd.attention`` (an 8-bit paged K/V cache and attention over it) are the
-operators between the linear layers of a decoder; the reference has neither.
+``tcfp_amd.norm`` (residual + RMS norm with FP8 output), ``tcfp_amd.rotary``
+(rotary positions), ``tcfp_amd.attention`` (attention within packed sequences, and
+over an 8-bit paged K/V cache) and ``tcfp_amd.loss`` (cross entropy of a linear
+head, logits never stored) are the operators between and behind the linear layers
+of a decoder; the reference has none of them.
 """
-from . import attention, core, cuda_ext, kernels, nn, norm  # noqa: F401
+from . import attention, core, cuda_ext, kernels, loss, nn, norm, rotary  # noqa: F401
 from .core import (  # noqa: F401
     ErrorFeedbackState,
     FP8Config,

@@ -162,6 +162,28 @@ _SIGNATURES = {
                              _i64, _i32, _i32, _i32, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
                              _i64, _i64, _i32, _i64, _i64, ctypes.c_float, _i32, _i64, _c_void_p,
                              _c_void_p, ctypes.c_size_t, _c_void_p],
+    "tcfp_rotary": [_c_void_p, _i64, _i64, _i32, _c_void_p, _i64, _i64, _i32, _i32, _i64, _i32,
+                    _c_void_p, _c_void_p, _i32, _i32, ctypes.c_float, _i32, _c_void_p, _c_void_p,
+                    _c_void_p],
+    "tcfp_packed_attention": [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,
+                              _c_void_p, _c_void_p, _i64, _i64, _i64, _i32, _i32, _i32, _i64,
+                              ctypes.c_float, _i32, _i64, _c_void_p, _c_void_p, _c_void_p],
+    "tcfp_packed_attention_backward_workspace_bytes": [_i64, _i64, _i64, _i64, _i32, _i32, _i32],
+    "tcfp_packed_attention_backward": [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p,
+                                       _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+                                       _c_void_p, _c_void_p, _i64, _i64, _i64, _i32, _i32, _i32,
+                                       _i64, _i64, ctypes.c_float, _i32, _i64, _c_void_p,
+                                       _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t,
+                                       _c_void_p],
+    "tcfp_linear_cross_entropy_workspace_bytes": [_i64, _i64],
+    "tcfp_linear_cross_entropy": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64,
+                                  _i64, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p,
+                                  ctypes.c_size_t, _c_void_p],
+    "tcfp_linear_cross_entropy_backward_workspace_bytes": [_i64, _i64, _i64, _i32, _i32],
+    "tcfp_linear_cross_entropy_backward": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64,
+                                           _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64,
+                                           _i64, _c_void_p, _c_void_p, _c_void_p,
+                                           ctypes.c_size_t, _c_void_p],
     "tcfp_gemm_set_tile_policy": [_i32],
     "tcfp_dual_quantize_set_candidates": [_i32],
     "tcfp_transpose_u8": [_c_void_p, _i64, _i64, _c_void_p, _c_void_p],
@@ -182,6 +204,9 @@ _RESTYPE = {
     "tcfp_quantize_batch_workspace_bytes": ctypes.c_size_t,
     "tcfp_rms_norm_backward_workspace_bytes": ctypes.c_size_t,
     "tcfp_paged_attention_workspace_bytes": ctypes.c_size_t,
+    "tcfp_packed_attention_backward_workspace_bytes": ctypes.c_size_t,
+    "tcfp_linear_cross_entropy_workspace_bytes": ctypes.c_size_t,
+    "tcfp_linear_cross_entropy_backward_workspace_bytes": ctypes.c_size_t,
 }
 
 _lib = None

@@ -1,7 +1,11 @@
-"""An 8-bit paged K/V cache and attention over it (HIP, gfx950; no reference
-counterpart).
+"""Attention (HIP, gfx950; no reference counterpart): within packed sequences, with
+its gradients, and over an 8-bit paged K/V cache.
 
-The cache holds, for K and for V, E4M3 codes ``[pages, kv_heads, page_size,
+In training (and wherever keys and values are at hand in bf16)
+:func:`packed_attention` attends the sequences of a batch that lie one after
+another in one tensor; it stores no scores, and its gradients form them again.
+
+For serving, the cache holds, for K and for V, E4M3 codes ``[pages, kv_heads, page_size,
 dim]`` and one power-of-two exponent per token and head (int8 ``[pages,
 kv_heads, page_size]``): the block format of ``kernels.block_quantize_fp8``
 with the head as the block.  A token's place is its *slot*, ``page * page_size
@@ -26,7 +30,127 @@ import torch
 
 from . import _hip
 
-__all__ = ["kv_cache_write", "kv_cache_read", "paged_attention", "PagedKVCache", "CacheBatch"]
+__all__ = ["packed_attention", "packed_attention_forward", "packed_attention_backward",
+           "kv_cache_write", "kv_cache_read", "paged_attention", "PagedKVCache", "CacheBatch"]
+
+
+def packed_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    seq_start: torch.Tensor,
+    *,
+    max_len: int,
+    key_start: torch.Tensor | None = None,
+    max_key_len: int | None = None,
+    scale: float | None = None,
+    causal: bool = True,
+    window: int = 0,
+) -> torch.Tensor:
+    """Attention within each of a batch's packed sequences, bf16 [tokens, heads, dim].
+
+    ``q`` [tokens, heads, dim], ``k`` and ``v`` [keys, kv_heads, dim] are bf16 (slices
+    of a QKV projection's output are taken as they are), ``dim`` 64, 128 or 256;
+    ``heads`` is a multiple of ``kv_heads``, neighbouring query heads share one.
+    Sequence b has the rows ``seq_start[b]`` to ``seq_start[b + 1]`` (int32
+    [sequences + 1], not decreasing) of q, and of k and v too unless ``key_start``
+    gives those rows of their own: with more keys than queries the queries are the
+    last tokens of the sequence.
+
+    A query at position p of its sequence sees the keys up to p (``causal``) that are
+    less than ``window`` positions back (``window`` > 0); without ``causal`` it sees
+    all keys of the sequence, within the window behind it.  A query that sees
+    nothing, and one that belongs to no sequence, gets zeros and a zero gradient.
+    What is not finite stays within its sequence.  ``scale`` is ``dim ** -0.5`` by
+    default.
+
+    ``max_len`` and ``max_key_len`` (``max_len`` by default, with ``key_start`` all
+    keys) bound the sequences' lengths and size the launches; lengths past them are
+    answered rightly, only slower.
+
+    Differentiable in q, k and v, once; results and gradients do not depend on the
+    launches' timing.
+    """
+    how = (seq_start, key_start, int(max_len), None if max_key_len is None else int(max_key_len),
+           None if scale is None else float(scale), bool(causal), int(window))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _PackedAttention.apply(q, k, v, *how)
+    return _packed_forward(q, k, v, *how, need_lse=False)[0]
+
+
+def _packed_forward(q, k, v, seq_start, key_start, max_len, max_key_len, scale, causal, window,
+                    need_lse):
+    if max_key_len is not None and max_key_len < 0:
+        raise ValueError("max_len and max_key_len must not be negative")
+    return _hip.host().packed_attention(q, k, v, seq_start, key_start, max_len, scale, causal,
+                                        window, need_lse)
+
+
+def packed_attention_forward(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    seq_start: torch.Tensor,
+    *,
+    max_len: int,
+    key_start: torch.Tensor | None = None,
+    scale: float | None = None,
+    causal: bool = True,
+    window: int = 0,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(out, lse)``: :func:`packed_attention` without autograd and, for
+    :func:`packed_attention_backward`, fp32 [heads, tokens]: log2 of each query's sum
+    of 2^(score * log2 e), +inf where it sees nothing (of queries that belong to no
+    sequence nothing is written)."""
+    return _packed_forward(q, k, v, seq_start, key_start, int(max_len), None,
+                           None if scale is None else float(scale), bool(causal), int(window),
+                           need_lse=True)
+
+
+def packed_attention_backward(
+    grad_out: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    lse: torch.Tensor,
+    seq_start: torch.Tensor,
+    *,
+    max_len: int,
+    key_start: torch.Tensor | None = None,
+    max_key_len: int | None = None,
+    scale: float | None = None,
+    causal: bool = True,
+    window: int = 0,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(grad_q, grad_k, grad_v)`` of :func:`packed_attention` in bf16, from its
+    inputs and what :func:`packed_attention_forward` returned for them."""
+    return _hip.host().packed_attention_backward(
+        grad_out, q, k, v, out, lse, seq_start, key_start, int(max_len),
+        None if max_key_len is None else int(max_key_len),
+        None if scale is None else float(scale), bool(causal), int(window))
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, seq_start, key_start, max_len, max_key_len, scale, causal, window):
+        out, lse = _packed_forward(q, k, v, seq_start, key_start, max_len, max_key_len, scale,
+                                   causal, window, need_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, seq_start, key_start)
+        ctx.how = max_len, max_key_len, scale, causal, window
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        q, k, v, out, lse, seq_start, key_start = ctx.saved_tensors
+        max_len, max_key_len, scale, causal, window = ctx.how
+        dq, dk, dv = packed_attention_backward(
+            grad, q, k, v, out, lse, seq_start, max_len=max_len, key_start=key_start,
+            max_key_len=max_key_len, scale=scale, causal=causal, window=window)
+        need = ctx.needs_input_grad
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
+                None, None, None, None, None, None, None)
 
 
 def kv_cache_write(

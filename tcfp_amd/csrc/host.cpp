@@ -1057,6 +1057,306 @@ Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
   return out;
 }
 
+// ---- a decoder's training step -------------------------------------------------
+
+// [tokens, heads, dim] as a kernel takes it: dim contiguous, the strides of axes
+// that have a single place made up.
+struct Heads {
+  Tensor t;
+  int64_t token, head;
+};
+Heads strided_heads(const Tensor& x) {
+  const auto of = [](const Tensor& t) {
+    const int64_t head = t.size(1) > 1 ? t.stride(1) : t.size(2);
+    return Heads{t, t.size(0) > 1 ? t.stride(0) : t.size(1) * head, head};
+  };
+  const int64_t unit = 16 / x.element_size();
+  const Heads h = of(x);
+  // (strides past a descriptor's reach, or negative ones, are copied too)
+  if ((x.stride(2) == 1 || x.size(2) == 1) && h.token % unit == 0 && h.head % unit == 0 &&
+      h.token >= 0 && h.token <= (1 << 23) && h.head >= 0 && al16(x))
+    return h;
+  const Tensor c = x.contiguous();
+  const Tensor w = al16(c) ? c : c.clone();
+  return {w, w.size(1) * w.size(2), w.size(2)};
+}
+void need_bf16(const Tensor& t, const char* name) {
+  if (t.scalar_type() != at::kBFloat16)
+    type_error(std::string(name) + " must be torch.bfloat16, got " + dtype_str(t.scalar_type()));
+}
+
+Outs rotary(const Tensor& q_, const OptT& k_, const Tensor& positions_, const Tensor& freqs_,
+            bool interleaved, double amplitude, bool inverse) {
+  OnGpu g;
+  g.add(q_);
+  g.add(k_);
+  g.add(positions_);
+  g.add(freqs_);
+  const c10::DeviceGuard guard(g.device());
+  if (q_.dim() != 3)
+    value_error("q must have shape (tokens, heads, dim), got " + shape_str(q_.sizes()));
+  const int64_t tokens = q_.size(0), dim = q_.size(2);
+  const int dt = in_dtype(q_);
+  if (k_) {
+    check_heads(*k_, 0, dim, "k");
+    if (k_->scalar_type() != q_.scalar_type())
+      type_error(std::string("q and k must have one dtype, got ") + dtype_str(q_.scalar_type()) +
+                 " and " + dtype_str(k_->scalar_type()));
+    if (k_->size(0) != tokens)
+      value_error("q has " + std::to_string(tokens) + " tokens, k " + std::to_string(k_->size(0)));
+  }
+  if (positions_.scalar_type() != at::kLong)
+    type_error(std::string("positions must be torch.int64, got ") +
+               dtype_str(positions_.scalar_type()));
+  if (positions_.dim() != 1 || positions_.size(0) != tokens)
+    value_error("positions must have shape (" + std::to_string(tokens) + ",), got " +
+                shape_str(positions_.sizes()));
+  if (freqs_.scalar_type() != at::kDouble)
+    type_error(std::string("freqs must be torch.float64, got ") + dtype_str(freqs_.scalar_type()));
+  if (freqs_.dim() != 1 || freqs_.size(0) < 1 || 2 * freqs_.size(0) > dim ||
+      freqs_.size(0) > 2048)
+    value_error("freqs must have 1 to " + std::to_string(std::min<int64_t>(dim / 2, 2048)) +
+                " entries, one a pair of columns, got shape " + shape_str(freqs_.sizes()));
+  if (dim > 65536 || q_.size(1) > 65535 || (k_ && k_->size(1) > 65535))
+    value_error("at most 65535 heads of 65536 columns");
+  const Tensor positions = positions_.contiguous(), freqs = freqs_.contiguous();
+  const Heads q = strided_heads(q_), k = k_ ? strided_heads(*k_) : Heads{};
+  Tensor qo = g.empty(q_.sizes(), q_.scalar_type()), ko;
+  if (k_) ko = g.empty(k_->sizes(), k_->scalar_type());
+  check(tcfp_rotary(ptr(q.t), q.token, q.head, int(q_.size(1)), ptr(k.t), k.token, k.head,
+                    k_ ? int(k_->size(1)) : 0, dt, tokens, int(dim), ptr<int64_t>(positions),
+                    ptr<double>(freqs), int(2 * freqs.size(0)), interleaved ? 1 : 0,
+                    float(amplitude), inverse ? 1 : 0, ptr(qo), ptr(ko), g.stream()),
+        "rotary_embedding");
+  return outs(qo, ko);
+}
+
+// The arguments that attention within packed sequences and its backward share.
+struct PackedIn {
+  Heads q, k, v;
+  Tensor q_starts, k_starts;
+  int64_t tokens, keys, batch, max_len, max_key_len;
+  int heads, kv_heads, dim;
+  float scale;
+};
+PackedIn packed_inputs(OnGpu& g, const Tensor& q, const Tensor& k, const Tensor& v,
+                       const Tensor& starts, const OptT& key_starts, int64_t max_len,
+                       std::optional<int64_t> max_key_len, std::optional<double> scale,
+                       int64_t window) {
+  need_bf16(q, "q");
+  need_bf16(k, "k");
+  need_bf16(v, "v");
+  if (q.dim() != 3)
+    value_error("q must have shape (tokens, heads, dim), got " + shape_str(q.sizes()));
+  PackedIn p;
+  const int64_t dim = q.size(2), heads = q.size(1);
+  if (dim != 64 && dim != 128 && dim != 256)
+    value_error("the head dimension must be 64, 128 or 256, got " + std::to_string(dim));
+  check_heads(k, 0, dim, "k");
+  if (v.sizes() != k.sizes())
+    value_error("v must have k's shape " + shape_str(k.sizes()) + ", got " + shape_str(v.sizes()));
+  const int64_t kv_heads = k.size(1);
+  if (kv_heads < 1 || heads < 1 || heads > 65535 || heads % kv_heads != 0)
+    value_error("q's heads (" + std::to_string(heads) + ") must be a multiple of k's (" +
+                std::to_string(kv_heads) + ")");
+  p.tokens = q.size(0);
+  p.keys = k.size(0);
+  if (p.tokens > (1 << 29) || p.keys > (1 << 29)) value_error("at most 2^29 tokens");
+  const auto check_starts = [](const Tensor& t, const char* name) {
+    if (t.scalar_type() != at::kInt)
+      type_error(std::string(name) + " must be torch.int32, got " + dtype_str(t.scalar_type()));
+    if (t.dim() != 1 || t.size(0) < 1)
+      value_error(std::string(name) + " must have shape (sequences + 1,), got " +
+                  shape_str(t.sizes()));
+  };
+  check_starts(starts, "seq_start");
+  p.batch = starts.size(0) - 1;
+  p.q_starts = starts.contiguous();
+  p.k_starts = p.q_starts;
+  if (key_starts) {
+    check_starts(*key_starts, "key_start");
+    if (key_starts->size(0) != p.batch + 1)
+      value_error("key_start must have shape (" + std::to_string(p.batch + 1) + ",), got " +
+                  shape_str(key_starts->sizes()));
+    p.k_starts = key_starts->contiguous();
+  } else if (p.keys != p.tokens) {
+    value_error("q has " + std::to_string(p.tokens) + " tokens, k " + std::to_string(p.keys) +
+                ": key_start is needed");
+  }
+  if (p.batch > 65535) value_error("at most 65535 sequences, got " + std::to_string(p.batch));
+  if (p.batch == 0 && (p.tokens > 0 || p.keys > 0))
+    value_error("there are tokens but no sequences");
+  if (max_len < 0 || (max_key_len && *max_key_len < 0))
+    value_error("max_len and max_key_len must not be negative");
+  if (window < 0) value_error("window must not be negative, got " + std::to_string(window));
+  if (scale && !std::isfinite(float(*scale)))
+    value_error("scale must be finite, got " + std::to_string(*scale));
+  p.max_len = std::min(max_len, p.tokens);
+  p.max_key_len = std::min(max_key_len.value_or(key_starts ? p.keys : max_len), p.keys);
+  p.heads = int(heads);
+  p.kv_heads = int(kv_heads);
+  p.dim = int(dim);
+  p.scale = float(scale.value_or(1.0 / std::sqrt(double(dim))));
+  p.q = strided_heads(q);
+  p.k = strided_heads(k);
+  p.v = strided_heads(v);
+  return p;
+}
+
+Outs packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& starts,
+                      const OptT& key_starts, int64_t max_len, std::optional<double> scale,
+                      bool causal, int64_t window, bool need_lse) {
+  OnGpu g;
+  g.add(q);
+  g.add(k);
+  g.add(v);
+  g.add(starts);
+  g.add(key_starts);
+  const c10::DeviceGuard guard(g.device());
+  const PackedIn p =
+      packed_inputs(g, q, k, v, starts, key_starts, max_len, std::nullopt, scale, window);
+  Tensor out = g.empty({p.tokens, p.heads, p.dim}, at::kBFloat16), lse;
+  if (need_lse) lse = g.empty({p.heads, p.tokens}, at::kFloat);
+  check(tcfp_packed_attention(ptr(p.q.t), p.q.token, p.q.head, ptr(p.k.t), p.k.token, p.k.head,
+                              ptr(p.v.t), p.v.token, p.v.head, ptr<int32_t>(p.q_starts),
+                              ptr<int32_t>(p.k_starts), p.batch, p.tokens, p.keys, p.heads,
+                              p.kv_heads, p.dim, p.max_len, p.scale, causal ? 1 : 0, window,
+                              ptr(out), f32(lse), g.stream()),
+        "packed_attention");
+  return outs(out, lse);
+}
+
+Outs packed_attention_backward(const Tensor& grad, const Tensor& q, const Tensor& k,
+                               const Tensor& v, const Tensor& out_, const Tensor& lse_,
+                               const Tensor& starts, const OptT& key_starts, int64_t max_len,
+                               std::optional<int64_t> max_key_len, std::optional<double> scale,
+                               bool causal, int64_t window) {
+  OnGpu g;
+  g.add(grad);
+  g.add(q);
+  g.add(k);
+  g.add(v);
+  g.add(out_);
+  g.add(lse_);
+  g.add(starts);
+  g.add(key_starts);
+  const c10::DeviceGuard guard(g.device());
+  const PackedIn p =
+      packed_inputs(g, q, k, v, starts, key_starts, max_len, max_key_len, scale, window);
+  need_bf16(grad, "grad_out");
+  need_bf16(out_, "out");
+  for (const auto& [name, t] : {std::pair<const char*, const Tensor*>{"grad_out", &grad},
+                                std::pair<const char*, const Tensor*>{"out", &out_}})
+    if (t->sizes() != q.sizes())
+      value_error(std::string(name) + " must have q's shape " + shape_str(q.sizes()) + ", got " +
+                  shape_str(t->sizes()));
+  if (lse_.scalar_type() != at::kFloat || lse_.dim() != 2 || lse_.size(0) != p.heads ||
+      lse_.size(1) != p.tokens)
+    value_error("lse must hold a float32 for each head and token, shape (" +
+                std::to_string(p.heads) + ", " + std::to_string(p.tokens) + ")");
+  const Heads go = strided_heads(grad);
+  const Tensor out = whole(out_), lse = lse_.contiguous();
+  Tensor dq = g.empty(q.sizes(), at::kBFloat16), dk = g.empty(k.sizes(), at::kBFloat16),
+         dv = g.empty(v.sizes(), at::kBFloat16), ws;
+  const size_t nb = tcfp_packed_attention_backward_workspace_bytes(
+      p.tokens, p.keys, p.batch, p.max_key_len, p.heads, p.kv_heads, p.dim);
+  if (nb) ws = g.empty({int64_t(nb)}, at::kByte);
+  check(tcfp_packed_attention_backward(
+            ptr(go.t), go.token, go.head, ptr(p.q.t), p.q.token, p.q.head, ptr(p.k.t), p.k.token,
+            p.k.head, ptr(p.v.t), p.v.token, p.v.head, ptr(out), f32(lse),
+            ptr<int32_t>(p.q_starts), ptr<int32_t>(p.k_starts), p.batch, p.tokens, p.keys, p.heads,
+            p.kv_heads, p.dim, p.max_len, p.max_key_len, p.scale, causal ? 1 : 0, window, ptr(dq),
+            ptr(dk), ptr(dv), ptr(ws), nb, g.stream()),
+        "packed_attention_backward");
+  return outs(dq, dk, dv);
+}
+
+// The head's operands, checked.
+struct HeadIn {
+  Rows h, w;
+  Tensor targets;
+};
+HeadIn head_inputs(const Tensor& hidden, const Tensor& weight, const Tensor& targets) {
+  need_bf16(hidden, "hidden");
+  need_bf16(weight, "weight");
+  HeadIn in;
+  in.h = rows_of(hidden, "hidden");
+  if (weight.dim() != 2 || weight.size(1) != in.h.cols || weight.size(0) < 1)
+    value_error("weight must have shape (classes, " + std::to_string(in.h.cols) + "), got " +
+                shape_str(weight.sizes()));
+  if (in.h.cols < 8 || in.h.cols % 8 != 0)
+    value_error("the hidden dimension must be a multiple of 8, got " + std::to_string(in.h.cols));
+  in.w = rows_of(weight, "weight");
+  for (Rows* r : {&in.h, &in.w})  // (a single row's stride means nothing)
+    if (r->ld < r->cols || r->rows <= 1) r->ld = r->cols;
+  if (targets.scalar_type() != at::kLong)
+    type_error(std::string("targets must be torch.int64, got ") +
+               dtype_str(targets.scalar_type()));
+  if (targets.sizes() != hidden.sizes().slice(0, size_t(hidden.dim() - 1)))
+    value_error("targets must have shape " +
+                shape_str(hidden.sizes().slice(0, size_t(hidden.dim() - 1))) + ", got " +
+                shape_str(targets.sizes()));
+  in.targets = targets.contiguous();
+  return in;
+}
+
+// -> (losses, lse, total): total only with `reduce`, the losses' mean or sum and
+// the tokens that count.
+Outs linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& targets,
+                          int64_t ignore, bool reduce, bool mean) {
+  OnGpu g;
+  g.add(hidden);
+  g.add(weight);
+  g.add(targets);
+  const c10::DeviceGuard guard(g.device());
+  const HeadIn in = head_inputs(hidden, weight, targets);
+  Tensor losses = g.empty(targets.sizes(), at::kFloat), lse = g.empty({in.h.rows}, at::kFloat), total;
+  if (reduce) total = g.empty({2}, at::kFloat);
+  const size_t nb = tcfp_linear_cross_entropy_workspace_bytes(in.h.rows, in.w.rows);
+  Tensor ws = g.empty({int64_t(std::max<size_t>(nb, 16))}, at::kByte);
+  check(tcfp_linear_cross_entropy(ptr(in.h.t), in.h.ld, ptr(in.w.t), in.w.ld,
+                                  ptr<int64_t>(in.targets), ignore, in.h.rows, in.w.rows,
+                                  in.h.cols, f32(losses), f32(lse), mean ? 1 : 0, f32(total),
+                                  ptr(ws), nb, g.stream()),
+        "linear_cross_entropy");
+  return outs(losses, lse, total);
+}
+
+Outs linear_cross_entropy_backward(const Tensor& grad_, const Tensor& hidden, const Tensor& weight,
+                                   const Tensor& targets, const Tensor& lse_, const OptT& count,
+                                   int64_t ignore, bool need_h, bool need_w) {
+  OnGpu g;
+  g.add(grad_);
+  g.add(hidden);
+  g.add(weight);
+  g.add(targets);
+  g.add(lse_);
+  g.add(count);
+  const c10::DeviceGuard guard(g.device());
+  const HeadIn in = head_inputs(hidden, weight, targets);
+  if (lse_.scalar_type() != at::kFloat || lse_.numel() != in.h.rows)
+    value_error("lse must hold a float32 for each of the " + std::to_string(in.h.rows) +
+                " tokens");
+  if (grad_.scalar_type() != at::kFloat || (grad_.dim() != 0 && grad_.sizes() != targets.sizes()))
+    value_error("grad must be one float32, or hold one for each token");
+  if (count && (count->scalar_type() != at::kFloat || count->numel() != 1))
+    value_error("count must be one float32");
+  const bool each = grad_.dim() != 0;
+  const Tensor grad = grad_.contiguous(), lse = lse_.contiguous();
+  Tensor dh, dw;
+  if (need_h) dh = g.empty(hidden.sizes(), at::kBFloat16);
+  if (need_w) dw = g.empty(weight.sizes(), at::kBFloat16);
+  const size_t nb = tcfp_linear_cross_entropy_backward_workspace_bytes(
+      in.h.rows, in.w.rows, in.h.cols, need_h ? 1 : 0, need_w ? 1 : 0);
+  Tensor ws = g.empty({int64_t(std::max<size_t>(nb, 16))}, at::kByte);
+  check(tcfp_linear_cross_entropy_backward(
+            ptr(in.h.t), in.h.ld, ptr(in.w.t), in.w.ld, ptr<int64_t>(in.targets), ignore, f32(lse),
+            f32(grad), each ? 1 : 0, f32(opt(count)), in.h.rows, in.w.rows, in.h.cols, ptr(dh),
+            ptr(dw), ptr(ws), nb, g.stream()),
+        "linear_cross_entropy_backward");
+  return outs(dh, dw);
+}
+
 }  // namespace
 
 namespace pybind11::detail {
@@ -1112,4 +1412,9 @@ PYBIND11_MODULE(_tcfp_host, m) {
   m.def("kv_cache_write", &kv_cache_write, NoGil());
   m.def("kv_cache_read", &kv_cache_read, NoGil());
   m.def("paged_attention", &paged_attention, NoGil());
+  m.def("rotary", &rotary, NoGil());
+  m.def("packed_attention", &packed_attention, NoGil());
+  m.def("packed_attention_backward", &packed_attention_backward, NoGil());
+  m.def("linear_cross_entropy", &linear_cross_entropy, NoGil());
+  m.def("linear_cross_entropy_backward", &linear_cross_entropy_backward, NoGil());
 }

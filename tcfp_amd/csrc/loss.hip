@@ -1,0 +1,738 @@
+// Softmax cross entropy of a linear head over a large vocabulary, and its
+// gradients (gfx950).
+//
+//   z = h W^T,  lse = log sum exp z,  loss = lse - z[target]
+//   g = (softmax(z) - onehot(target)) * grad,  dh = g W,  dW = g^T h
+//
+// h [tokens, dim] and W [vocab, dim] are bf16; z is never stored.  Forward: one
+// product whose epilogue reduces every 256 (128) classes of a token to their
+// maximum and sum of exponentials, which a small launch joins.  Backward: for
+// a run of classes at a time, whose g [tokens, run] in bf16 fits a bounded
+// workspace, z is formed again with g as the epilogue, and g is the operand of
+// the products of dh, which are added up over the runs in fp32, and of dW, whose
+// rows the run owns.  g is rounded to bf16 once (2^-9 of each value, as the
+// results themselves are); all sums are fp32.
+#include <algorithm>
+
+#include "mfma_tiles.h"
+
+using namespace tcfp;
+
+namespace {
+
+// ---- the products -----------------------------------------------------------
+//
+// C[n][m] = sum over k of B[n][k] A[m][k] with both operands read as they lie in
+// memory: rows along k, or (TA, TB) rows of one k each, which LDS transposes on
+// the way into the registers.  So W serves z = h W^T and dh = g W, and g serves
+// dh = g W and dW = g^T h, without transposed copies.
+//
+// A workgroup owns T x T of C.  T = 256: eight waves, 2 along m and 4 along n,
+// 128 x 64 each; two stages of 64 k in LDS (128 KiB), one workgroup a CU.
+// T = 128: four waves of 64 x 64 and four stages, for outputs of few tiles.
+// A stage's copies are issued as soon as every wave has read its last operands
+// of the stage whose place they take, in the middle of that stage's products.
+constexpr int kStageK = 64;
+
+template <int T>
+struct Shape {
+  static constexpr int WAVES = T == 256 ? 8 : 4, THREADS = 64 * WAVES;
+  static constexpr int STAGES = T == 256 ? 2 : 4;
+  static constexpr int MB = T / 64, NB = 2;  // 32-row and 32-column blocks of a wave
+  static constexpr int WAVES_M = 2;
+  static constexpr int OPERAND = T * kStageK * 2, STAGE = 2 * OPERAND;
+};
+
+struct Product {
+  const uint16_t *a, *b;
+  int64_t lda, ldb;  // elements
+  int m, n, k;
+  int tiles_m, tiles_n;
+  int k_run;         // k of a split (blockIdx.y), a multiple of 64
+  // results: bf16 or fp32 [n, m], rows ldo apart
+  void* out;
+  int64_t ldo;
+  int64_t split_stride;
+  int add;           // fp32: to what is there
+  // the loss
+  const int64_t* targets;
+  int64_t ignore;
+  int64_t first;     // class of m = 0
+  int64_t classes;   // of the whole vocabulary
+  float2* part;      // [tiles_m, n]: maximum in units of log2, sum
+  float* picked;     // [n]: z of the target
+  const float* lse;
+  const float* grad;       // one a token (grad_step 1) or for all (0)
+  int grad_step;
+  const float* count;      // nullptr, or what grad is divided by
+};
+
+enum Epilogue { kBf16, kFp32, kStats, kGrad };
+
+// Offsets of one operand's copies into LDS: 4 instructions a wave and stage.
+// Rows along k: instruction q brings the rows 8 q ... of 128 bytes, whose eight
+// chunks of 16 bytes are permuted by (row / 2) % 8; rows of one k: instruction q
+// brings 1024 / (2 T) rows, whose chunks are permuted by 4 (row % 4), so that the
+// reads below meet every bank once.
+template <int T, bool ROWS_OF_K>
+struct Copies {
+  uint32_t off0, off1, step;
+  bool past0, past1;  // this lane's chunk lies outside
+  int chunk0, chunk1;
+  TCFP_DEV void init(int wave, int lane, int64_t ld, int at, int extent) {
+    if constexpr (!ROWS_OF_K) {
+      const int row = 32 * wave + (lane >> 3);
+      chunk0 = (lane & 7) ^ ((lane >> 4) & 7);
+      chunk1 = (lane & 7) ^ ((4 + (lane >> 4)) & 7);
+      off0 = uint32_t(row * ld * 2) + chunk0 * 16;
+      off1 = uint32_t(row * ld * 2) + chunk1 * 16;
+      step = uint32_t(8 * ld * 2);
+      past0 = past1 = false;
+    } else {
+      constexpr int CH = T / 8, R = 64 / CH;  // chunks of a row, rows an instruction
+      const int row = 4 * R * wave + lane / CH;
+      // (row % 4 of instruction i: for R == 2 it depends on i's parity)
+      chunk0 = (lane % CH) ^ (4 * ((lane / CH) & 3));
+      chunk1 = (lane % CH) ^ (4 * ((R + lane / CH) & 3));
+      off0 = uint32_t(row * ld * 2) + chunk0 * 16;
+      off1 = uint32_t(row * ld * 2) + chunk1 * 16;
+      step = uint32_t(R * ld * 2);
+      past0 = at + chunk0 * 8 >= extent;
+      past1 = at + chunk1 * 8 >= extent;
+    }
+  }
+};
+
+template <int T, bool TA, bool TB, int EPI>
+__global__ __launch_bounds__(Shape<T>::THREADS, 1) void product_kernel(Product g) {
+  using S = Shape<T>;
+  __shared__ __align__(16) uint8_t lds[S::STAGES * S::STAGE];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int wm = wave % S::WAVES_M, wn = wave / S::WAVES_M;
+
+  // Each XCD (workgroup b is on XCD b % 8) takes a run of tiles, in groups of
+  // four tile rows along n, so that its L2 holds both operands' panels.
+  int m0, n0;
+  {
+    const int tiles = g.tiles_m * g.tiles_n;
+    int l = int(blockIdx.x);
+    l = (l & 7) * (tiles >> 3) + min(l & 7, tiles & 7) + (l >> 3);
+    const int per = 4 * g.tiles_m, first = l / per * 4, rows = min(g.tiles_n - first, 4);
+    n0 = (first + l % per % rows) * T;
+    m0 = l % per / rows * T;
+  }
+  const int k0 = int(blockIdx.y) * g.k_run, k1 = min(g.k, k0 + g.k_run);
+  const int stages = (k1 - k0 + kStageK - 1) / kStageK;
+
+  Copies<T, TA> ca;
+  Copies<T, TB> cb;
+  ca.init(wave, lane, g.lda, m0, g.m);
+  cb.init(wave, lane, g.ldb, n0, g.n);
+  const uint32_t lds0 = lds_offset(lds);
+  // the copies of one operand's stage at k into LDS at `to` (whole chunks of 16
+  // bytes: behind an odd number of classes g has zeros)
+  auto copy_operand = [&](auto& c, auto of_k, const uint16_t* p, int64_t ld, int at, int extent, int k,
+                          uint32_t to) {
+    constexpr bool OF_K = decltype(of_k)::value;
+    const bool live = k < k1;
+    const uint16_t* base;
+    int64_t span;
+    if constexpr (OF_K) {
+      base = p + int64_t(k) * ld + at;
+      span = (int64_t(min(k1 - k, kStageK)) - 1) * ld + ((extent - at + 7) & ~7);
+    } else {
+      base = p + int64_t(at) * ld + k;
+      span = (int64_t(min(extent - at, T)) - 1) * ld + ((k1 - k + 7) & ~7);
+    }
+    const v4i rsrc = make_rsrc(base, live ? uint32_t(span * 2) : 0u);
+    uint32_t o0 = c.past0 ? kOutOfRange : c.off0, o1 = c.past1 ? kOutOfRange : c.off1;
+    if constexpr (!OF_K) {
+      // (a run of k ends inside a row)
+      if (k + c.chunk0 * 8 >= k1) o0 = kOutOfRange;
+      if (k + c.chunk1 * 8 >= k1) o1 = kOutOfRange;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) copy16(rsrc, ((i & 1) ? o1 : o0) + i * c.step, to + i * 1024);
+  };
+  auto copy_stage = [&](int t) {
+    const uint32_t to = lds0 + uint32_t(t % S::STAGES) * S::STAGE + uint32_t(wave) * 4096;
+    const int k = k0 + t * kStageK;
+    copy_operand(ca, std::integral_constant<bool, TA>{}, g.a, g.lda, m0, g.m, k, to);
+    copy_operand(cb, std::integral_constant<bool, TB>{}, g.b, g.ldb, n0, g.n, k, to + S::OPERAND);
+  };
+
+  // operand reads: block x of 32 rows (columns), k step s of 16
+  const int swz = (col >> 1) & 7;
+  const int grp = (lane >> 4) & 1, i16 = lane & 15;
+  auto read_rows = [&](const uint8_t* base, int x, int s) {
+    return read16(base + (32 * x + col) * 128 + (((2 * s + half) ^ swz) << 4));
+  };
+  auto read_of_k = [&](const uint8_t* base, int x, int s) {
+    const int row = 16 * s + 8 * half + (i16 >> 2);
+    const int chunk = (4 * x + 2 * grp + ((i16 & 3) >> 1)) ^ (4 * (i16 >> 2));
+    const uint8_t* p = base + row * (2 * T) + chunk * 16 + (i16 & 1) * 8;
+    return read_transposed(p, p + 4 * (2 * T));
+  };
+  struct Frags {
+    v8bf a[2][S::MB], b[2][S::NB];
+  };
+  auto read_half = [&](Frags& f, int t, int h) {
+    const uint8_t* st = lds + (t % S::STAGES) * S::STAGE;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int x = 0; x < S::MB; ++x)
+        f.a[s][x] = TA ? read_of_k(st, wm * S::MB + x, 2 * h + s)
+                       : read_rows(st, wm * S::MB + x, 2 * h + s);
+#pragma unroll
+      for (int x = 0; x < S::NB; ++x)
+        f.b[s][x] = TB ? read_of_k(st + S::OPERAND, wn * S::NB + x, 2 * h + s)
+                       : read_rows(st + S::OPERAND, wn * S::NB + x, 2 * h + s);
+    }
+  };
+  v16f acc[S::MB][S::NB];
+#pragma unroll
+  for (int x = 0; x < S::MB; ++x)
+#pragma unroll
+    for (int y = 0; y < S::NB; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
+  auto multiply = [&](const Frags& f, int s) {
+#pragma unroll
+    for (int x = 0; x < S::MB; ++x)
+#pragma unroll
+      for (int y = 0; y < S::NB; ++y) acc[x][y] = mfma(f.a[s][x], f.b[s][y], acc[x][y]);
+  };
+  // (keeps the products where they stand, ahead of the barrier and copies that
+  // follow)
+  auto pin = [&]() {
+#pragma unroll
+    for (int x = 0; x < S::MB; ++x)
+#pragma unroll
+      for (int y = 0; y < S::NB; ++y) asm volatile("" : "+v"(acc[x][y]));
+  };
+
+  // (copies past the last stage read nothing and keep the count of what is in
+  // flight)
+  constexpr int kAhead = 8 * (S::STAGES - 2);
+#pragma unroll
+  for (int t = 0; t < S::STAGES - 1; ++t) copy_stage(t);
+  wait_and_sync<kAhead>();
+  Frags f0, f1;
+  copy_stage(S::STAGES - 1);
+  read_half(f0, 0, 0);
+  for (int t = 0; t < stages; ++t) {
+    read_half(f1, t, 1);
+    multiply(f0, 0);
+    pin();
+    wait_and_sync<kAhead>();
+    multiply(f0, 1);
+    pin();
+    __builtin_amdgcn_sched_barrier(0);
+    copy_stage(t + S::STAGES);
+    __builtin_amdgcn_sched_barrier(0);
+    read_half(f0, t + 1, 0);
+    multiply(f1, 0);
+    multiply(f1, 1);
+  }
+  // (the copies still in flight read nothing, but write zeros)
+  wait_and_sync<0>();
+
+  // ---- epilogues: acc[x][y][r] is m = m_of(x, r), n = n_of(y) ----------------
+  const int mw = wm * S::MB * 32, nw = wn * 64;
+  auto m_of = [&](int x, int r) { return mw + 32 * x + 8 * (r >> 2) + 4 * half + (r & 3); };
+  if constexpr (EPI == kFp32) {
+    float* out = static_cast<float*>(g.out) + int64_t(blockIdx.y) * g.split_stride;
+#pragma unroll
+    for (int y = 0; y < S::NB; ++y) {
+      const int n = n0 + nw + 32 * y + col;
+      if (n >= g.n) continue;
+#pragma unroll
+      for (int x = 0; x < S::MB; ++x)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int m = m0 + m_of(x, 4 * q);
+          if (m >= g.m) continue;
+          float4* p = reinterpret_cast<float4*>(out + int64_t(n) * g.ldo + m);
+          float4 v = make_float4(acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2],
+                                 acc[x][y][4 * q + 3]);
+          if (g.add) {
+            const float4 o = *p;
+            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+          }
+          *p = v;
+        }
+    }
+    return;
+  }
+  if constexpr (EPI == kStats) {
+    float2* both = reinterpret_cast<float2*>(lds);  // [wave along m][n of the tile]
+#pragma unroll
+    for (int y = 0; y < S::NB; ++y) {
+      const int n = n0 + nw + 32 * y + col;
+      const bool in = n < g.n;
+      const int64_t want = in ? g.targets[n] - g.first - m0 : -1;
+      const int w = want >= 0 && want < T ? int(want) : -1;
+      // the target's place among the lane's values, if it is there
+      const int rel = w - mw - 4 * half;
+      const bool mine = w >= 0 && m0 + w < g.m && rel >= 0 && rel < 32 * S::MB && (rel & 4) == 0;
+      float top = -INFINITY, sum = 0.0f, pick = 0.0f;
+      if (m0 + T > g.m) {
+#pragma unroll
+        for (int x = 0; x < S::MB; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (m0 + m_of(x, r) >= g.m) acc[x][y][r] = -INFINITY;
+      }
+#pragma unroll
+      for (int x = 0; x < S::MB; ++x) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          pick = rel == 32 * x + 8 * (r >> 2) + (r & 3) ? acc[x][y][r] : pick;
+          top = fmaxf(top, acc[x][y][r]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float off = top == -INFINITY ? 0.0f : top * kLog2e;
+#pragma unroll
+      for (int x = 0; x < S::MB; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          sum += exp2_fast(__builtin_fmaf(acc[x][y][r], kLog2e, -off));
+      sum += __shfl_xor(sum, 32);
+      if (half == 0) both[wm * T + nw + 32 * y + col] = make_float2(off, sum);
+      if (mine) g.picked[n] = pick;
+    }
+    __syncthreads();
+    const int t = threadIdx.x, n = n0 + t;
+    if (t < T && n < g.n) {
+      const float2 p = both[t], q = both[T + t];
+      // (a wave without classes has sum 0 and must not raise the maximum)
+      const float top = q.y == 0.0f ? p.x : p.y == 0.0f ? q.x : fmaxf(p.x, q.x);
+      const float sum = p.y * exp2_fast(p.x - top) + (q.y == 0.0f ? 0.0f : q.y * exp2_fast(q.x - top));
+      g.part[int64_t(m0 / T) * g.n + n] = make_float2(top, sum);
+    }
+    return;
+  }
+  if constexpr (EPI == kBf16 || EPI == kGrad) {
+    constexpr int ROW = 2 * T, CH = ROW / 16;
+#pragma unroll
+    for (int y = 0; y < S::NB; ++y) {
+      const int nl = nw + 32 * y + col, n = n0 + nl;
+      float scale = 0.0f, off = 0.0f;
+      int w = -1;
+      bool keep = false;
+      if constexpr (EPI == kGrad) {
+        if (n < g.n) {
+          const int64_t target = g.targets[n], want = target - g.first - m0;
+          keep = target != g.ignore;
+          w = want >= 0 && want < T ? int(want) : -1;
+          scale = g.grad[int64_t(n) * g.grad_step];
+          if (g.count) scale /= *g.count;
+          // (a target outside the vocabulary has a loss that is NaN, and so are
+          // its gradients)
+          if (target < 0 || target >= g.classes) scale = NAN;
+          off = g.lse[n] * kLog2e;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < S::MB; ++x)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int m = m_of(x, 4 * q);
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            v[r] = acc[x][y][4 * q + r];
+            if constexpr (EPI == kGrad) {
+              float p = exp2_fast(__builtin_fmaf(v[r], kLog2e, -off));
+              if (m + r == w) p -= 1.0f;
+              v[r] = keep && m0 + m + r < g.m ? p * scale : 0.0f;
+            }
+          }
+          const int chunk = (m >> 3) ^ (nl & (CH - 1));
+          *reinterpret_cast<uint2*>(lds + nl * ROW + chunk * 16 + (m & 4) * 2) =
+              make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+        }
+    }
+    __syncthreads();
+    uint16_t* out = static_cast<uint16_t*>(g.out);
+    // (of g whole tiles are written: what lies behind the classes is zero)
+    const int cols = EPI == kGrad ? m0 + T : g.m;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < T * CH; i += S::THREADS) {
+      const int nl = i / CH, c = i % CH, n = n0 + nl, m = m0 + c * 8;
+      if (n < g.n && m < cols)
+        *reinterpret_cast<uint4*>(out + int64_t(n) * g.ldo + m) =
+            *reinterpret_cast<const uint4*>(lds + nl * ROW + ((c ^ (nl & (CH - 1))) << 4));
+    }
+  }
+}
+
+// ---- the joins ----------------------------------------------------------------
+
+// Every token's lse and loss from its partial maxima and sums; sums[block] =
+// (sum of the block's losses, tokens that count).  32 tokens a block, eight
+// threads each.
+__global__ __launch_bounds__(256) void join_losses_kernel(
+    const float2* __restrict__ part, int parts, const float* __restrict__ picked,
+    const int64_t* __restrict__ targets, int64_t ignore, int64_t classes, int tokens,
+    float* __restrict__ losses, float* __restrict__ lse, double2* __restrict__ sums) {
+  __shared__ float2 s[8][32];
+  const int tl = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int t = int(blockIdx.x) * 32 + tl;
+  float top = -INFINITY, sum = 0.0f;
+  if (t < tokens)
+    for (int i = slice; i < parts; i += 8) {
+      const float2 p = part[int64_t(i) * tokens + t];
+      if (p.y == 0.0f) continue;
+      const float next = fmaxf(top, p.x);
+      sum = (sum == 0.0f ? 0.0f : sum * exp2_fast(top - next)) + p.y * exp2_fast(p.x - next);
+      top = next;
+    }
+  s[slice][tl] = make_float2(top, sum);
+  __syncthreads();
+  double loss = 0.0, count = 0.0;
+  if (slice == 0 && t < tokens) {
+    for (int i = 1; i < 8; ++i) {
+      const float2 p = s[i][tl];
+      if (p.y == 0.0f) continue;
+      const float next = fmaxf(top, p.x);
+      sum = (sum == 0.0f ? 0.0f : sum * exp2_fast(top - next)) + p.y * exp2_fast(p.x - next);
+      top = next;
+    }
+    const float l = (top + log2_fast(sum)) * kLn2;
+    const int64_t target = targets[t];
+    const bool keep = target != ignore;
+    const float each = !keep ? 0.0f : target < 0 || target >= classes ? NAN : l - picked[t];
+    lse[t] = l;
+    losses[t] = each;
+    loss = each;
+    count = keep ? 1.0 : 0.0;
+  }
+  if (sums && threadIdx.x < 64) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      loss += __shfl_xor(loss, o);
+      count += __shfl_xor(count, o);
+    }
+    if (threadIdx.x == 0) sums[blockIdx.x] = make_double2(loss, count);
+  }
+}
+
+// total[0] = the losses' sum or mean, total[1] = the tokens that count; one
+// workgroup, in one order.
+__global__ __launch_bounds__(256) void total_loss_kernel(const double2* __restrict__ sums, int n,
+                                                         int mean, float* __restrict__ total) {
+  __shared__ double2 s[256];
+  double a = 0.0, b = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256) a += sums[i].x, b += sums[i].y;
+  s[threadIdx.x] = make_double2(a, b);
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (int(threadIdx.x) < o) {
+      s[threadIdx.x].x += s[threadIdx.x + o].x;
+      s[threadIdx.x].y += s[threadIdx.x + o].y;
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    total[0] = float(mean ? s[0].x / s[0].y : s[0].x);
+    total[1] = float(s[0].y);
+  }
+}
+
+// out = the sum of `splits` fp32 [n, m] arrays in bf16, in order; eight columns a
+// thread.
+__global__ __launch_bounds__(256) void round_sum_kernel(const float* __restrict__ part, int splits,
+                                                        int64_t stride, int64_t eights,
+                                                        uint16_t* __restrict__ out) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= eights) return;
+  float v[8] = {};
+  for (int s = 0; s < splits; ++s) {
+    const float4* p = reinterpret_cast<const float4*>(part + s * stride) + 2 * i;
+    const float4 a = p[0], b = p[1];
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+  }
+  reinterpret_cast<uint4*>(out)[i] =
+      make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+}
+
+// ---- plans ----------------------------------------------------------------------
+
+constexpr int kCus = 256;
+// g of a run of classes takes at most this much of the workspace, but for runs
+// of 256 classes.
+constexpr int64_t kRunBytes = int64_t(256) << 20;
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+int launch_status() { return hipGetLastError() == hipSuccess ? TCFP_OK : TCFP_ERR_HIP; }
+
+// The tile of z: 256 where that gives every CU one.
+int logits_tile(int64_t tokens, int64_t classes) {
+  return ceil_div(tokens, 256) * ceil_div(classes, 256) >= kCus ? 256 : 128;
+}
+// Classes of a run of the backward pass (a multiple of 256, whole tiles).
+int64_t run_of(int64_t tokens, int64_t vocab) {
+  // (rows of a run stay within a descriptor's reach)
+  const int64_t most = std::clamp<int64_t>(
+      kRunBytes / (2 * std::max<int64_t>(tokens, 1)) / 256, 1, 4096) * 256;
+  const int64_t all = ceil_div(vocab, 256) * 256;
+  const int64_t runs = ceil_div(all, most);
+  return ceil_div(ceil_div(all, runs), 256) * 256;
+}
+// How C [n, m] over k is cut: tile, splits of k.
+struct Cut {
+  int tile, splits, k_run;
+};
+Cut cut_of(int64_t n, int64_t m, int64_t k) {
+  Cut c{256, 1, int(ceil_div(k, kStageK) * kStageK)};
+  if (ceil_div(n, 256) * ceil_div(m, 256) >= kCus) return c;
+  c.tile = 128;
+  const int64_t tiles = ceil_div(n, 128) * ceil_div(m, 128);
+  // splits of at least eight stages, to one workgroup a CU
+  int64_t splits = std::min(kCus / std::max<int64_t>(tiles, 1), k / (8 * kStageK));
+  if (splits < 2) return c;
+  c.k_run = int(ceil_div(ceil_div(k, splits), kStageK) * kStageK);
+  c.splits = int(ceil_div(k, c.k_run));
+  return c;
+}
+
+template <int T, bool TA, bool TB, int EPI>
+int launch(Product p, int splits, hipStream_t st) {
+  p.tiles_m = int(ceil_div(p.m, T));
+  p.tiles_n = int(ceil_div(p.n, T));
+  const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
+  if (!grid_x_fits(tiles, Shape<T>::THREADS) || tiles > INT32_MAX) return TCFP_ERR_SHAPE;
+  product_kernel<T, TA, TB, EPI>
+      <<<dim3(unsigned(tiles), unsigned(splits)), Shape<T>::THREADS, 0, st>>>(p);
+  return launch_status();
+}
+template <bool TA, bool TB, int EPI>
+int launch_tile(int tile, const Product& p, int splits, hipStream_t st) {
+  return tile == 256 ? launch<256, TA, TB, EPI>(p, splits, st)
+                     : launch<128, TA, TB, EPI>(p, splits, st);
+}
+
+struct Layout {
+  int64_t run;      // classes
+  Cut dh, dw;
+  size_t g, sum_h, sum_w;  // bytes: g of a run, fp32 sums of dh and of dW
+};
+Layout layout_of(int64_t tokens, int64_t vocab, int64_t dim, bool need_h, bool need_w) {
+  Layout l{};
+  l.run = run_of(tokens, vocab);
+  l.g = align256(size_t(tokens) * size_t(l.run) * 2);
+  if (need_h) {
+    l.dh = cut_of(tokens, dim, l.run);
+    if (l.dh.splits > 1 || l.run < vocab)
+      l.sum_h = align256(size_t(l.dh.splits) * size_t(tokens) * size_t(dim) * 4);
+  }
+  if (need_w) {
+    l.dw = cut_of(std::min(l.run, vocab), dim, tokens);
+    if (l.dw.splits > 1)
+      l.sum_w = align256(size_t(l.dw.splits) * size_t(std::min(l.run, vocab)) * size_t(dim) * 4);
+  }
+  return l;
+}
+
+int check_sizes(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int64_t tokens,
+                int64_t vocab, int64_t dim) {
+  if (tokens < 0 || vocab < 1 || dim < 8 || dim % 8 || tokens > INT32_MAX / 2 ||
+      vocab > INT32_MAX / 2 || dim > INT32_MAX / 2 || ldh < dim || ldw < dim)
+    return TCFP_ERR_SHAPE;
+  // (32-bit offsets within a tile's rows)
+  if (256 * ldh * 2 + dim * 2 >= kMaxSpan || 256 * ldw * 2 + dim * 2 >= kMaxSpan)
+    return TCFP_ERR_SHAPE;
+  if (!aligned16(hidden) || !aligned16(weight) || ldh % 8 || ldw % 8) return TCFP_ERR_ALIGN;
+  return TCFP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tcfp_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t vocab) {
+  if (tokens <= 0 || vocab <= 0) return 0;
+  const int64_t parts = ceil_div(vocab, logits_tile(tokens, vocab));
+  return align256(size_t(parts) * size_t(tokens) * 8) + align256(size_t(tokens) * 4) +
+         align256(size_t(ceil_div(tokens, 32)) * 16);
+}
+
+int tcfp_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+                              const int64_t* targets, int64_t ignore, int64_t tokens,
+                              int64_t vocab, int64_t dim, float* losses, float* lse, int mean,
+                              float* total, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  const int rc = check_sizes(hidden, ldh, weight, ldw, tokens, vocab, dim);
+  if (rc != TCFP_OK) return rc;
+  if (!workspace || workspace_bytes < tcfp_linear_cross_entropy_workspace_bytes(tokens, vocab) ||
+      !aligned16(workspace)) {
+    if (tokens > 0) return TCFP_ERR_WORKSPACE;
+  }
+  const auto st = static_cast<hipStream_t>(stream);
+  if (tokens == 0) {
+    if (total) total_loss_kernel<<<1, 256, 0, st>>>(nullptr, 0, mean, total);
+    return launch_status();
+  }
+  const int tile = logits_tile(tokens, vocab);
+  const int64_t parts = ceil_div(vocab, tile);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  Product p{};
+  p.a = static_cast<const uint16_t*>(weight);
+  p.b = static_cast<const uint16_t*>(hidden);
+  p.lda = ldw;
+  p.ldb = ldh;
+  p.m = int(vocab);
+  p.n = int(tokens);
+  p.k = int(dim);
+  p.k_run = int(ceil_div(dim, kStageK) * kStageK);
+  p.targets = targets;
+  p.classes = vocab;
+  p.part = reinterpret_cast<float2*>(ws);
+  ws += align256(size_t(parts) * size_t(tokens) * 8);
+  p.picked = reinterpret_cast<float*>(ws);
+  ws += align256(size_t(tokens) * 4);
+  double2* sums = total ? reinterpret_cast<double2*>(ws) : nullptr;
+  const int done = launch_tile<false, false, kStats>(tile, p, 1, st);
+  if (done != TCFP_OK) return done;
+  const unsigned blocks = unsigned(ceil_div(tokens, 32));
+  join_losses_kernel<<<blocks, 256, 0, st>>>(p.part, int(parts), p.picked, targets, ignore, vocab,
+                                             int(tokens), losses, lse, sums);
+  if (total) total_loss_kernel<<<1, 256, 0, st>>>(sums, int(blocks), mean, total);
+  return launch_status();
+}
+
+size_t tcfp_linear_cross_entropy_backward_workspace_bytes(int64_t tokens, int64_t vocab,
+                                                          int64_t dim, int need_hidden,
+                                                          int need_weight) {
+  if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
+  const Layout l = layout_of(tokens, vocab, dim, need_hidden != 0, need_weight != 0);
+  return l.g + l.sum_h + l.sum_w;
+}
+
+int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const void* weight,
+                                       int64_t ldw, const int64_t* targets, int64_t ignore,
+                                       const float* lse, const float* grad, int64_t grad_step,
+                                       const float* count, int64_t tokens, int64_t vocab,
+                                       int64_t dim, void* grad_hidden, void* grad_weight,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_sizes(hidden, ldh, weight, ldw, tokens, vocab, dim);
+  if (rc != TCFP_OK) return rc;
+  if (!aligned16(grad_hidden) || !aligned16(grad_weight)) return TCFP_ERR_ALIGN;
+  if (grad_step != 0 && grad_step != 1) return TCFP_ERR_SHAPE;
+  const bool need_h = grad_hidden != nullptr, need_w = grad_weight != nullptr;
+  if (!need_h && !need_w) return TCFP_OK;
+  const auto st = static_cast<hipStream_t>(stream);
+  if (tokens == 0) {
+    if (need_w) {
+      const int64_t eights = vocab * dim / 8;
+      if (!grid_x_fits(ceil_div(eights, 256), 256)) return TCFP_ERR_SHAPE;
+      round_sum_kernel<<<unsigned(ceil_div(eights, 256)), 256, 0, st>>>(
+          nullptr, 0, 0, eights, static_cast<uint16_t*>(grad_weight));
+    }
+    return launch_status();
+  }
+  const Layout l = layout_of(tokens, vocab, dim, need_h, need_w);
+  if (!workspace || workspace_bytes < l.g + l.sum_h + l.sum_w || !aligned16(workspace))
+    return TCFP_ERR_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  uint16_t* g = reinterpret_cast<uint16_t*>(ws);
+  float* sum_h = reinterpret_cast<float*>(ws + l.g);
+  float* sum_w = reinterpret_cast<float*>(ws + l.g + l.sum_h);
+  const auto* h = static_cast<const uint16_t*>(hidden);
+  const auto* w = static_cast<const uint16_t*>(weight);
+  auto round_sum = [&](const float* part, int splits, int64_t values, uint16_t* out) {
+    const int64_t eights = values / 8, blocks = ceil_div(eights, 256);
+    if (!grid_x_fits(blocks, 256)) return int(TCFP_ERR_SHAPE);
+    round_sum_kernel<<<unsigned(blocks), 256, 0, st>>>(part, splits, values, eights, out);
+    return launch_status();
+  };
+  for (int64_t v0 = 0; v0 < vocab; v0 += l.run) {
+    const int64_t classes = std::min(l.run, vocab - v0);
+    Product p{};
+    p.a = w + v0 * ldw;
+    p.b = h;
+    p.lda = ldw;
+    p.ldb = ldh;
+    p.m = int(classes);
+    p.n = int(tokens);
+    p.k = int(dim);
+    p.k_run = int(ceil_div(dim, kStageK) * kStageK);
+    p.out = g;
+    p.ldo = l.run;
+    p.targets = targets;
+    p.ignore = ignore;
+    p.first = v0;
+    p.classes = vocab;
+    p.lse = lse;
+    p.grad = grad;
+    p.grad_step = int(grad_step);
+    p.count = count;
+    int done = launch_tile<false, false, kGrad>(logits_tile(tokens, classes), p, 1, st);
+    if (done != TCFP_OK) return done;
+    if (need_h) {
+      // dh[t][d] += sum over the run's classes of g[t][v] W[v][d]
+      Product q{};
+      q.a = w + v0 * ldw;
+      q.b = g;
+      q.lda = ldw;
+      q.ldb = l.run;
+      q.m = int(dim);
+      q.n = int(tokens);
+      q.k = int(classes);
+      q.k_run = l.dh.k_run;
+      if (l.sum_h) {
+        q.out = sum_h;
+        q.ldo = dim;
+        q.split_stride = tokens * dim;
+        q.add = v0 > 0;
+        // (a last, shorter run may leave splits without classes: nothing to add)
+        const int splits = v0 > 0 ? int(std::min<int64_t>(l.dh.splits, ceil_div(classes, l.dh.k_run)))
+                                  : l.dh.splits;
+        done = launch_tile<true, false, kFp32>(l.dh.tile, q, splits, st);
+      } else {
+        q.out = grad_hidden;
+        q.ldo = dim;
+        done = launch_tile<true, false, kBf16>(l.dh.tile, q, 1, st);
+      }
+      if (done != TCFP_OK) return done;
+    }
+    if (need_w) {
+      // dW[v][d] = sum over tokens of g[t][v] h[t][d]
+      Product q{};
+      q.a = h;
+      q.b = g;
+      q.lda = ldh;
+      q.ldb = l.run;
+      q.m = int(dim);
+      q.n = int(classes);
+      q.k = int(tokens);
+      q.k_run = l.dw.k_run;
+      uint16_t* out = static_cast<uint16_t*>(grad_weight) + v0 * dim;
+      q.ldo = dim;
+      if (l.dw.splits > 1) {
+        q.out = sum_w;
+        q.split_stride = classes * dim;
+        done = launch_tile<true, true, kFp32>(l.dw.tile, q, l.dw.splits, st);
+        if (done == TCFP_OK) done = round_sum(sum_w, l.dw.splits, classes * dim, out);
+      } else {
+        q.out = out;
+        done = launch_tile<true, true, kBf16>(l.dw.tile, q, 1, st);
+      }
+      if (done != TCFP_OK) return done;
+    }
+  }
+  if (need_h && l.sum_h)
+    return round_sum(sum_h, l.dh.splits, tokens * dim, static_cast<uint16_t*>(grad_hidden));
+  return TCFP_OK;
+}
+
+}  // extern "C"

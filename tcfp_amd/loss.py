@@ -1,0 +1,113 @@
+"""Softmax cross entropy of a linear head over a large vocabulary, with its
+gradients, without storing the logits (HIP, gfx950; no reference counterpart).
+
+The head of a language model multiplies the last hidden states with a weight of
+one row a class; its logits, tokens x classes, are the largest matrix of a
+training step.  Here the product's own epilogue reduces them to each token's
+maximum and sum of exponentials, and the backward pass forms them again, a run of
+classes at a time: memory beside the inputs and gradients stays bounded (the
+backward's workspace: 256 MiB for the run's gradients of the logits, and fp32
+sums of the hidden states' gradient).
+
+Every op runs on the tensors' GPU and current stream; there is no CPU path.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _hip
+
+__all__ = ["linear_cross_entropy", "linear_cross_entropy_forward", "linear_cross_entropy_backward"]
+
+
+def linear_cross_entropy(
+    hidden: torch.Tensor,
+    weight: torch.Tensor,
+    targets: torch.Tensor,
+    *,
+    ignore_index: int = -100,
+    reduction: str = "mean",
+) -> torch.Tensor:
+    """Cross entropy of ``hidden @ weight.T`` with ``targets``, fp32.
+
+    ``hidden`` [..., D] and ``weight`` [classes, D] are bf16 (a head kept in fp32 is
+    cast where it is used: ``weight.bfloat16()``), D a multiple of 8, rows of 2-D
+    tensors may be apart; ``targets`` [...] int64.  Tokens whose target is
+    ``ignore_index`` are left out: their loss is 0, their hidden state gets a zero
+    gradient, and the mean is over the others (NaN if there are none).  A target that
+    is neither that nor a class gives NaN.  Products and sums are fp32 (the
+    reduction's fp64).
+
+    ``reduction`` is ``"mean"``, ``"sum"`` or ``"none"`` (a loss for every token).
+    Differentiable in ``hidden`` and ``weight``, once; gradients are bf16.  The hidden
+    states of tokens left out are read all the same: a value there that is not
+    finite reaches the weight's gradient.
+    """
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _LinearCrossEntropy.apply(hidden, weight, targets, int(ignore_index), reduction)
+    losses, _, total = _forward(hidden, weight, targets, ignore_index, reduction)
+    return losses if reduction == "none" else total[0]
+
+
+def _forward(hidden, weight, targets, ignore_index, reduction):
+    return _hip.host().linear_cross_entropy(hidden, weight, targets, int(ignore_index),
+                                            reduction != "none", reduction == "mean")
+
+
+def linear_cross_entropy_forward(
+    hidden: torch.Tensor,
+    weight: torch.Tensor,
+    targets: torch.Tensor,
+    *,
+    ignore_index: int = -100,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(losses, lse)`` of every token, fp32: :func:`linear_cross_entropy` without
+    autograd or reduction, and the log sum of exponentials of its logits, which
+    :func:`linear_cross_entropy_backward` takes."""
+    return _forward(hidden, weight, targets, ignore_index, "none")[:2]
+
+
+def linear_cross_entropy_backward(
+    grad: torch.Tensor,
+    hidden: torch.Tensor,
+    weight: torch.Tensor,
+    targets: torch.Tensor,
+    lse: torch.Tensor,
+    *,
+    count: torch.Tensor | None = None,
+    ignore_index: int = -100,
+    need_hidden_grad: bool = True,
+    need_weight_grad: bool = True,
+) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """``(grad_hidden, grad_weight)`` in bf16 (None where not asked for) of
+    :func:`linear_cross_entropy`.
+
+    ``grad`` (fp32) is the gradient of every token's loss, or one value for all of
+    them, which ``count`` (one fp32 value on the device: the tokens of a mean)
+    divides; ``lse`` is what :func:`linear_cross_entropy_forward` returned.
+    """
+    return _hip.host().linear_cross_entropy_backward(grad, hidden, weight, targets, lse, count,
+                                                     int(ignore_index), bool(need_hidden_grad),
+                                                     bool(need_weight_grad))
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
+        losses, lse, total = _forward(hidden, weight, targets, ignore_index, reduction)
+        count = total[1] if reduction == "mean" else None
+        ctx.save_for_backward(hidden, weight, targets, lse, count)
+        ctx.ignore_index = ignore_index
+        return losses if reduction == "none" else total[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        hidden, weight, targets, lse, count = ctx.saved_tensors
+        need_h, need_w = ctx.needs_input_grad[:2]
+        dh, dw = linear_cross_entropy_backward(
+            grad, hidden, weight, targets, lse, count=count, ignore_index=ctx.ignore_index,
+            need_hidden_grad=need_h, need_weight_grad=need_w)
+        return dh, dw, None, None, None

@@ -1,0 +1,335 @@
+"""Cross entropy of a linear head and its gradients against the formulas in 64 bits.
+
+Tolerances (per element).  A sum of n products in fp32 is within n 2^-23 of the sum
+of their sizes (each of n additions off by half a step, or a whole one where the
+matrix cores cut bits off): a logit within dz = D 2^-23 sum |h w|.  A softmax
+probability is then off by 2 dz + 2^-20 of itself (both exponentials, their
+arguments and the sum of V terms, which is within V 2^-24 of itself), a loss by
+twice the largest dz and 2^-22 of the sizes it is a difference of.  The gradient of
+a logit is rounded to bf16, 2^-8 of itself, and so is each result."""
+import math
+
+import pytest
+import torch
+
+from tcfp_amd import loss as L
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+HALF = 2.0**-8
+
+
+def inputs(dev, tokens, d, vocab, seed=0, ignored=0.0, spread=2.0):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(tokens, d, generator=g).to(BF16).to(dev)
+    w = (torch.randn(vocab, d, generator=g) * (spread / math.sqrt(d))).to(BF16).to(dev)
+    t = torch.randint(0, vocab, (tokens,), generator=g)
+    if ignored:
+        t[torch.rand(tokens, generator=g) < ignored] = -100
+    return h, w, t.to(dev)
+
+
+class Exact:
+    """Losses, gradients and how far each may be off, in 64 bits on the CPU."""
+
+    def __init__(self, h, w, t, grad=None, ignore=-100):
+        h, w, t = h.detach().double().cpu(), w.detach().double().cpu(), t.cpu()
+        d, v = h.shape[1], w.shape[0]
+        z = h @ w.t()
+        dz = d * 2.0**-23 * (h.abs() @ w.abs().t())
+        self.kept = t != ignore
+        at = t.clamp(min=0)[:, None]
+        self.lse = torch.logsumexp(z, 1)
+        picked = z.gather(1, at)[:, 0]
+        self.losses = (self.lse - picked) * self.kept
+        top = dz.amax(1)
+        self.lse_tol = top + 2.0**-21 + v * 2.0**-24 + 2.0**-22 * self.lse.abs()
+        self.losses_tol = self.lse_tol + top + 2.0**-22 * (self.lse.abs() + picked.abs())
+        if grad is None:
+            return
+        grad = grad.double().cpu() * self.kept
+        p = torch.exp(z - self.lse[:, None])
+        g = p.clone()
+        g.scatter_add_(1, at, torch.full_like(picked, -1.0)[:, None])
+        g *= grad[:, None]
+        eps = dz + self.lse_tol[:, None] + 2.0**-20
+        g_tol = HALF * g.abs() + (1 + HALF) * (eps * p + 2.0**-23) * grad.abs()[:, None]
+        # (2^-23: p - 1 at the target, and the gradient's own rounding)
+        self.dh = g @ w
+        self.dw = g.t() @ h
+        n = h.shape[0]
+        self.dh_tol = HALF * self.dh.abs() + (1 + HALF) * (g_tol + v * 2.0**-23 * g.abs()) @ w.abs()
+        self.dw_tol = HALF * self.dw.abs() + (1 + HALF) * (g_tol + n * 2.0**-23 * g.abs()).t() @ h.abs()
+
+
+def within(got, want, tol, what):
+    err = (got.detach().double().cpu() - want).abs()
+    assert got.shape == want.shape
+    assert (err <= tol).all(), (what, float((err / tol.clamp(min=1e-300)).max()))
+
+
+SHAPES = [(1, 8, 1), (1, 64, 5), (3, 72, 100), (64, 256, 256), (65, 128, 257), (130, 264, 1001),
+          (300, 64, 129), (17, 1000, 4100), (512, 512, 2048), (1100, 88, 130), (5, 40, 33000)]
+
+
+@pytest.mark.parametrize("tokens,d,vocab", SHAPES)
+def test_losses(dev, tokens, d, vocab):
+    print(f"[loss] forward {tokens} {d} {vocab}", flush=True)
+    h, w, t = inputs(dev, tokens, d, vocab, ignored=0.2 if tokens > 3 else 0.0)
+    e = Exact(h, w, t)
+    losses, lse = L.linear_cross_entropy_forward(h, w, t)
+    assert losses.dtype == lse.dtype == torch.float32
+    within(losses, e.losses, e.losses_tol, "losses")
+    within(lse, e.lse, e.lse_tol, "lse")
+    assert torch.equal(L.linear_cross_entropy(h, w, t, reduction="none"), losses)
+    total = L.linear_cross_entropy(h, w, t, reduction="sum")
+    mean = L.linear_cross_entropy(h, w, t)
+    s = float(e.losses.sum())
+    room = float(e.losses_tol.sum()) + 2.0**-24 * abs(s)
+    assert abs(float(total) - s) <= room
+    count = int(e.kept.sum())
+    assert abs(float(mean) - s / count) <= room / count
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("tokens,d,vocab", SHAPES)
+def test_gradients(dev, tokens, d, vocab, reduction):
+    print(f"[loss] backward {tokens} {d} {vocab} {reduction}", flush=True)
+    h, w, t = inputs(dev, tokens, d, vocab, seed=1, ignored=0.2 if tokens > 3 else 0.0)
+    h.requires_grad_()
+    w.requires_grad_()
+    out = L.linear_cross_entropy(h, w, t, reduction=reduction)
+    if reduction == "none":
+        up = torch.randn(tokens, generator=torch.Generator().manual_seed(2)).to(dev)
+    else:
+        up = torch.tensor(1.75, device=dev)
+    dh, dw = torch.autograd.grad(out, (h, w), up)
+    each = up.double().cpu().expand(tokens)
+    if reduction == "mean":
+        each = each / int((t != -100).sum())
+    e = Exact(h, w, t, each)
+    assert dh.dtype == dw.dtype == BF16
+    within(dh, e.dh, e.dh_tol, "dh")
+    within(dw, e.dw, e.dw_tol, "dw")
+    assert not dh[(t == -100)].any()
+
+
+def test_runs_of_classes_add_up(dev):
+    """More tokens x classes than a run's workspace: 70000 x 4100 x 2 bytes in three
+    runs, held against single rows and columns in 64 bits."""
+    tokens, d, vocab = 70000, 16, 4100
+    h, w, t = inputs(dev, tokens, d, vocab, seed=3)
+    nb = L._hip.lib().tcfp_linear_cross_entropy_backward_workspace_bytes(tokens, vocab, d, 1, 1)
+    assert nb < 2 * tokens * vocab  # g as a whole would take more
+    h.requires_grad_()
+    w.requires_grad_()
+    dh, dw = torch.autograd.grad(L.linear_cross_entropy(h, w, t, reduction="sum"), (h, w))
+    hd, wd = h.detach().double(), w.detach().double()
+    z = torch.mm(hd, wd.t().contiguous())
+    lse = torch.logsumexp(z, 1)
+    p = torch.exp(z - lse[:, None])
+    p[torch.arange(tokens, device=dev), t] -= 1.0
+    # z within D 2^-23 sum |h w| <= 2^-14 here, p with it
+    eps = d * 2.0**-23 * float((hd.abs().amax(0) * wd.abs().amax(0)).sum()) * 3 + 2.0**-20 + vocab * 2.0**-24
+    tol = (HALF * 1.01 + eps) * p.abs() + eps
+    want = torch.mm(p, wd)
+    room = HALF * want.abs() + torch.mm(tol, wd.abs()) + vocab * 2.0**-23 * torch.mm(p.abs(), wd.abs())
+    assert ((dh.double() - want).abs() <= room).all()
+    want = torch.mm(p.t().contiguous(), hd)
+    pa = p.abs().t().contiguous()
+    room = HALF * want.abs() + torch.mm(tol.t().contiguous(), hd.abs()) + tokens * 2.0**-23 * torch.mm(pa, hd.abs())
+    assert ((dw.double() - want).abs() <= room).all()
+
+
+@pytest.mark.parametrize("which", ["hidden", "weight"])
+def test_one_gradient_alone(dev, which):
+    h, w, t = inputs(dev, 70, 64, 300, seed=4)
+    h.requires_grad_(which == "hidden")
+    w.requires_grad_(which == "weight")
+    (h if which == "hidden" else w).retain_grad()
+    L.linear_cross_entropy(h, w, t).backward()
+    both = L.linear_cross_entropy_forward(h, w, t)
+    count = torch.tensor(70.0, device=dev)
+    dh, dw = L.linear_cross_entropy_backward(torch.tensor(1.0, device=dev), h.detach(), w.detach(), t,
+                                             both[1], count=count)
+    assert torch.equal(h.grad if which == "hidden" else w.grad, dh if which == "hidden" else dw)
+
+
+def test_gradient_against_differences(dev):
+    """Along directions on which h +- e d and w +- e d are exact in bf16: what the
+    difference differs from the 64-bit gradient by (its third order) is known, the
+    rest are the losses' and the gradients' tolerances."""
+    g = torch.Generator().manual_seed(5)
+    tokens, d, vocab, e = 20, 32, 40, 1 / 16
+    h = (torch.randint(-16, 17, (tokens, d), generator=g) / 16).to(BF16).to(dev)
+    w = (torch.randint(-8, 9, (vocab, d), generator=g) / 16).to(BF16).to(dev)
+    t = torch.randint(0, vocab, (tokens,), generator=g).to(dev)
+    for leaf in ("h", "w"):
+        x = h if leaf == "h" else w
+        move = (torch.randint(-1, 2, x.shape, generator=g) * e).to(BF16).to(dev)
+        pairs = [(h + s * move, w) if leaf == "h" else (h, w + s * move) for s in (1, -1)]
+        exact = [Exact(*p, t) for p in pairs]
+        slope = sum(s * L.linear_cross_entropy(*p, t, reduction="sum").double().cpu()
+                    for s, p in zip((1, -1), pairs)) / 2
+        want = sum(s * x.losses.sum() for s, x in zip((1, -1), exact)) / 2
+        room = sum(float(x.losses_tol.sum()) + 2.0**-24 * float(x.losses.sum()) for x in exact)
+        assert abs(float(slope - want)) <= room
+        a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+        grads = torch.autograd.grad(L.linear_cross_entropy(a, b, t, reduction="sum"), (a, b))
+        ref = Exact(h, w, t, torch.ones(tokens))
+        got, right, tol = ((grads[0], ref.dh, ref.dh_tol) if leaf == "h"
+                           else (grads[1], ref.dw, ref.dw_tol))
+        step = move.double().cpu()
+        third = abs(float((right * step).sum() - want))
+        assert abs(float((got.double().cpu() * step).sum() - slope)) <= (
+            third + room + float((tol * step.abs()).sum()))
+
+
+def test_strides_and_leading_axes(dev):
+    h, w, t = inputs(dev, 24, 64, 50, seed=6)
+    want = L.linear_cross_entropy(h, w, t, reduction="none")
+    wide = torch.zeros(24, 96, dtype=BF16, device=dev)
+    wide[:, 16:80] = h
+    tall = torch.zeros(50, 80, dtype=BF16, device=dev)
+    tall[:, 8:72] = w
+    assert torch.equal(L.linear_cross_entropy(wide[:, 16:80], tall[:, 8:72], t, reduction="none"), want)
+    assert torch.equal(L.linear_cross_entropy(wide[:, 16:80].clone()[:, :], tall[:, 8:72], t,
+                                              reduction="none"), want)
+    odd = torch.zeros(24 * 64 + 1, dtype=BF16, device=dev)[1:].view(24, 64)
+    odd.copy_(h)
+    assert torch.equal(L.linear_cross_entropy(odd, w.t().contiguous().t(), t, reduction="none"), want)
+    three = L.linear_cross_entropy(h.view(2, 12, 64), w, t.view(2, 12), reduction="none")
+    assert torch.equal(three, want.view(2, 12))
+    a = h.view(2, 12, 64).clone().requires_grad_()
+    (grad,) = torch.autograd.grad(L.linear_cross_entropy(a, w, t.view(2, 12)), a)
+    b = h.clone().requires_grad_()
+    (flat,) = torch.autograd.grad(L.linear_cross_entropy(b, w, t), b)
+    assert torch.equal(grad.view(24, 64), flat)
+    one = L.linear_cross_entropy(h[0], w, t[0], reduction="none")
+    assert one.shape == () and torch.equal(one, want[0])
+
+
+def test_targets_left_out_and_outside(dev):
+    h, w, t = inputs(dev, 12, 64, 50, seed=7)
+    t[:] = -100
+    assert math.isnan(float(L.linear_cross_entropy(h, w, t)))
+    assert float(L.linear_cross_entropy(h, w, t, reduction="sum")) == 0.0
+    hg, wg = h.clone().requires_grad_(), w.clone().requires_grad_()
+    dh, dw = torch.autograd.grad(L.linear_cross_entropy(hg, wg, t, reduction="sum"), (hg, wg))
+    assert not dh.any() and not dw.any()
+    t = torch.arange(12, device=dev)
+    t[3], t[5] = 50, -7
+    losses = L.linear_cross_entropy(h, w, t, reduction="none")
+    bad = torch.zeros(12, dtype=torch.bool)
+    bad[[3, 5]] = True
+    assert torch.equal(torch.isnan(losses).cpu(), bad)
+    (dh,) = torch.autograd.grad(L.linear_cross_entropy(hg, w, t, reduction="sum"), hg)
+    assert torch.equal(torch.isnan(dh).any(1).cpu(), bad)
+    # another index to leave out, one of the classes
+    t = torch.arange(12, device=dev) % 3
+    losses = L.linear_cross_entropy(h, w, t, ignore_index=1, reduction="none")
+    assert torch.equal(losses == 0, t == 1)
+
+
+def test_what_is_not_finite(dev):
+    h, w, t = inputs(dev, 40, 64, 300, seed=8)
+    h = h.clone()
+    h[7, 3] = math.nan
+    h[9] = 1e38  # logits of both signs past fp32
+    losses = L.linear_cross_entropy(h, w, t, reduction="none")
+    bad = torch.zeros(40, dtype=torch.bool)
+    bad[[7, 9]] = True
+    assert torch.equal(~torch.isfinite(losses).cpu(), bad)
+    # what a token that is left out holds reaches no other token's loss or gradient
+    t2 = t.clone()
+    t2[[7, 9]] = -100
+    hg = h.clone().requires_grad_()
+    loss = L.linear_cross_entropy(hg, w, t2)
+    assert math.isfinite(float(loss))
+    (dh,) = torch.autograd.grad(loss, hg)
+    assert torch.isfinite(dh).all() and not dh[[7, 9]].any()
+
+
+def test_large_logits(dev):
+    """Logits of some +-2000: exponentials only of differences."""
+    h, w, t = inputs(dev, 33, 64, 500, seed=9, spread=500.0)
+    e = Exact(h, w, t, torch.ones(33))
+    within(L.linear_cross_entropy(h, w, t, reduction="none"), e.losses, e.losses_tol, "losses")
+
+
+def test_no_tokens(dev):
+    h = torch.zeros(0, 64, dtype=BF16, device=dev).requires_grad_()
+    w = torch.ones(50, 64, dtype=BF16, device=dev).requires_grad_()
+    t = torch.zeros(0, dtype=torch.int64, device=dev)
+    assert L.linear_cross_entropy(h, w, t, reduction="none").shape == (0,)
+    loss = L.linear_cross_entropy(h, w, t, reduction="sum")
+    assert float(loss) == 0.0
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    assert dh.shape == (0, 64) and not dw.any()
+    assert math.isnan(float(L.linear_cross_entropy(h, w, t)))
+
+
+def test_bits_repeat_and_streams(dev):
+    h, w, t = inputs(dev, 700, 264, 1500, seed=10, ignored=0.1)
+    h.requires_grad_()
+    w.requires_grad_()
+
+    def once():
+        loss = L.linear_cross_entropy(h, w, t)
+        return (loss.detach(), *torch.autograd.grad(loss, (h, w)))
+
+    want = once()
+    assert all(torch.equal(a, b) for a, b in zip(once(), want))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = once()
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_graph(dev):
+    h, w, t = inputs(dev, 300, 128, 600, seed=11)
+    x = h.clone()
+    _, lse0 = L.linear_cross_entropy_forward(x, w, t)
+    one = torch.tensor(1.0, device=dev)
+
+    def both():
+        losses, lse = L.linear_cross_entropy_forward(x, w, t)
+        return (losses, *L.linear_cross_entropy_backward(one, x, w, t, lse))
+
+    both()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both()
+    for i in range(3):
+        x.copy_(h * (i + 1))
+        eager = both()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_refusals(dev):
+    h, w, t = inputs(dev, 4, 64, 10)
+    for exc, args in [
+            (TypeError, (h.float(), w, t)), (TypeError, (h, w.float(), t)),
+            (TypeError, (h, w, t.int())), (ValueError, (h, w[:, :32], t)),
+            (ValueError, (h, w[0], t)), (ValueError, (h, w, t[:3])), (ValueError, (h, w[:0], t)),
+            (ValueError, (h[:, :60].contiguous(), w[:, :60].contiguous(), t)),
+            (RuntimeError, (h.cpu(), w, t)), (RuntimeError, (h, w, t.cpu()))]:
+        with pytest.raises(exc):
+            L.linear_cross_entropy(*args)
+    with pytest.raises(ValueError):
+        L.linear_cross_entropy(h, w, t, reduction="max")
+    lse = torch.zeros(4, device=dev)
+    g = torch.ones(4, device=dev)
+    for args in [(g[:3], h, w, t, lse), (g.double(), h, w, t, lse), (g, h, w, t, lse[:3])]:
+        with pytest.raises(ValueError):
+            L.linear_cross_entropy_backward(*args)
+    a = h.clone().requires_grad_()
+    (grad,) = torch.autograd.grad(L.linear_cross_entropy(a, w, t), a, create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()
