@@ -765,9 +765,11 @@ int tcfp_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, in
  * keys j <= p (causal) with j > p - window (window > 0).  A query that sees
  * nothing, and one outside the sequences, gets zeros.
  * out = softmax(scale * q K^T) V with scores, maxima and sums in f32, the weights
- * rounded to bf16 before the second product.  lse [heads, tokens] f32 (may be
- * NULL): log2 of the sum of 2^(score * log2 e), +inf for a query that sees
- * nothing; not written for one outside the sequences.
+ * rounded to bf16 before the second product.  For the backward (either may be
+ * NULL; neither is written for a query outside the sequences): lse [heads, tokens]
+ * f32, log2 of the sum of 2^(score * log2 e), +inf for a query that sees nothing;
+ * out_low [tokens, heads, dim], what out's rounding to bf16 left, in 2^-8 of its
+ * last place: the f32 bits are (out << 16) + (out_low << 8).
  * max_len bounds the sequences' queries and sizes the launch (longer ones are
  * still answered rightly, only slower).  What is not finite stays within its
  * sequence.  No workspace; results do not depend on the launch's timing. */
@@ -777,11 +779,11 @@ int tcfp_packed_attention(const void* q, int64_t q_token_stride, int64_t q_head_
                           const int32_t* q_starts, const int32_t* k_starts, int64_t batch,
                           int64_t tokens, int64_t keys, int heads, int kv_heads, int dim,
                           int64_t max_len, float scale, int causal, int64_t window, void* out,
-                          float* lse, void* stream);
+                          int8_t* out_low, float* lse, void* stream);
 
 /* Its gradients: dq [tokens, heads, dim], dk and dv [keys, kv_heads, dim] bf16,
- * contiguous, from grad_out (strided like q), the inputs, and out and lse as the
- * forward wrote them.  The gradients of a K/V head are summed in f32 over the
+ * contiguous, from grad_out (strided like q), the inputs, and out, out_low and lse
+ * as the forward wrote them.  The gradients of a K/V head are summed in f32 over the
  * query heads that share it, in an order that the sizes fix; rows outside the
  * sequences get zeros.  dS is rounded to bf16 before the products it goes into.
  * max_key_len bounds the sequences' keys.  workspace:
@@ -793,7 +795,7 @@ int tcfp_packed_attention_backward(
     const void* grad_out, int64_t go_token_stride, int64_t go_head_stride, const void* q,
     int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
     int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
-    const void* out, const float* lse, const int32_t* q_starts, const int32_t* k_starts,
+    const void* out, const int8_t* out_low, const float* lse, const int32_t* q_starts, const int32_t* k_starts,
     int64_t batch, int64_t tokens, int64_t keys, int heads, int kv_heads, int dim,
     int64_t max_len, int64_t max_key_len, float scale, int causal, int64_t window, void* dq,
     void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);

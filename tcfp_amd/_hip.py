@@ -167,11 +167,13 @@ _SIGNATURES = {
                     _c_void_p],
     "tcfp_packed_attention": [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,
                               _c_void_p, _c_void_p, _i64, _i64, _i64, _i32, _i32, _i32, _i64,
-                              ctypes.c_float, _i32, _i64, _c_void_p, _c_void_p, _c_void_p],
+                              ctypes.c_float, _i32, _i64, _c_void_p, _c_void_p, _c_void_p,
+                              _c_void_p],
     "tcfp_packed_attention_backward_workspace_bytes": [_i64, _i64, _i64, _i64, _i32, _i32, _i32],
     "tcfp_packed_attention_backward": [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p,
                                        _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
-                                       _c_void_p, _c_void_p, _i64, _i64, _i64, _i32, _i32, _i32,
+                                       _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i32,
+                                       _i32, _i32,
                                        _i64, _i64, ctypes.c_float, _i32, _i64, _c_void_p,
                                        _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t,
                                        _c_void_p],

@@ -75,15 +75,15 @@ def packed_attention(
            None if scale is None else float(scale), bool(causal), int(window))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _PackedAttention.apply(q, k, v, *how)
-    return _packed_forward(q, k, v, *how, need_lse=False)[0]
+    return _packed_forward(q, k, v, *how, for_backward=False)[0]
 
 
 def _packed_forward(q, k, v, seq_start, key_start, max_len, max_key_len, scale, causal, window,
-                    need_lse):
+                    for_backward):
     if max_key_len is not None and max_key_len < 0:
         raise ValueError("max_len and max_key_len must not be negative")
     return _hip.host().packed_attention(q, k, v, seq_start, key_start, max_len, scale, causal,
-                                        window, need_lse)
+                                        window, for_backward)
 
 
 def packed_attention_forward(
@@ -97,14 +97,15 @@ def packed_attention_forward(
     scale: float | None = None,
     causal: bool = True,
     window: int = 0,
-) -> tuple[torch.Tensor, torch.Tensor]:
-    """``(out, lse)``: :func:`packed_attention` without autograd and, for
-    :func:`packed_attention_backward`, fp32 [heads, tokens]: log2 of each query's sum
-    of 2^(score * log2 e), +inf where it sees nothing (of queries that belong to no
-    sequence nothing is written)."""
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(out, out_low, lse)``: :func:`packed_attention` without autograd, and what
+    :func:`packed_attention_backward` needs of it: int8 [tokens, heads, dim], the next
+    eight bits of ``out`` (in 2^-8 of bf16's last place), and fp32 [heads, tokens], log2
+    of each query's sum of 2^(score * log2 e), +inf where it sees nothing.  (Of queries
+    that belong to no sequence the latter two hold nothing.)"""
     return _packed_forward(q, k, v, seq_start, key_start, int(max_len), None,
                            None if scale is None else float(scale), bool(causal), int(window),
-                           need_lse=True)
+                           for_backward=True)
 
 
 def packed_attention_backward(
@@ -113,6 +114,7 @@ def packed_attention_backward(
     k: torch.Tensor,
     v: torch.Tensor,
     out: torch.Tensor,
+    out_low: torch.Tensor,
     lse: torch.Tensor,
     seq_start: torch.Tensor,
     *,
@@ -126,7 +128,7 @@ def packed_attention_backward(
     """``(grad_q, grad_k, grad_v)`` of :func:`packed_attention` in bf16, from its
     inputs and what :func:`packed_attention_forward` returned for them."""
     return _hip.host().packed_attention_backward(
-        grad_out, q, k, v, out, lse, seq_start, key_start, int(max_len),
+        grad_out, q, k, v, out, out_low, lse, seq_start, key_start, int(max_len),
         None if max_key_len is None else int(max_key_len),
         None if scale is None else float(scale), bool(causal), int(window))
 
@@ -134,19 +136,19 @@ def packed_attention_backward(
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, seq_start, key_start, max_len, max_key_len, scale, causal, window):
-        out, lse = _packed_forward(q, k, v, seq_start, key_start, max_len, max_key_len, scale,
-                                   causal, window, need_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse, seq_start, key_start)
+        out, low, lse = _packed_forward(q, k, v, seq_start, key_start, max_len, max_key_len, scale,
+                                        causal, window, for_backward=True)
+        ctx.save_for_backward(q, k, v, out, low, lse, seq_start, key_start)
         ctx.how = max_len, max_key_len, scale, causal, window
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, out, lse, seq_start, key_start = ctx.saved_tensors
+        q, k, v, out, low, lse, seq_start, key_start = ctx.saved_tensors
         max_len, max_key_len, scale, causal, window = ctx.how
         dq, dk, dv = packed_attention_backward(
-            grad, q, k, v, out, lse, seq_start, max_len=max_len, key_start=key_start,
+            grad, q, k, v, out, low, lse, seq_start, max_len=max_len, key_start=key_start,
             max_key_len=max_key_len, scale=scale, causal=causal, window=window)
         need = ctx.needs_input_grad
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,

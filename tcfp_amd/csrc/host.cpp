@@ -1205,7 +1205,7 @@ PackedIn packed_inputs(OnGpu& g, const Tensor& q, const Tensor& k, const Tensor&
 
 Outs packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& starts,
                       const OptT& key_starts, int64_t max_len, std::optional<double> scale,
-                      bool causal, int64_t window, bool need_lse) {
+                      bool causal, int64_t window, bool for_backward) {
   OnGpu g;
   g.add(q);
   g.add(k);
@@ -1215,20 +1215,23 @@ Outs packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
   const c10::DeviceGuard guard(g.device());
   const PackedIn p =
       packed_inputs(g, q, k, v, starts, key_starts, max_len, std::nullopt, scale, window);
-  Tensor out = g.empty({p.tokens, p.heads, p.dim}, at::kBFloat16), lse;
-  if (need_lse) lse = g.empty({p.heads, p.tokens}, at::kFloat);
+  Tensor out = g.empty({p.tokens, p.heads, p.dim}, at::kBFloat16), low, lse;
+  if (for_backward) {
+    low = g.empty(out.sizes(), at::kChar);
+    lse = g.empty({p.heads, p.tokens}, at::kFloat);
+  }
   check(tcfp_packed_attention(ptr(p.q.t), p.q.token, p.q.head, ptr(p.k.t), p.k.token, p.k.head,
                               ptr(p.v.t), p.v.token, p.v.head, ptr<int32_t>(p.q_starts),
                               ptr<int32_t>(p.k_starts), p.batch, p.tokens, p.keys, p.heads,
                               p.kv_heads, p.dim, p.max_len, p.scale, causal ? 1 : 0, window,
-                              ptr(out), f32(lse), g.stream()),
+                              ptr(out), exps(low), f32(lse), g.stream()),
         "packed_attention");
-  return outs(out, lse);
+  return outs(out, low, lse);
 }
 
 Outs packed_attention_backward(const Tensor& grad, const Tensor& q, const Tensor& k,
-                               const Tensor& v, const Tensor& out_, const Tensor& lse_,
-                               const Tensor& starts, const OptT& key_starts, int64_t max_len,
+                               const Tensor& v, const Tensor& out_, const Tensor& low_,
+                               const Tensor& lse_, const Tensor& starts, const OptT& key_starts, int64_t max_len,
                                std::optional<int64_t> max_key_len, std::optional<double> scale,
                                bool causal, int64_t window) {
   OnGpu g;
@@ -1237,6 +1240,7 @@ Outs packed_attention_backward(const Tensor& grad, const Tensor& q, const Tensor
   g.add(k);
   g.add(v);
   g.add(out_);
+  g.add(low_);
   g.add(lse_);
   g.add(starts);
   g.add(key_starts);
@@ -1245,8 +1249,11 @@ Outs packed_attention_backward(const Tensor& grad, const Tensor& q, const Tensor
       packed_inputs(g, q, k, v, starts, key_starts, max_len, max_key_len, scale, window);
   need_bf16(grad, "grad_out");
   need_bf16(out_, "out");
+  if (low_.scalar_type() != at::kChar)
+    type_error(std::string("out_low must be torch.int8, got ") + dtype_str(low_.scalar_type()));
   for (const auto& [name, t] : {std::pair<const char*, const Tensor*>{"grad_out", &grad},
-                                std::pair<const char*, const Tensor*>{"out", &out_}})
+                                std::pair<const char*, const Tensor*>{"out", &out_},
+                                std::pair<const char*, const Tensor*>{"out_low", &low_}})
     if (t->sizes() != q.sizes())
       value_error(std::string(name) + " must have q's shape " + shape_str(q.sizes()) + ", got " +
                   shape_str(t->sizes()));
@@ -1255,7 +1262,7 @@ Outs packed_attention_backward(const Tensor& grad, const Tensor& q, const Tensor
     value_error("lse must hold a float32 for each head and token, shape (" +
                 std::to_string(p.heads) + ", " + std::to_string(p.tokens) + ")");
   const Heads go = strided_heads(grad);
-  const Tensor out = whole(out_), lse = lse_.contiguous();
+  const Tensor out = whole(out_), low = whole(low_), lse = lse_.contiguous();
   Tensor dq = g.empty(q.sizes(), at::kBFloat16), dk = g.empty(k.sizes(), at::kBFloat16),
          dv = g.empty(v.sizes(), at::kBFloat16), ws;
   const size_t nb = tcfp_packed_attention_backward_workspace_bytes(
@@ -1263,7 +1270,7 @@ Outs packed_attention_backward(const Tensor& grad, const Tensor& q, const Tensor
   if (nb) ws = g.empty({int64_t(nb)}, at::kByte);
   check(tcfp_packed_attention_backward(
             ptr(go.t), go.token, go.head, ptr(p.q.t), p.q.token, p.q.head, ptr(p.k.t), p.k.token,
-            p.k.head, ptr(p.v.t), p.v.token, p.v.head, ptr(out), f32(lse),
+            p.k.head, ptr(p.v.t), p.v.token, p.v.head, ptr(out), exps(low), f32(lse),
             ptr<int32_t>(p.q_starts), ptr<int32_t>(p.k_starts), p.batch, p.tokens, p.keys, p.heads,
             p.kv_heads, p.dim, p.max_len, p.max_key_len, p.scale, causal ? 1 : 0, window, ptr(dq),
             ptr(dk), ptr(dv), ptr(ws), nb, g.stream()),

@@ -37,6 +37,7 @@ struct Packed {
   const uint16_t *q, *k, *v, *go;  // [tokens, heads, dim], [keys, kv_heads, dim]
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, go_token, go_head;
   uint16_t* o;            // contiguous: written forward, read backward
+  int8_t* low;            // what o's rounding left, see low_part()
   uint16_t *dq, *dk, *dv;  // contiguous
   float* lse;             // [heads, tokens]: log2 of the sum, +inf where nothing is seen
   float* delta;           // [heads, tokens]
@@ -110,6 +111,13 @@ TCFP_DEV int swizzle(int row) {
 template <int D>
 constexpr int kTileBytes = kStep * D * 2;
 
+// Hides an offset's origin from the compiler, which would otherwise keep all that
+// is derived from it in registers through the loop, where none are free.
+TCFP_DEV int fresh(int off) {
+  asm volatile("" : "+v"(off));
+  return off;
+}
+
 // The wave's share (instructions wave, wave + NW, ...) of the copy of rows
 // [row, row + kStep) of x, of which the first `rows` there are.
 template <int D, int NW>
@@ -118,31 +126,39 @@ TCFP_DEV void copy_tile(const uint16_t* x, int64_t ld, int64_t row, int rows, ui
   constexpr int CH = D / 8, R = 64 / CH, N = kStep / R / NW;
   const v4i rsrc = make_rsrc(
       x + row * ld, rows > 0 ? uint32_t((int64_t(min(rows, kStep) - 1) * ld + D) * 2) : 0u);
+  const int r = wave * R + lane / CH;
+  const uint32_t off = fresh(r * int(ld) * 2), chunk = fresh(((lane % CH) ^ swizzle<D>(r)) << 4);
+  const uint32_t step = uint32_t(NW * R * 2) * uint32_t(ld);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int r = (i * NW + wave) * R + lane / CH;
-    copy16(rsrc, uint32_t(r * ld * 2) + (((lane % CH) ^ swizzle<D>(r)) << 4),
+  for (int i = 0; i < N; ++i)  // (the swizzle of row i NW R + r is the two's)
+    copy16(rsrc, off + (chunk ^ (swizzle<D>(i * NW * R) << 4)) + uint32_t(i) * step,
            lds + uint32_t((i * NW + wave) * 1024));
-  }
 }
 
-// Operand "rows along lanes": rows x + lane % 32 of the tile, columns 16 s + 8
-// (lane / 32) ....
+// Where a lane reads its operands of a tile:
+// * "rows along lanes": row x + lane % 32, columns 16 d + 8 (lane / 32) ...;
+// * "columns along lanes": column 32 x + lane % 32 of the rows r0 + 4 (lane / 32) +
+//   {0 ... 3, 8 ... 11}, r0 a multiple of 16: the rows that the lane's accumulators
+//   8 (r0 / 16 % 2) ... of a 32-row block hold.
+// Both are one offset in which d and x flip bits.
 template <int D>
-TCFP_DEV v8bf by_rows(const uint8_t* tile, int x, int s, int lane) {
-  const int row = x + (lane & 31);
-  return read16(tile + row * (2 * D) + (((2 * s + (lane >> 5)) ^ swizzle<D>(row)) << 4));
+struct Lanes {
+  int rows, columns;
+  TCFP_DEV void init(int lane) {
+    const int row = lane & 31, half = lane >> 5, i = lane & 15, r = 4 * half + (i >> 2);
+    rows = row * (2 * D) + ((half ^ swizzle<D>(row)) << 4);
+    columns = r * (2 * D) + (((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ swizzle<D>(r)) << 4) +
+              (i & 1) * 8;
+  }
+};
+template <int D>
+TCFP_DEV v8bf by_rows(const uint8_t* lds, int off, int x, int d) {
+  return read16(lds + (off ^ (d << 5)) + x * (2 * D));
 }
-// Operand "columns along lanes": columns 32 x + lane % 32, of rows r0 + 4 (lane /
-// 32) + {0 ... 3, 8 ... 11}: the rows that the lane's accumulators 8 (r0 / 16 % 2)
-// ... of a 32-row block hold.
 template <int D>
-TCFP_DEV v8bf by_columns(const uint8_t* tile, int x, int r0, int lane) {
-  const int i = lane & 15, row = r0 + 4 * (lane >> 5) + (i >> 2);
-  const int chunk = 4 * x + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-  const int at = (i & 1) * 8;
-  return read_transposed(tile + row * (2 * D) + ((chunk ^ swizzle<D>(row)) << 4) + at,
-                         tile + (row + 8) * (2 * D) + ((chunk ^ swizzle<D>(row + 8)) << 4) + at);
+TCFP_DEV v8bf by_columns(const uint8_t* lds, int off, int x, int r0) {
+  const int at = off ^ (x << 6);
+  return read_transposed(lds + at + r0 * (2 * D), lds + (at ^ 32) + (r0 + 8) * (2 * D));
 }
 
 // A lane's operand of its own row in memory: columns 16 s + 8 half ....
@@ -181,6 +197,17 @@ TCFP_DEV v16f zeros() {
 #pragma unroll
   for (int r = 0; r < 16; ++r) z[r] = 0.0f;
   return z;
+}
+
+// What rounding x to bf16 left, in 2^-8 of bf16's last place: delta = rowsum(dO * O)
+// takes O with eight bits more.  From the rounded O alone, short rows lose: dK of
+// 32 sequences of 128 tokens was 2.7e-3 off where its own rounding is 1.7e-3.
+TCFP_DEV uint32_t low_part(float x) {
+  const int bits = __float_as_int(x), high = int(pack2(x, x) & 0xFFFF0000u);
+  return uint32_t(min((bits - high + 128) >> 8, 127)) & 0xFFu;
+}
+TCFP_DEV float with_low(uint32_t high, uint32_t low, int byte) {
+  return __int_as_float(int(high) + (int(low << (24 - 8 * byte)) >> 24) * 256);
 }
 
 // A wave's transposed result, columns across the registers, as rows of bf16.
@@ -228,6 +255,8 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_forward_kern
     if (b == a.batch - 1) zero_rows<D>(a.o, s.q0 + s.nq, a.tokens, a.heads, head, 1);
   }
   const uint32_t lds0 = lds_offset(lds);
+  Lanes<D> at_lane;
+  at_lane.init(lane);
   const int tiles = (s.nq + 32 * NW - 1) / (32 * NW);
   // (the last tiles, which see the most keys, first; a bound on the lengths that
   // is too small gives a workgroup several)
@@ -259,14 +288,14 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_forward_kern
       wait_and_sync<0>();  // this step is there, the one before it read
       if (key + kStep < end) fetch(key + kStep, buf ^ 1);
       if (idle || key >= w_hi || key + kStep <= w_lo) continue;
-      const uint8_t* kt = lds + buf * 2 * TILE;
-      const uint8_t* vt = kt + TILE;
+      const int k_off = fresh(buf * 2 * TILE + at_lane.rows);
+      const int v_off = fresh(buf * 2 * TILE + TILE + at_lane.columns);
       v16f e[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         e[x] = zeros();
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) e[x] = mfma(by_rows<D>(kt, 32 * x, d, lane), q[d], e[x]);
+        for (int d = 0; d < D / 16; ++d) e[x] = mfma(by_rows<D>(lds, k_off, 32 * x, d), q[d], e[x]);
       }
       if (key < w_lo_max || key + kStep > w_hi_min) {
 #pragma unroll
@@ -302,13 +331,25 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_forward_kern
       for (int x = 0; x < 4; ++x) {
         const v8bf p = pack8(e[x >> 1], 8 * (x & 1));
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] = mfma(by_columns<D>(vt, i, 16 * x, lane), p, o[i]);
+        for (int i = 0; i < D / 32; ++i) o[i] = mfma(by_columns<D>(lds, v_off, i, 16 * x), p, o[i]);
       }
     }
     l += other_half(l);
     if (r0 + 32 * wave + col <= last) {
-      store_row<D>(a.o + (int64_t(s.q0 + row) * a.heads + head) * D, o, l == 0.0f ? 0.0f : 1.0f / l,
-                   half);
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int64_t at_row = (int64_t(s.q0 + row) * a.heads + head) * D;
+      store_row<D>(a.o + at_row, o, inv, half);
+      if (a.low) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w |= low_part(o[i][4 * g + r] * inv) << (8 * r);
+            *reinterpret_cast<uint32_t*>(a.low + at_row + 32 * i + 8 * g + 4 * half) = w;
+          }
+      }
       if (a.lse && half == 0)
         a.lse[int64_t(head) * a.tokens + s.q0 + row] =
             l == 0.0f ? INFINITY : m * a.c + log2_fast(l);
@@ -336,6 +377,8 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dq_kernel(Pa
     if (b == a.batch - 1) zero_rows<D>(a.dq, s.q0 + s.nq, a.tokens, a.heads, head, 1);
   }
   const uint32_t lds0 = lds_offset(lds);
+  Lanes<D> at_lane;
+  at_lane.init(lane);
   const int tiles = (s.nq + 32 * NW - 1) / (32 * NW);
   for (int at = tiles - 1 - tile; at >= 0; at -= a.tiles) {
     const int r0 = at * 32 * NW, last = min(r0 + 32 * NW, s.nq) - 1;
@@ -361,9 +404,15 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dq_kernel(Pa
     float delta = 0.0f;
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) {
-      const v8bf o = *reinterpret_cast<const v8bf*>(a.o + hrow * D + 16 * d + 8 * half);
+      const int64_t at_o = hrow * D + 16 * d + 8 * half;
+      const uint4 o = *reinterpret_cast<const uint4*>(a.o + at_o);
+      const uint2 low = *reinterpret_cast<const uint2*>(a.low + at_o);
+      const uint32_t ow[4] = {o.x, o.y, o.z, o.w}, lw[2] = {low.x, low.y};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(float(o[j]), float(go[d][j]), delta);
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t high = j & 1 ? ow[j / 2] & 0xFFFF0000u : ow[j / 2] << 16;
+        delta = __builtin_fmaf(with_low(high, lw[j / 4], j % 4), float(go[d][j]), delta);
+      }
     }
     delta += other_half(delta);
     const int64_t stat = int64_t(head) * a.tokens + s.q0 + row;
@@ -378,16 +427,17 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dq_kernel(Pa
       wait_and_sync<0>();
       if (key + kStep < end) fetch(key + kStep, buf ^ 1);
       if (idle || key >= w_hi || key + kStep <= w_lo) continue;
-      const uint8_t* kt = lds + buf * 2 * TILE;
-      const uint8_t* vt = kt + TILE;
       const bool masked = key < w_lo_max || key + kStep > w_hi_min;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
+        const int k_off = fresh(buf * 2 * TILE + at_lane.rows);
+        const int kt_off = fresh(buf * 2 * TILE + at_lane.columns);
         v16f e = zeros(), dp = zeros();
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) e = mfma(by_rows<D>(kt, 32 * x, d, lane), q[d], e);
+        for (int d = 0; d < D / 16; ++d) e = mfma(by_rows<D>(lds, k_off, 32 * x, d), q[d], e);
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) dp = mfma(by_rows<D>(vt, 32 * x, d, lane), go[d], dp);
+        for (int d = 0; d < D / 16; ++d)
+          dp = mfma(by_rows<D>(lds + TILE, k_off, 32 * x, d), go[d], dp);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           e[r] = exp2_fast(__builtin_fmaf(e[r], a.c, -lse)) * (dp[r] - delta);
@@ -403,7 +453,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dq_kernel(Pa
           const v8bf ds = pack8(e, 8 * y);
 #pragma unroll
           for (int i = 0; i < D / 32; ++i)
-            dq[i] = mfma(by_columns<D>(kt, i, 32 * x + 16 * y, lane), ds, dq[i]);
+            dq[i] = mfma(by_columns<D>(lds, kt_off, i, 32 * x + 16 * y), ds, dq[i]);
         }
       }
     }
@@ -436,6 +486,8 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dkv_kernel(P
   const int heads_each = (a.group + a.parts - 1) / a.parts;
   const int g0 = part * heads_each, g1 = min(g0 + heads_each, a.group);
   const uint32_t lds0 = lds_offset(lds);
+  Lanes<D> at_lane;
+  at_lane.init(lane);
   for (int j0 = tile * 32 * NW; j0 < s.nk; j0 += a.tiles * 32 * NW) {
     const int last = min(j0 + 32 * NW, s.nk) - 1;
     // queries that see some of the tile's keys
@@ -461,8 +513,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dkv_kernel(P
     for (int i = 0; i < D / 32; ++i) dk[i] = zeros(), dv[i] = zeros();
     const int steps = begin < end ? (end - begin + kStep - 1) / kStep : 0;
     const int total = steps * (g1 - g0);
-    auto fetch = [&](int i, int buf) {
-      const int g = g0 + i / steps, at = begin + (i % steps) * kStep;
+    auto fetch = [&](int g, int at, int buf) {
       const int head = kvh * a.group + g;
       const uint32_t to = lds0 + uint32_t(buf) * BUF;
       copy_tile<D, NW>(a.q + int64_t(head) * a.q_head, a.q_token, s.q0 + at, s.nq - at, to, wave,
@@ -473,28 +524,36 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dkv_kernel(P
       // products are masked)
       if (wave < 2) {
         const float* x = (wave ? a.delta : a.lse) + int64_t(head) * a.tokens + s.q0 + at;
-        copy4(make_rsrc(x, uint32_t(min(s.nq - at, kStep) * 4)), uint32_t(lane * 4),
+        const uint32_t me = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+        copy4(make_rsrc(x, uint32_t(min(s.nq - at, kStep) * 4)), me * 4,
               to + 2 * TILE + uint32_t(wave) * (kStep * 4));
       }
     };
-    if (total > 0) fetch(0, 0);
+    int g = g0, at = begin, next_g = g0, next_at = begin;
+    auto advance = [&]() {
+      next_at += kStep;
+      if (next_at >= end) next_at = begin, ++next_g;
+    };
+    if (total > 0) fetch(g, at, 0);
     int buf = 0;
     for (int i = 0; i < total; ++i, buf ^= 1) {
       wait_and_sync<0>();
-      if (i + 1 < total) fetch(i + 1, buf ^ 1);
-      const int at = begin + (i % steps) * kStep;
-      const uint8_t* qt = lds + buf * BUF;
-      const uint8_t* gt = qt + TILE;
-      const float* stats = reinterpret_cast<const float*>(gt + TILE);
-#pragma unroll
+      g = next_g, at = next_at;
+      advance();
+      if (i + 1 < total) fetch(next_g, next_at, buf ^ 1);
+      const float* stats = reinterpret_cast<const float*>(lds + buf * BUF + 2 * TILE);
+#pragma unroll 1
       for (int x = 0; x < 2; ++x) {
         const int r0 = at + 32 * x;
         if (idle || r0 + 32 <= w_begin || r0 >= w_end) continue;
+        const int r_off = fresh(buf * BUF + 32 * x * (2 * D) + at_lane.rows);
+        const int c_off = fresh(buf * BUF + 32 * x * (2 * D) + at_lane.columns);
         v16f e = zeros(), dp = zeros();
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) e = mfma(by_rows<D>(qt, 32 * x, d, lane), k[d], e);
+        for (int d = 0; d < D / 16; ++d) dp = mfma(by_rows<D>(lds + TILE, r_off, 0, d), v[d], dp);
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) dp = mfma(by_rows<D>(gt, 32 * x, d, lane), v[d], dp);
+        for (int d = 0; d < D / 16; ++d) e = mfma(by_rows<D>(lds, r_off, 0, d), k[d], e);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4 l4 = *reinterpret_cast<const float4*>(stats + 32 * x + 8 * g + 4 * half);
@@ -515,15 +574,16 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dkv_kernel(P
             if (qi < first || qi >= past) e[r] = 0.0f, dp[r] = 0.0f;
           }
         }
+        const v8bf p[2] = {pack8(e, 0), pack8(e, 8)}, ds[2] = {pack8(dp, 0), pack8(dp, 8)};
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const v8bf p = pack8(e, 8 * y), ds = pack8(dp, 8 * y);
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
-            dv[j] = mfma(by_columns<D>(gt, j, 32 * x + 16 * y, lane), p, dv[j]);
-            dk[j] = mfma(by_columns<D>(qt, j, 32 * x + 16 * y, lane), ds, dk[j]);
+            dv[j] = mfma(by_columns<D>(lds + TILE, c_off, j, 16 * y), p[y], dv[j]);
+            dk[j] = mfma(by_columns<D>(lds, c_off, j, 16 * y), ds[y], dk[j]);
           }
-        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     if (j0 + 32 * wave + col <= last) {
@@ -585,14 +645,15 @@ int launch_status() { return hipGetLastError() == hipSuccess ? TCFP_OK : TCFP_ER
 // Waves of a workgroup.
 constexpr int kWaves = 4;
 
-// Parts of a group's heads in the dK, dV launch: one, but where the keys' tiles
-// are fewer than the workgroups the card holds at once.
+// Parts of a group's heads in the dK, dV launch: one, but where there are not twice
+// as many tiles of keys as workgroups that the card holds at once (of a causal
+// sequence the first tile has twice the mean's queries).
 int parts_of(int64_t keys, int64_t batch, int64_t max_key_len, int kv_heads, int group, int dim) {
   const int64_t rows = 32 * kWaves;
   const int64_t tiles =
       std::min(ceil_div(std::max<int64_t>(max_key_len, 1), rows) * batch, keys / rows + batch);
-  const int64_t room = (dim == 256 ? kCus : 2 * kCus) / std::max<int64_t>(tiles * kv_heads, 1);
-  return int(std::clamp<int64_t>(room, 1, group));
+  const int64_t want = (dim == 256 ? 2 : 4) * kCus;
+  return int(std::clamp<int64_t>(ceil_div(want, std::max<int64_t>(tiles * kv_heads, 1)), 1, group));
 }
 
 struct Sizes {
@@ -661,13 +722,13 @@ int tcfp_packed_attention(const void* q, int64_t q_token_stride, int64_t q_head_
                           const int32_t* q_starts, const int32_t* k_starts, int64_t batch,
                           int64_t tokens, int64_t keys, int heads, int kv_heads, int dim,
                           int64_t max_len, float scale, int causal, int64_t window, void* out,
-                          float* lse, void* stream) {
+                          int8_t* out_low, float* lse, void* stream) {
   const Sizes z{tokens, keys, batch, max_len, 0, window, heads, kv_heads, dim, scale};
   if (const int rc = check_sizes(z)) return rc;
   if (const int rc = check_rows(q, q_token_stride, q_head_stride)) return rc;
   if (const int rc = check_rows(k, k_token_stride, k_head_stride)) return rc;
   if (const int rc = check_rows(v, v_token_stride, v_head_stride)) return rc;
-  if (!aligned16(out)) return TCFP_ERR_ALIGN;
+  if (!aligned16(out) || !aligned16(out_low)) return TCFP_ERR_ALIGN;
   if (tokens == 0) return TCFP_OK;
   Packed a = arguments(z, causal != 0);
   a.q = static_cast<const uint16_t*>(q);
@@ -679,6 +740,7 @@ int tcfp_packed_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   a.q_starts = q_starts;
   a.k_starts = k_starts;
   a.o = static_cast<uint16_t*>(out);
+  a.low = out_low;
   a.lse = lse;
   a.tiles = tiles_of(max_len, tokens);
   const auto st = static_cast<hipStream_t>(stream);
@@ -700,7 +762,7 @@ int tcfp_packed_attention_backward(
     const void* grad_out, int64_t go_token_stride, int64_t go_head_stride, const void* q,
     int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
     int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
-    const void* out, const float* lse, const int32_t* q_starts, const int32_t* k_starts,
+    const void* out, const int8_t* out_low, const float* lse, const int32_t* q_starts, const int32_t* k_starts,
     int64_t batch, int64_t tokens, int64_t keys, int heads, int kv_heads, int dim, int64_t max_len,
     int64_t max_key_len, float scale, int causal, int64_t window, void* dq, void* dk, void* dv,
     void* workspace, size_t workspace_bytes, void* stream) {
@@ -710,7 +772,7 @@ int tcfp_packed_attention_backward(
   if (const int rc = check_rows(q, q_token_stride, q_head_stride)) return rc;
   if (const int rc = check_rows(k, k_token_stride, k_head_stride)) return rc;
   if (const int rc = check_rows(v, v_token_stride, v_head_stride)) return rc;
-  if (!aligned16(out) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return TCFP_ERR_ALIGN;
+  if (!aligned16(out) || !aligned16(out_low) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return TCFP_ERR_ALIGN;
   if (tokens == 0 && keys == 0) return TCFP_OK;
   const size_t need = tcfp_packed_attention_backward_workspace_bytes(
       tokens, keys, batch, max_key_len, heads, kv_heads, dim);
@@ -728,6 +790,7 @@ int tcfp_packed_attention_backward(
   a.q_starts = q_starts;
   a.k_starts = k_starts;
   a.o = const_cast<uint16_t*>(static_cast<const uint16_t*>(out));
+  a.low = const_cast<int8_t*>(out_low);
   a.lse = const_cast<float*>(lse);
   a.dq = static_cast<uint16_t*>(dq);
   a.dk = static_cast<uint16_t*>(dk);

@@ -301,8 +301,8 @@ def test_graph(dev):
     x, at = q.clone(), i32(starts, dev)
 
     def both():
-        o, lse = A.packed_attention_forward(x, k, v, at, max_len=150)
-        return (o, *A.packed_attention_backward(go, x, k, v, o, lse, at, max_len=150))
+        o, low, lse = A.packed_attention_forward(x, k, v, at, max_len=150)
+        return (o, *A.packed_attention_backward(go, x, k, v, o, low, lse, at, max_len=150))
 
     both()
     graph = torch.cuda.CUDAGraph()
@@ -352,9 +352,13 @@ def test_refusals(dev):
             (RuntimeError, dict(q=q.cpu())), (RuntimeError, dict(at=at.cpu()))]:
         with pytest.raises(exc):
             call(**kw)
-    o, lse = A.packed_attention_forward(q, k, v, at, max_len=6)
-    for exc, args in [(ValueError, (go[:5], q, k, v, o, lse)), (ValueError, (go, q, k, v, o, lse[:3])),
-                      (TypeError, (go.float(), q, k, v, o, lse)), (ValueError, (go, q, k, v, o[:5], lse))]:
+    o, low, lse = A.packed_attention_forward(q, k, v, at, max_len=6)
+    for exc, args in [(ValueError, (go[:5], q, k, v, o, low, lse)),
+                      (ValueError, (go, q, k, v, o, low, lse[:3])),
+                      (TypeError, (go.float(), q, k, v, o, low, lse)),
+                      (ValueError, (go, q, k, v, o[:5], low, lse)),
+                      (TypeError, (go, q, k, v, o, low.float(), lse)),
+                      (ValueError, (go, q, k, v, o, low[:5], lse))]:
         with pytest.raises(exc):
             A.packed_attention_backward(*args, at, max_len=6)
     a = q.clone().requires_grad_()
