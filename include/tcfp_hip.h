@@ -805,17 +805,17 @@ int tcfp_packed_attention_backward(
  *   hidden [tokens, dim], weight [vocab, dim] bf16, rows ldh / ldw apart
  *   (multiples of 8, 16-byte aligned), dim % 8 == 0.
  * A token whose target is `ignore` has loss 0; one whose target is neither that
- * nor a class has loss NaN.  lse [tokens] f32: log sum exp z.  total (may be
- * NULL): [0] the sum of the losses, or (mean != 0) their mean over the tokens that
- * are not ignored (NaN if all are), [1] the number of those; summed in f64 in an
- * order that the sizes fix.  workspace: ..._workspace_bytes, any contents, 16-byte
+ * nor a class has loss NaN.  lse [tokens] f32: log sum exp z.  total and count (both
+ * or neither): one f32 each, the sum of the losses, or (mean != 0) their mean over
+ * the tokens that are not ignored (NaN if all are), and the number of those; summed
+ * in f64 in an order that the sizes fix.  workspace: ..._workspace_bytes, any contents, 16-byte
  * aligned. */
-size_t tcfp_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t vocab);
+size_t tcfp_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim);
 int tcfp_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                               const int64_t* targets, int64_t ignore, int64_t tokens,
                               int64_t vocab, int64_t dim, float* losses, float* lse, int mean,
-                              float* total, void* workspace, size_t workspace_bytes,
-                              void* stream);
+                              float* total, float* count, void* workspace,
+                              size_t workspace_bytes, void* stream);
 
 /* Its gradients: g[t] = (softmax(z[t]) - onehot(targets[t])) * grad[t * grad_step]
  * (/ *count, if count is not NULL), 0 for an ignored token;

@@ -177,10 +177,10 @@ _SIGNATURES = {
                                        _i64, _i64, ctypes.c_float, _i32, _i64, _c_void_p,
                                        _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t,
                                        _c_void_p],
-    "tcfp_linear_cross_entropy_workspace_bytes": [_i64, _i64],
+    "tcfp_linear_cross_entropy_workspace_bytes": [_i64, _i64, _i64],
     "tcfp_linear_cross_entropy": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64,
                                   _i64, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p,
-                                  ctypes.c_size_t, _c_void_p],
+                                  _c_void_p, ctypes.c_size_t, _c_void_p],
     "tcfp_linear_cross_entropy_backward_workspace_bytes": [_i64, _i64, _i64, _i32, _i32],
     "tcfp_linear_cross_entropy_backward": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64,
                                            _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64,

@@ -71,19 +71,10 @@ def packed_attention(
     Differentiable in q, k and v, once; results and gradients do not depend on the
     launches' timing.
     """
-    how = (seq_start, key_start, int(max_len), None if max_key_len is None else int(max_key_len),
-           None if scale is None else float(scale), bool(causal), int(window))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _PackedAttention.apply(q, k, v, *how)
-    return _packed_forward(q, k, v, *how, for_backward=False)[0]
-
-
-def _packed_forward(q, k, v, seq_start, key_start, max_len, max_key_len, scale, causal, window,
-                    for_backward):
-    if max_key_len is not None and max_key_len < 0:
-        raise ValueError("max_len and max_key_len must not be negative")
-    return _hip.host().packed_attention(q, k, v, seq_start, key_start, max_len, scale, causal,
-                                        window, for_backward)
+    return _hip.host().packed_attention(
+        q, k, v, seq_start, key_start, int(max_len),
+        None if max_key_len is None else int(max_key_len),
+        None if scale is None else float(scale), bool(causal), int(window))
 
 
 def packed_attention_forward(
@@ -103,9 +94,9 @@ def packed_attention_forward(
     eight bits of ``out`` (in 2^-8 of bf16's last place), and fp32 [heads, tokens], log2
     of each query's sum of 2^(score * log2 e), +inf where it sees nothing.  (Of queries
     that belong to no sequence the latter two hold nothing.)"""
-    return _packed_forward(q, k, v, seq_start, key_start, int(max_len), None,
-                           None if scale is None else float(scale), bool(causal), int(window),
-                           for_backward=True)
+    return _hip.host().packed_attention_forward(
+        q, k, v, seq_start, key_start, int(max_len), None if scale is None else float(scale),
+        bool(causal), int(window), True)
 
 
 def packed_attention_backward(
@@ -131,28 +122,6 @@ def packed_attention_backward(
         grad_out, q, k, v, out, out_low, lse, seq_start, key_start, int(max_len),
         None if max_key_len is None else int(max_key_len),
         None if scale is None else float(scale), bool(causal), int(window))
-
-
-class _PackedAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, seq_start, key_start, max_len, max_key_len, scale, causal, window):
-        out, low, lse = _packed_forward(q, k, v, seq_start, key_start, max_len, max_key_len, scale,
-                                        causal, window, for_backward=True)
-        ctx.save_for_backward(q, k, v, out, low, lse, seq_start, key_start)
-        ctx.how = max_len, max_key_len, scale, causal, window
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        q, k, v, out, low, lse, seq_start, key_start = ctx.saved_tensors
-        max_len, max_key_len, scale, causal, window = ctx.how
-        dq, dk, dv = packed_attention_backward(
-            grad, q, k, v, out, low, lse, seq_start, max_len=max_len, key_start=key_start,
-            max_key_len=max_key_len, scale=scale, causal=causal, window=window)
-        need = ctx.needs_input_grad
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
-                None, None, None, None, None, None, None)
 
 
 def kv_cache_write(

@@ -20,6 +20,8 @@
 #include <Python.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
@@ -1307,8 +1309,8 @@ HeadIn head_inputs(const Tensor& hidden, const Tensor& weight, const Tensor& tar
   return in;
 }
 
-// -> (losses, lse, total): total only with `reduce`, the losses' mean or sum and
-// the tokens that count.
+// -> (losses, lse, total, count): the latter two only with `reduce`, the losses' mean
+// or sum and the tokens that count.
 Outs linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& targets,
                           int64_t ignore, bool reduce, bool mean) {
   OnGpu g;
@@ -1317,16 +1319,17 @@ Outs linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tens
   g.add(targets);
   const c10::DeviceGuard guard(g.device());
   const HeadIn in = head_inputs(hidden, weight, targets);
-  Tensor losses = g.empty(targets.sizes(), at::kFloat), lse = g.empty({in.h.rows}, at::kFloat), total;
-  if (reduce) total = g.empty({2}, at::kFloat);
-  const size_t nb = tcfp_linear_cross_entropy_workspace_bytes(in.h.rows, in.w.rows);
+  Tensor losses = g.empty(targets.sizes(), at::kFloat), lse = g.empty({in.h.rows}, at::kFloat), total,
+         count;
+  if (reduce) total = g.empty({}, at::kFloat), count = g.empty({}, at::kFloat);
+  const size_t nb = tcfp_linear_cross_entropy_workspace_bytes(in.h.rows, in.w.rows, in.h.cols);
   Tensor ws = g.empty({int64_t(std::max<size_t>(nb, 16))}, at::kByte);
   check(tcfp_linear_cross_entropy(ptr(in.h.t), in.h.ld, ptr(in.w.t), in.w.ld,
                                   ptr<int64_t>(in.targets), ignore, in.h.rows, in.w.rows,
                                   in.h.cols, f32(losses), f32(lse), mean ? 1 : 0, f32(total),
-                                  ptr(ws), nb, g.stream()),
+                                  f32(count), ptr(ws), nb, g.stream()),
         "linear_cross_entropy");
-  return outs(losses, lse, total);
+  return outs(losses, lse, total, count);
 }
 
 Outs linear_cross_entropy_backward(const Tensor& grad_, const Tensor& hidden, const Tensor& weight,
@@ -1362,6 +1365,161 @@ Outs linear_cross_entropy_backward(const Tensor& grad_, const Tensor& hidden, co
             ptr(dw), ptr(ws), nb, g.stream()),
         "linear_cross_entropy_backward");
   return outs(dh, dw);
+}
+
+// ---- the same with gradients ----------------------------------------------------
+//
+// Autograd nodes in C++: a Python node's forward and backward cost some 25 us of
+// host time each, as much as the kernels of a small layer.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  return std::any_of(ts.begin(), ts.end(),
+                     [](const Tensor* t) { return t->defined() && t->requires_grad(); });
+}
+// Runs a backward's op; what it raises becomes an error that the autograd engine
+// hands to the caller.
+template <typename F>
+variable_list in_engine(F f) {
+  try {
+    return f().t;
+  } catch (const Raise& r) {
+    TORCH_CHECK(false, r.msg);
+  }
+}
+// Gradients that cannot be differentiated once more say so if they are.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& t : grads)
+    if (t.defined()) {
+      Tensor one = t.detach();
+      one.set_requires_grad(true);
+      auto error = std::make_shared<torch::autograd::DelayedError>(
+          "this operator's gradient has no gradient of its own (differentiable once)", 1);
+      t = (*error)({one})[0];
+    }
+  return grads;
+}
+
+Outs rotary_with_grad(const Tensor& q, const OptT& k, const Tensor& positions, const Tensor& freqs,
+                      bool interleaved, double amplitude, bool inverse);
+
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptT& k,
+                               const Tensor& positions, const Tensor& freqs, bool interleaved,
+                               double amplitude, bool inverse) {
+    ctx->save_for_backward({positions, freqs});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["amplitude"] = amplitude;
+    ctx->saved_data["inverse"] = inverse;
+    Outs o = rotary(q, k, positions, freqs, interleaved, amplitude, inverse);
+    if (!k) o.t.pop_back();
+    return o.t;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    // (a linear map: its gradient is the other turn, and has one itself)
+    const bool has_k = grads.size() == 2;
+    const variable_list saved = ctx->get_saved_variables();
+    const bool need_q = ctx->needs_input_grad(0), need_k = has_k && ctx->needs_input_grad(1);
+    variable_list out(7);
+    if (!need_q && !need_k) return out;
+    const variable_list got = in_engine([&] {
+      return rotary_with_grad(grads[need_q ? 0 : 1], need_q && need_k ? OptT(grads[1]) : OptT(),
+                              saved[0], saved[1], ctx->saved_data["interleaved"].toBool(),
+                              ctx->saved_data["amplitude"].toDouble(),
+                              !ctx->saved_data["inverse"].toBool());
+    });
+    out[need_q ? 0 : 1] = got[0];
+    if (need_q && need_k) out[1] = got[1];
+    return out;
+  }
+};
+
+Outs rotary_with_grad(const Tensor& q, const OptT& k, const Tensor& positions, const Tensor& freqs,
+                      bool interleaved, double amplitude, bool inverse) {
+  if (!wants_grad({&q, &opt(k)}))
+    return rotary(q, k, positions, freqs, interleaved, amplitude, inverse);
+  Outs o{RotaryNode::apply(q, k, positions, freqs, interleaved, amplitude, inverse)};
+  if (!k) o.t.emplace_back();
+  return o;
+}
+
+struct PackedNode : torch::autograd::Function<PackedNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const Tensor& starts, const OptT& key_starts, int64_t max_len,
+                        std::optional<int64_t> max_key_len, std::optional<double> scale,
+                        bool causal, int64_t window) {
+    Outs o = packed_attention(q, k, v, starts, key_starts, max_len, scale, causal, window, true);
+    ctx->save_for_backward({q, k, v, o.t[0], o.t[1], o.t[2], starts, opt(key_starts)});
+    ctx->saved_data["max_len"] = max_len;
+    ctx->saved_data["max_key_len"] = max_key_len;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["window"] = window;
+    return o.t[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    auto& how = ctx->saved_data;
+    variable_list got = in_engine([&] {
+      const at::NoGradGuard no_grad;
+      return packed_attention_backward(
+          grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7].defined() ? OptT(s[7]) : OptT(),
+          how["max_len"].toInt(), how["max_key_len"].toOptional<int64_t>(),
+          how["scale"].toOptional<double>(), how["causal"].toBool(), how["window"].toInt());
+    });
+    for (size_t i = 0; i < 3; ++i)
+      if (!ctx->needs_input_grad(i)) got[i].reset();
+    got = once(std::move(got));
+    got.resize(10);
+    return got;
+  }
+};
+
+Tensor packed_attention_with_grad(const Tensor& q, const Tensor& k, const Tensor& v,
+                                  const Tensor& starts, const OptT& key_starts, int64_t max_len,
+                                  std::optional<int64_t> max_key_len, std::optional<double> scale,
+                                  bool causal, int64_t window) {
+  if (max_key_len && *max_key_len < 0)
+    value_error("max_len and max_key_len must not be negative");
+  if (!wants_grad({&q, &k, &v}))
+    return packed_attention(q, k, v, starts, key_starts, max_len, scale, causal, window, false).t[0];
+  return PackedNode::apply(q, k, v, starts, key_starts, max_len, max_key_len, scale, causal,
+                           window);
+}
+
+struct LossNode : torch::autograd::Function<LossNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight,
+                        const Tensor& targets, int64_t ignore, bool reduce, bool mean) {
+    Outs o = linear_cross_entropy(hidden, weight, targets, ignore, reduce, mean);
+    ctx->save_for_backward({hidden, weight, targets, o.t[1], mean ? o.t[3] : Tensor()});
+    ctx->saved_data["ignore"] = ignore;
+    return reduce ? o.t[2] : o.t[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    variable_list got = in_engine([&] {
+      const at::NoGradGuard no_grad;
+      return linear_cross_entropy_backward(
+          grads[0], s[0], s[1], s[2], s[3], s[4].defined() ? OptT(s[4]) : OptT(),
+          ctx->saved_data["ignore"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+    });
+    got = once(std::move(got));
+    got.resize(6);
+    return got;
+  }
+};
+
+Tensor linear_cross_entropy_with_grad(const Tensor& hidden, const Tensor& weight,
+                                      const Tensor& targets, int64_t ignore, bool reduce,
+                                      bool mean) {
+  if (wants_grad({&hidden, &weight}))
+    return LossNode::apply(hidden, weight, targets, ignore, reduce, mean);
+  const Outs o = linear_cross_entropy(hidden, weight, targets, ignore, reduce, mean);
+  return reduce ? o.t[2] : o.t[0];
 }
 
 }  // namespace
@@ -1419,9 +1577,11 @@ PYBIND11_MODULE(_tcfp_host, m) {
   m.def("kv_cache_write", &kv_cache_write, NoGil());
   m.def("kv_cache_read", &kv_cache_read, NoGil());
   m.def("paged_attention", &paged_attention, NoGil());
-  m.def("rotary", &rotary, NoGil());
-  m.def("packed_attention", &packed_attention, NoGil());
+  m.def("rotary_embedding", &rotary_with_grad, NoGil());
+  m.def("packed_attention", &packed_attention_with_grad, NoGil());
+  m.def("packed_attention_forward", &packed_attention, NoGil());
   m.def("packed_attention_backward", &packed_attention_backward, NoGil());
-  m.def("linear_cross_entropy", &linear_cross_entropy, NoGil());
+  m.def("linear_cross_entropy", &linear_cross_entropy_with_grad, NoGil());
+  m.def("linear_cross_entropy_forward", &linear_cross_entropy, NoGil());
   m.def("linear_cross_entropy_backward", &linear_cross_entropy_backward, NoGil());
 }

@@ -13,6 +13,8 @@
 // rows the run owns.  g is rounded to bf16 once (2^-9 of each value, as the
 // results themselves are); all sums are fp32.
 #include <algorithm>
+#include <cmath>
+#include <utility>
 
 #include "mfma_tiles.h"
 
@@ -27,17 +29,19 @@ namespace {
 // the way into the registers.  So W serves z = h W^T and dh = g W, and g serves
 // dh = g W and dW = g^T h, without transposed copies.
 //
-// A workgroup owns T x T of C.  T = 256: eight waves, 2 along m and 4 along n,
-// 128 x 64 each; two stages of 64 k in LDS (128 KiB), one workgroup a CU.
-// T = 128: four waves of 64 x 64 and four stages, for outputs of few tiles.
+// A workgroup owns T x T of C over a run of k (a split).  T = 256: eight waves, 2
+// along m and 4 along n, 128 x 64 each; two stages of 64 k in LDS (128 KiB), one
+// workgroup a CU.  T = 128: four waves of 64 x 64; four stages (one workgroup a CU:
+// what streams one operand from HBM, or has few tiles) or two (two workgroups, of
+// which one multiplies while the other waits or stores).  cost() says which is taken.
 // A stage's copies are issued as soon as every wave has read its last operands
 // of the stage whose place they take, in the middle of that stage's products.
 constexpr int kStageK = 64;
 
-template <int T>
+template <int T, int ST>
 struct Shape {
   static constexpr int WAVES = T == 256 ? 8 : 4, THREADS = 64 * WAVES;
-  static constexpr int STAGES = T == 256 ? 2 : 4;
+  static constexpr int STAGES = ST;
   static constexpr int MB = T / 64, NB = 2;  // 32-row and 32-column blocks of a wave
   static constexpr int WAVES_M = 2;
   static constexpr int OPERAND = T * kStageK * 2, STAGE = 2 * OPERAND;
@@ -48,7 +52,7 @@ struct Product {
   int64_t lda, ldb;  // elements
   int m, n, k;
   int tiles_m, tiles_n;
-  int k_run;         // k of a split (blockIdx.y), a multiple of 64
+  int splits, k_run; // of k, the latter a multiple of 64
   // results: bf16 or fp32 [n, m], rows ldo apart
   void* out;
   int64_t ldo;
@@ -61,6 +65,7 @@ struct Product {
   int64_t classes;   // of the whole vocabulary
   float2* part;      // [tiles_m, n]: maximum in units of log2, sum
   float* picked;     // [n]: z of the target
+  int* done;         // cleared for the launch that joins the parts
   const float* lse;
   const float* grad;       // one a token (grad_step 1) or for all (0)
   int grad_step;
@@ -103,27 +108,29 @@ struct Copies {
   }
 };
 
-template <int T, bool TA, bool TB, int EPI>
-__global__ __launch_bounds__(Shape<T>::THREADS, 1) void product_kernel(Product g) {
-  using S = Shape<T>;
+template <int T, int ST, bool TA, bool TB, int EPI>
+__global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) void product_kernel(Product g) {
+  using S = Shape<T, ST>;
   __shared__ __align__(16) uint8_t lds[S::STAGES * S::STAGE];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int wm = wave % S::WAVES_M, wn = wave / S::WAVES_M;
 
-  // Each XCD (workgroup b is on XCD b % 8) takes a run of tiles, in groups of
-  // four tile rows along n, so that its L2 holds both operands' panels.
-  int m0, n0;
+  // Each XCD (workgroup b is on XCD b % 8) takes a run of the splits' tiles, in
+  // groups of four tile rows along n, so that its L2 holds both operands' panels.
+  int m0, n0, split;
   {
-    const int tiles = g.tiles_m * g.tiles_n;
+    const int tiles = g.tiles_m * g.tiles_n, units = tiles * g.splits;
     int l = int(blockIdx.x);
-    l = (l & 7) * (tiles >> 3) + min(l & 7, tiles & 7) + (l >> 3);
+    l = (l & 7) * (units >> 3) + min(l & 7, units & 7) + (l >> 3);
+    split = l / tiles;
+    l -= split * tiles;
     const int per = 4 * g.tiles_m, first = l / per * 4, rows = min(g.tiles_n - first, 4);
     n0 = (first + l % per % rows) * T;
     m0 = l % per / rows * T;
   }
-  const int k0 = int(blockIdx.y) * g.k_run, k1 = min(g.k, k0 + g.k_run);
+  const int k0 = split * g.k_run, k1 = min(g.k, k0 + g.k_run);
   const int stages = (k1 - k0 + kStageK - 1) / kStageK;
 
   Copies<T, TA> ca;
@@ -211,7 +218,11 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 1) void product_kernel(Product g
 #pragma unroll
     for (int x = 0; x < S::MB; ++x)
 #pragma unroll
-      for (int y = 0; y < S::NB; ++y) asm volatile("" : "+v"(acc[x][y]));
+      for (int y = 0; y < S::NB; ++y) {
+        // (where a wave has 512 registers its accumulators lie in the second half)
+        if constexpr (T == 256 || ST == 2) asm volatile("" : "+v"(acc[x][y]));
+        else asm volatile("" : "+a"(acc[x][y]));
+      }
   };
 
   // (copies past the last stage read nothing and keep the count of what is in
@@ -244,7 +255,7 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 1) void product_kernel(Product g
   const int mw = wm * S::MB * 32, nw = wn * 64;
   auto m_of = [&](int x, int r) { return mw + 32 * x + 8 * (r >> 2) + 4 * half + (r & 3); };
   if constexpr (EPI == kFp32) {
-    float* out = static_cast<float*>(g.out) + int64_t(blockIdx.y) * g.split_stride;
+    float* out = static_cast<float*>(g.out) + int64_t(split) * g.split_stride;
 #pragma unroll
     for (int y = 0; y < S::NB; ++y) {
       const int n = n0 + nw + 32 * y + col;
@@ -269,6 +280,7 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 1) void product_kernel(Product g
   }
   if constexpr (EPI == kStats) {
     float2* both = reinterpret_cast<float2*>(lds);  // [wave along m][n of the tile]
+    if (blockIdx.x == 0 && threadIdx.x == 0) *g.done = 0;
 #pragma unroll
     for (int y = 0; y < S::NB; ++y) {
       const int n = n0 + nw + 32 * y + col;
@@ -323,13 +335,13 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 1) void product_kernel(Product g
     for (int y = 0; y < S::NB; ++y) {
       const int nl = nw + 32 * y + col, n = n0 + nl;
       float scale = 0.0f, off = 0.0f;
-      int w = -1;
+      int rel = -1;  // the target's place among the lane's values
       bool keep = false;
       if constexpr (EPI == kGrad) {
         if (n < g.n) {
           const int64_t target = g.targets[n], want = target - g.first - m0;
           keep = target != g.ignore;
-          w = want >= 0 && want < T ? int(want) : -1;
+          rel = want >= 0 && want < T ? int(want) - mw - 4 * half : -1;
           scale = g.grad[int64_t(n) * g.grad_step];
           if (g.count) scale /= *g.count;
           // (a target outside the vocabulary has a loss that is NaN, and so are
@@ -348,9 +360,15 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 1) void product_kernel(Product g
           for (int r = 0; r < 4; ++r) {
             v[r] = acc[x][y][4 * q + r];
             if constexpr (EPI == kGrad) {
-              float p = exp2_fast(__builtin_fmaf(v[r], kLog2e, -off));
-              if (m + r == w) p -= 1.0f;
-              v[r] = keep && m0 + m + r < g.m ? p * scale : 0.0f;
+              const float p = exp2_fast(__builtin_fmaf(v[r], kLog2e, -off));
+              v[r] = keep ? (p - (rel == 32 * x + 8 * q + r ? 1.0f : 0.0f)) * scale : 0.0f;
+            }
+          }
+          if constexpr (EPI == kGrad) {
+            if (m0 + T > g.m) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (m0 + m + r >= g.m) v[r] = 0.0f;
             }
           }
           const int chunk = (m >> 3) ^ (nl & (CH - 1));
@@ -374,36 +392,43 @@ __global__ __launch_bounds__(Shape<T>::THREADS, 1) void product_kernel(Product g
 
 // ---- the joins ----------------------------------------------------------------
 
-// Every token's lse and loss from its partial maxima and sums; sums[block] =
-// (sum of the block's losses, tokens that count).  32 tokens a block, eight
-// threads each.
+// Every token's lse and loss from its partial maxima and sums: eight tokens a
+// block, 32 threads each, then, for `total`, by the block that is done last, the sum
+// of all blocks' sums in their order: total[0] = the losses' sum or mean, total[1] =
+// the tokens that count.  (A launch of its own for that took 4.8 us; the counter
+// `done` is cleared by the launch before.)
+constexpr int kJoinTokens = 8;
 __global__ __launch_bounds__(256) void join_losses_kernel(
     const float2* __restrict__ part, int parts, const float* __restrict__ picked,
     const int64_t* __restrict__ targets, int64_t ignore, int64_t classes, int tokens,
-    float* __restrict__ losses, float* __restrict__ lse, double2* __restrict__ sums) {
-  __shared__ float2 s[8][32];
-  const int tl = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int t = int(blockIdx.x) * 32 + tl;
+    float* __restrict__ losses, float* __restrict__ lse, double* __restrict__ sums, int* done,
+    int mean, float* __restrict__ total, float* __restrict__ count_out) {
+  __shared__ float2 s[32][kJoinTokens];
+  __shared__ double2 d[256];
+  __shared__ bool last;
+  const int tl = threadIdx.x % kJoinTokens, slice = threadIdx.x / kJoinTokens;
+  const int t = int(blockIdx.x) * kJoinTokens + tl;
   float top = -INFINITY, sum = 0.0f;
+  auto add = [&](const float2& p) {
+    if (p.y == 0.0f) return;
+    const float next = fmaxf(top, p.x);
+    sum = (sum == 0.0f ? 0.0f : sum * exp2_fast(top - next)) + p.y * exp2_fast(p.x - next);
+    top = next;
+  };
   if (t < tokens)
-    for (int i = slice; i < parts; i += 8) {
-      const float2 p = part[int64_t(i) * tokens + t];
-      if (p.y == 0.0f) continue;
-      const float next = fmaxf(top, p.x);
-      sum = (sum == 0.0f ? 0.0f : sum * exp2_fast(top - next)) + p.y * exp2_fast(p.x - next);
-      top = next;
+    for (int i = slice; i < parts; i += 4 * 32) {
+      float2 p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        p[j] = i + 32 * j < parts ? part[int64_t(i + 32 * j) * tokens + t] : make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) add(p[j]);
     }
   s[slice][tl] = make_float2(top, sum);
   __syncthreads();
   double loss = 0.0, count = 0.0;
   if (slice == 0 && t < tokens) {
-    for (int i = 1; i < 8; ++i) {
-      const float2 p = s[i][tl];
-      if (p.y == 0.0f) continue;
-      const float next = fmaxf(top, p.x);
-      sum = (sum == 0.0f ? 0.0f : sum * exp2_fast(top - next)) + p.y * exp2_fast(p.x - next);
-      top = next;
-    }
+    for (int i = 1; i < 32; ++i) add(s[i][tl]);
     const float l = (top + log2_fast(sum)) * kLn2;
     const int64_t target = targets[t];
     const bool keep = target != ignore;
@@ -413,36 +438,48 @@ __global__ __launch_bounds__(256) void join_losses_kernel(
     loss = each;
     count = keep ? 1.0 : 0.0;
   }
-  if (sums && threadIdx.x < 64) {
+  if (!total) return;
+  if (threadIdx.x < 64) {  // (the block's tokens are its first eight threads)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = kJoinTokens / 2; o > 0; o >>= 1) {
       loss += __shfl_xor(loss, o);
       count += __shfl_xor(count, o);
     }
-    if (threadIdx.x == 0) sums[blockIdx.x] = make_double2(loss, count);
+    if (threadIdx.x == 0) {
+      // (past this XCD's L2, as what reads them may run on another)
+      __hip_atomic_store(sums + 2 * blockIdx.x, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(sums + 2 * blockIdx.x + 1, count, __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+      last = __hip_atomic_fetch_add(done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+             int(gridDim.x) - 1;
+    }
   }
-}
-
-// total[0] = the losses' sum or mean, total[1] = the tokens that count; one
-// workgroup, in one order.
-__global__ __launch_bounds__(256) void total_loss_kernel(const double2* __restrict__ sums, int n,
-                                                         int mean, float* __restrict__ total) {
-  __shared__ double2 s[256];
+  __syncthreads();
+  if (!last) return;
   double a = 0.0, b = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) a += sums[i].x, b += sums[i].y;
-  s[threadIdx.x] = make_double2(a, b);
+  for (int i = threadIdx.x; i < int(gridDim.x); i += 256) {
+    a += __hip_atomic_load(sums + 2 * i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    b += __hip_atomic_load(sums + 2 * i + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  d[threadIdx.x] = make_double2(a, b);
   __syncthreads();
   for (int o = 128; o > 0; o >>= 1) {
     if (int(threadIdx.x) < o) {
-      s[threadIdx.x].x += s[threadIdx.x + o].x;
-      s[threadIdx.x].y += s[threadIdx.x + o].y;
+      d[threadIdx.x].x += d[threadIdx.x + o].x;
+      d[threadIdx.x].y += d[threadIdx.x + o].y;
     }
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    total[0] = float(mean ? s[0].x / s[0].y : s[0].x);
-    total[1] = float(s[0].y);
+    *total = float(mean ? d[0].x / d[0].y : d[0].x);
+    *count_out = float(d[0].y);
   }
+}
+
+// The total of no tokens.
+__global__ void no_tokens_kernel(int mean, float* total, float* count) {
+  *total = mean ? NAN : 0.0f;
+  *count = 0.0f;
 }
 
 // out = the sum of `splits` fp32 [n, m] arrays in bf16, in order; eight columns a
@@ -475,9 +512,45 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 int launch_status() { return hipGetLastError() == hipSuccess ? TCFP_OK : TCFP_ERR_HIP; }
 
-// The tile of z: 256 where that gives every CU one.
-int logits_tile(int64_t tokens, int64_t classes) {
-  return ceil_div(tokens, 256) * ceil_div(classes, 256) >= kCus ? 256 : 128;
+// How C [n, m] over k is computed: tile, stages in LDS, splits of k.
+struct Cut {
+  int tile, ring, splits, k_run;
+};
+// What `units` tiles of `stages` each take, us, by what was measured: a stage 1.5,
+// 0.55 and (two workgroups on a CU) 0.98 us, first loads and result 9.5, 4 and 5; e.g.
+// 2048 x 8192 over 4096: 107 us in tiles of 256, 125 with 128 and two stages, 150
+// with four; 64 x 32768 over 4096, where W comes from HBM: 55 with 128 and four
+// stages, 73 with two; 1000 x 8192 over 1056: 28 with two, 33 with four.
+double cost(int tile, int ring, int64_t units, int64_t stages) {
+  if (tile == 256)
+    return double(ceil_div(units, kCus)) * (std::max(1.5 * double(stages), 4.0) + 9.5);
+  if (ring == 4) return double(ceil_div(units, kCus)) * (0.55 * double(stages) + 4);
+  const int64_t rounds = units / (2 * kCus), rest = units - rounds * 2 * kCus;
+  return double(rounds) * (0.98 * double(stages) + 5) +
+         (rest > kCus ? 0.98 * double(stages) + 5 : rest > 0 ? 0.7 * double(stages) + 4 : 0.0);
+}
+// Splits write fp32 parts, 3.5 TB/s with their sum, and take a launch more.
+Cut cut_of(int64_t n, int64_t m, int64_t k, bool may_split) {
+  const int64_t stages = std::max<int64_t>(ceil_div(k, kStageK), 1);
+  Cut best{};
+  double least = INFINITY;
+  for (const auto& [tile, ring] : {std::pair<int, int>{256, 2}, {128, 2}, {128, 4}}) {
+    const int64_t tiles = ceil_div(n, tile) * ceil_div(m, tile);
+    for (int64_t s = 1; s <= (may_split ? std::min<int64_t>(64, stages) : 1); ++s) {
+      if (s > 1 && tiles * s > 2 * kCus) break;
+      const int64_t each = ceil_div(stages, s);
+      const double t = cost(tile, ring, tiles * s, each) +
+                       (s > 1 ? double(n) * double(m) * 8 * double(s) / 3.5e6 + 4 : 0.0);
+      if (t < least) {
+        least = t;
+        best = {tile, ring, int(ceil_div(stages, each)), int(each * kStageK)};
+      }
+    }
+  }
+  return best;
+}
+Cut logits_cut(int64_t tokens, int64_t classes, int64_t dim) {
+  return cut_of(tokens, classes, dim, false);
 }
 // Classes of a run of the backward pass (a multiple of 256, whole tiles).
 int64_t run_of(int64_t tokens, int64_t vocab) {
@@ -488,37 +561,24 @@ int64_t run_of(int64_t tokens, int64_t vocab) {
   const int64_t runs = ceil_div(all, most);
   return ceil_div(ceil_div(all, runs), 256) * 256;
 }
-// How C [n, m] over k is cut: tile, splits of k.
-struct Cut {
-  int tile, splits, k_run;
-};
-Cut cut_of(int64_t n, int64_t m, int64_t k) {
-  Cut c{256, 1, int(ceil_div(k, kStageK) * kStageK)};
-  if (ceil_div(n, 256) * ceil_div(m, 256) >= kCus) return c;
-  c.tile = 128;
-  const int64_t tiles = ceil_div(n, 128) * ceil_div(m, 128);
-  // splits of at least eight stages, to one workgroup a CU
-  int64_t splits = std::min(kCus / std::max<int64_t>(tiles, 1), k / (8 * kStageK));
-  if (splits < 2) return c;
-  c.k_run = int(ceil_div(ceil_div(k, splits), kStageK) * kStageK);
-  c.splits = int(ceil_div(k, c.k_run));
-  return c;
-}
 
-template <int T, bool TA, bool TB, int EPI>
-int launch(Product p, int splits, hipStream_t st) {
+template <int T, int ST, bool TA, bool TB, int EPI>
+int launch(Product p, hipStream_t st) {
+  constexpr int THREADS = Shape<T, ST>::THREADS;
   p.tiles_m = int(ceil_div(p.m, T));
   p.tiles_n = int(ceil_div(p.n, T));
-  const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
-  if (!grid_x_fits(tiles, Shape<T>::THREADS) || tiles > INT32_MAX) return TCFP_ERR_SHAPE;
-  product_kernel<T, TA, TB, EPI>
-      <<<dim3(unsigned(tiles), unsigned(splits)), Shape<T>::THREADS, 0, st>>>(p);
+  const int64_t units = int64_t(p.tiles_m) * p.tiles_n * p.splits;
+  if (!grid_x_fits(units, THREADS) || units > INT32_MAX) return TCFP_ERR_SHAPE;
+  product_kernel<T, ST, TA, TB, EPI><<<unsigned(units), THREADS, 0, st>>>(p);
   return launch_status();
 }
 template <bool TA, bool TB, int EPI>
-int launch_tile(int tile, const Product& p, int splits, hipStream_t st) {
-  return tile == 256 ? launch<256, TA, TB, EPI>(p, splits, st)
-                     : launch<128, TA, TB, EPI>(p, splits, st);
+int launch_cut(const Cut& c, Product p, hipStream_t st) {
+  p.splits = c.splits;
+  p.k_run = c.k_run;
+  return c.tile == 256 ? launch<256, 2, TA, TB, EPI>(p, st)
+         : c.ring == 2 ? launch<128, 2, TA, TB, EPI>(p, st)
+                       : launch<128, 4, TA, TB, EPI>(p, st);
 }
 
 struct Layout {
@@ -531,12 +591,12 @@ Layout layout_of(int64_t tokens, int64_t vocab, int64_t dim, bool need_h, bool n
   l.run = run_of(tokens, vocab);
   l.g = align256(size_t(tokens) * size_t(l.run) * 2);
   if (need_h) {
-    l.dh = cut_of(tokens, dim, l.run);
+    l.dh = cut_of(tokens, dim, std::min(l.run, vocab), true);
     if (l.dh.splits > 1 || l.run < vocab)
       l.sum_h = align256(size_t(l.dh.splits) * size_t(tokens) * size_t(dim) * 4);
   }
   if (need_w) {
-    l.dw = cut_of(std::min(l.run, vocab), dim, tokens);
+    l.dw = cut_of(std::min(l.run, vocab), dim, tokens, true);
     if (l.dw.splits > 1)
       l.sum_w = align256(size_t(l.dw.splits) * size_t(std::min(l.run, vocab)) * size_t(dim) * 4);
   }
@@ -559,31 +619,32 @@ int check_sizes(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
 
 extern "C" {
 
-size_t tcfp_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t vocab) {
-  if (tokens <= 0 || vocab <= 0) return 0;
-  const int64_t parts = ceil_div(vocab, logits_tile(tokens, vocab));
+size_t tcfp_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim) {
+  if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
+  const int64_t parts = ceil_div(vocab, logits_cut(tokens, vocab, dim).tile);
   return align256(size_t(parts) * size_t(tokens) * 8) + align256(size_t(tokens) * 4) +
-         align256(size_t(ceil_div(tokens, 32)) * 16);
+         align256(size_t(ceil_div(tokens, kJoinTokens)) * 16) + 256;
 }
 
 int tcfp_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                               const int64_t* targets, int64_t ignore, int64_t tokens,
                               int64_t vocab, int64_t dim, float* losses, float* lse, int mean,
-                              float* total, void* workspace, size_t workspace_bytes,
+                              float* total, float* count, void* workspace, size_t workspace_bytes,
                               void* stream) {
   const int rc = check_sizes(hidden, ldh, weight, ldw, tokens, vocab, dim);
   if (rc != TCFP_OK) return rc;
-  if (!workspace || workspace_bytes < tcfp_linear_cross_entropy_workspace_bytes(tokens, vocab) ||
+  if (!total != !count) return TCFP_ERR_SHAPE;
+  if (!workspace || workspace_bytes < tcfp_linear_cross_entropy_workspace_bytes(tokens, vocab, dim) ||
       !aligned16(workspace)) {
     if (tokens > 0) return TCFP_ERR_WORKSPACE;
   }
   const auto st = static_cast<hipStream_t>(stream);
   if (tokens == 0) {
-    if (total) total_loss_kernel<<<1, 256, 0, st>>>(nullptr, 0, mean, total);
+    if (total) no_tokens_kernel<<<1, 1, 0, st>>>(mean, total, count);
     return launch_status();
   }
-  const int tile = logits_tile(tokens, vocab);
-  const int64_t parts = ceil_div(vocab, tile);
+  const Cut cut = logits_cut(tokens, vocab, dim);
+  const int64_t parts = ceil_div(vocab, cut.tile);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Product p{};
   p.a = static_cast<const uint16_t*>(weight);
@@ -593,20 +654,20 @@ int tcfp_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weigh
   p.m = int(vocab);
   p.n = int(tokens);
   p.k = int(dim);
-  p.k_run = int(ceil_div(dim, kStageK) * kStageK);
   p.targets = targets;
   p.classes = vocab;
   p.part = reinterpret_cast<float2*>(ws);
   ws += align256(size_t(parts) * size_t(tokens) * 8);
   p.picked = reinterpret_cast<float*>(ws);
   ws += align256(size_t(tokens) * 4);
-  double2* sums = total ? reinterpret_cast<double2*>(ws) : nullptr;
-  const int done = launch_tile<false, false, kStats>(tile, p, 1, st);
-  if (done != TCFP_OK) return done;
-  const unsigned blocks = unsigned(ceil_div(tokens, 32));
+  const unsigned blocks = unsigned(ceil_div(tokens, kJoinTokens));
+  double* sums = reinterpret_cast<double*>(ws);
+  p.done = reinterpret_cast<int*>(ws + align256(size_t(blocks) * 16));
+  const int rc_product = launch_cut<false, false, kStats>(cut, p, st);
+  if (rc_product != TCFP_OK) return rc_product;
   join_losses_kernel<<<blocks, 256, 0, st>>>(p.part, int(parts), p.picked, targets, ignore, vocab,
-                                             int(tokens), losses, lse, sums);
-  if (total) total_loss_kernel<<<1, 256, 0, st>>>(sums, int(blocks), mean, total);
+                                             int(tokens), losses, lse, sums, p.done, mean, total,
+                                             count);
   return launch_status();
 }
 
@@ -665,7 +726,6 @@ int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const vo
     p.m = int(classes);
     p.n = int(tokens);
     p.k = int(dim);
-    p.k_run = int(ceil_div(dim, kStageK) * kStageK);
     p.out = g;
     p.ldo = l.run;
     p.targets = targets;
@@ -676,7 +736,7 @@ int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const vo
     p.grad = grad;
     p.grad_step = int(grad_step);
     p.count = count;
-    int done = launch_tile<false, false, kGrad>(logits_tile(tokens, classes), p, 1, st);
+    int done = launch_cut<false, false, kGrad>(logits_cut(tokens, classes, dim), p, st);
     if (done != TCFP_OK) return done;
     if (need_h) {
       // dh[t][d] += sum over the run's classes of g[t][v] W[v][d]
@@ -688,20 +748,19 @@ int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const vo
       q.m = int(dim);
       q.n = int(tokens);
       q.k = int(classes);
-      q.k_run = l.dh.k_run;
       if (l.sum_h) {
         q.out = sum_h;
         q.ldo = dim;
         q.split_stride = tokens * dim;
         q.add = v0 > 0;
         // (a last, shorter run may leave splits without classes: nothing to add)
-        const int splits = v0 > 0 ? int(std::min<int64_t>(l.dh.splits, ceil_div(classes, l.dh.k_run)))
-                                  : l.dh.splits;
-        done = launch_tile<true, false, kFp32>(l.dh.tile, q, splits, st);
+        Cut cut = l.dh;
+        if (v0 > 0) cut.splits = int(std::min<int64_t>(cut.splits, ceil_div(classes, cut.k_run)));
+        done = launch_cut<true, false, kFp32>(cut, q, st);
       } else {
         q.out = grad_hidden;
         q.ldo = dim;
-        done = launch_tile<true, false, kBf16>(l.dh.tile, q, 1, st);
+        done = launch_cut<true, false, kBf16>(l.dh, q, st);
       }
       if (done != TCFP_OK) return done;
     }
@@ -715,17 +774,16 @@ int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const vo
       q.m = int(dim);
       q.n = int(classes);
       q.k = int(tokens);
-      q.k_run = l.dw.k_run;
       uint16_t* out = static_cast<uint16_t*>(grad_weight) + v0 * dim;
       q.ldo = dim;
       if (l.dw.splits > 1) {
         q.out = sum_w;
         q.split_stride = classes * dim;
-        done = launch_tile<true, true, kFp32>(l.dw.tile, q, l.dw.splits, st);
+        done = launch_cut<true, true, kFp32>(l.dw, q, st);
         if (done == TCFP_OK) done = round_sum(sum_w, l.dw.splits, classes * dim, out);
       } else {
         q.out = out;
-        done = launch_tile<true, true, kBf16>(l.dw.tile, q, 1, st);
+        done = launch_cut<true, true, kBf16>(l.dw, q, st);
       }
       if (done != TCFP_OK) return done;
     }

@@ -45,13 +45,6 @@ def linear_cross_entropy(
     """
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        return _LinearCrossEntropy.apply(hidden, weight, targets, int(ignore_index), reduction)
-    losses, _, total = _forward(hidden, weight, targets, ignore_index, reduction)
-    return losses if reduction == "none" else total[0]
-
-
-def _forward(hidden, weight, targets, ignore_index, reduction):
     return _hip.host().linear_cross_entropy(hidden, weight, targets, int(ignore_index),
                                             reduction != "none", reduction == "mean")
 
@@ -66,7 +59,8 @@ def linear_cross_entropy_forward(
     """``(losses, lse)`` of every token, fp32: :func:`linear_cross_entropy` without
     autograd or reduction, and the log sum of exponentials of its logits, which
     :func:`linear_cross_entropy_backward` takes."""
-    return _forward(hidden, weight, targets, ignore_index, "none")[:2]
+    return _hip.host().linear_cross_entropy_forward(hidden, weight, targets, int(ignore_index),
+                                                    False, False)[:2]
 
 
 def linear_cross_entropy_backward(
@@ -91,23 +85,3 @@ def linear_cross_entropy_backward(
     return _hip.host().linear_cross_entropy_backward(grad, hidden, weight, targets, lse, count,
                                                      int(ignore_index), bool(need_hidden_grad),
                                                      bool(need_weight_grad))
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index, reduction):
-        losses, lse, total = _forward(hidden, weight, targets, ignore_index, reduction)
-        count = total[1] if reduction == "mean" else None
-        ctx.save_for_backward(hidden, weight, targets, lse, count)
-        ctx.ignore_index = ignore_index
-        return losses if reduction == "none" else total[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        hidden, weight, targets, lse, count = ctx.saved_tensors
-        need_h, need_w = ctx.needs_input_grad[:2]
-        dh, dw = linear_cross_entropy_backward(
-            grad, hidden, weight, targets, lse, count=count, ignore_index=ctx.ignore_index,
-            need_hidden_grad=need_h, need_weight_grad=need_w)
-        return dh, dw, None, None, None

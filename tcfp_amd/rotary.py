@@ -78,34 +78,8 @@ def rotary_embedding(
     Angles are formed in fp64, products in fp32, results rounded once, in new
     tensors.
 
-    Differentiable in ``q`` and ``k``: the gradient is turned the other way.
+    Differentiable in ``q`` and ``k``, any number of times: the gradient is turned the
+    other way.
     """
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotary.apply(q, k, positions, freqs, bool(interleaved), float(amplitude),
-                             bool(inverse))
-    return _hip.host().rotary(q, k, positions, freqs, bool(interleaved), float(amplitude),
-                              bool(inverse))
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, freqs, interleaved, amplitude, inverse):
-        ctx.save_for_backward(positions, freqs)
-        ctx.how = interleaved, amplitude, inverse
-        return _hip.host().rotary(q, k, positions, freqs, interleaved, amplitude, inverse)
-
-    @staticmethod
-    def backward(ctx, grad_q, grad_k):
-        # (a linear map: its gradient is differentiable like itself)
-        interleaved, amplitude, inverse = ctx.how
-        positions, freqs = ctx.saved_tensors
-        if not ctx.needs_input_grad[0]:
-            grad_q, grad_k = None, rotary_embedding(
-                grad_k, None, positions, freqs, interleaved=interleaved, amplitude=amplitude,
-                inverse=not inverse)[0]
-        else:
-            need_k = ctx.needs_input_grad[1]
-            grad_q, grad_k = rotary_embedding(
-                grad_q, grad_k if need_k else None, positions, freqs, interleaved=interleaved,
-                amplitude=amplitude, inverse=not inverse)
-        return grad_q, grad_k, None, None, None, None, None
+    return _hip.host().rotary_embedding(q, k, positions, freqs, bool(interleaved),
+                                        float(amplitude), bool(inverse))
