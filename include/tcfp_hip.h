@@ -817,7 +817,28 @@ int tcfp_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weigh
                               float* total, float* count, void* workspace,
                               size_t workspace_bytes, void* stream);
 
-/* Its gradients: g[t] = (softmax(z[t]) - onehot(targets[t])) * grad[t * grad_step]
+/* The same with the gradients of total: grad_hidden and grad_weight (bf16,
+ * contiguous, either may be NULL) of the losses' sum or mean, in three products, as the
+ * logits' exponentials stay in the workspace (16 bits each) until they are used.
+ * ..._workspace_bytes is 0 where those would take more than 1 GiB (or for more than
+ * 2^20 classes or 524280 tokens): such sizes are refused, and take the pair of
+ * functions above and below. */
+size_t tcfp_linear_cross_entropy_train_workspace_bytes(int64_t tokens, int64_t vocab,
+                                                       int64_t dim, int need_hidden,
+                                                       int need_weight);
+int tcfp_linear_cross_entropy_train(const void* hidden, int64_t ldh, const void* weight,
+                                    int64_t ldw, const int64_t* targets, int64_t ignore,
+                                    int64_t tokens, int64_t vocab, int64_t dim, float* losses,
+                                    float* lse, int mean, float* total, float* count,
+                                    void* grad_hidden, void* grad_weight, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* a and b (bf16, numbers of values multiples of 8, 16-byte aligned) times *by, in
+ * place; untouched where *by is 1. */
+int tcfp_scale_bf16(void* a, int64_t a_values, void* b, int64_t b_values, const float* by,
+                    void* stream);
+
+/* The gradients alone: g[t] = (softmax(z[t]) - onehot(targets[t])) * grad[t * grad_step]
  * (/ *count, if count is not NULL), 0 for an ignored token;
  *   grad_hidden = g weight, grad_weight = g^T hidden,
  * bf16, contiguous, either may be NULL.  grad_step is 1 (a gradient a token) or 0

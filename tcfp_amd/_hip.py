@@ -181,6 +181,12 @@ _SIGNATURES = {
     "tcfp_linear_cross_entropy": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64,
                                   _i64, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p,
                                   _c_void_p, ctypes.c_size_t, _c_void_p],
+    "tcfp_linear_cross_entropy_train_workspace_bytes": [_i64, _i64, _i64, _i32, _i32],
+    "tcfp_linear_cross_entropy_train": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64,
+                                        _i64, _i64, _c_void_p, _c_void_p, _i32, _c_void_p,
+                                        _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                                        ctypes.c_size_t, _c_void_p],
+    "tcfp_scale_bf16": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _c_void_p],
     "tcfp_linear_cross_entropy_backward_workspace_bytes": [_i64, _i64, _i64, _i32, _i32],
     "tcfp_linear_cross_entropy_backward": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64,
                                            _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64,
@@ -208,6 +214,7 @@ _RESTYPE = {
     "tcfp_paged_attention_workspace_bytes": ctypes.c_size_t,
     "tcfp_packed_attention_backward_workspace_bytes": ctypes.c_size_t,
     "tcfp_linear_cross_entropy_workspace_bytes": ctypes.c_size_t,
+    "tcfp_linear_cross_entropy_train_workspace_bytes": ctypes.c_size_t,
     "tcfp_linear_cross_entropy_backward_workspace_bytes": ctypes.c_size_t,
 }
 

@@ -1367,6 +1367,33 @@ Outs linear_cross_entropy_backward(const Tensor& grad_, const Tensor& hidden, co
   return outs(dh, dw);
 }
 
+// -> (losses, lse, total, count, dh, dw): with the gradients of total, where their
+// workspace has room (no result otherwise).
+std::optional<Outs> linear_cross_entropy_train(const Tensor& hidden, const Tensor& weight,
+                                               const Tensor& targets, int64_t ignore, bool mean,
+                                               bool need_h, bool need_w) {
+  OnGpu g;
+  g.add(hidden);
+  g.add(weight);
+  g.add(targets);
+  const c10::DeviceGuard guard(g.device());
+  const HeadIn in = head_inputs(hidden, weight, targets);
+  const size_t nb = tcfp_linear_cross_entropy_train_workspace_bytes(
+      in.h.rows, in.w.rows, in.h.cols, need_h ? 1 : 0, need_w ? 1 : 0);
+  if (nb == 0) return std::nullopt;
+  Tensor losses = g.empty(targets.sizes(), at::kFloat), lse = g.empty({in.h.rows}, at::kFloat),
+         total = g.empty({}, at::kFloat), count = g.empty({}, at::kFloat), dh, dw;
+  if (need_h) dh = g.empty(hidden.sizes(), at::kBFloat16);
+  if (need_w) dw = g.empty(weight.sizes(), at::kBFloat16);
+  Tensor ws = g.empty({int64_t(nb)}, at::kByte);
+  check(tcfp_linear_cross_entropy_train(ptr(in.h.t), in.h.ld, ptr(in.w.t), in.w.ld,
+                                        ptr<int64_t>(in.targets), ignore, in.h.rows, in.w.rows,
+                                        in.h.cols, f32(losses), f32(lse), mean ? 1 : 0, f32(total),
+                                        f32(count), ptr(dh), ptr(dw), ptr(ws), nb, g.stream()),
+        "linear_cross_entropy");
+  return outs(losses, lse, total, count, dh, dw);
+}
+
 // ---- the same with gradients ----------------------------------------------------
 //
 // Autograd nodes in C++: a Python node's forward and backward cost some 25 us of
@@ -1491,22 +1518,51 @@ Tensor packed_attention_with_grad(const Tensor& q, const Tensor& k, const Tensor
                            window);
 }
 
+// The gradients of a sum or mean are made with the forward, for a gradient of the
+// loss of 1; the backward multiplies them with what that turns out to be and hands
+// them over.  A second backward through the same node, and one of every token's
+// loss, forms the logits again.
 struct LossNode : torch::autograd::Function<LossNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight,
                         const Tensor& targets, int64_t ignore, bool reduce, bool mean) {
-    Outs o = linear_cross_entropy(hidden, weight, targets, ignore, reduce, mean);
+    std::optional<Outs> made;
+    if (reduce)
+      made = linear_cross_entropy_train(hidden, weight, targets, ignore, mean,
+                                        hidden.requires_grad(), weight.requires_grad());
+    if (made) ctx->saved_data["made"] = variable_list{made->t[4], made->t[5]};
+    Outs o = made ? std::move(*made)
+                  : linear_cross_entropy(hidden, weight, targets, ignore, reduce, mean);
     ctx->save_for_backward({hidden, weight, targets, o.t[1], mean ? o.t[3] : Tensor()});
     ctx->saved_data["ignore"] = ignore;
     return reduce ? o.t[2] : o.t[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
-    variable_list got = in_engine([&] {
-      const at::NoGradGuard no_grad;
-      return linear_cross_entropy_backward(
-          grads[0], s[0], s[1], s[2], s[3], s[4].defined() ? OptT(s[4]) : OptT(),
-          ctx->saved_data["ignore"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
-    });
+    const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    variable_list got;
+    if (const auto made = ctx->saved_data.find("made"); made != ctx->saved_data.end()) {
+      got = made->second.toTensorVector();
+      ctx->saved_data.erase(made);
+      if (!need_h) got[0].reset();
+      if (!need_w) got[1].reset();
+      in_engine([&] {
+        const c10::DeviceGuard guard(grads[0].device());
+        OnGpu g;
+        g.add(grads[0]);
+        const auto values = [](const Tensor& t) { return t.defined() ? t.numel() : 0; };
+        check(tcfp_scale_bf16(ptr(got[0]), values(got[0]), ptr(got[1]), values(got[1]),
+                              f32(grads[0]), g.stream()),
+              "linear_cross_entropy_backward");
+        return Outs{};
+      });
+    } else {
+      got = in_engine([&] {
+        const at::NoGradGuard no_grad;
+        return linear_cross_entropy_backward(grads[0], s[0], s[1], s[2], s[3],
+                                             s[4].defined() ? OptT(s[4]) : OptT(),
+                                             ctx->saved_data["ignore"].toInt(), need_h, need_w);
+      });
+    }
     got = once(std::move(got));
     got.resize(6);
     return got;

@@ -4,14 +4,19 @@
 //   z = h W^T,  lse = log sum exp z,  loss = lse - z[target]
 //   g = (softmax(z) - onehot(target)) * grad,  dh = g W,  dW = g^T h
 //
-// h [tokens, dim] and W [vocab, dim] are bf16; z is never stored.  Forward: one
-// product whose epilogue reduces every 256 (128) classes of a token to their
-// maximum and sum of exponentials, which a small launch joins.  Backward: for
-// a run of classes at a time, whose g [tokens, run] in bf16 fits a bounded
-// workspace, z is formed again with g as the epilogue, and g is the operand of
-// the products of dh, which are added up over the runs in fp32, and of dW, whose
-// rows the run owns.  g is rounded to bf16 once (2^-9 of each value, as the
-// results themselves are); all sums are fp32.
+// h [tokens, dim] and W [vocab, dim] are bf16.  Forward: one product whose epilogue
+// reduces every 256 (128) classes of a token to their maximum and sum of
+// exponentials, which a small launch joins; z is not stored.
+//
+// Gradients, where they are wanted of the losses' sum or mean and tokens x classes
+// take at most 1 GiB of workspace in 16 bits: with the forward, three products in
+// all.  The first one's epilogue leaves exp(z - maximum of its tile) in fp16 (11
+// bits, as it is rounded once more), a pass turns it into g in bf16 in place, and g
+// is the operand of dh and dW.  Otherwise (more, or a gradient for every token's
+// loss) the backward forms z again for a run of classes at a time, with g as the
+// epilogue: dh is added up over the runs in fp32, of dW a run has its rows.  g is
+// rounded to bf16 (2^-9 of each value, as the results themselves are); all sums are
+// fp32.
 #include <algorithm>
 #include <cmath>
 #include <utility>
@@ -37,6 +42,12 @@ namespace {
 // A stage's copies are issued as soon as every wave has read its last operands
 // of the stage whose place they take, in the middle of that stage's products.
 constexpr int kStageK = 64;
+
+TCFP_DEV uint32_t half2(float a, float b) {
+  typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+  const v2h v = {(_Float16)a, (_Float16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
 
 template <int T, int ST>
 struct Shape {
@@ -72,7 +83,8 @@ struct Product {
   const float* count;      // nullptr, or what grad is divided by
 };
 
-enum Epilogue { kBf16, kFp32, kStats, kGrad };
+// kStats: parts of the losses; kExps: those and the exponentials; kGrad: g.
+enum Epilogue { kBf16, kFp32, kStats, kExps, kGrad };
 
 // Offsets of one operand's copies into LDS: 4 instructions a wave and stage.
 // Rows along k: instruction q brings the rows 8 q ... of 128 bytes, whose eight
@@ -111,7 +123,9 @@ struct Copies {
 template <int T, int ST, bool TA, bool TB, int EPI>
 __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) void product_kernel(Product g) {
   using S = Shape<T, ST>;
+  constexpr bool STATS = EPI == kStats || EPI == kExps;
   __shared__ __align__(16) uint8_t lds[S::STAGES * S::STAGE];
+  __shared__ float tops[STATS ? 2 : 1][T], exps[STATS ? 2 : 1][T];  // [wave along m][n]
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -278,8 +292,7 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
     }
     return;
   }
-  if constexpr (EPI == kStats) {
-    float2* both = reinterpret_cast<float2*>(lds);  // [wave along m][n of the tile]
+  if constexpr (STATS) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *g.done = 0;
 #pragma unroll
     for (int y = 0; y < S::NB; ++y) {
@@ -290,7 +303,7 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
       // the target's place among the lane's values, if it is there
       const int rel = w - mw - 4 * half;
       const bool mine = w >= 0 && m0 + w < g.m && rel >= 0 && rel < 32 * S::MB && (rel & 4) == 0;
-      float top = -INFINITY, sum = 0.0f, pick = 0.0f;
+      float top = -INFINITY, pick = 0.0f;
       if (m0 + T > g.m) {
 #pragma unroll
         for (int x = 0; x < S::MB; ++x)
@@ -308,28 +321,37 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
         __builtin_amdgcn_sched_barrier(0);
       }
       top = fmaxf(top, __shfl_xor(top, 32));
+      if (half == 0) tops[wm][nw + 32 * y + col] = top;
+      if (mine) g.picked[n] = pick;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int y = 0; y < S::NB; ++y) {
+      const int nl = nw + 32 * y + col;
+      const float top = fmaxf(tops[0][nl], tops[1][nl]);
       const float off = top == -INFINITY ? 0.0f : top * kLog2e;
+      float sum = 0.0f;
 #pragma unroll
       for (int x = 0; x < S::MB; ++x)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          sum += exp2_fast(__builtin_fmaf(acc[x][y][r], kLog2e, -off));
+        for (int r = 0; r < 16; ++r) {
+          const float e = exp2_fast(__builtin_fmaf(acc[x][y][r], kLog2e, -off));
+          sum += e;
+          if constexpr (EPI == kExps) acc[x][y][r] = e;
+        }
       sum += __shfl_xor(sum, 32);
-      if (half == 0) both[wm * T + nw + 32 * y + col] = make_float2(off, sum);
-      if (mine) g.picked[n] = pick;
+      if (half == 0) exps[wm][nl] = sum;
     }
     __syncthreads();
     const int t = threadIdx.x, n = n0 + t;
     if (t < T && n < g.n) {
-      const float2 p = both[t], q = both[T + t];
-      // (a wave without classes has sum 0 and must not raise the maximum)
-      const float top = q.y == 0.0f ? p.x : p.y == 0.0f ? q.x : fmaxf(p.x, q.x);
-      const float sum = p.y * exp2_fast(p.x - top) + (q.y == 0.0f ? 0.0f : q.y * exp2_fast(q.x - top));
-      g.part[int64_t(m0 / T) * g.n + n] = make_float2(top, sum);
+      const float top = fmaxf(tops[0][t], tops[1][t]);
+      g.part[int64_t(m0 / T) * g.n + n] =
+          make_float2(top == -INFINITY ? 0.0f : top * kLog2e, exps[0][t] + exps[1][t]);
     }
-    return;
+    if constexpr (EPI == kStats) return;
   }
-  if constexpr (EPI == kBf16 || EPI == kGrad) {
+  if constexpr (EPI == kBf16 || EPI == kGrad || EPI == kExps) {
     constexpr int ROW = 2 * T, CH = ROW / 16;
 #pragma unroll
     for (int y = 0; y < S::NB; ++y) {
@@ -373,13 +395,15 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
           }
           const int chunk = (m >> 3) ^ (nl & (CH - 1));
           *reinterpret_cast<uint2*>(lds + nl * ROW + chunk * 16 + (m & 4) * 2) =
-              make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+              EPI == kExps ? make_uint2(half2(v[0], v[1]), half2(v[2], v[3]))
+                           : make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
         }
     }
     __syncthreads();
     uint16_t* out = static_cast<uint16_t*>(g.out);
-    // (of g whole tiles are written: what lies behind the classes is zero)
-    const int cols = EPI == kGrad ? m0 + T : g.m;
+    // (of g and the exponentials whole tiles are written: what lies behind the
+    // classes is zero)
+    const int cols = EPI == kBf16 ? g.m : m0 + T;
 #pragma unroll 4
     for (int i = threadIdx.x; i < T * CH; i += S::THREADS) {
       const int nl = i / CH, c = i % CH, n = n0 + nl, m = m0 + c * 8;
@@ -392,19 +416,45 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
 
 // ---- the joins ----------------------------------------------------------------
 
-// Every token's lse and loss from its partial maxima and sums: eight tokens a
-// block, 32 threads each, then, for `total`, by the block that is done last, the sum
-// of all blocks' sums in their order: total[0] = the losses' sum or mean, total[1] =
-// the tokens that count.  (A launch of its own for that took 4.8 us; the counter
-// `done` is cleared by the launch before.)
-constexpr int kJoinTokens = 8;
-__global__ __launch_bounds__(256) void join_losses_kernel(
+// Every token's lse and loss from its partial maxima and sums: 32 tokens a block, 32
+// threads each, and the block's sum of losses and tokens that count into sums.  With
+// `done`, the counter that the launch before cleared, the block that is last adds up
+// all of them: a launch less, but every block publishes its sums past its XCD's L2
+// (4096 tokens in 512 blocks: 15 us against 4), so for few blocks only.
+constexpr int kJoinTokens = 32, kJoinThreads = 32 * kJoinTokens, kJoinLast = 32;
+
+// The losses' sum or mean, and the tokens that count, from n blocks' sums, in one
+// order.
+template <typename Load>
+TCFP_DEV void add_up(int n, int mean, Load load, float* total, float* count) {
+  __shared__ double2 d[256];
+  const int t = threadIdx.x;
+  if (t < 256) {
+    double a = 0.0, b = 0.0;
+    for (int i = t; i < n; i += 256) a += load(2 * i), b += load(2 * i + 1);
+    d[t] = make_double2(a, b);
+  }
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (t < o) d[t].x += d[t + o].x, d[t].y += d[t + o].y;
+    __syncthreads();
+  }
+  if (t == 0) {
+    *total = float(mean ? d[0].x / d[0].y : d[0].x);
+    *count = float(d[0].y);
+  }
+}
+__global__ __launch_bounds__(256) void total_loss_kernel(const double* __restrict__ sums, int n,
+                                                         int mean, float* total, float* count) {
+  add_up(n, mean, [&](int i) { return sums[i]; }, total, count);
+}
+
+__global__ __launch_bounds__(kJoinThreads) void join_losses_kernel(
     const float2* __restrict__ part, int parts, const float* __restrict__ picked,
     const int64_t* __restrict__ targets, int64_t ignore, int64_t classes, int tokens,
-    float* __restrict__ losses, float* __restrict__ lse, double* __restrict__ sums, int* done,
-    int mean, float* __restrict__ total, float* __restrict__ count_out) {
+    float* __restrict__ losses, float* __restrict__ lse, double* sums, int* done, int mean,
+    float* total, float* count_out) {
   __shared__ float2 s[32][kJoinTokens];
-  __shared__ double2 d[256];
   __shared__ bool last;
   const int tl = threadIdx.x % kJoinTokens, slice = threadIdx.x / kJoinTokens;
   const int t = int(blockIdx.x) * kJoinTokens + tl;
@@ -438,15 +488,17 @@ __global__ __launch_bounds__(256) void join_losses_kernel(
     loss = each;
     count = keep ? 1.0 : 0.0;
   }
-  if (!total) return;
-  if (threadIdx.x < 64) {  // (the block's tokens are its first eight threads)
+  if (!sums) return;
+  if (threadIdx.x < 64) {  // (the block's tokens are its first 32 threads)
 #pragma unroll
     for (int o = kJoinTokens / 2; o > 0; o >>= 1) {
       loss += __shfl_xor(loss, o);
       count += __shfl_xor(count, o);
     }
-    if (threadIdx.x == 0) {
-      // (past this XCD's L2, as what reads them may run on another)
+    if (threadIdx.x == 0 && !done) {
+      sums[2 * blockIdx.x] = loss;
+      sums[2 * blockIdx.x + 1] = count;
+    } else if (threadIdx.x == 0) {
       __hip_atomic_store(sums + 2 * blockIdx.x, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __hip_atomic_store(sums + 2 * blockIdx.x + 1, count, __ATOMIC_RELAXED,
                          __HIP_MEMORY_SCOPE_AGENT);
@@ -454,32 +506,74 @@ __global__ __launch_bounds__(256) void join_losses_kernel(
              int(gridDim.x) - 1;
     }
   }
+  if (!done) return;
   __syncthreads();
   if (!last) return;
-  double a = 0.0, b = 0.0;
-  for (int i = threadIdx.x; i < int(gridDim.x); i += 256) {
-    a += __hip_atomic_load(sums + 2 * i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    b += __hip_atomic_load(sums + 2 * i + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  d[threadIdx.x] = make_double2(a, b);
-  __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (int(threadIdx.x) < o) {
-      d[threadIdx.x].x += d[threadIdx.x + o].x;
-      d[threadIdx.x].y += d[threadIdx.x + o].y;
-    }
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    *total = float(mean ? d[0].x / d[0].y : d[0].x);
-    *count_out = float(d[0].y);
-  }
+  add_up(int(gridDim.x), mean,
+         [&](int i) {
+           return __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+         },
+         total, count_out);
 }
 
 // The total of no tokens.
 __global__ void no_tokens_kernel(int mean, float* total, float* count) {
   *total = mean ? NAN : 0.0f;
   *count = 0.0f;
+}
+
+// The exponentials of tokens x classes (fp16, rows ld apart, relative to the maxima of
+// their tiles) turned into g (bf16) in place, eight a thread.
+template <int T>
+__global__ __launch_bounds__(256) void exps_to_grad_kernel(
+    uint16_t* __restrict__ x, int64_t ld, const float2* __restrict__ part,
+    const float* __restrict__ lse, const int64_t* __restrict__ targets, int64_t ignore,
+    int64_t classes, int tokens, const float* __restrict__ count) {
+  const int t = int(blockIdx.y) * 8 + threadIdx.x / 32;
+  if (t >= tokens) return;
+  const int64_t target = targets[t];
+  const bool keep = target != ignore;
+  float c = count ? 1.0f / *count : 1.0f;
+  if (target < 0 || target >= classes) c = NAN;  // (as its loss)
+  const float l = lse[t] * kLog2e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t v0 = (int64_t(blockIdx.x) * 128 + i * 32 + threadIdx.x % 32) * 8;
+    if (v0 >= classes) return;
+    const float f = exp2_fast(part[v0 / T * tokens + t].x - l) * c;
+    uint4* p = reinterpret_cast<uint4*>(x + int64_t(t) * ld + v0);
+    typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+    const v8h e = __builtin_bit_cast(v8h, *p);
+    const int at = target >= v0 && target < v0 + 8 ? int(target - v0) : -1;
+    float g[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      // (what lies behind the classes stays zero)
+      const float z = v0 + j < classes ? float(e[j]) * f - (j == at ? c : 0.0f) : 0.0f;
+      g[j] = keep ? z : 0.0f;
+    }
+    *p = make_uint4(pack2(g[0], g[1]), pack2(g[2], g[3]), pack2(g[4], g[5]), pack2(g[6], g[7]));
+  }
+}
+
+// Two arrays of bf16, eights of them, times *by, in place; nothing is to be done
+// for 1, what the gradient of a loss is most of the time.
+__global__ __launch_bounds__(256) void scale_kernel(uint16_t* a, int64_t a_eights, uint16_t* b,
+                                                    int64_t b_eights, const float* by) {
+  const float f = *by;
+  if (f == 1.0f) return;
+  const int64_t step = int64_t(gridDim.x) * 256;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < a_eights + b_eights; i += step) {
+    uint4* p = i < a_eights ? reinterpret_cast<uint4*>(a) + i
+                            : reinterpret_cast<uint4*>(b) + (i - a_eights);
+    const uint4 x = *p;
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      y[j] = pack2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xFFFF0000u) * f);
+    *p = make_uint4(y[0], y[1], y[2], y[3]);
+  }
 }
 
 // out = the sum of `splits` fp32 [n, m] arrays in bf16, in order; eight columns a
@@ -506,6 +600,8 @@ constexpr int kCus = 256;
 // g of a run of classes takes at most this much of the workspace, but for runs
 // of 256 classes.
 constexpr int64_t kRunBytes = int64_t(256) << 20;
+// What g of all classes may take where the forward makes the gradients.
+constexpr int64_t kTrainBytes = int64_t(1) << 30;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -581,6 +677,10 @@ int launch_cut(const Cut& c, Product p, hipStream_t st) {
                        : launch<128, 4, TA, TB, EPI>(p, st);
 }
 
+// Elements from a row of g to the next: 256 bytes more than whole tiles, as rows a power
+// of two apart meet the same channels of the memory.
+int64_t row_of(int64_t run) { return run + 128; }
+
 struct Layout {
   int64_t run;      // classes
   Cut dh, dw;
@@ -589,7 +689,7 @@ struct Layout {
 Layout layout_of(int64_t tokens, int64_t vocab, int64_t dim, bool need_h, bool need_w) {
   Layout l{};
   l.run = run_of(tokens, vocab);
-  l.g = align256(size_t(tokens) * size_t(l.run) * 2);
+  l.g = align256(size_t(tokens) * size_t(row_of(l.run)) * 2);
   if (need_h) {
     l.dh = cut_of(tokens, dim, std::min(l.run, vocab), true);
     if (l.dh.splits > 1 || l.run < vocab)
@@ -615,15 +715,148 @@ int check_sizes(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
   return TCFP_OK;
 }
 
+// The workspace of one pass over all classes at once.
+Layout train_layout(int64_t tokens, int64_t vocab, int64_t dim, bool need_h, bool need_w) {
+  Layout l{};
+  l.run = ceil_div(vocab, 256) * 256;
+  l.g = align256(size_t(tokens) * size_t(row_of(l.run)) * 2);
+  if (need_h) {
+    l.dh = cut_of(tokens, dim, vocab, true);
+    if (l.dh.splits > 1) l.sum_h = align256(size_t(l.dh.splits) * size_t(tokens) * size_t(dim) * 4);
+  }
+  if (need_w) {
+    l.dw = cut_of(vocab, dim, tokens, true);
+    if (l.dw.splits > 1) l.sum_w = align256(size_t(l.dw.splits) * size_t(vocab) * size_t(dim) * 4);
+  }
+  return l;
+}
+
+struct Head {
+  const void* hidden;
+  int64_t ldh;
+  const void* weight;
+  int64_t ldw;
+  const int64_t* targets;
+  int64_t ignore, tokens, vocab, dim;
+};
+// z of the classes [v0, v0 + classes).
+Product head_product(const Head& h, int64_t v0, int64_t classes) {
+  Product p{};
+  p.a = static_cast<const uint16_t*>(h.weight) + v0 * h.ldw;
+  p.b = static_cast<const uint16_t*>(h.hidden);
+  p.lda = h.ldw;
+  p.ldb = h.ldh;
+  p.m = int(classes);
+  p.n = int(h.tokens);
+  p.k = int(h.dim);
+  p.targets = h.targets;
+  p.ignore = h.ignore;
+  p.first = v0;
+  p.classes = h.vocab;
+  return p;
+}
+
+// Workspace of losses_of(): parts, the targets' logits, sums of blocks, a counter.
+size_t parts_bytes(int64_t tokens, int64_t vocab, int64_t dim) {
+  const int64_t parts = ceil_div(vocab, logits_cut(tokens, vocab, dim).tile);
+  return align256(size_t(parts) * size_t(tokens) * 8) + align256(size_t(tokens) * 4) +
+         align256(size_t(ceil_div(tokens, kJoinTokens)) * 16) + 256;
+}
+// Losses, and with exps (rows ld apart) what exps_to_grad_kernel takes.
+int losses_of(const Head& h, float* losses, float* lse, int mean, float* total, float* count,
+              uint8_t* ws, uint16_t* exps, int64_t ld, hipStream_t st) {
+  const Cut cut = logits_cut(h.tokens, h.vocab, h.dim);
+  const int64_t parts = ceil_div(h.vocab, cut.tile);
+  const unsigned blocks = unsigned(ceil_div(h.tokens, kJoinTokens));
+  Product p = head_product(h, 0, h.vocab);
+  p.out = exps;
+  p.ldo = ld;
+  p.part = reinterpret_cast<float2*>(ws);
+  ws += align256(size_t(parts) * size_t(h.tokens) * 8);
+  p.picked = reinterpret_cast<float*>(ws);
+  ws += align256(size_t(h.tokens) * 4);
+  double* sums = total ? reinterpret_cast<double*>(ws) : nullptr;
+  p.done = reinterpret_cast<int*>(ws + align256(size_t(blocks) * 16));
+  const bool last = blocks <= kJoinLast;
+  const int rc = exps ? launch_cut<false, false, kExps>(cut, p, st)
+                      : launch_cut<false, false, kStats>(cut, p, st);
+  if (rc != TCFP_OK) return rc;
+  join_losses_kernel<<<blocks, kJoinThreads, 0, st>>>(
+      p.part, int(parts), p.picked, h.targets, h.ignore, h.vocab, int(h.tokens), losses, lse, sums,
+      last && total ? p.done : nullptr, mean, total, count);
+  if (total && !last)
+    total_loss_kernel<<<1, 256, 0, st>>>(sums, int(blocks), mean, total, count);
+  return launch_status();
+}
+
+int round_sum(const float* part, int splits, int64_t values, void* out, hipStream_t st) {
+  const int64_t eights = values / 8, blocks = ceil_div(eights, 256);
+  if (!grid_x_fits(blocks, 256)) return TCFP_ERR_SHAPE;
+  round_sum_kernel<<<unsigned(blocks), 256, 0, st>>>(part, splits, values, eights,
+                                                     static_cast<uint16_t*>(out));
+  return launch_status();
+}
+
+// What g of the classes [v0, v0 + classes) gives: their rows of dW, and their part of
+// dh (into sum_h where the layout has it: added up over the runs).
+int products_of(const Head& h, const Layout& l, const uint16_t* g, int64_t v0, int64_t classes,
+                void* grad_hidden, void* grad_weight, float* sum_h, float* sum_w,
+                hipStream_t st) {
+  if (grad_hidden) {
+    // dh[t][d] += sum over the classes of g[t][v] W[v][d]
+    Product q{};
+    q.a = static_cast<const uint16_t*>(h.weight) + v0 * h.ldw;
+    q.b = g;
+    q.lda = h.ldw;
+    q.ldb = row_of(l.run);
+    q.m = int(h.dim);
+    q.n = int(h.tokens);
+    q.k = int(classes);
+    q.ldo = h.dim;
+    int done;
+    if (l.sum_h) {
+      q.out = sum_h;
+      q.split_stride = h.tokens * h.dim;
+      q.add = v0 > 0;
+      // (a last, shorter run may leave splits without classes: nothing to add)
+      Cut cut = l.dh;
+      if (v0 > 0) cut.splits = int(std::min<int64_t>(cut.splits, ceil_div(classes, cut.k_run)));
+      done = launch_cut<true, false, kFp32>(cut, q, st);
+    } else {
+      q.out = grad_hidden;
+      done = launch_cut<true, false, kBf16>(l.dh, q, st);
+    }
+    if (done != TCFP_OK) return done;
+  }
+  if (!grad_weight) return TCFP_OK;
+  // dW[v][d] = sum over tokens of g[t][v] h[t][d]
+  Product q{};
+  q.a = static_cast<const uint16_t*>(h.hidden);
+  q.b = g;
+  q.lda = h.ldh;
+  q.ldb = row_of(l.run);
+  q.m = int(h.dim);
+  q.n = int(classes);
+  q.k = int(h.tokens);
+  q.ldo = h.dim;
+  uint16_t* out = static_cast<uint16_t*>(grad_weight) + v0 * h.dim;
+  if (l.dw.splits == 1) {
+    q.out = out;
+    return launch_cut<true, true, kBf16>(l.dw, q, st);
+  }
+  q.out = sum_w;
+  q.split_stride = classes * h.dim;
+  const int done = launch_cut<true, true, kFp32>(l.dw, q, st);
+  return done != TCFP_OK ? done : round_sum(sum_w, l.dw.splits, classes * h.dim, out, st);
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t tcfp_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim) {
   if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
-  const int64_t parts = ceil_div(vocab, logits_cut(tokens, vocab, dim).tile);
-  return align256(size_t(parts) * size_t(tokens) * 8) + align256(size_t(tokens) * 4) +
-         align256(size_t(ceil_div(tokens, kJoinTokens)) * 16) + 256;
+  return parts_bytes(tokens, vocab, dim);
 }
 
 int tcfp_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
@@ -634,40 +867,74 @@ int tcfp_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weigh
   const int rc = check_sizes(hidden, ldh, weight, ldw, tokens, vocab, dim);
   if (rc != TCFP_OK) return rc;
   if (!total != !count) return TCFP_ERR_SHAPE;
-  if (!workspace || workspace_bytes < tcfp_linear_cross_entropy_workspace_bytes(tokens, vocab, dim) ||
-      !aligned16(workspace)) {
-    if (tokens > 0) return TCFP_ERR_WORKSPACE;
-  }
   const auto st = static_cast<hipStream_t>(stream);
   if (tokens == 0) {
     if (total) no_tokens_kernel<<<1, 1, 0, st>>>(mean, total, count);
     return launch_status();
   }
-  const Cut cut = logits_cut(tokens, vocab, dim);
-  const int64_t parts = ceil_div(vocab, cut.tile);
+  if (!workspace || workspace_bytes < parts_bytes(tokens, vocab, dim) || !aligned16(workspace))
+    return TCFP_ERR_WORKSPACE;
+  return losses_of({hidden, ldh, weight, ldw, targets, ignore, tokens, vocab, dim}, losses, lse,
+                   mean, total, count, static_cast<uint8_t*>(workspace), nullptr, 0, st);
+}
+
+size_t tcfp_linear_cross_entropy_train_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim,
+                                                       int need_hidden, int need_weight) {
+  // (the second and third: the grid of the pass over g, a descriptor's reach)
+  if (tokens <= 0 || vocab <= 0 || dim <= 0 || tokens > 65535 * 8 || vocab > 1 << 20) return 0;
+  const Layout l = train_layout(tokens, vocab, dim, need_hidden != 0, need_weight != 0);
+  if (int64_t(l.g) > kTrainBytes) return 0;
+  return l.g + l.sum_h + l.sum_w + parts_bytes(tokens, vocab, dim);
+}
+
+int tcfp_linear_cross_entropy_train(const void* hidden, int64_t ldh, const void* weight,
+                                    int64_t ldw, const int64_t* targets, int64_t ignore,
+                                    int64_t tokens, int64_t vocab, int64_t dim, float* losses,
+                                    float* lse, int mean, float* total, float* count,
+                                    void* grad_hidden, void* grad_weight, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  const int rc = check_sizes(hidden, ldh, weight, ldw, tokens, vocab, dim);
+  if (rc != TCFP_OK) return rc;
+  if (!aligned16(grad_hidden) || !aligned16(grad_weight)) return TCFP_ERR_ALIGN;
+  const bool need_h = grad_hidden != nullptr, need_w = grad_weight != nullptr;
+  const size_t need =
+      tcfp_linear_cross_entropy_train_workspace_bytes(tokens, vocab, dim, need_h, need_w);
+  if (need == 0 || !total || !count) return TCFP_ERR_SHAPE;
+  if (!workspace || workspace_bytes < need || !aligned16(workspace)) return TCFP_ERR_WORKSPACE;
+  const auto st = static_cast<hipStream_t>(stream);
+  const Head head{hidden, ldh, weight, ldw, targets, ignore, tokens, vocab, dim};
+  const Layout l = train_layout(tokens, vocab, dim, need_h, need_w);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  Product p{};
-  p.a = static_cast<const uint16_t*>(weight);
-  p.b = static_cast<const uint16_t*>(hidden);
-  p.lda = ldw;
-  p.ldb = ldh;
-  p.m = int(vocab);
-  p.n = int(tokens);
-  p.k = int(dim);
-  p.targets = targets;
-  p.classes = vocab;
-  p.part = reinterpret_cast<float2*>(ws);
-  ws += align256(size_t(parts) * size_t(tokens) * 8);
-  p.picked = reinterpret_cast<float*>(ws);
-  ws += align256(size_t(tokens) * 4);
-  const unsigned blocks = unsigned(ceil_div(tokens, kJoinTokens));
-  double* sums = reinterpret_cast<double*>(ws);
-  p.done = reinterpret_cast<int*>(ws + align256(size_t(blocks) * 16));
-  const int rc_product = launch_cut<false, false, kStats>(cut, p, st);
-  if (rc_product != TCFP_OK) return rc_product;
-  join_losses_kernel<<<blocks, 256, 0, st>>>(p.part, int(parts), p.picked, targets, ignore, vocab,
-                                             int(tokens), losses, lse, sums, p.done, mean, total,
-                                             count);
+  uint16_t* g = reinterpret_cast<uint16_t*>(ws);
+  uint8_t* parts = ws + l.g + l.sum_h + l.sum_w;
+  int done = losses_of(head, losses, lse, mean, total, count, parts, g, row_of(l.run), st);
+  if (done != TCFP_OK) return done;
+  const dim3 grid(unsigned(ceil_div(vocab, 1024)), unsigned(ceil_div(tokens, 8)));
+  const auto* part = reinterpret_cast<const float2*>(parts);
+  const float* each = mean ? count : nullptr;
+  if (logits_cut(tokens, vocab, dim).tile == 256)
+    exps_to_grad_kernel<256><<<grid, 256, 0, st>>>(g, row_of(l.run), part, lse, targets, ignore, vocab,
+                                                   int(tokens), each);
+  else
+    exps_to_grad_kernel<128><<<grid, 256, 0, st>>>(g, row_of(l.run), part, lse, targets, ignore, vocab,
+                                                   int(tokens), each);
+  if (launch_status() != TCFP_OK) return TCFP_ERR_HIP;
+  done = products_of(head, l, g, 0, vocab, grad_hidden, grad_weight,
+                     reinterpret_cast<float*>(ws + l.g),
+                     reinterpret_cast<float*>(ws + l.g + l.sum_h), st);
+  if (done != TCFP_OK || !l.sum_h) return done;
+  return round_sum(reinterpret_cast<float*>(ws + l.g), l.dh.splits, tokens * dim, grad_hidden, st);
+}
+
+int tcfp_scale_bf16(void* a, int64_t a_values, void* b, int64_t b_values, const float* by,
+                    void* stream) {
+  if (a_values < 0 || b_values < 0 || a_values % 8 || b_values % 8) return TCFP_ERR_SHAPE;
+  if (!aligned16(a) || !aligned16(b)) return TCFP_ERR_ALIGN;
+  const int64_t eights = (a_values + b_values) / 8;
+  if (eights == 0) return TCFP_OK;
+  scale_kernel<<<unsigned(std::min<int64_t>(ceil_div(eights, 256), 8 * kCus)), 256, 0,
+                 static_cast<hipStream_t>(stream)>>>(static_cast<uint16_t*>(a), a_values / 8,
+                                                     static_cast<uint16_t*>(b), b_values / 8, by);
   return launch_status();
 }
 
@@ -708,88 +975,22 @@ int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const vo
   uint16_t* g = reinterpret_cast<uint16_t*>(ws);
   float* sum_h = reinterpret_cast<float*>(ws + l.g);
   float* sum_w = reinterpret_cast<float*>(ws + l.g + l.sum_h);
-  const auto* h = static_cast<const uint16_t*>(hidden);
-  const auto* w = static_cast<const uint16_t*>(weight);
-  auto round_sum = [&](const float* part, int splits, int64_t values, uint16_t* out) {
-    const int64_t eights = values / 8, blocks = ceil_div(eights, 256);
-    if (!grid_x_fits(blocks, 256)) return int(TCFP_ERR_SHAPE);
-    round_sum_kernel<<<unsigned(blocks), 256, 0, st>>>(part, splits, values, eights, out);
-    return launch_status();
-  };
+  const Head head{hidden, ldh, weight, ldw, targets, ignore, tokens, vocab, dim};
   for (int64_t v0 = 0; v0 < vocab; v0 += l.run) {
     const int64_t classes = std::min(l.run, vocab - v0);
-    Product p{};
-    p.a = w + v0 * ldw;
-    p.b = h;
-    p.lda = ldw;
-    p.ldb = ldh;
-    p.m = int(classes);
-    p.n = int(tokens);
-    p.k = int(dim);
+    Product p = head_product(head, v0, classes);
     p.out = g;
-    p.ldo = l.run;
-    p.targets = targets;
-    p.ignore = ignore;
-    p.first = v0;
-    p.classes = vocab;
+    p.ldo = row_of(l.run);
     p.lse = lse;
     p.grad = grad;
     p.grad_step = int(grad_step);
     p.count = count;
     int done = launch_cut<false, false, kGrad>(logits_cut(tokens, classes, dim), p, st);
+    if (done == TCFP_OK)
+      done = products_of(head, l, g, v0, classes, grad_hidden, grad_weight, sum_h, sum_w, st);
     if (done != TCFP_OK) return done;
-    if (need_h) {
-      // dh[t][d] += sum over the run's classes of g[t][v] W[v][d]
-      Product q{};
-      q.a = w + v0 * ldw;
-      q.b = g;
-      q.lda = ldw;
-      q.ldb = l.run;
-      q.m = int(dim);
-      q.n = int(tokens);
-      q.k = int(classes);
-      if (l.sum_h) {
-        q.out = sum_h;
-        q.ldo = dim;
-        q.split_stride = tokens * dim;
-        q.add = v0 > 0;
-        // (a last, shorter run may leave splits without classes: nothing to add)
-        Cut cut = l.dh;
-        if (v0 > 0) cut.splits = int(std::min<int64_t>(cut.splits, ceil_div(classes, cut.k_run)));
-        done = launch_cut<true, false, kFp32>(cut, q, st);
-      } else {
-        q.out = grad_hidden;
-        q.ldo = dim;
-        done = launch_cut<true, false, kBf16>(l.dh, q, st);
-      }
-      if (done != TCFP_OK) return done;
-    }
-    if (need_w) {
-      // dW[v][d] = sum over tokens of g[t][v] h[t][d]
-      Product q{};
-      q.a = h;
-      q.b = g;
-      q.lda = ldh;
-      q.ldb = l.run;
-      q.m = int(dim);
-      q.n = int(classes);
-      q.k = int(tokens);
-      uint16_t* out = static_cast<uint16_t*>(grad_weight) + v0 * dim;
-      q.ldo = dim;
-      if (l.dw.splits > 1) {
-        q.out = sum_w;
-        q.split_stride = classes * dim;
-        done = launch_cut<true, true, kFp32>(l.dw, q, st);
-        if (done == TCFP_OK) done = round_sum(sum_w, l.dw.splits, classes * dim, out);
-      } else {
-        q.out = out;
-        done = launch_cut<true, true, kBf16>(l.dw, q, st);
-      }
-      if (done != TCFP_OK) return done;
-    }
   }
-  if (need_h && l.sum_h)
-    return round_sum(sum_h, l.dh.splits, tokens * dim, static_cast<uint16_t*>(grad_hidden));
+  if (need_h && l.sum_h) return round_sum(sum_h, l.dh.splits, tokens * dim, grad_hidden, st);
   return TCFP_OK;
 }
 

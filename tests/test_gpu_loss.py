@@ -6,7 +6,10 @@ matrix cores cut bits off): a logit within dz = D 2^-23 sum |h w|.  A softmax
 probability is then off by 2 dz + 2^-20 of itself (both exponentials, their
 arguments and the sum of V terms, which is within V 2^-24 of itself), a loss by
 twice the largest dz and 2^-22 of the sizes it is a difference of.  The gradient of
-a logit is rounded to bf16, 2^-8 of itself, and so is each result."""
+a logit is rounded to bf16, 2^-8 of itself, and so is each result.  Where the forward
+makes the gradients (a sum or mean) the exponentials are rounded to fp16 in between,
+2^-11 of themselves and 2^-25 at least (of the largest probability of 256 classes, 1 at
+most), and the results are rounded once more when the loss's gradient is not 1."""
 import math
 
 import pytest
@@ -33,7 +36,7 @@ def inputs(dev, tokens, d, vocab, seed=0, ignored=0.0, spread=2.0):
 class Exact:
     """Losses, gradients and how far each may be off, in 64 bits on the CPU."""
 
-    def __init__(self, h, w, t, grad=None, ignore=-100):
+    def __init__(self, h, w, t, grad=None, ignore=-100, made=True):
         h, w, t = h.detach().double().cpu(), w.detach().double().cpu(), t.cpu()
         d, v = h.shape[1], w.shape[0]
         z = h @ w.t()
@@ -53,14 +56,16 @@ class Exact:
         g = p.clone()
         g.scatter_add_(1, at, torch.full_like(picked, -1.0)[:, None])
         g *= grad[:, None]
-        eps = dz + self.lse_tol[:, None] + 2.0**-20
-        g_tol = HALF * g.abs() + (1 + HALF) * (eps * p + 2.0**-23) * grad.abs()[:, None]
+        eps = dz + self.lse_tol[:, None] + 2.0**-20 + (2.0**-11 if made else 0.0)
+        g_tol = HALF * g.abs() + (1 + HALF) * (
+            eps * p + 2.0**-23 + (2.0**-25 if made else 0.0)) * grad.abs()[:, None]
         # (2^-23: p - 1 at the target, and the gradient's own rounding)
         self.dh = g @ w
         self.dw = g.t() @ h
         n = h.shape[0]
-        self.dh_tol = HALF * self.dh.abs() + (1 + HALF) * (g_tol + v * 2.0**-23 * g.abs()) @ w.abs()
-        self.dw_tol = HALF * self.dw.abs() + (1 + HALF) * (g_tol + n * 2.0**-23 * g.abs()).t() @ h.abs()
+        out = 2 * HALF + HALF * HALF if made else HALF
+        self.dh_tol = out * self.dh.abs() + (1 + out) * (g_tol + v * 2.0**-23 * g.abs()) @ w.abs()
+        self.dw_tol = out * self.dw.abs() + (1 + out) * (g_tol + n * 2.0**-23 * g.abs()).t() @ h.abs()
 
 
 def within(got, want, tol, what):
@@ -108,23 +113,26 @@ def test_gradients(dev, tokens, d, vocab, reduction):
     each = up.double().cpu().expand(tokens)
     if reduction == "mean":
         each = each / int((t != -100).sum())
-    e = Exact(h, w, t, each)
+    e = Exact(h, w, t, each, made=reduction != "none")
     assert dh.dtype == dw.dtype == BF16
     within(dh, e.dh, e.dh_tol, "dh")
     within(dw, e.dw, e.dw_tol, "dw")
     assert not dh[(t == -100)].any()
 
 
-def test_runs_of_classes_add_up(dev):
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_runs_of_classes_add_up(dev, reduction):
     """More tokens x classes than a run's workspace: 70000 x 4100 x 2 bytes in three
-    runs, held against single rows and columns in 64 bits."""
+    runs where every token's loss has a gradient, held against 64 bits; the sum's
+    gradients come with the forward."""
     tokens, d, vocab = 70000, 16, 4100
     h, w, t = inputs(dev, tokens, d, vocab, seed=3)
     nb = L._hip.lib().tcfp_linear_cross_entropy_backward_workspace_bytes(tokens, vocab, d, 1, 1)
     assert nb < 2 * tokens * vocab  # g as a whole would take more
     h.requires_grad_()
     w.requires_grad_()
-    dh, dw = torch.autograd.grad(L.linear_cross_entropy(h, w, t, reduction="sum"), (h, w))
+    out = L.linear_cross_entropy(h, w, t, reduction=reduction)
+    dh, dw = torch.autograd.grad(out, (h, w), torch.ones_like(out))
     hd, wd = h.detach().double(), w.detach().double()
     z = torch.mm(hd, wd.t().contiguous())
     lse = torch.logsumexp(z, 1)
@@ -132,6 +140,8 @@ def test_runs_of_classes_add_up(dev):
     p[torch.arange(tokens, device=dev), t] -= 1.0
     # z within D 2^-23 sum |h w| <= 2^-14 here, p with it
     eps = d * 2.0**-23 * float((hd.abs().amax(0) * wd.abs().amax(0)).sum()) * 3 + 2.0**-20 + vocab * 2.0**-24
+    if reduction == "sum":
+        eps += 2.0**-11
     tol = (HALF * 1.01 + eps) * p.abs() + eps
     want = torch.mm(p, wd)
     room = HALF * want.abs() + torch.mm(tol, wd.abs()) + vocab * 2.0**-23 * torch.mm(p.abs(), wd.abs())
@@ -142,18 +152,65 @@ def test_runs_of_classes_add_up(dev):
     assert ((dw.double() - want).abs() <= room).all()
 
 
+def test_the_largest_workspace(dev):
+    """1 GiB of exponentials and no more: beyond, and for more classes than a
+    descriptor reaches, the logits are formed twice."""
+    size = L._hip.lib().tcfp_linear_cross_entropy_train_workspace_bytes
+    assert size(16320, 32768, 64, 1, 1) < 1 << 31 and size(16385, 32768, 64, 1, 1) == 0
+    assert size(4, 1 << 20, 64, 1, 1) > 0 and size(4, (1 << 20) + 1, 64, 1, 1) == 0
+    assert size(16320, 32768, 64, 1, 1) > 0 and size(524281, 8, 64, 1, 1) == 0
+    assert size(524280, 256, 64, 1, 1) > 0
+    h, w, t = inputs(dev, 3, 8, (1 << 20) + 3, seed=12, spread=8.0)
+    t[1] = (1 << 20) + 2
+    h.requires_grad_()
+    w.requires_grad_()
+    dh, dw = torch.autograd.grad(L.linear_cross_entropy(h, w, t, reduction="sum"), (h, w))
+    e = Exact(h, w, t, torch.ones(3), made=False)
+    within(dh, e.dh, e.dh_tol, "dh")
+    within(dw, e.dw, e.dw_tol, "dw")
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_second_backward(dev, reduction):
+    """Of a kept graph: the first one is handed what the forward made, the second forms
+    the logits again."""
+    h, w, t = inputs(dev, 90, 64, 700, seed=13, ignored=0.2)
+    h.requires_grad_()
+    w.requires_grad_()
+    out = L.linear_cross_entropy(h, w, t, reduction=reduction)
+    up = torch.full_like(out, 0.3)
+    e = Exact(h, w, t, (up if reduction == "none" else up / int((t != -100).sum())).expand(90))
+    for _ in range(3):
+        dh, dw = torch.autograd.grad(out, (h, w), up, retain_graph=True)
+        within(dh, e.dh, e.dh_tol, "dh")
+        within(dw, e.dw, e.dw_tol, "dw")
+
+
 @pytest.mark.parametrize("which", ["hidden", "weight"])
 def test_one_gradient_alone(dev, which):
     h, w, t = inputs(dev, 70, 64, 300, seed=4)
     h.requires_grad_(which == "hidden")
     w.requires_grad_(which == "weight")
-    (h if which == "hidden" else w).retain_grad()
     L.linear_cross_entropy(h, w, t).backward()
-    both = L.linear_cross_entropy_forward(h, w, t)
-    count = torch.tensor(70.0, device=dev)
-    dh, dw = L.linear_cross_entropy_backward(torch.tensor(1.0, device=dev), h.detach(), w.detach(), t,
-                                             both[1], count=count)
-    assert torch.equal(h.grad if which == "hidden" else w.grad, dh if which == "hidden" else dw)
+    a, b = h.detach().clone().requires_grad_(), w.detach().clone().requires_grad_()
+    both = torch.autograd.grad(L.linear_cross_entropy(a, b, t), (a, b))
+    if which == "hidden":
+        assert torch.equal(h.grad, both[0]) and w.grad is None
+    else:
+        assert torch.equal(w.grad, both[1]) and h.grad is None
+    # the same without autograd
+    lse = L.linear_cross_entropy_forward(h, w, t)[1]
+    e = Exact(h, w, t, torch.full((70,), 1 / 70), made=False)
+    dh, dw = L.linear_cross_entropy_backward(
+        torch.tensor(1.0, device=dev), h.detach(), w.detach(), t, lse,
+        count=torch.tensor(70.0, device=dev), need_hidden_grad=which == "hidden",
+        need_weight_grad=which == "weight")
+    if which == "hidden":
+        within(dh, e.dh, e.dh_tol, "dh")
+        assert dw is None
+    else:
+        within(dw, e.dw, e.dw_tol, "dw")
+        assert dh is None
 
 
 def test_gradient_against_differences(dev):
