@@ -35,11 +35,14 @@ namespace {
 // dh = g W and dW = g^T h, without transposed copies.
 //
 // A workgroup owns T x T of C over a run of k (a split).  T = 256: eight waves, 2
-// along m and 4 along n, 128 x 64 each; two stages of 64 k in LDS (128 KiB), one
-// workgroup a CU.  T = 128: four waves of 64 x 64; four stages (one workgroup a CU:
-// what streams one operand from HBM, or has few tiles) or two (two workgroups, of
-// which one multiplies while the other waits or stores).  cost() says which is taken.
-// A stage's copies are issued as soon as every wave has read its last operands
+// along m and 4 along n, 128 x 64 each; two stages of 64 k in LDS (128 KiB); one
+// workgroup a CU, which takes tile after tile: the next one's first stages are on
+// their way while a result is written, and its stores drain while the next one is
+// multiplied (8192 x 32768 over 4096 with the exponentials, a workgroup a tile:
+// 2066 us, so: 1886).  T = 128: four waves of 64 x 64; four stages (one workgroup
+// a CU: what streams one operand from HBM, or has few tiles) or two (two workgroups,
+// of which one multiplies while the other waits or stores).  cost() says which is
+// taken.  A stage's copies are issued as soon as every wave has read its last operands
 // of the stage whose place they take, in the middle of that stage's products.
 constexpr int kStageK = 64;
 
@@ -86,102 +89,110 @@ struct Product {
 // kStats: parts of the losses; kExps: those and the exponentials; kGrad: g.
 enum Epilogue { kBf16, kFp32, kStats, kExps, kGrad };
 
-// Offsets of one operand's copies into LDS: 4 instructions a wave and stage.
+// One operand's copies into LDS: 4 instructions a wave and stage.
 // Rows along k: instruction q brings the rows 8 q ... of 128 bytes, whose eight
 // chunks of 16 bytes are permuted by (row / 2) % 8; rows of one k: instruction q
 // brings 1024 / (2 T) rows, whose chunks are permuted by 4 (row % 4), so that the
-// reads below meet every bank once.
-template <int T, bool ROWS_OF_K>
+// reads meet every bank once.
+template <int T, bool OF_K>
 struct Copies {
-  uint32_t off0, off1, step;
-  bool past0, past1;  // this lane's chunk lies outside
-  int chunk0, chunk1;
-  TCFP_DEV void init(int wave, int lane, int64_t ld, int at, int extent) {
-    if constexpr (!ROWS_OF_K) {
-      const int row = 32 * wave + (lane >> 3);
-      chunk0 = (lane & 7) ^ ((lane >> 4) & 7);
-      chunk1 = (lane & 7) ^ ((4 + (lane >> 4)) & 7);
-      off0 = uint32_t(row * ld * 2) + chunk0 * 16;
-      off1 = uint32_t(row * ld * 2) + chunk1 * 16;
-      step = uint32_t(8 * ld * 2);
-      past0 = past1 = false;
+  uint32_t off0, off1, step;  // of even and odd instructions
+  int at0, at1;               // their chunks' first k (column)
+  TCFP_DEV void init(int wave, int lane, int64_t ld) {
+    constexpr int CH = OF_K ? T / 8 : 8, R = 64 / CH;  // chunks of a row, rows an instruction
+    const int row = 4 * R * wave + lane / CH;
+    int c0, c1;
+    if constexpr (OF_K) {
+      c0 = (lane % CH) ^ (4 * ((lane / CH) & 3));
+      c1 = (lane % CH) ^ (4 * ((R + lane / CH) & 3));
     } else {
-      constexpr int CH = T / 8, R = 64 / CH;  // chunks of a row, rows an instruction
-      const int row = 4 * R * wave + lane / CH;
-      // (row % 4 of instruction i: for R == 2 it depends on i's parity)
-      chunk0 = (lane % CH) ^ (4 * ((lane / CH) & 3));
-      chunk1 = (lane % CH) ^ (4 * ((R + lane / CH) & 3));
-      off0 = uint32_t(row * ld * 2) + chunk0 * 16;
-      off1 = uint32_t(row * ld * 2) + chunk1 * 16;
-      step = uint32_t(R * ld * 2);
-      past0 = at + chunk0 * 8 >= extent;
-      past1 = at + chunk1 * 8 >= extent;
+      c0 = (lane & 7) ^ ((lane >> 4) & 7);
+      c1 = (lane & 7) ^ ((4 + (lane >> 4)) & 7);
     }
+    off0 = uint32_t(row * ld * 2) + c0 * 16;
+    off1 = uint32_t(row * ld * 2) + c1 * 16;
+    step = uint32_t(R * ld * 2);
+    at0 = c0 * 8;
+    at1 = c1 * 8;
+  }
+  // The stage at k of rows (columns) [at, extent), k up to k1, into LDS at `to`; nothing
+  // but zeros from k1 on.  (Whole chunks of 16 bytes: behind an odd number of classes g
+  // has zeros.)
+  TCFP_DEV void issue(const uint16_t* p, int64_t ld, int at, int extent, int k, int k1,
+                      uint32_t to) const {
+    const uint16_t* base;
+    int64_t span;
+    int left;  // of what a row holds
+    if constexpr (OF_K) {
+      base = p + int64_t(k) * ld + at;
+      left = extent - at;
+      span = (int64_t(min(k1 - k, kStageK)) - 1) * ld + ((left + 7) & ~7);
+    } else {
+      base = p + int64_t(at) * ld + k;
+      left = k1 - k;
+      span = (int64_t(min(extent - at, T)) - 1) * ld + ((left + 7) & ~7);
+    }
+    const v4i rsrc = make_rsrc(base, k < k1 ? uint32_t(span * 2) : 0u);
+    const uint32_t o0 = at0 >= left ? kOutOfRange : off0, o1 = at1 >= left ? kOutOfRange : off1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) copy16(rsrc, ((i & 1) ? o1 : o0) + i * step, to + i * 1024);
   }
 };
 
+// What of C a workgroup computes.
+struct Unit {
+  int m0, n0, k0, k1, split, stages;
+};
+// Each XCD (workgroup b is on XCD b % 8) takes a run of the splits' tiles, in groups of
+// four tile rows along n, so that its L2 holds both operands' panels.
+template <int T>
+TCFP_DEV Unit unit_at(const Product& g, int l) {
+  Unit u;
+  const int tiles = g.tiles_m * g.tiles_n, units = tiles * g.splits;
+  l = (l & 7) * (units >> 3) + min(l & 7, units & 7) + (l >> 3);
+  u.split = l / tiles;
+  l -= u.split * tiles;
+  const int per = 4 * g.tiles_m, first = l / per * 4, rows = min(g.tiles_n - first, 4);
+  u.n0 = (first + l % per % rows) * T;
+  u.m0 = l % per / rows * T;
+  u.k0 = u.split * g.k_run;
+  u.k1 = min(g.k, u.k0 + g.k_run);
+  // (two at least, of which a second one may be zeros)
+  u.stages = max((u.k1 - u.k0 + kStageK - 1) / kStageK, T == 256 ? 2 : 0);
+  return u;
+}
+
+// Waits for the wave's LDS operations, then for the workgroup; copies and stores go on.
+TCFP_DEV void sync_lds() { wait_and_sync<63>(); }
+
 template <int T, int ST, bool TA, bool TB, int EPI>
-__global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) void product_kernel(Product g) {
+__global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) void product_kernel(
+    Product g) {
   using S = Shape<T, ST>;
-  constexpr bool STATS = EPI == kStats || EPI == kExps;
-  __shared__ __align__(16) uint8_t lds[S::STAGES * S::STAGE];
-  __shared__ float tops[STATS ? 2 : 1][T], exps[STATS ? 2 : 1][T];  // [wave along m][n]
+  constexpr bool STATS = EPI == kStats || EPI == kExps, MANY = T == 256;
+  // Of each wave 4 KiB beside the stages (or, where the workgroup has one tile, in their
+  // place when they are done with): what the epilogue takes, and its result on its way
+  // to rows.
+  constexpr int PRIVATE = 4096;
+  __shared__ __align__(16) uint8_t lds[S::STAGES * S::STAGE + (MANY ? S::WAVES * PRIVATE : 0)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int wm = wave % S::WAVES_M, wn = wave / S::WAVES_M;
-
-  // Each XCD (workgroup b is on XCD b % 8) takes a run of the splits' tiles, in
-  // groups of four tile rows along n, so that its L2 holds both operands' panels.
-  int m0, n0, split;
-  {
-    const int tiles = g.tiles_m * g.tiles_n, units = tiles * g.splits;
-    int l = int(blockIdx.x);
-    l = (l & 7) * (units >> 3) + min(l & 7, units & 7) + (l >> 3);
-    split = l / tiles;
-    l -= split * tiles;
-    const int per = 4 * g.tiles_m, first = l / per * 4, rows = min(g.tiles_n - first, 4);
-    n0 = (first + l % per % rows) * T;
-    m0 = l % per / rows * T;
-  }
-  const int k0 = split * g.k_run, k1 = min(g.k, k0 + g.k_run);
-  const int stages = (k1 - k0 + kStageK - 1) / kStageK;
+  uint8_t* const spare = lds + (MANY ? S::STAGES * S::STAGE : 0);
+  uint8_t* const own = spare + wave * PRIVATE;
+  if (STATS && blockIdx.x == 0 && threadIdx.x == 0) *g.done = 0;
 
   Copies<T, TA> ca;
   Copies<T, TB> cb;
-  ca.init(wave, lane, g.lda, m0, g.m);
-  cb.init(wave, lane, g.ldb, n0, g.n);
+  ca.init(wave, lane, g.lda);
+  cb.init(wave, lane, g.ldb);
   const uint32_t lds0 = lds_offset(lds);
-  // the copies of one operand's stage at k into LDS at `to` (whole chunks of 16
-  // bytes: behind an odd number of classes g has zeros)
-  auto copy_operand = [&](auto& c, auto of_k, const uint16_t* p, int64_t ld, int at, int extent, int k,
-                          uint32_t to) {
-    constexpr bool OF_K = decltype(of_k)::value;
-    const bool live = k < k1;
-    const uint16_t* base;
-    int64_t span;
-    if constexpr (OF_K) {
-      base = p + int64_t(k) * ld + at;
-      span = (int64_t(min(k1 - k, kStageK)) - 1) * ld + ((extent - at + 7) & ~7);
-    } else {
-      base = p + int64_t(at) * ld + k;
-      span = (int64_t(min(extent - at, T)) - 1) * ld + ((k1 - k + 7) & ~7);
-    }
-    const v4i rsrc = make_rsrc(base, live ? uint32_t(span * 2) : 0u);
-    uint32_t o0 = c.past0 ? kOutOfRange : c.off0, o1 = c.past1 ? kOutOfRange : c.off1;
-    if constexpr (!OF_K) {
-      // (a run of k ends inside a row)
-      if (k + c.chunk0 * 8 >= k1) o0 = kOutOfRange;
-      if (k + c.chunk1 * 8 >= k1) o1 = kOutOfRange;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) copy16(rsrc, ((i & 1) ? o1 : o0) + i * c.step, to + i * 1024);
-  };
-  auto copy_stage = [&](int t) {
-    const uint32_t to = lds0 + uint32_t(t % S::STAGES) * S::STAGE + uint32_t(wave) * 4096;
-    const int k = k0 + t * kStageK;
-    copy_operand(ca, std::integral_constant<bool, TA>{}, g.a, g.lda, m0, g.m, k, to);
-    copy_operand(cb, std::integral_constant<bool, TB>{}, g.b, g.ldb, n0, g.n, k, to + S::OPERAND);
+  auto copy_stage = [&](const Unit& u, int t, int buf) {
+    const uint32_t to = lds0 + uint32_t(buf) * S::STAGE + uint32_t(wave) * 4096;
+    const int k = u.k0 + t * kStageK;
+    ca.issue(g.a, g.lda, u.m0, g.m, k, u.k1, to);
+    cb.issue(g.b, g.ldb, u.n0, g.n, k, u.k1, to + S::OPERAND);
   };
 
   // operand reads: block x of 32 rows (columns), k step s of 16
@@ -199,8 +210,8 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
   struct Frags {
     v8bf a[2][S::MB], b[2][S::NB];
   };
-  auto read_half = [&](Frags& f, int t, int h) {
-    const uint8_t* st = lds + (t % S::STAGES) * S::STAGE;
+  auto read_half = [&](Frags& f, int buf, int h) {
+    const uint8_t* st = lds + buf * S::STAGE;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
@@ -214,12 +225,14 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
     }
   };
   v16f acc[S::MB][S::NB];
+  auto clear = [&]() {
 #pragma unroll
-  for (int x = 0; x < S::MB; ++x)
+    for (int x = 0; x < S::MB; ++x)
 #pragma unroll
-    for (int y = 0; y < S::NB; ++y)
+      for (int y = 0; y < S::NB; ++y)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
+  };
   auto multiply = [&](const Frags& f, int s) {
 #pragma unroll
     for (int x = 0; x < S::MB; ++x)
@@ -239,178 +252,303 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
       }
   };
 
-  // (copies past the last stage read nothing and keep the count of what is in
-  // flight)
-  constexpr int kAhead = 8 * (S::STAGES - 2);
-#pragma unroll
-  for (int t = 0; t < S::STAGES - 1; ++t) copy_stage(t);
-  wait_and_sync<kAhead>();
-  Frags f0, f1;
-  copy_stage(S::STAGES - 1);
-  read_half(f0, 0, 0);
-  for (int t = 0; t < stages; ++t) {
-    read_half(f1, t, 1);
-    multiply(f0, 0);
-    pin();
-    wait_and_sync<kAhead>();
-    multiply(f0, 1);
-    pin();
-    __builtin_amdgcn_sched_barrier(0);
-    copy_stage(t + S::STAGES);
-    __builtin_amdgcn_sched_barrier(0);
-    read_half(f0, t + 1, 0);
-    multiply(f1, 0);
-    multiply(f1, 1);
-  }
-  // (the copies still in flight read nothing, but write zeros)
-  wait_and_sync<0>();
-
-  // ---- epilogues: acc[x][y][r] is m = m_of(x, r), n = n_of(y) ----------------
+  // ---- what the epilogue takes of the wave's 64 tokens (the loss's products): target,
+  // lse and gradient, brought into the wave's own LDS with the tile's first stages
+  // (loaded in the epilogue, each wait for them would wait for the next tile's copies)
+  constexpr int TAKEN = EPI == kGrad ? 4 : STATS ? 2 : 0;
   const int mw = wm * S::MB * 32, nw = wn * 64;
-  auto m_of = [&](int x, int r) { return mw + 32 * x + 8 * (r >> 2) + 4 * half + (r & 3); };
-  if constexpr (EPI == kFp32) {
-    float* out = static_cast<float*>(g.out) + int64_t(split) * g.split_stride;
-#pragma unroll
-    for (int y = 0; y < S::NB; ++y) {
-      const int n = n0 + nw + 32 * y + col;
-      if (n >= g.n) continue;
-#pragma unroll
-      for (int x = 0; x < S::MB; ++x)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int m = m0 + m_of(x, 4 * q);
-          if (m >= g.m) continue;
-          float4* p = reinterpret_cast<float4*>(out + int64_t(n) * g.ldo + m);
-          float4 v = make_float4(acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2],
-                                 acc[x][y][4 * q + 3]);
-          if (g.add) {
-            const float4 o = *p;
-            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-          }
-          *p = v;
-        }
+  auto take = [&](const Unit& u) {
+    if constexpr (MANY && TAKEN > 0) {
+      const int n = u.n0 + nw, there = min(max(g.n - n, 0), 64);
+      const uint32_t to = lds_offset(own), lane4 = uint32_t(lane) * 4;
+      const v4i t = make_rsrc(g.targets + n, uint32_t(there) * 8);
+      copy4(t, 2 * lane4, to);
+      copy4(t, 2 * lane4 + 4, to + 256);
+      if constexpr (EPI == kGrad) {
+        copy4(make_rsrc(g.lse + n, uint32_t(there) * 4), lane4, to + 512);
+        copy4(make_rsrc(g.grad + n, g.grad_step ? uint32_t(there) * 4 : 0u), lane4, to + 768);
+      }
     }
-    return;
-  }
-  if constexpr (STATS) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) *g.done = 0;
+  };
+  struct Token {
+    int64_t target;
+    float lse, grad;
+  };
+  auto token_of = [&](const Unit& u, int y, int col) {  // (of a row past the tokens: anything)
+    Token t{};
+    if constexpr (MANY) {
+      const uint8_t* p = own + (32 * y + col) * 4;
+      t.target = int64_t(uint64_t(*reinterpret_cast<const uint32_t*>(p)) |
+                         uint64_t(*reinterpret_cast<const uint32_t*>(p + 256)) << 32);
+      if constexpr (EPI == kGrad) {
+        t.lse = *reinterpret_cast<const float*>(p + 512);
+        t.grad = g.grad_step ? *reinterpret_cast<const float*>(p + 768) : *g.grad;
+      }
+    } else {
+      const int64_t n = min(u.n0 + nw + 32 * y + col, g.n - 1);
+      t.target = g.targets[n];
+      if constexpr (EPI == kGrad) {
+        t.lse = g.lse[n];
+        t.grad = g.grad[n * g.grad_step];
+      }
+    }
+    return t;
+  };
+  // the target's place among the lane's values of the tile, negative if it is not there
+  auto place_of = [&](const Unit& u, int64_t target, int half) {
+    const int64_t w = target - g.first - u.m0;
+    return w >= 0 && w < min(T, g.m - u.m0) ? int(w) - mw - 4 * half : -1;
+  };
+
+  // ---- results: acc[x][y][r] is m = mw + 4 half + 32 x + 8 (r / 4) + r % 4, n = nw + 32
+  // y + col of the tile
+  constexpr int STORES = S::NB * (S::MB / 2) * 4;  // instructions a wave
+  // 16-bit values as rows: 32 x 64 at a time through the wave's own LDS, and out in
+  // runs of 128 bytes (all instructions are issued, so that they can be counted)
+  auto store_rows = [&](const Unit& u, int cols, int lane, auto value) {
+    const int col = lane & 31, half = lane >> 5, swz = (col >> 1) & 7;
+    const int64_t row = g.ldo * 2;
+    const int rows = min(g.n - u.n0 - nw, 64);
+    const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(
+        static_cast<uint16_t*>(g.out) + int64_t(u.n0 + nw) * g.ldo + u.m0, 0,
+        rows > 0 ? int(uint32_t((rows - 1) * row) + uint32_t(cols - u.m0) * 2) : 0, 0x00020000);
 #pragma unroll
-    for (int y = 0; y < S::NB; ++y) {
-      const int n = n0 + nw + 32 * y + col;
-      const bool in = n < g.n;
-      const int64_t want = in ? g.targets[n] - g.first - m0 : -1;
-      const int w = want >= 0 && want < T ? int(want) : -1;
-      // the target's place among the lane's values, if it is there
-      const int rel = w - mw - 4 * half;
-      const bool mine = w >= 0 && m0 + w < g.m && rel >= 0 && rel < 32 * S::MB && (rel & 4) == 0;
-      float top = -INFINITY, pick = 0.0f;
-      if (m0 + T > g.m) {
+    for (int y = 0; y < S::NB; ++y)
+#pragma unroll
+      for (int xp = 0; xp < S::MB / 2; ++xp) {
+#pragma unroll
+        for (int x = 2 * xp; x < 2 * xp + 2; ++x)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int c = 4 * (x & 1) + q;
+            *reinterpret_cast<uint2*>(own + col * 128 + ((c ^ swz) << 4) + half * 8) = value(x, y, q);
+          }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + (lane >> 3), c = lane & 7;
+          typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+          const u4 w = *reinterpret_cast<const u4*>(own + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
+          const int m = mw + 64 * xp + 8 * c;
+          const uint32_t at = u.m0 + m < cols ? uint32_t((32 * y + r) * row) + uint32_t(m) * 2
+                                              : kOutOfRange;
+          __builtin_amdgcn_raw_buffer_store_b128(w, out, at, 0, 0);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+  };
+  auto finish = [&](const Unit& u) {
+    // (what it derives from the lane is not kept through the products)
+    const int lane = fresh(threadIdx.x & 63), col = lane & 31, half = lane >> 5;
+    // classes of the lane's part of the tile, behind whose end are zeros
+    const int there = g.m - u.m0 - mw - 4 * half;
+    if constexpr (EPI == kFp32) {
+      float* out = static_cast<float*>(g.out) + int64_t(u.split) * g.split_stride;
+#pragma unroll
+      for (int y = 0; y < S::NB; ++y) {
+        const int n = u.n0 + nw + 32 * y + col;
+        if (n >= g.n) continue;
 #pragma unroll
         for (int x = 0; x < S::MB; ++x)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (m0 + m_of(x, r) >= g.m) acc[x][y][r] = -INFINITY;
+          for (int q = 0; q < 4; ++q) {
+            const int m = u.m0 + mw + 4 * half + 32 * x + 8 * q;
+            if (m >= g.m) continue;
+            float4* p = reinterpret_cast<float4*>(out + int64_t(n) * g.ldo + m);
+            float4 v = make_float4(acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2],
+                                   acc[x][y][4 * q + 3]);
+            if (g.add) {
+              const float4 o = *p;
+              v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+            }
+            *p = v;
+          }
+      }
+    }
+    if constexpr (EPI == kBf16)
+      store_rows(u, g.m, lane, [&](int x, int y, int q) {
+        const v16f& e = acc[x][y];
+        return make_uint2(pack2(e[4 * q], e[4 * q + 1]), pack2(e[4 * q + 2], e[4 * q + 3]));
+      });
+    if constexpr (EPI == kGrad) {
+      // (of g and the exponentials whole tiles are written: what lies behind the classes
+      // is zero)
+      float off[2], scale[2];
+      int rel[2];
+      bool keep[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const Token t = token_of(u, y, col);
+        keep[y] = t.target != g.ignore;
+        rel[y] = place_of(u, t.target, half);
+        scale[y] = g.count ? t.grad / *g.count : t.grad;
+        // (a target outside the vocabulary has a loss that is NaN, and so are its
+        // gradients)
+        if (t.target < 0 || t.target >= g.classes) scale[y] = NAN;
+        off[y] = t.lse * kLog2e;
+      }
+      store_rows(u, u.m0 + T, lane, [&](int x, int y, int q) {
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = exp2_fast(__builtin_fmaf(acc[x][y][4 * q + r], kLog2e, -off[y]));
+          v[r] = keep[y] ? (p - (rel[y] == 32 * x + 8 * q + r ? 1.0f : 0.0f)) * scale[y] : 0.0f;
+        }
+        if (u.m0 + T > g.m) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            v[r] = __int_as_float(__float_as_int(v[r]) & ((32 * x + 8 * q + r - there) >> 31));
+        }
+        return make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+      });
+    }
+    if constexpr (STATS) {
+      // maxima and sums of the two waves along m meet in their own LDS, [64] each
+      float* const mine = reinterpret_cast<float*>(own + 1024);
+      const float* const other = reinterpret_cast<const float*>(spare + (wave ^ 1) * PRIVATE + 1024);
+      int rel[2];
+#pragma unroll
+      for (int y = 0; y < S::NB; ++y) rel[y] = place_of(u, token_of(u, y, col).target, half);
+#pragma unroll
+      for (int y = 0; y < S::NB; ++y) {
+        const int n = u.n0 + nw + 32 * y + col;
+        const bool here = n < g.n && rel[y] >= 0 && rel[y] < 32 * S::MB && (rel[y] & 4) == 0;
+        if (__ballot(here)) {  // (few of the tiles hold a target of theirs)
+          // 32 x 32 values through the wave's LDS, where a lane can pick
+          float* const at = reinterpret_cast<float*>(own) + col * 32 + 4 * half;
+#pragma unroll
+          for (int x = 0; x < S::MB; ++x) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<float4*>(at + 8 * q) =
+                  make_float4(acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2],
+                              acc[x][y][4 * q + 3]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (here && rel[y] >> 5 == x) g.picked[n] = at[rel[y] & 31];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          }
+        }
       }
 #pragma unroll
-      for (int x = 0; x < S::MB; ++x) {
+      for (int y = 0; y < S::NB; ++y) {
+        float top = -INFINITY;
+        if (u.m0 + T > g.m) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          pick = rel == 32 * x + 8 * (r >> 2) + (r & 3) ? acc[x][y][r] : pick;
-          top = fmaxf(top, acc[x][y][r]);
+          for (int x = 0; x < S::MB; ++x) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              acc[x][y][r] = 32 * x + 8 * (r >> 2) + (r & 3) < there ? acc[x][y][r] : -INFINITY;
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
+#pragma unroll
+        for (int x = 0; x < S::MB; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[x][y][r]);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (half == 0) mine[32 * y + col] = top;
+      }
+      sync_lds();
+#pragma unroll
+      for (int y = 0; y < S::NB; ++y) {
+        const float top = fmaxf(mine[32 * y + col], other[32 * y + col]);
+        const float off = top == -INFINITY ? 0.0f : top * kLog2e;
+        float sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < S::MB; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float e = exp2_fast(__builtin_fmaf(acc[x][y][r], kLog2e, -off));
+            sum += e;
+            if constexpr (EPI == kExps) acc[x][y][r] = e;
+          }
+        sum += __shfl_xor(sum, 32);
+        if (half == 0) mine[64 + 32 * y + col] = sum;
+      }
+      sync_lds();
+      const int n = u.n0 + nw + lane;
+      if (wm == 0 && n < g.n) {
+        const float top = fmaxf(mine[lane], other[lane]);
+        g.part[int64_t(u.m0 / T) * g.n + n] =
+            make_float2(top == -INFINITY ? 0.0f : top * kLog2e, mine[64 + lane] + other[64 + lane]);
+      }
+      if constexpr (EPI == kExps) {
+        sync_lds();
+        store_rows(u, u.m0 + T, lane, [&](int x, int y, int q) {
+          const v16f& e = acc[x][y];
+          return make_uint2(half2(e[4 * q], e[4 * q + 1]), half2(e[4 * q + 2], e[4 * q + 3]));
+        });
+      }
+    }
+  };
+
+  Unit u = unit_at<T>(g, int(blockIdx.x));
+  Frags f0, f1;
+  clear();
+  if constexpr (MANY) {
+    const int units = g.tiles_m * g.tiles_n * g.splits;
+    // instructions in flight behind a tile's second stage: the result's stores (at
+    // least), and what the next epilogue takes
+    constexpr int BEHIND = (EPI == kBf16 || EPI == kGrad || EPI == kExps ? STORES : 0) + TAKEN;
+    copy_stage(u, 0, 0);
+    copy_stage(u, 1, 1);
+    take(u);
+    wait_and_sync<8 + TAKEN>();
+    read_half(f0, 0, 0);
+    int buf = 0;
+    for (int at = int(blockIdx.x); at < units; at += int(gridDim.x)) {
+      const bool more = at + int(gridDim.x) < units;
+      Unit next = u;
+      if (more) next = unit_at<T>(g, at + int(gridDim.x));
+      else next.k1 = next.k0;  // (copies read nothing)
+      for (int t = 0; t < u.stages; ++t, buf ^= 1) {
+        read_half(f1, buf, 1);
+        multiply(f0, 0);
+        pin();
+        if (t == 0 && at >= int(gridDim.x)) wait_and_sync<BEHIND>();
+        else wait_and_sync<0>();
+        multiply(f0, 1);
+        pin();
         __builtin_amdgcn_sched_barrier(0);
+        const bool last = t + 2 >= u.stages;
+        copy_stage(last ? next : u, last ? t + 2 - u.stages : t + 2, buf);
+        __builtin_amdgcn_sched_barrier(0);
+        // (after the last stage: the next tile's first one)
+        read_half(f0, buf ^ 1, 0);
+        multiply(f1, 0);
+        multiply(f1, 1);
       }
-      top = fmaxf(top, __shfl_xor(top, 32));
-      if (half == 0) tops[wm][nw + 32 * y + col] = top;
-      if (mine) g.picked[n] = pick;
+      finish(u);
+      clear();
+      u = next;
+      if (more) take(u);
     }
-    __syncthreads();
+    // (copies still in flight read nothing, but write zeros)
+    wait_and_sync<0>();
+  } else {
+    // (copies past the last stage read nothing and keep the count of what is in flight)
+    constexpr int kAhead = 8 * (S::STAGES - 2);
 #pragma unroll
-    for (int y = 0; y < S::NB; ++y) {
-      const int nl = nw + 32 * y + col;
-      const float top = fmaxf(tops[0][nl], tops[1][nl]);
-      const float off = top == -INFINITY ? 0.0f : top * kLog2e;
-      float sum = 0.0f;
-#pragma unroll
-      for (int x = 0; x < S::MB; ++x)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float e = exp2_fast(__builtin_fmaf(acc[x][y][r], kLog2e, -off));
-          sum += e;
-          if constexpr (EPI == kExps) acc[x][y][r] = e;
-        }
-      sum += __shfl_xor(sum, 32);
-      if (half == 0) exps[wm][nl] = sum;
+    for (int t = 0; t < S::STAGES - 1; ++t) copy_stage(u, t, t);
+    wait_and_sync<kAhead>();
+    copy_stage(u, S::STAGES - 1, S::STAGES - 1);
+    read_half(f0, 0, 0);
+    for (int t = 0; t < u.stages; ++t) {
+      read_half(f1, t % S::STAGES, 1);
+      multiply(f0, 0);
+      pin();
+      wait_and_sync<kAhead>();
+      multiply(f0, 1);
+      pin();
+      __builtin_amdgcn_sched_barrier(0);
+      copy_stage(u, t + S::STAGES, t % S::STAGES);
+      __builtin_amdgcn_sched_barrier(0);
+      read_half(f0, (t + 1) % S::STAGES, 0);
+      multiply(f1, 0);
+      multiply(f1, 1);
     }
-    __syncthreads();
-    const int t = threadIdx.x, n = n0 + t;
-    if (t < T && n < g.n) {
-      const float top = fmaxf(tops[0][t], tops[1][t]);
-      g.part[int64_t(m0 / T) * g.n + n] =
-          make_float2(top == -INFINITY ? 0.0f : top * kLog2e, exps[0][t] + exps[1][t]);
-    }
-    if constexpr (EPI == kStats) return;
-  }
-  if constexpr (EPI == kBf16 || EPI == kGrad || EPI == kExps) {
-    constexpr int ROW = 2 * T, CH = ROW / 16;
-#pragma unroll
-    for (int y = 0; y < S::NB; ++y) {
-      const int nl = nw + 32 * y + col, n = n0 + nl;
-      float scale = 0.0f, off = 0.0f;
-      int rel = -1;  // the target's place among the lane's values
-      bool keep = false;
-      if constexpr (EPI == kGrad) {
-        if (n < g.n) {
-          const int64_t target = g.targets[n], want = target - g.first - m0;
-          keep = target != g.ignore;
-          rel = want >= 0 && want < T ? int(want) - mw - 4 * half : -1;
-          scale = g.grad[int64_t(n) * g.grad_step];
-          if (g.count) scale /= *g.count;
-          // (a target outside the vocabulary has a loss that is NaN, and so are
-          // its gradients)
-          if (target < 0 || target >= g.classes) scale = NAN;
-          off = g.lse[n] * kLog2e;
-        }
-      }
-#pragma unroll
-      for (int x = 0; x < S::MB; ++x)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int m = m_of(x, 4 * q);
-          float v[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            v[r] = acc[x][y][4 * q + r];
-            if constexpr (EPI == kGrad) {
-              const float p = exp2_fast(__builtin_fmaf(v[r], kLog2e, -off));
-              v[r] = keep ? (p - (rel == 32 * x + 8 * q + r ? 1.0f : 0.0f)) * scale : 0.0f;
-            }
-          }
-          if constexpr (EPI == kGrad) {
-            if (m0 + T > g.m) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (m0 + m + r >= g.m) v[r] = 0.0f;
-            }
-          }
-          const int chunk = (m >> 3) ^ (nl & (CH - 1));
-          *reinterpret_cast<uint2*>(lds + nl * ROW + chunk * 16 + (m & 4) * 2) =
-              EPI == kExps ? make_uint2(half2(v[0], v[1]), half2(v[2], v[3]))
-                           : make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
-        }
-    }
-    __syncthreads();
-    uint16_t* out = static_cast<uint16_t*>(g.out);
-    // (of g and the exponentials whole tiles are written: what lies behind the
-    // classes is zero)
-    const int cols = EPI == kBf16 ? g.m : m0 + T;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < T * CH; i += S::THREADS) {
-      const int nl = i / CH, c = i % CH, n = n0 + nl, m = m0 + c * 8;
-      if (n < g.n && m < cols)
-        *reinterpret_cast<uint4*>(out + int64_t(n) * g.ldo + m) =
-            *reinterpret_cast<const uint4*>(lds + nl * ROW + ((c ^ (nl & (CH - 1))) << 4));
-    }
+    wait_and_sync<0>();
+    finish(u);
   }
 }
 
@@ -665,7 +803,9 @@ int launch(Product p, hipStream_t st) {
   p.tiles_n = int(ceil_div(p.n, T));
   const int64_t units = int64_t(p.tiles_m) * p.tiles_n * p.splits;
   if (!grid_x_fits(units, THREADS) || units > INT32_MAX) return TCFP_ERR_SHAPE;
-  product_kernel<T, ST, TA, TB, EPI><<<unsigned(units), THREADS, 0, st>>>(p);
+  // (tiles of 256: a workgroup a CU, which takes several)
+  const unsigned grid = unsigned(T == 256 ? std::min<int64_t>(units, kCus) : units);
+  product_kernel<T, ST, TA, TB, EPI><<<grid, THREADS, 0, st>>>(p);
   return launch_status();
 }
 template <bool TA, bool TB, int EPI>

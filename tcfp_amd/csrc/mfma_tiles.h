@@ -49,12 +49,22 @@ TCFP_DEV void copy16(v4i rsrc, uint32_t off, uint32_t lds) {
                : "memory");
 }
 
-// The same, 4 bytes a lane: into LDS at lds + 4 * lane.
+// The same, 4 bytes a lane: into LDS at lds + 4 * lane.  (Its descriptor may come out
+// of vector registers, which takes five wait states.)
 TCFP_DEV void copy4(v4i rsrc, uint32_t off, uint32_t lds) {
-  asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
+#pragma unroll
+  for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
+  asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds"
                :
                : "v"(off), "s"(rsrc), "{m0}"(lds)
                : "memory");
+}
+
+// Hides a value's origin from the compiler, which would otherwise keep all that is
+// derived from it in registers through a loop, where none are free.
+TCFP_DEV int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 // Waits until at most N of the wave's vector memory operations are in flight and

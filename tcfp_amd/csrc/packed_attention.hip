@@ -111,13 +111,6 @@ TCFP_DEV int swizzle(int row) {
 template <int D>
 constexpr int kTileBytes = kStep * D * 2;
 
-// Hides an offset's origin from the compiler, which would otherwise keep all that
-// is derived from it in registers through the loop, where none are free.
-TCFP_DEV int fresh(int off) {
-  asm volatile("" : "+v"(off));
-  return off;
-}
-
 // The wave's share (instructions wave, wave + NW, ...) of the copy of rows
 // [row, row + kStep) of x, of which the first `rows` there are.
 template <int D, int NW>
