@@ -1,13 +1,16 @@
 """Train a small decoder on TCFP-12 layers, then generate from it through the
 8-bit paged K/V cache.
 
-    python examples/generate.py [--steps 600] [--tokens 64]
+    python examples/generate.py [--steps 600] [--tokens 64] [--rotary]
 
 The model is the repository's small transformer (d_model 256, 4 layers, 4 heads,
 FFN 1024, vocab 256) with root-mean-square norms: every norm stands in front of
 a linear layer that reads FP8 codes, so ``TCFPNormLinear`` quantises where it
-normalises.  Serving lays the weight codes out once; a step of a batch -- whole
-prompts or one token each -- is, per layer,
+normalises.  Positions are a learned table, or with ``--rotary`` turns of the
+queries and keys.  Training attends a batch's sequences packed one after another
+and takes the loss from the hidden states, without the logits.  Serving lays the
+weight codes out once; a step of a batch -- whole prompts or one token each -- is,
+per layer,
 
     rms_norm_quantize -> QKV GEMM -> cache write -> paged attention
     -> block_quantize -> output GEMM
@@ -30,7 +33,9 @@ sys.path.insert(0, str(Path(__file__).resolve().parent.parent))
 
 from tcfp_amd import kernels as K  # noqa: E402
 from tcfp_amd import norm  # noqa: E402
-from tcfp_amd.attention import PagedKVCache  # noqa: E402
+from tcfp_amd.attention import PagedKVCache, packed_attention  # noqa: E402
+from tcfp_amd.loss import linear_cross_entropy  # noqa: E402
+from tcfp_amd.rotary import rotary_embedding, rotary_frequencies  # noqa: E402
 from tcfp_amd.nn import TCFPLinear, TCFPNormLinear, TCFPRMSNorm  # noqa: E402
 
 VOCAB, BLOCK = 256, 64
@@ -45,41 +50,58 @@ class Layer(nn.Module):
         self.fc1 = TCFPNormLinear(d, ffn, scale_block_size=BLOCK)
         self.fc2 = TCFPLinear(ffn, d, use_tensor_cores=True, scale_block_size=BLOCK)
 
-    def forward(self, x, h):
-        """``x``: what the layer before adds to the residual stream ``h``."""
+    def forward(self, x, h, starts, turn):
+        """``x``: what the layer before adds to the residual stream ``h``; ``starts``:
+        where the batch's sequences begin; ``turn``: positions and frequencies."""
         qkv, h = self.qkv(x, h)
         b, t, c = h.shape
-        q, k, v = (z.contiguous() for z in
-                   qkv.float().reshape(b, t, 3, self.heads, -1).permute(2, 0, 3, 1, 4))
-        att = torch.matmul(q, k.transpose(-2, -1).contiguous()) / q.shape[-1] ** 0.5
-        mask = torch.triu(torch.ones(t, t, dtype=torch.bool, device=x.device), 1)
-        att = F.softmax(att.masked_fill(mask, float("-inf")), dim=-1)
-        y = torch.matmul(att, v).transpose(1, 2).reshape(b, t, c)
-        z, h = self.fc1(self.proj(y), h)
+        q, k, v = qkv.bfloat16().reshape(b * t, 3, self.heads, -1).unbind(1)
+        if turn is not None:
+            q, k = rotary_embedding(q, k, *turn)
+        y = packed_attention(q, k, v, starts, max_len=t).reshape(b, t, c)
+        z, h = self.fc1(self.proj(y.to(h.dtype)), h)
         return self.fc2(F.gelu(z)), h
 
 
 class Decoder(nn.Module):
     def __init__(self, d: int = 256, layers: int = 4, heads: int = 4, ffn: int = 1024,
-                 positions: int = 256) -> None:
+                 positions: int = 256, rotary: bool = False) -> None:
         super().__init__()
-        self.tok, self.pos = nn.Embedding(VOCAB, d), nn.Embedding(positions, d)
+        self.tok, self.positions = nn.Embedding(VOCAB, d), positions
+        self.pos = None if rotary else nn.Embedding(positions, d)
+        self.register_buffer("freqs", rotary_frequencies(d // heads) if rotary else None,
+                             persistent=False)
         self.layers = nn.ModuleList(Layer(d, heads, ffn) for _ in range(layers))
         self.norm = TCFPRMSNorm(d)
         for m in self.modules():
             if isinstance(m, (nn.Embedding, TCFPLinear)):
                 nn.init.normal_(m.weight, std=0.02)
 
-    def forward(self, idx):
-        if idx.shape[1] > self.pos.num_embeddings:
-            raise ValueError(f"{idx.shape[1]} tokens, the model has {self.pos.num_embeddings} "
-                             "positions")
+    def embed(self, idx, pos):
+        """What the first layer adds to the residual stream, and the stream."""
         h = self.tok(idx)
-        x = self.pos(torch.arange(idx.shape[1], device=idx.device)).expand_as(h)
+        return (torch.zeros_like(h) if self.pos is None else self.pos(pos).expand_as(h)), h
+
+    def hidden(self, idx):
+        """The hidden states in front of the head."""
+        b, t = idx.shape
+        if t > self.positions:
+            raise ValueError(f"{t} tokens, the model has {self.positions} positions")
+        pos = torch.arange(t, device=idx.device)
+        x, h = self.embed(idx, pos)
+        starts = torch.arange(0, b * t + 1, t, dtype=torch.int32, device=idx.device)
+        turn = None if self.freqs is None else (pos.repeat(b), self.freqs)
         for layer in self.layers:
-            x, h = layer(x, h)
-        y, _ = self.norm(x, h)
-        return y.float() @ self.tok.weight.t()
+            x, h = layer(x, h, starts, turn)
+        return self.norm(x, h)[0]
+
+    def forward(self, idx):
+        return self.hidden(idx).float() @ self.tok.weight.t()
+
+    def loss(self, idx, targets):
+        """Mean cross entropy, with the head in bf16 and its logits nowhere."""
+        return linear_cross_entropy(self.hidden(idx).bfloat16(), self.tok.weight.bfloat16(),
+                                    targets)
 
 
 class Server:
@@ -107,7 +129,7 @@ class Server:
         model, dev = self.model, self.model.tok.weight.device
         starts = [self.cache.length(s) for s in seqs]
         # (an index that a table does not have would end the process on the GPU)
-        room = model.pos.num_embeddings
+        room = model.positions
         if any(a + len(t) > room for a, t in zip(starts, tokens)):
             raise ValueError(f"a sequence would pass the model's {room} positions")
         if any(not 0 <= t < model.tok.num_embeddings for ts in tokens for t in ts):
@@ -116,12 +138,14 @@ class Server:
         idx = torch.tensor([t for ts in tokens for t in ts], device=dev)
         pos = torch.tensor([a + i for a, t in zip(starts, tokens) for i in range(len(t))],
                            device=dev)
-        h, x = model.tok(idx), model.pos(pos)
+        x, h = model.embed(idx, pos)
         for i, layer in enumerate(model.layers):
             q8, e, h, _ = norm.rms_norm_quantize(x, layer.qkv.norm_weight, h, eps=layer.qkv.eps,
                                                  block_size=BLOCK)
             qkv = self._linear(layer.qkv, q8, e, torch.bfloat16)
             q, k, v = (z.unflatten(1, (self.heads, self.dim)) for z in qkv.chunk(3, 1))
+            if model.freqs is not None:
+                q, k = rotary_embedding(q, k, pos, model.freqs)
             self.cache.write(i, k, v, batch)
             y = self.cache.attend(i, q, batch)
             x = self._linear(layer.proj, *K.block_quantize_fp8(y.flatten(1), BLOCK))
@@ -178,7 +202,7 @@ def train(model: Decoder, steps: int, seq: int = 128, batch: int = 32, seed: int
         for g in opt.param_groups:
             g["lr"] = 1e-3 * min(1.0, (step + 1) / 20)
         data = patterns(batch, seq + 1, gen).to(dev)
-        loss = F.cross_entropy(model(data[:, :-1]).reshape(-1, VOCAB), data[:, 1:].reshape(-1))
+        loss = model.loss(data[:, :-1], data[:, 1:])
         opt.zero_grad(set_to_none=True)
         loss.backward()
         nn.utils.clip_grad_norm_(model.parameters(), 1.0)
@@ -191,9 +215,10 @@ def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--steps", type=int, default=600)
     ap.add_argument("--tokens", type=int, default=64)
+    ap.add_argument("--rotary", action="store_true", help="rotary instead of learned positions")
     a = ap.parse_args()
     torch.manual_seed(0)
-    model = Decoder().cuda()
+    model = Decoder(rotary=a.rotary).cuda()
     losses = train(model, a.steps)
     print(f"loss {losses[0]:.3f} -> {losses[-1]:.3f} in {a.steps} steps", flush=True)
     server = Server(model)

@@ -638,15 +638,29 @@ int launch_status() { return hipGetLastError() == hipSuccess ? TCFP_OK : TCFP_ER
 // Waves of a workgroup.
 constexpr int kWaves = 4;
 
-// Parts of a group's heads in the dK, dV launch: one, but where there are not twice
-// as many tiles of keys as workgroups that the card holds at once (of a causal
-// sequence the first tile has twice the mean's queries).
+// Parts of a group's heads in the dK, dV launch, by what they are about to take, us: a
+// step of 64 queries, heads of 128, 2.6 for a workgroup alone on a CU and 4.2 beside
+// another; the longest chain of steps -- of a causal sequence the first tile of keys has
+// twice the mean's -- against all of them over the card; the parts' writing and joining,
+// 4.5 TB/s.  (32 / 8 heads of 128, the whole backward: one sequence of 8192 4000 us in
+// one part, 1770 in two; four of up to 4096 1310 and 1063; six of up to 1000 198 in two,
+// 199 in four.)
 int parts_of(int64_t keys, int64_t batch, int64_t max_key_len, int kv_heads, int group, int dim) {
-  const int64_t rows = 32 * kWaves;
-  const int64_t tiles =
-      std::min(ceil_div(std::max<int64_t>(max_key_len, 1), rows) * batch, keys / rows + batch);
-  const int64_t want = (dim == 256 ? 2 : 4) * kCus;
-  return int(std::clamp<int64_t>(ceil_div(want, std::max<int64_t>(tiles * kv_heads, 1)), 1, group));
+  const int64_t rows = 32 * kWaves, longest = std::max<int64_t>(std::min(max_key_len, keys), 1);
+  const double tiles =
+      double(std::min(ceil_div(longest, rows) * batch, keys / rows + batch) * kv_heads);
+  const double steps = double(ceil_div(longest, kStep)) * dim / 128;
+  const double slots = dim == 256 ? kCus : 2 * kCus;
+  int best = 1;
+  double least = INFINITY;
+  for (int parts = 1; parts <= group; ++parts) {
+    const double step = tiles * parts > kCus ? 4.2 : 2.6;
+    const double t = std::max(steps * double(ceil_div(group, parts)) * step,
+                              0.5 * steps * group * tiles / slots * 4.2) +
+                     (parts > 1 ? 5 + double(parts) * double(keys) * kv_heads * dim * 16 / 4.5e6 : 0);
+    if (t < least) least = t, best = parts;
+  }
+  return best;
 }
 
 struct Sizes {
