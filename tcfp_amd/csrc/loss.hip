@@ -817,10 +817,6 @@ int launch_cut(const Cut& c, Product p, hipStream_t st) {
                        : launch<128, 4, TA, TB, EPI>(p, st);
 }
 
-// Elements from a row of g to the next: 256 bytes more than whole tiles, as rows a power
-// of two apart meet the same channels of the memory.
-int64_t row_of(int64_t run) { return run + 128; }
-
 struct Layout {
   int64_t run;      // classes
   Cut dh, dw;
@@ -829,7 +825,7 @@ struct Layout {
 Layout layout_of(int64_t tokens, int64_t vocab, int64_t dim, bool need_h, bool need_w) {
   Layout l{};
   l.run = run_of(tokens, vocab);
-  l.g = align256(size_t(tokens) * size_t(row_of(l.run)) * 2);
+  l.g = align256(size_t(tokens) * size_t(l.run) * 2);
   if (need_h) {
     l.dh = cut_of(tokens, dim, std::min(l.run, vocab), true);
     if (l.dh.splits > 1 || l.run < vocab)
@@ -859,7 +855,7 @@ int check_sizes(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
 Layout train_layout(int64_t tokens, int64_t vocab, int64_t dim, bool need_h, bool need_w) {
   Layout l{};
   l.run = ceil_div(vocab, 256) * 256;
-  l.g = align256(size_t(tokens) * size_t(row_of(l.run)) * 2);
+  l.g = align256(size_t(tokens) * size_t(l.run) * 2);
   if (need_h) {
     l.dh = cut_of(tokens, dim, vocab, true);
     if (l.dh.splits > 1) l.sum_h = align256(size_t(l.dh.splits) * size_t(tokens) * size_t(dim) * 4);
@@ -948,7 +944,7 @@ int products_of(const Head& h, const Layout& l, const uint16_t* g, int64_t v0, i
     q.a = static_cast<const uint16_t*>(h.weight) + v0 * h.ldw;
     q.b = g;
     q.lda = h.ldw;
-    q.ldb = row_of(l.run);
+    q.ldb = l.run;
     q.m = int(h.dim);
     q.n = int(h.tokens);
     q.k = int(classes);
@@ -974,7 +970,7 @@ int products_of(const Head& h, const Layout& l, const uint16_t* g, int64_t v0, i
   q.a = static_cast<const uint16_t*>(h.hidden);
   q.b = g;
   q.lda = h.ldh;
-  q.ldb = row_of(l.run);
+  q.ldb = l.run;
   q.m = int(h.dim);
   q.n = int(classes);
   q.k = int(h.tokens);
@@ -1047,16 +1043,16 @@ int tcfp_linear_cross_entropy_train(const void* hidden, int64_t ldh, const void*
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint16_t* g = reinterpret_cast<uint16_t*>(ws);
   uint8_t* parts = ws + l.g + l.sum_h + l.sum_w;
-  int done = losses_of(head, losses, lse, mean, total, count, parts, g, row_of(l.run), st);
+  int done = losses_of(head, losses, lse, mean, total, count, parts, g, l.run, st);
   if (done != TCFP_OK) return done;
   const dim3 grid(unsigned(ceil_div(vocab, 1024)), unsigned(ceil_div(tokens, 8)));
   const auto* part = reinterpret_cast<const float2*>(parts);
   const float* each = mean ? count : nullptr;
   if (logits_cut(tokens, vocab, dim).tile == 256)
-    exps_to_grad_kernel<256><<<grid, 256, 0, st>>>(g, row_of(l.run), part, lse, targets, ignore, vocab,
+    exps_to_grad_kernel<256><<<grid, 256, 0, st>>>(g, l.run, part, lse, targets, ignore, vocab,
                                                    int(tokens), each);
   else
-    exps_to_grad_kernel<128><<<grid, 256, 0, st>>>(g, row_of(l.run), part, lse, targets, ignore, vocab,
+    exps_to_grad_kernel<128><<<grid, 256, 0, st>>>(g, l.run, part, lse, targets, ignore, vocab,
                                                    int(tokens), each);
   if (launch_status() != TCFP_OK) return TCFP_ERR_HIP;
   done = products_of(head, l, g, 0, vocab, grad_hidden, grad_weight,
@@ -1120,7 +1116,7 @@ int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const vo
     const int64_t classes = std::min(l.run, vocab - v0);
     Product p = head_product(head, v0, classes);
     p.out = g;
-    p.ldo = row_of(l.run);
+    p.ldo = l.run;
     p.lse = lse;
     p.grad = grad;
     p.grad_step = int(grad_step);

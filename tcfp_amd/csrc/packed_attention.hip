@@ -459,7 +459,10 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dq_kernel(Pa
 //
 // A workgroup takes 32 NW keys of a K/V head, a wave 32 of them, whose K and V stay
 // in registers; the queries of the group's heads (of a part of them, where the keys
-// alone would not fill the card) come in steps of 64 with their dO, L and delta.
+// alone would not fill the card) come in steps of 64 with their dO, L and delta.  Of a
+// wave's 256 registers 192 hold its K, V, dK and dV (heads of 128): the phases of 32
+// queries -- S and dP, P and dS, the sums -- are kept apart, and the other workgroup on
+// the CU fills the matrix cores meanwhile.
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dkv_kernel(Packed a) {
   constexpr int TILE = kTileBytes<D>, STATS = 2 * kStep * 4, BUF = 2 * TILE + STATS;
@@ -535,7 +538,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dkv_kernel(P
       advance();
       if (i + 1 < total) fetch(next_g, next_at, buf ^ 1);
       const float* stats = reinterpret_cast<const float*>(lds + buf * BUF + 2 * TILE);
-#pragma unroll 1
+#pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int r0 = at + 32 * x;
         if (idle || r0 + 32 <= w_begin || r0 >= w_end) continue;

@@ -133,12 +133,12 @@ def test_workspaces():
         assert f(0, 100, 64, 1, 1) == f(-1, 100, 64, 1, 1) == f(4, 0, 64, 1, 1) == 0
         # what is not wanted takes nothing
         assert f(1000, 50001, 1056, 0, 1) <= f(1000, 50001, 1056, 1, 1)
-    # the logits' gradients of a run stay within 256 MiB (and the rows' padding), of a
-    # whole pass within 1 GiB
+    # the logits' gradients of a run stay within 256 MiB (or are a run of 256 classes), of
+    # a whole pass within 1 GiB
     for tokens in (1, 100, 8192, 100000, 400000):
         for vocab in (256, 50001, 1 << 20, 5 << 20):
-            assert back(tokens, vocab, 64, 0, 0) <= (256 << 20) + 1024 * tokens
-            assert train(tokens, vocab, 64, 0, 0) <= (1 << 30) + (1 << 28)
+            assert back(tokens, vocab, 64, 0, 0) <= max(256 << 20, 512 * tokens)
+            assert train(tokens, vocab, 64, 0, 0) <= (1 << 30) + (1 << 28)  # (parts, sums)
     packed = lib.tcfp_packed_attention_backward_workspace_bytes
     assert packed(100, 100, 0, 100, 4, 2, 64) == packed(100, 100, 1, 100, 4, 3, 64) == 0
     # delta; with many tiles of keys no parts beside it
