@@ -795,7 +795,8 @@ int tcfp_packed_attention_backward(
     const void* grad_out, int64_t go_token_stride, int64_t go_head_stride, const void* q,
     int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
     int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
-    const void* out, const int8_t* out_low, const float* lse, const int32_t* q_starts, const int32_t* k_starts,
+    const void* out, const int8_t* out_low, const float* lse, const int32_t* q_starts,
+    const int32_t* k_starts,
     int64_t batch, int64_t tokens, int64_t keys, int heads, int kv_heads, int dim,
     int64_t max_len, int64_t max_key_len, float scale, int causal, int64_t window, void* dq,
     void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);

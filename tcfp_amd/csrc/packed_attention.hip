@@ -393,7 +393,8 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dq_kernel(Pa
     v8bf q[D / 16], go[D / 16];
     const int64_t hrow = int64_t(s.q0 + row) * a.heads + head;
     load_row<D>(a.q + int64_t(s.q0 + row) * a.q_token + int64_t(head) * a.q_head, half, true, q);
-    load_row<D>(a.go + int64_t(s.q0 + row) * a.go_token + int64_t(head) * a.go_head, half, true, go);
+    load_row<D>(a.go + int64_t(s.q0 + row) * a.go_token + int64_t(head) * a.go_head, half, true,
+                go);
     float delta = 0.0f;
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) {
@@ -619,7 +620,8 @@ __global__ __launch_bounds__(256) void packed_join_kernel(Packed a, int64_t eigh
   if (row >= k_first && row < k_past) {
     const float* p = a.part + int64_t(blockIdx.y) * whole + i * 8;
     for (int s = 0; s < a.parts; ++s, p += 2 * whole) {
-      const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+      const float4 x = reinterpret_cast<const float4*>(p)[0];
+      const float4 y = reinterpret_cast<const float4*>(p)[1];
       v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
       v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
     }
@@ -660,7 +662,7 @@ int parts_of(int64_t keys, int64_t batch, int64_t max_key_len, int kv_heads, int
     const double step = tiles * parts > kCus ? 4.2 : 2.6;
     const double t = std::max(steps * double(ceil_div(group, parts)) * step,
                               0.5 * steps * group * tiles / slots * 4.2) +
-                     (parts > 1 ? 5 + double(parts) * double(keys) * kv_heads * dim * 16 / 4.5e6 : 0);
+                     (parts > 1 ? 5 + 16 / 4.5e6 * parts * double(keys) * kv_heads * dim : 0);
     if (t < least) least = t, best = parts;
   }
   return best;
@@ -675,8 +677,8 @@ int check_sizes(const Sizes& z) {
   if (z.dim != 64 && z.dim != 128 && z.dim != 256) return TCFP_ERR_SHAPE;
   if (z.tokens < 0 || z.keys < 0 || z.tokens > kMostRows || z.keys > kMostRows || z.batch < 0 ||
       z.batch > 65535 || z.heads <= 0 || z.heads > 65535 || z.kv_heads <= 0 ||
-      z.heads % z.kv_heads || z.max_len < 0 || z.max_key_len < 0 || z.window < 0 ||
-      !std::isfinite(z.scale))
+      z.heads % z.kv_heads || z.batch * z.heads > 1 << 30 || z.max_len < 0 || z.max_key_len < 0 ||
+      z.window < 0 || !std::isfinite(z.scale))
     return TCFP_ERR_SHAPE;
   if ((z.tokens > 0 || z.keys > 0) && z.batch == 0) return TCFP_ERR_SHAPE;
   return TCFP_OK;
@@ -703,13 +705,14 @@ Packed arguments(const Sizes& z, bool causal) {
   a.sets = int(z.batch * z.kv_heads);
   return a;
 }
-// Workgroups of a launch with `members` of each set and `tiles` of each of those.
-int64_t workgroups(const Packed& a, int members) {
+// Tiles of a sequence and head in a launch with `members` of each set, and its workgroups.
+// A bound far past the lengths (all keys of a batch of many sequences) is cut: a
+// workgroup takes the tiles that are left over, one after another.
+int64_t lay_out(Packed& a, int64_t max_len, int64_t rows, int members) {
   const int64_t sets = a.sets >= 8 ? (a.sets + 7) / 8 * 8 : a.sets;
-  return sets * members * a.tiles;
-}
-int tiles_of(int64_t max_len, int64_t rows) {
-  return int(std::max<int64_t>(ceil_div(std::min(max_len, rows), 32 * kWaves), 1));
+  const int64_t each = sets * members, most = std::max<int64_t>((int64_t(1) << 22) / each, 1);
+  a.tiles = int(std::clamp<int64_t>(ceil_div(std::min(max_len, rows), 32 * kWaves), 1, most));
+  return each * a.tiles;
 }
 
 #define TCFP_PACKED(KERNEL, GRID)                                                       \
@@ -752,9 +755,8 @@ int tcfp_packed_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   a.o = static_cast<uint16_t*>(out);
   a.low = out_low;
   a.lse = lse;
-  a.tiles = tiles_of(max_len, tokens);
   const auto st = static_cast<hipStream_t>(stream);
-  TCFP_PACKED(packed_forward_kernel, workgroups(a, a.group));
+  TCFP_PACKED(packed_forward_kernel, lay_out(a, max_len, tokens, a.group));
   return TCFP_OK;
 }
 
@@ -772,17 +774,18 @@ int tcfp_packed_attention_backward(
     const void* grad_out, int64_t go_token_stride, int64_t go_head_stride, const void* q,
     int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
     int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
-    const void* out, const int8_t* out_low, const float* lse, const int32_t* q_starts, const int32_t* k_starts,
-    int64_t batch, int64_t tokens, int64_t keys, int heads, int kv_heads, int dim, int64_t max_len,
-    int64_t max_key_len, float scale, int causal, int64_t window, void* dq, void* dk, void* dv,
-    void* workspace, size_t workspace_bytes, void* stream) {
+    const void* out, const int8_t* out_low, const float* lse, const int32_t* q_starts,
+    const int32_t* k_starts, int64_t batch, int64_t tokens, int64_t keys, int heads, int kv_heads,
+    int dim, int64_t max_len, int64_t max_key_len, float scale, int causal, int64_t window,
+    void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream) {
   const Sizes z{tokens, keys, batch, max_len, max_key_len, window, heads, kv_heads, dim, scale};
   if (const int rc = check_sizes(z)) return rc;
   if (const int rc = check_rows(grad_out, go_token_stride, go_head_stride)) return rc;
   if (const int rc = check_rows(q, q_token_stride, q_head_stride)) return rc;
   if (const int rc = check_rows(k, k_token_stride, k_head_stride)) return rc;
   if (const int rc = check_rows(v, v_token_stride, v_head_stride)) return rc;
-  if (!aligned16(out) || !aligned16(out_low) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return TCFP_ERR_ALIGN;
+  if (!aligned16(out) || !aligned16(out_low) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
+    return TCFP_ERR_ALIGN;
   if (tokens == 0 && keys == 0) return TCFP_OK;
   const size_t need = tcfp_packed_attention_backward_workspace_bytes(
       tokens, keys, batch, max_key_len, heads, kv_heads, dim);
@@ -809,14 +812,10 @@ int tcfp_packed_attention_backward(
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                     align256(size_t(tokens) * size_t(heads) * 4));
   const auto st = static_cast<hipStream_t>(stream);
-  if (tokens > 0) {
-    a.tiles = tiles_of(max_len, tokens);
-    TCFP_PACKED(packed_dq_kernel, workgroups(a, a.group));
-  }
+  if (tokens > 0) TCFP_PACKED(packed_dq_kernel, lay_out(a, max_len, tokens, a.group));
   if (keys > 0) {
-    a.tiles = tiles_of(max_key_len, keys);
     a.parts = parts_of(keys, batch, max_key_len, kv_heads, a.group, dim);
-    TCFP_PACKED(packed_dkv_kernel, workgroups(a, a.parts));
+    TCFP_PACKED(packed_dkv_kernel, lay_out(a, max_key_len, keys, a.parts));
     if (a.parts > 1) {
       const int64_t eights = keys * kv_heads * dim / 8, blocks = ceil_div(eights, 256);
       if (!grid_x_fits(blocks, 256)) return TCFP_ERR_SHAPE;

@@ -98,7 +98,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Rotary r) {
     const float2* cs = turn + t * r.pairs;
     if (e >= turned) {
       const int at = rotary + (e - turned) * N;
-      if constexpr (VEC) *reinterpret_cast<uint4*>(y + at) = *reinterpret_cast<const uint4*>(x + at);
+      if constexpr (VEC)
+        *reinterpret_cast<uint4*>(y + at) = *reinterpret_cast<const uint4*>(x + at);
       else y[at] = x[at];
       continue;
     }
@@ -176,7 +177,8 @@ extern "C" int tcfp_rotary(const void* q, int64_t q_token_stride, int64_t q_head
   // card, else four, whose angles keep its threads busy.
   r.per_block = tokens < 1024 || r.pairs > kMostPairs / 4 ? 1 : 4;
   const int64_t blocks = (tokens + r.per_block - 1) / r.per_block;
-  if (!grid_x_fits(blocks, kThreads) || int64_t(r.per_block) * (q_heads + k_heads) * dim > INT32_MAX)
+  if (!grid_x_fits(blocks, kThreads) ||
+      int64_t(r.per_block) * (q_heads + k_heads) * dim > INT32_MAX)
     return TCFP_ERR_SHAPE;
   const auto st = static_cast<hipStream_t>(stream);
   const size_t lds = size_t(r.per_block) * r.pairs * sizeof(float2);

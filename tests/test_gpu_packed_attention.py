@@ -179,6 +179,34 @@ def test_bounds_that_are_too_small(dev):
     compare(dev, *data, max_len=1)
 
 
+def test_many_short_sequences_under_a_far_bound(dev):
+    """Keys of their own without a bound: all keys of the batch for every sequence."""
+    lens = [1 + i % 3 for i in range(700)]
+    keys = [1 + i % 5 for i in range(700)]
+    q, k, v, go, starts, kstarts = inputs(dev, lens, 2, 1, 64, keys, seed=20)
+    x = [y.detach().requires_grad_() for y in (q, k, v)]
+    o = A.packed_attention(*x, i32(starts, dev), max_len=10**9, key_start=i32(kstarts, dev))
+    got = (o.detach(), *torch.autograd.grad(o, x, go))
+    want = exact(q, k, v, go, starts, kstarts, 0.125, True, 0)
+    for n, y in zip(("o", "dq", "dk", "dv"), got):
+        within(y, want[n], n)
+
+
+def test_more_tiles_than_workgroups(dev):
+    """Sequences times heads times tiles past what a launch holds (4 million workgroups):
+    one long sequence among many of one token."""
+    long, heads = 15000, 8
+    lens = [1] * 2500 + [long] + [1] * 2499
+    q, k, v, go, starts, _ = inputs(dev, lens, heads, heads, 64, seed=21)
+    got = run(dev, q, k, v, go, starts, starts, window=200)
+    at = slice(2500, 2500 + long)
+    q, k, v, go = (x[at] for x in (q, k, v, go))
+    want = run(dev, q, k, v, go, [0, long], [0, long], window=200)
+    for x, y in zip(got, want):
+        # (the same values, but for dK and dV's sums if they are split another way)
+        torch.testing.assert_close(x[at], y, rtol=3 * HALF, atol=2e-4 * float(y.abs().max()))
+
+
 def test_rows_outside_the_sequences(dev):
     q, k, v, go, _, _ = inputs(dev, [100], 4, 2, 64, seed=6)
     q, k, v, go = (x.clone() for x in (q, k, v, go))

@@ -97,7 +97,8 @@ def test_packed_attention_refused():
     for kw in (dict(dim=32), dict(dim=96), dict(heads=3, kv=2), dict(heads=0), dict(kv=0), dict(batch=0),
                dict(batch=70000), dict(tokens=-1), dict(keys=-1), dict(tokens=(1 << 29) + 1),
                dict(longest=-1), dict(window=-1), dict(scale=math.inf), dict(scale=math.nan),
-               dict(token=-64), dict(token=1 << 24)):
+               dict(token=-64), dict(token=1 << 24),
+               dict(batch=65535, heads=65535)):
         assert packed_call(**kw) == shape, kw
     for kw in (dict(q=PTR + 2), dict(token=130), dict(head=65)):
         assert "align" in packed_call(**kw).lower(), kw
