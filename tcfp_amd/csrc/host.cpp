@@ -1233,7 +1233,8 @@ Outs packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
 
 Outs packed_attention_backward(const Tensor& grad, const Tensor& q, const Tensor& k,
                                const Tensor& v, const Tensor& out_, const Tensor& low_,
-                               const Tensor& lse_, const Tensor& starts, const OptT& key_starts, int64_t max_len,
+                               const Tensor& lse_, const Tensor& starts, const OptT& key_starts,
+                               int64_t max_len,
                                std::optional<int64_t> max_key_len, std::optional<double> scale,
                                bool causal, int64_t window) {
   OnGpu g;
@@ -1319,8 +1320,8 @@ Outs linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tens
   g.add(targets);
   const c10::DeviceGuard guard(g.device());
   const HeadIn in = head_inputs(hidden, weight, targets);
-  Tensor losses = g.empty(targets.sizes(), at::kFloat), lse = g.empty({in.h.rows}, at::kFloat), total,
-         count;
+  Tensor losses = g.empty(targets.sizes(), at::kFloat), lse = g.empty({in.h.rows}, at::kFloat),
+         total, count;
   if (reduce) total = g.empty({}, at::kFloat), count = g.empty({}, at::kFloat);
   const size_t nb = tcfp_linear_cross_entropy_workspace_bytes(in.h.rows, in.w.rows, in.h.cols);
   Tensor ws = g.empty({int64_t(std::max<size_t>(nb, 16))}, at::kByte);
@@ -1513,15 +1514,29 @@ Tensor packed_attention_with_grad(const Tensor& q, const Tensor& k, const Tensor
   if (max_key_len && *max_key_len < 0)
     value_error("max_len and max_key_len must not be negative");
   if (!wants_grad({&q, &k, &v}))
-    return packed_attention(q, k, v, starts, key_starts, max_len, scale, causal, window, false).t[0];
+    return packed_attention(q, k, v, starts, key_starts, max_len, scale, causal, window, false)
+        .t[0];
   return PackedNode::apply(q, k, v, starts, key_starts, max_len, max_key_len, scale, causal,
                            window);
 }
 
+// The capture that records the current stream's work; 0 outside of captures.
+unsigned long long capture_id(const Tensor& on) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const auto stream = c10::hip::getCurrentHIPStream(on.device().index()).stream();
+  if (hipStreamGetCaptureInfo(stream, &status, &id) != hipSuccess ||
+      status == hipStreamCaptureStatusNone)
+    return 0;
+  return id;
+}
+
 // The gradients of a sum or mean are made with the forward, for a gradient of the
-// loss of 1; the backward multiplies them with what that turns out to be and hands
-// them over.  A second backward through the same node, and one of every token's
-// loss, forms the logits again.
+// loss of 1; the backward multiplies them in place with what that turns out to be
+// (rounding them a second time if it is no power of two) and hands them over.  A second
+// backward through the same node, one that is captured without its forward (whose
+// replays would multiply again and again), and one of every token's loss form the
+// logits again.
 struct LossNode : torch::autograd::Function<LossNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight,
                         const Tensor& targets, int64_t ignore, bool reduce, bool mean) {
@@ -1529,7 +1544,10 @@ struct LossNode : torch::autograd::Function<LossNode> {
     if (reduce)
       made = linear_cross_entropy_train(hidden, weight, targets, ignore, mean,
                                         hidden.requires_grad(), weight.requires_grad());
-    if (made) ctx->saved_data["made"] = variable_list{made->t[4], made->t[5]};
+    if (made) {
+      ctx->saved_data["made"] = variable_list{made->t[4], made->t[5]};
+      ctx->saved_data["capture"] = int64_t(capture_id(hidden));
+    }
     Outs o = made ? std::move(*made)
                   : linear_cross_entropy(hidden, weight, targets, ignore, reduce, mean);
     ctx->save_for_backward({hidden, weight, targets, o.t[1], mean ? o.t[3] : Tensor()});
@@ -1540,7 +1558,9 @@ struct LossNode : torch::autograd::Function<LossNode> {
     const variable_list s = ctx->get_saved_variables();
     const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
     variable_list got;
-    if (const auto made = ctx->saved_data.find("made"); made != ctx->saved_data.end()) {
+    if (const auto made = ctx->saved_data.find("made");
+        made != ctx->saved_data.end() &&
+        ctx->saved_data["capture"].toInt() == int64_t(capture_id(grads[0]))) {
       got = made->second.toTensorVector();
       ctx->saved_data.erase(made);
       if (!need_h) got[0].reset();

@@ -10,9 +10,10 @@
 //
 // Gradients, where they are wanted of the losses' sum or mean and tokens x classes
 // take at most 1 GiB of workspace in 16 bits: with the forward, three products in
-// all.  The first one's epilogue leaves exp(z - maximum of its tile) in fp16 (11
-// bits, as it is rounded once more), a pass turns it into g in bf16 in place, and g
-// is the operand of dh and dW.  Otherwise (more, or a gradient for every token's
+// all.  The first one's epilogue leaves 2^15 exp(z - maximum of its tile) in fp16 (11
+// bits, as it is rounded once more; down to 2^-29 of the maximum, fewer to 2^-39: rare
+// classes keep their gradients), a pass turns it into g in bf16 in place, and g is the
+// operand of dh and dW.  Otherwise (more, or a gradient for every token's
 // loss) the backward forms z again for a run of classes at a time, with g as the
 // epilogue: dh is added up over the runs in fp32, of dW a run has its rows.  g is
 // rounded to bf16 (2^-9 of each value, as the results themselves are); all sums are
@@ -85,6 +86,9 @@ struct Product {
   int grad_step;
   const float* count;      // nullptr, or what grad is divided by
 };
+
+// What the exponentials, 1 at most, are stored times.
+constexpr float kExpsUp = 32768.0f;
 
 // kStats: parts of the losses; kExps: those and the exponentials; kGrad: g.
 enum Epilogue { kBf16, kFp32, kStats, kExps, kGrad };
@@ -321,7 +325,8 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int c = 4 * (x & 1) + q;
-            *reinterpret_cast<uint2*>(own + col * 128 + ((c ^ swz) << 4) + half * 8) = value(x, y, q);
+            *reinterpret_cast<uint2*>(own + col * 128 + ((c ^ swz) << 4) + half * 8) =
+                value(x, y, q);
           }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -405,7 +410,8 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
     if constexpr (STATS) {
       // maxima and sums of the two waves along m meet in their own LDS, [64] each
       float* const mine = reinterpret_cast<float*>(own + 1024);
-      const float* const other = reinterpret_cast<const float*>(spare + (wave ^ 1) * PRIVATE + 1024);
+      const float* const other =
+          reinterpret_cast<const float*>(spare + (wave ^ 1) * PRIVATE + 1024);
       int rel[2];
 #pragma unroll
       for (int y = 0; y < S::NB; ++y) rel[y] = place_of(u, token_of(u, y, col).target, half);
@@ -476,7 +482,8 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
         sync_lds();
         store_rows(u, u.m0 + T, lane, [&](int x, int y, int q) {
           const v16f& e = acc[x][y];
-          return make_uint2(half2(e[4 * q], e[4 * q + 1]), half2(e[4 * q + 2], e[4 * q + 3]));
+          return make_uint2(half2(e[4 * q] * kExpsUp, e[4 * q + 1] * kExpsUp),
+                            half2(e[4 * q + 2] * kExpsUp, e[4 * q + 3] * kExpsUp));
         });
       }
     }
@@ -608,7 +615,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_losses_kernel(
       float2 p[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        p[j] = i + 32 * j < parts ? part[int64_t(i + 32 * j) * tokens + t] : make_float2(0.0f, 0.0f);
+        p[j] = i + 32 * j < parts ? part[int64_t(i + 32 * j) * tokens + t]
+                                  : make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int j = 0; j < 4; ++j) add(p[j]);
     }
@@ -660,8 +668,8 @@ __global__ void no_tokens_kernel(int mean, float* total, float* count) {
   *count = 0.0f;
 }
 
-// The exponentials of tokens x classes (fp16, rows ld apart, relative to the maxima of
-// their tiles) turned into g (bf16) in place, eight a thread.
+// The exponentials of tokens x classes (fp16, rows ld apart, kExpsUp times those relative
+// to the maxima of their tiles) turned into g (bf16) in place, eight a thread.
 template <int T>
 __global__ __launch_bounds__(256) void exps_to_grad_kernel(
     uint16_t* __restrict__ x, int64_t ld, const float2* __restrict__ part,
@@ -678,7 +686,7 @@ __global__ __launch_bounds__(256) void exps_to_grad_kernel(
   for (int i = 0; i < 4; ++i) {
     const int64_t v0 = (int64_t(blockIdx.x) * 128 + i * 32 + threadIdx.x % 32) * 8;
     if (v0 >= classes) return;
-    const float f = exp2_fast(part[v0 / T * tokens + t].x - l) * c;
+    const float f = exp2_fast(part[v0 / T * tokens + t].x - l) * (c / kExpsUp);
     uint4* p = reinterpret_cast<uint4*>(x + int64_t(t) * ld + v0);
     typedef _Float16 v8h __attribute__((ext_vector_type(8)));
     const v8h e = __builtin_bit_cast(v8h, *p);
@@ -914,6 +922,7 @@ int losses_of(const Head& h, float* losses, float* lse, int mean, float* total, 
   double* sums = total ? reinterpret_cast<double*>(ws) : nullptr;
   p.done = reinterpret_cast<int*>(ws + align256(size_t(blocks) * 16));
   const bool last = blocks <= kJoinLast;
+  if (!grid_x_fits(blocks, kJoinThreads)) return TCFP_ERR_SHAPE;
   const int rc = exps ? launch_cut<false, false, kExps>(cut, p, st)
                       : launch_cut<false, false, kStats>(cut, p, st);
   if (rc != TCFP_OK) return rc;
