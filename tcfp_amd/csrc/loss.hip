@@ -2,8 +2,12 @@
 // gradients (gfx950).
 //
 //   z = h W^T,  lse = log sum exp z,  loss = lse - z[target]
-//   g = (softmax(z) - onehot(target)) * grad,  dh = g W,  dW = g^T h
+//   g = (softmax(z) - onehot(target)) * grad / unit,  dh = unit g W,  dW = unit g^T h
 //
+// (unit: the gradient of a sum, that of a mean over the tokens that count, or the
+// largest of all tokens'.  With it in g, every g of a target would be the same number
+// near -unit, whose rounding to bf16 all tokens' gradients would share: 3.6e-3 off
+// where the results' own rounding is 1.7e-3.)
 // h [tokens, dim] and W [vocab, dim] are bf16.  Forward: one product whose epilogue
 // reduces every 256 (128) classes of a token to their maximum and sum of
 // exponentials, which a small launch joins; z is not stored.
@@ -82,10 +86,13 @@ struct Product {
   float* picked;     // [n]: z of the target
   int* done;         // cleared for the launch that joins the parts
   const float* lse;
-  const float* grad;       // one a token (grad_step 1) or for all (0)
-  int grad_step;
-  const float* count;      // nullptr, or what grad is divided by
+  const float* grad;       // nullptr, or one a token, divided by *up
+  const float *up, *over;  // unit is *up / *over, nullptr: 1 (bf16 results are times unit)
 };
+TCFP_DEV float unit_of(const float* up, const float* over) {
+  const float u = up ? *up : 1.0f, o = over ? *over : 1.0f;
+  return o == 0.0f ? 0.0f : u / o;  // (no tokens that count: no gradients)
+}
 
 // What the exponentials, 1 at most, are stored times.
 constexpr float kExpsUp = 32768.0f;
@@ -187,6 +194,9 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
   uint8_t* const own = spare + wave * PRIVATE;
   if (STATS && blockIdx.x == 0 && threadIdx.x == 0) *g.done = 0;
 
+  // (kept in a scalar register)
+  const float unit = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(
+      EPI == kBf16 ? unit_of(g.up, g.over) : EPI == kGrad && g.grad ? *g.up : 1.0f)));
   Copies<T, TA> ca;
   Copies<T, TB> cb;
   ca.init(wave, lane, g.lda);
@@ -270,7 +280,7 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
       copy4(t, 2 * lane4 + 4, to + 256);
       if constexpr (EPI == kGrad) {
         copy4(make_rsrc(g.lse + n, uint32_t(there) * 4), lane4, to + 512);
-        copy4(make_rsrc(g.grad + n, g.grad_step ? uint32_t(there) * 4 : 0u), lane4, to + 768);
+        copy4(make_rsrc(g.grad + n, g.grad ? uint32_t(there) * 4 : 0u), lane4, to + 768);
       }
     }
   };
@@ -286,14 +296,14 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
                          uint64_t(*reinterpret_cast<const uint32_t*>(p + 256)) << 32);
       if constexpr (EPI == kGrad) {
         t.lse = *reinterpret_cast<const float*>(p + 512);
-        t.grad = g.grad_step ? *reinterpret_cast<const float*>(p + 768) : *g.grad;
+        t.grad = g.grad ? *reinterpret_cast<const float*>(p + 768) : 1.0f;
       }
     } else {
       const int64_t n = min(u.n0 + nw + 32 * y + col, g.n - 1);
       t.target = g.targets[n];
       if constexpr (EPI == kGrad) {
         t.lse = g.lse[n];
-        t.grad = g.grad[n * g.grad_step];
+        t.grad = g.grad ? g.grad[n] : 1.0f;
       }
     }
     return t;
@@ -373,7 +383,8 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
     if constexpr (EPI == kBf16)
       store_rows(u, g.m, lane, [&](int x, int y, int q) {
         const v16f& e = acc[x][y];
-        return make_uint2(pack2(e[4 * q], e[4 * q + 1]), pack2(e[4 * q + 2], e[4 * q + 3]));
+        return make_uint2(pack2(e[4 * q] * unit, e[4 * q + 1] * unit),
+                          pack2(e[4 * q + 2] * unit, e[4 * q + 3] * unit));
       });
     if constexpr (EPI == kGrad) {
       // (of g and the exponentials whole tiles are written: what lies behind the classes
@@ -386,7 +397,7 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
         const Token t = token_of(u, y, col);
         keep[y] = t.target != g.ignore;
         rel[y] = place_of(u, t.target, half);
-        scale[y] = g.count ? t.grad / *g.count : t.grad;
+        scale[y] = g.grad ? t.grad / unit : 1.0f;
         // (a target outside the vocabulary has a loss that is NaN, and so are its
         // gradients)
         if (t.target < 0 || t.target >= g.classes) scale[y] = NAN;
@@ -674,13 +685,12 @@ template <int T>
 __global__ __launch_bounds__(256) void exps_to_grad_kernel(
     uint16_t* __restrict__ x, int64_t ld, const float2* __restrict__ part,
     const float* __restrict__ lse, const int64_t* __restrict__ targets, int64_t ignore,
-    int64_t classes, int tokens, const float* __restrict__ count) {
+    int64_t classes, int tokens) {
   const int t = int(blockIdx.y) * 8 + threadIdx.x / 32;
   if (t >= tokens) return;
   const int64_t target = targets[t];
   const bool keep = target != ignore;
-  float c = count ? 1.0f / *count : 1.0f;
-  if (target < 0 || target >= classes) c = NAN;  // (as its loss)
+  const float c = target < 0 || target >= classes ? NAN : 1.0f;  // (as its loss)
   const float l = lse[t] * kLog2e;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -722,10 +732,29 @@ __global__ __launch_bounds__(256) void scale_kernel(uint16_t* a, int64_t a_eight
   }
 }
 
-// out = the sum of `splits` fp32 [n, m] arrays in bf16, in order; eight columns a
-// thread.
+// The largest of the tokens' gradients that is finite; 1 if that is 0.
+__global__ __launch_bounds__(1024) void largest_kernel(const float* __restrict__ grad, int tokens,
+                                                       float* unit) {
+  __shared__ float s[16];
+  float top = 0.0f;
+  for (int64_t i = threadIdx.x; i < tokens; i += 1024) {
+    const float x = fabsf(grad[i]);
+    if (x < INFINITY) top = fmaxf(top, x);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (threadIdx.x % 64 == 0) s[threadIdx.x / 64] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+  *unit = top == 0.0f ? 1.0f : top;
+}
+
+// out = the sum of `splits` fp32 [n, m] arrays times unit in bf16, in order; eight
+// columns a thread.
 __global__ __launch_bounds__(256) void round_sum_kernel(const float* __restrict__ part, int splits,
                                                         int64_t stride, int64_t eights,
+                                                        const float* up, const float* over,
                                                         uint16_t* __restrict__ out) {
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (i >= eights) return;
@@ -736,6 +765,9 @@ __global__ __launch_bounds__(256) void round_sum_kernel(const float* __restrict_
     v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
     v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
   }
+  const float unit = unit_of(up, over);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] *= unit;
   reinterpret_cast<uint4*>(out)[i] =
       make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
 }
@@ -934,19 +966,21 @@ int losses_of(const Head& h, float* losses, float* lse, int mean, float* total, 
   return launch_status();
 }
 
-int round_sum(const float* part, int splits, int64_t values, void* out, hipStream_t st) {
+int round_sum(const float* part, int splits, int64_t values, const float* up, const float* over,
+              void* out, hipStream_t st) {
   const int64_t eights = values / 8, blocks = ceil_div(eights, 256);
   if (!grid_x_fits(blocks, 256)) return TCFP_ERR_SHAPE;
-  round_sum_kernel<<<unsigned(blocks), 256, 0, st>>>(part, splits, values, eights,
+  round_sum_kernel<<<unsigned(blocks), 256, 0, st>>>(part, splits, values, eights, up, over,
                                                      static_cast<uint16_t*>(out));
   return launch_status();
 }
 
 // What g of the classes [v0, v0 + classes) gives: their rows of dW, and their part of
-// dh (into sum_h where the layout has it: added up over the runs).
+// dh (into sum_h where the layout has it: added up over the runs, and not yet times
+// unit).
 int products_of(const Head& h, const Layout& l, const uint16_t* g, int64_t v0, int64_t classes,
-                void* grad_hidden, void* grad_weight, float* sum_h, float* sum_w,
-                hipStream_t st) {
+                const float* up, const float* over, void* grad_hidden, void* grad_weight,
+                float* sum_h, float* sum_w, hipStream_t st) {
   if (grad_hidden) {
     // dh[t][d] += sum over the classes of g[t][v] W[v][d]
     Product q{};
@@ -969,6 +1003,8 @@ int products_of(const Head& h, const Layout& l, const uint16_t* g, int64_t v0, i
       done = launch_cut<true, false, kFp32>(cut, q, st);
     } else {
       q.out = grad_hidden;
+      q.up = up;
+      q.over = over;
       done = launch_cut<true, false, kBf16>(l.dh, q, st);
     }
     if (done != TCFP_OK) return done;
@@ -987,12 +1023,16 @@ int products_of(const Head& h, const Layout& l, const uint16_t* g, int64_t v0, i
   uint16_t* out = static_cast<uint16_t*>(grad_weight) + v0 * h.dim;
   if (l.dw.splits == 1) {
     q.out = out;
+    q.up = up;
+    q.over = over;
     return launch_cut<true, true, kBf16>(l.dw, q, st);
   }
   q.out = sum_w;
   q.split_stride = classes * h.dim;
   const int done = launch_cut<true, true, kFp32>(l.dw, q, st);
-  return done != TCFP_OK ? done : round_sum(sum_w, l.dw.splits, classes * h.dim, out, st);
+  return done != TCFP_OK
+             ? done
+             : round_sum(sum_w, l.dw.splits, classes * h.dim, up, over, out, st);
 }
 
 }  // namespace
@@ -1059,16 +1099,17 @@ int tcfp_linear_cross_entropy_train(const void* hidden, int64_t ldh, const void*
   const float* each = mean ? count : nullptr;
   if (logits_cut(tokens, vocab, dim).tile == 256)
     exps_to_grad_kernel<256><<<grid, 256, 0, st>>>(g, l.run, part, lse, targets, ignore, vocab,
-                                                   int(tokens), each);
+                                                   int(tokens));
   else
     exps_to_grad_kernel<128><<<grid, 256, 0, st>>>(g, l.run, part, lse, targets, ignore, vocab,
-                                                   int(tokens), each);
+                                                   int(tokens));
   if (launch_status() != TCFP_OK) return TCFP_ERR_HIP;
-  done = products_of(head, l, g, 0, vocab, grad_hidden, grad_weight,
+  done = products_of(head, l, g, 0, vocab, nullptr, each, grad_hidden, grad_weight,
                      reinterpret_cast<float*>(ws + l.g),
                      reinterpret_cast<float*>(ws + l.g + l.sum_h), st);
   if (done != TCFP_OK || !l.sum_h) return done;
-  return round_sum(reinterpret_cast<float*>(ws + l.g), l.dh.splits, tokens * dim, grad_hidden, st);
+  return round_sum(reinterpret_cast<float*>(ws + l.g), l.dh.splits, tokens * dim, nullptr, each,
+                   grad_hidden, st);
 }
 
 int tcfp_scale_bf16(void* a, int64_t a_values, void* b, int64_t b_values, const float* by,
@@ -1088,7 +1129,7 @@ size_t tcfp_linear_cross_entropy_backward_workspace_bytes(int64_t tokens, int64_
                                                           int need_weight) {
   if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
   const Layout l = layout_of(tokens, vocab, dim, need_hidden != 0, need_weight != 0);
-  return l.g + l.sum_h + l.sum_w;
+  return l.g + l.sum_h + l.sum_w + 256;  // (and unit)
 }
 
 int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const void* weight,
@@ -1109,33 +1150,40 @@ int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const vo
       const int64_t eights = vocab * dim / 8;
       if (!grid_x_fits(ceil_div(eights, 256), 256)) return TCFP_ERR_SHAPE;
       round_sum_kernel<<<unsigned(ceil_div(eights, 256)), 256, 0, st>>>(
-          nullptr, 0, 0, eights, static_cast<uint16_t*>(grad_weight));
+          nullptr, 0, 0, eights, nullptr, nullptr, static_cast<uint16_t*>(grad_weight));
     }
     return launch_status();
   }
   const Layout l = layout_of(tokens, vocab, dim, need_h, need_w);
-  if (!workspace || workspace_bytes < l.g + l.sum_h + l.sum_w || !aligned16(workspace))
+  if (!workspace || workspace_bytes < l.g + l.sum_h + l.sum_w + 256 || !aligned16(workspace))
     return TCFP_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint16_t* g = reinterpret_cast<uint16_t*>(ws);
   float* sum_h = reinterpret_cast<float*>(ws + l.g);
   float* sum_w = reinterpret_cast<float*>(ws + l.g + l.sum_h);
   const Head head{hidden, ldh, weight, ldw, targets, ignore, tokens, vocab, dim};
+  const float* up = grad;
+  if (grad_step == 1) {
+    float* largest = reinterpret_cast<float*>(ws + l.g + l.sum_h + l.sum_w);
+    largest_kernel<<<1, 1024, 0, st>>>(grad, int(tokens), largest);
+    up = largest;
+  }
   for (int64_t v0 = 0; v0 < vocab; v0 += l.run) {
     const int64_t classes = std::min(l.run, vocab - v0);
     Product p = head_product(head, v0, classes);
     p.out = g;
     p.ldo = l.run;
     p.lse = lse;
-    p.grad = grad;
-    p.grad_step = int(grad_step);
-    p.count = count;
+    p.grad = grad_step == 1 ? grad : nullptr;
+    p.up = up;
     int done = launch_cut<false, false, kGrad>(logits_cut(tokens, classes, dim), p, st);
     if (done == TCFP_OK)
-      done = products_of(head, l, g, v0, classes, grad_hidden, grad_weight, sum_h, sum_w, st);
+      done = products_of(head, l, g, v0, classes, up, count, grad_hidden, grad_weight, sum_h,
+                         sum_w, st);
     if (done != TCFP_OK) return done;
   }
-  if (need_h && l.sum_h) return round_sum(sum_h, l.dh.splits, tokens * dim, grad_hidden, st);
+  if (need_h && l.sum_h)
+    return round_sum(sum_h, l.dh.splits, tokens * dim, up, count, grad_hidden, st);
   return TCFP_OK;
 }
 

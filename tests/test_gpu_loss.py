@@ -356,6 +356,34 @@ def test_large_logits(dev):
     within(L.linear_cross_entropy(h, w, t, reduction="none"), e.losses, e.losses_tol, "losses")
 
 
+@pytest.mark.parametrize("how", ["mean", "sum", "again", "each"])
+@pytest.mark.parametrize("tokens,d,vocab", [(255, 64, 3000), (255, 1024, 300)])
+def test_tokens_do_not_share_a_rounding(dev, tokens, d, vocab, how):
+    """1 / 255 lies half a step of bf16 from the nearest value: a factor that is rounded
+    with every target's gradient would be 2^-8 off for all of them.  The results' own
+    rounding is 2^-8 / sqrt(12) to 2^-8 / sqrt(3) of them, 1.7e-3 for even mantissas, and
+    the other factors' average out; the target's probability less 1 is off by 2^-9 at most."""
+    h, w, t = inputs(dev, tokens, d, vocab, seed=19)
+    hg, wg = h.clone().requires_grad_(), w.clone().requires_grad_()
+    factor = torch.full((), 1 / 255, device=dev)
+    if how in ("mean", "again"):
+        out = L.linear_cross_entropy(hg, wg, t)
+        if how == "again":
+            torch.autograd.grad(out, (hg, wg), retain_graph=True)
+        got = torch.autograd.grad(out, (hg, wg))
+    elif how == "sum":
+        out = L.linear_cross_entropy(hg, wg, t, reduction="sum")
+        torch.autograd.grad(out, (hg, wg), retain_graph=True)
+        got = torch.autograd.grad(out, (hg, wg), factor)
+    else:
+        out = L.linear_cross_entropy(hg, wg, t, reduction="none")
+        got = torch.autograd.grad(out, (hg, wg), factor.expand(tokens))
+    e = Exact(h, w, t, torch.full((tokens,), 1 / 255))
+    for x, want in zip(got, (e.dh, e.dw)):
+        off = (x.double().cpu() - want).norm() / want.norm()
+        assert off <= 2.6e-3, float(off)
+
+
 @pytest.mark.parametrize("reduction", ["sum", "none"])
 @pytest.mark.parametrize("tokens", [40, 600])
 def test_rare_classes_keep_their_gradients(dev, tokens, reduction):
