@@ -66,7 +66,8 @@ def packed_attention(
 
     ``max_len`` and ``max_key_len`` (``max_len`` by default, with ``key_start`` all
     keys) bound the sequences' lengths and size the launches; lengths past them are
-    answered rightly, only slower.
+    answered rightly, only slower.  Where both are at most 256 the gradients of q and k
+    are formed from more bits.
 
     Differentiable in q, k and v, once; results and gradients do not depend on the
     launches' timing.

@@ -6,8 +6,9 @@
 //
 // All operands are bf16; scores, maxima, sums, the row statistic L = log2 sum
 // 2^S and every accumulator are fp32.  P and dS are rounded to bf16 on their way
-// into the second products (2^-9 of each value, as the results are rounded
-// themselves).  No P is stored: the backward forms it again from L.
+// into the second products (2^-8 of each value at most, as the results are rounded
+// themselves), of short sequences what dS's rounding left is multiplied too (see
+// kShort).  No P is stored: the backward forms it again from L.
 //
 // Every product runs transposed so that what one leaves in the registers is what
 // the next one wants of the lane (the matrix instruction's columns are the
@@ -32,6 +33,12 @@ using namespace tcfp;
 namespace {
 
 constexpr int kStep = 64;  // rows of a tile in LDS
+// Where no sequence has more rows than this, dQ and dK take dS as two bf16, its rounding
+// and what that left: 1.7e-3 off, as the results' rounding, instead of 2.4e-3 (32
+// sequences of 128 tokens, 4 heads of 64: a backward pass of 18.5 us instead of 17.7,
+// less than its launches take the host).  For long ones the product more would be a
+// sixth of the pass.
+constexpr int kShort = 256;
 
 struct Packed {
   const uint16_t *q, *k, *v, *go;  // [tokens, heads, dim], [keys, kv_heads, dim]
@@ -184,6 +191,13 @@ TCFP_DEV v8bf pack8(const v16f& e, int z) {
   const v4i w = {int(pack2(e[z], e[z + 1])), int(pack2(e[z + 2], e[z + 3])),
                  int(pack2(e[z + 4], e[z + 5])), int(pack2(e[z + 6], e[z + 7]))};
   return __builtin_bit_cast(v8bf, w);
+}
+// What that rounding left.
+TCFP_DEV v8bf pack8_low(const v16f& e, int z, const v8bf& high) {
+  v16f rest;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) rest[j] = e[z + j] - float(high[j]);
+  return pack8(rest, 0);
 }
 TCFP_DEV v16f zeros() {
   v16f z;
@@ -355,7 +369,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_forward_kern
 //
 // As forward, with dO beside Q in registers; a step's two runs of 32 keys one after
 // the other.
-template <int D, int NW>
+template <int D, int NW, bool SHORT>
 __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dq_kernel(Packed a) {
   constexpr int TILE = kTileBytes<D>;
   __shared__ __align__(16) uint8_t lds[4 * TILE];
@@ -448,6 +462,12 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dq_kernel(Pa
 #pragma unroll
           for (int i = 0; i < D / 32; ++i)
             dq[i] = mfma(by_columns<D>(lds, kt_off, i, 32 * x + 16 * y), ds, dq[i]);
+          if constexpr (SHORT) {
+            const v8bf low = pack8_low(e, 8 * y, ds);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+              dq[i] = mfma(by_columns<D>(lds, kt_off, i, 32 * x + 16 * y), low, dq[i]);
+          }
         }
       }
     }
@@ -464,7 +484,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dq_kernel(Pa
 // wave's 256 registers 192 hold its K, V, dK and dV (heads of 128): the phases of 32
 // queries -- S and dP, P and dS, the sums -- are kept apart, and the other workgroup on
 // the CU fills the matrix cores meanwhile.
-template <int D, int NW>
+template <int D, int NW, bool SHORT>
 __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dkv_kernel(Packed a) {
   constexpr int TILE = kTileBytes<D>, STATS = 2 * kStep * 4, BUF = 2 * TILE + STATS;
   __shared__ __align__(16) uint8_t lds[2 * BUF];
@@ -580,6 +600,15 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dkv_kernel(P
             dv[j] = mfma(by_columns<D>(lds + TILE, c_off, j, 16 * y), p[y], dv[j]);
             dk[j] = mfma(by_columns<D>(lds, c_off, j, 16 * y), ds[y], dk[j]);
           }
+        if constexpr (SHORT) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const v8bf low = pack8_low(dp, 8 * y, ds[y]);
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j)
+              dk[j] = mfma(by_columns<D>(lds, c_off, j, 16 * y), low, dk[j]);
+          }
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -715,14 +744,15 @@ int64_t lay_out(Packed& a, int64_t max_len, int64_t rows, int members) {
   return each * a.tiles;
 }
 
-#define TCFP_PACKED(KERNEL, GRID)                                                       \
-  do {                                                                                  \
-    const int64_t n_ = GRID;                                                            \
-    if (n_ > INT32_MAX || !grid_x_fits(n_, 64 * kWaves)) return TCFP_ERR_SHAPE;         \
-    if (z.dim == 64) KERNEL<64, kWaves><<<unsigned(n_), 64 * kWaves, 0, st>>>(a);       \
-    else if (z.dim == 128) KERNEL<128, kWaves><<<unsigned(n_), 64 * kWaves, 0, st>>>(a); \
-    else KERNEL<256, kWaves><<<unsigned(n_), 64 * kWaves, 0, st>>>(a);                  \
-    if (launch_status() != TCFP_OK) return TCFP_ERR_HIP;                                \
+#define TCFP_PACKED(GRID, KERNEL, ...)                                                      \
+  do {                                                                                      \
+    const int64_t n_ = GRID;                                                                \
+    if (n_ > INT32_MAX || !grid_x_fits(n_, 64 * kWaves)) return TCFP_ERR_SHAPE;             \
+    const unsigned g_ = unsigned(n_), t_ = 64 * kWaves;                                     \
+    if (z.dim == 64) KERNEL<64, kWaves __VA_ARGS__><<<g_, t_, 0, st>>>(a);                  \
+    else if (z.dim == 128) KERNEL<128, kWaves __VA_ARGS__><<<g_, t_, 0, st>>>(a);           \
+    else KERNEL<256, kWaves __VA_ARGS__><<<g_, t_, 0, st>>>(a);                             \
+    if (launch_status() != TCFP_OK) return TCFP_ERR_HIP;                                    \
   } while (0)
 
 }  // namespace
@@ -756,7 +786,7 @@ int tcfp_packed_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   a.low = out_low;
   a.lse = lse;
   const auto st = static_cast<hipStream_t>(stream);
-  TCFP_PACKED(packed_forward_kernel, lay_out(a, max_len, tokens, a.group));
+  TCFP_PACKED(lay_out(a, max_len, tokens, a.group), packed_forward_kernel);
   return TCFP_OK;
 }
 
@@ -812,10 +842,17 @@ int tcfp_packed_attention_backward(
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                     align256(size_t(tokens) * size_t(heads) * 4));
   const auto st = static_cast<hipStream_t>(stream);
-  if (tokens > 0) TCFP_PACKED(packed_dq_kernel, lay_out(a, max_len, tokens, a.group));
+  const bool brief = std::max(max_len, max_key_len) <= kShort;
+  if (tokens > 0) {
+    const int64_t grid = lay_out(a, max_len, tokens, a.group);
+    if (brief) TCFP_PACKED(grid, packed_dq_kernel, , true);
+    else TCFP_PACKED(grid, packed_dq_kernel, , false);
+  }
   if (keys > 0) {
     a.parts = parts_of(keys, batch, max_key_len, kv_heads, a.group, dim);
-    TCFP_PACKED(packed_dkv_kernel, lay_out(a, max_key_len, keys, a.parts));
+    const int64_t grid = lay_out(a, max_key_len, keys, a.parts);
+    if (brief) TCFP_PACKED(grid, packed_dkv_kernel, , true);
+    else TCFP_PACKED(grid, packed_dkv_kernel, , false);
     if (a.parts > 1) {
       const int64_t eights = keys * kv_heads * dim / 8, blocks = ceil_div(eights, 256);
       if (!grid_x_fits(blocks, 256)) return TCFP_ERR_SHAPE;
