@@ -843,9 +843,10 @@ int tcfp_scale_bf16(void* a, int64_t a_values, void* b, int64_t b_values, const 
  * (/ *count, if count is not NULL), 0 for an ignored token;
  *   grad_hidden = g weight, grad_weight = g^T hidden,
  * bf16, contiguous, either may be NULL.  grad_step is 1 (a gradient a token) or 0
- * (one for all, of a sum, or with count of a mean).  z is formed again, for a run
- * of classes at a time whose g, rounded to bf16, takes at most 256 MiB of the
- * workspace; sums are f32.  hidden is read for ignored tokens too: a value that is
+ * (one for all, of a sum, or with count of a mean; a count of 0 gives zeros).  z is
+ * formed again, for a run of classes at a time whose g, rounded to bf16 before what
+ * all its tokens share is multiplied, takes at most 256 MiB of the workspace; sums are
+ * f32.  hidden is read for ignored tokens too: a value that is
  * not finite there reaches grad_weight. */
 size_t tcfp_linear_cross_entropy_backward_workspace_bytes(int64_t tokens, int64_t vocab,
                                                           int64_t dim, int need_hidden,

@@ -177,3 +177,47 @@ def test_the_example_serves_what_it_trains_with_turns(dev, example):
     assert rel(a, full) < 0.1
     with pytest.raises(ValueError, match="256 positions"):
         server.step(seqs, [[1] * 217, [1], [1]])
+
+
+def test_a_captured_step(dev):
+    """Forward and backward through all three in one graph: every replay is the eager
+    step, bit for bit, also between eager steps, and as the sequences change."""
+    heads, kv_heads, dim, vocab = 4, 2, 64, 300
+    lens = (130, 1, 69)
+    tokens = sum(lens)
+    g = torch.Generator().manual_seed(31)
+    x0 = torch.randn(tokens, (heads + 2 * kv_heads) * dim, generator=g).to(BF16).to(dev)
+    w0 = (torch.randn(vocab, heads * dim, generator=g) / 16).to(BF16).to(dev)
+    targets = torch.randint(0, vocab, (tokens,), generator=g).to(dev)
+    at = torch.tensor([0, 130, 131, 200], dtype=torch.int32, device=dev)
+    pos = torch.arange(tokens, device=dev)
+    freqs = rotary_frequencies(dim, device=dev)
+    by = torch.full((), 0.3, device=dev)
+
+    def step(x, w):
+        x, w = x.detach().requires_grad_(), w.detach().requires_grad_()  # (sharing memory)
+        q, k, v = x.unflatten(1, (-1, dim)).split((heads, kv_heads, kv_heads), 1)
+        q, k = rotary_embedding(q, k, pos, freqs)
+        y = packed_attention(q, k, v, at, max_len=tokens)
+        loss = linear_cross_entropy(y.flatten(1), w, targets)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w), by))
+
+    x, w = x0.clone(), w0.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = step(x, w)
+    for i, starts in enumerate(([0, 130, 131, 200], [0, 10, 190, 200], [0, 0, 200, 200])):
+        x.copy_(x0 * (1 + i / 4))
+        w.copy_(w0 * (1 - i / 4))
+        at.copy_(torch.tensor(starts, dtype=torch.int32))
+        want = step(x, w)
+        torch.cuda.synchronize()
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
