@@ -221,3 +221,65 @@ def test_a_captured_step(dev):
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def room(gib):
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"needs {gib} GiB of GPU memory")
+
+
+def test_attention_past_32_bits(dev):
+    """More than 2^32 values of q: its last sequence as if it were alone (the others are
+    zeros), turned and attended, with gradients."""
+    room(90)
+    heads, dim, n, tokens = 128, 128, 200, 270000
+    g = torch.Generator(device=dev).manual_seed(41)
+    part = [torch.randn(n, h, dim, device=dev, dtype=BF16, generator=g) for h in (heads, 1, 1, heads)]
+    pos = torch.arange(tokens, device=dev) % 4000
+    freqs = rotary_frequencies(dim, device=dev)
+
+    def run(q, k, v, go, pos, starts):
+        q, k, v = (x.requires_grad_() for x in (q, k, v))
+        a, b = rotary_embedding(q, k, pos, freqs)
+        at = torch.tensor(starts, dtype=torch.int32, device=dev)
+        o = packed_attention(a, b, v, at, max_len=n, window=64)
+        return (o.detach()[-n:], *(x[-n:] for x in torch.autograd.grad(o, (q, k, v), go)))
+
+    whole = []
+    for x in part:
+        whole.append(torch.zeros(tokens, *x.shape[1:], dtype=BF16, device=dev))
+        whole[-1][-n:] = x
+    assert whole[0].numel() > 2**32
+    got = run(*whole, pos, [*range(0, tokens - n + 1, n), tokens])
+    want = run(*part, pos[-n:], [0, n])
+    for x, y in zip(got, want):
+        # (how many parts a group's heads make is by the number of tiles)
+        torch.testing.assert_close(x, y, rtol=3 * 2.0**-8, atol=2e-4 * float(y.abs().max()))
+
+
+def test_loss_past_32_bits(dev):
+    """More than 2^32 values of the hidden states, in a row and with gradients; the last
+    tokens as if they were alone (the others are left out)."""
+    room(60)
+    tokens, d, vocab, n = 2_200_000, 2048, 96, 500
+    g = torch.Generator(device=dev).manual_seed(42)
+    part = torch.randn(n, d, device=dev, dtype=BF16, generator=g)
+    w = (torch.randn(vocab, d, device=dev, generator=g) / 32).to(BF16)
+    targets = torch.randint(0, vocab, (n,), device=dev, generator=g)
+    h = torch.zeros(tokens, d, dtype=BF16, device=dev)
+    h[-n:] = part
+    t = torch.full((tokens,), -100, device=dev)
+    t[-n:] = targets
+    assert h.numel() > 2**32
+
+    def run(h, w, t):
+        h, w = h.requires_grad_(), w.detach().requires_grad_()
+        loss = linear_cross_entropy(h, w, t)
+        dh, dw = torch.autograd.grad(loss, (h, w))
+        return loss.detach(), dh[-n:], dw
+
+    got, want = run(h, w, t), run(part, w, targets)
+    assert abs(float(got[0] - want[0])) <= 2.0**-20 * float(want[0])
+    # (alone the logits' gradients come from fp16: each side's roundings, a sum's order)
+    for x, y in zip(got[1:], want[1:]):
+        assert rel(x, y) <= 4 * 2.0**-8
