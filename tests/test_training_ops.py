@@ -138,7 +138,8 @@ def test_workspaces():
     # a whole pass within 1 GiB
     for tokens in (1, 100, 8192, 100000, 400000):
         for vocab in (256, 50001, 1 << 20, 5 << 20):
-            assert back(tokens, vocab, 64, 0, 0) <= max(256 << 20, 512 * tokens)
+            # (and 256 bytes, of which one float holds what all gradients are divided by)
+            assert back(tokens, vocab, 64, 0, 0) <= max(256 << 20, 512 * tokens) + 256
             assert train(tokens, vocab, 64, 0, 0) <= (1 << 30) + (1 << 28)  # (parts, sums)
     packed = lib.tcfp_packed_attention_backward_workspace_bytes
     assert packed(100, 100, 0, 100, 4, 2, 64) == packed(100, 100, 1, 100, 4, 3, 64) == 0
