@@ -4,10 +4,12 @@ gradients, without storing the logits (HIP, gfx950; no reference counterpart).
 The head of a language model multiplies the last hidden states with a weight of
 one row a class; its logits, tokens x classes, are the largest matrix of a
 training step.  Here the product's own epilogue reduces them to each token's
-maximum and sum of exponentials, and the backward pass forms them again, a run of
-classes at a time: memory beside the inputs and gradients stays bounded (the
-backward's workspace: 256 MiB for the run's gradients of the logits, and fp32
-sums of the hidden states' gradient).
+maximum and sum of exponentials.  The gradients of a sum or mean are made in the
+same call, from exponentials in 16 bits that take at most 1 GiB of workspace while it
+runs; where they would take more, and for gradients of every token's loss, the
+backward pass forms the logits again, a run of classes at a time (256 MiB for the
+run's gradients, and fp32 sums of the hidden states').  Memory beside the inputs and
+gradients stays bounded either way.
 
 Every op runs on the tensors' GPU and current stream; there is no CPU path.
 """
