@@ -1408,6 +1408,13 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return std::any_of(ts.begin(), ts.end(),
                      [](const Tensor* t) { return t->defined() && t->requires_grad(); });
 }
+// Of a tensor with a tangent the plain op would make a result without one, and it has no
+// rule to make it by: refused, whatever requires_grad and the grad mode say.
+void no_tangents(std::initializer_list<const Tensor*> ts, const char* what) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined())
+      runtime_error(std::string(what) + " has no forward-mode derivative");
+}
 // Runs a backward's op; what it raises becomes an error that the autograd engine
 // hands to the caller.
 template <typename F>
@@ -1468,6 +1475,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
 
 Outs rotary_with_grad(const Tensor& q, const OptT& k, const Tensor& positions, const Tensor& freqs,
                       bool interleaved, double amplitude, bool inverse) {
+  no_tangents({&q, &opt(k)}, "rotary_embedding");
   if (!wants_grad({&q, &opt(k)}))
     return rotary(q, k, positions, freqs, interleaved, amplitude, inverse);
   Outs o{RotaryNode::apply(q, k, positions, freqs, interleaved, amplitude, inverse)};
@@ -1511,6 +1519,7 @@ Tensor packed_attention_with_grad(const Tensor& q, const Tensor& k, const Tensor
                                   const Tensor& starts, const OptT& key_starts, int64_t max_len,
                                   std::optional<int64_t> max_key_len, std::optional<double> scale,
                                   bool causal, int64_t window) {
+  no_tangents({&q, &k, &v}, "packed_attention");
   if (max_key_len && *max_key_len < 0)
     value_error("max_len and max_key_len must not be negative");
   if (!wants_grad({&q, &k, &v}))
@@ -1592,6 +1601,7 @@ struct LossNode : torch::autograd::Function<LossNode> {
 Tensor linear_cross_entropy_with_grad(const Tensor& hidden, const Tensor& weight,
                                       const Tensor& targets, int64_t ignore, bool reduce,
                                       bool mean) {
+  no_tangents({&hidden, &weight}, "linear_cross_entropy");
   if (wants_grad({&hidden, &weight}))
     return LossNode::apply(hidden, weight, targets, ignore, reduce, mean);
   const Outs o = linear_cross_entropy(hidden, weight, targets, ignore, reduce, mean);
