@@ -344,6 +344,11 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_forward_kern
     l += other_half(l);
     if (r0 + 32 * wave + col <= last) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      // (nothing is seen: a weight of 0 times what others' values hold may be NaN)
+      if (l == 0.0f) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) o[i] = zeros();
+      }
       const int64_t at_row = (int64_t(s.q0 + row) * a.heads + head) * D;
       store_row<D>(a.o + at_row, o, inv, half);
       if (a.low) {
@@ -470,6 +475,10 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void packed_dq_kernel(Pa
           }
         }
       }
+    }
+    if (lse == INFINITY) {  // (nothing is seen, as forward)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) dq[i] = zeros();
     }
     if (live) store_row<D>(a.dq + hrow * D, dq, a.scale, half);
     __syncthreads();
