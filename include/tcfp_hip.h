@@ -806,11 +806,12 @@ int tcfp_packed_attention_backward(
  *   hidden [tokens, dim], weight [vocab, dim] bf16, rows ldh / ldw apart
  *   (multiples of 8, 16-byte aligned), dim % 8 == 0.
  * A token whose target is `ignore` has loss 0; one whose target is neither that
- * nor a class has loss NaN.  lse [tokens] f32: log sum exp z.  total and count (both
- * or neither): one f32 each, the sum of the losses, or (mean != 0) their mean over
- * the tokens that are not ignored (NaN if all are), and the number of those; summed
- * in f64 in an order that the sizes fix.  workspace: ..._workspace_bytes, any contents, 16-byte
- * aligned. */
+ * nor a class has loss NaN.  Losses are formed from differences of logits: off by 2^-23
+ * and their own rounding whatever the logits' size, never below 0.  lse [tokens] f32:
+ * log sum exp z.  total and count (both or neither): one f32 each, the sum of the
+ * losses, or (mean != 0) their mean over the tokens that are not ignored (NaN if all
+ * are), and the number of those; summed in f64 in an order that the sizes fix.
+ * workspace: ..._workspace_bytes, any contents, 16-byte aligned. */
 size_t tcfp_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim);
 int tcfp_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                               const int64_t* targets, int64_t ignore, int64_t tokens,
@@ -843,20 +844,22 @@ int tcfp_scale_bf16(void* a, int64_t a_values, void* b, int64_t b_values, const 
  * (/ *count, if count is not NULL), 0 for an ignored token;
  *   grad_hidden = g weight, grad_weight = g^T hidden,
  * bf16, contiguous, either may be NULL.  grad_step is 1 (a gradient a token) or 0
- * (one for all, of a sum, or with count of a mean; a count of 0 gives zeros).  z is
- * formed again, for a run of classes at a time whose g, rounded to bf16 before what
- * all its tokens share is multiplied, takes at most 256 MiB of the workspace; sums are
- * f32.  hidden is read for ignored tokens too: a value that is
- * not finite there reaches grad_weight. */
+ * (one for all, of a sum, or with count of a mean; a count of 0 gives zeros).  losses
+ * [tokens]: the target's softmax(z) - 1 is formed from them, or if NULL from lse, whose
+ * rounding is in it then.  z is formed again, for a run of classes at a time whose g,
+ * rounded to bf16 before what all its tokens share is multiplied, takes at most 256 MiB
+ * of the workspace; sums are f32.  hidden is read for ignored tokens too: a value that
+ * is not finite there reaches grad_weight. */
 size_t tcfp_linear_cross_entropy_backward_workspace_bytes(int64_t tokens, int64_t vocab,
                                                           int64_t dim, int need_hidden,
                                                           int need_weight);
 int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const void* weight,
                                        int64_t ldw, const int64_t* targets, int64_t ignore,
-                                       const float* lse, const float* grad, int64_t grad_step,
-                                       const float* count, int64_t tokens, int64_t vocab,
-                                       int64_t dim, void* grad_hidden, void* grad_weight,
-                                       void* workspace, size_t workspace_bytes, void* stream);
+                                       const float* lse, const float* losses, const float* grad,
+                                       int64_t grad_step, const float* count, int64_t tokens,
+                                       int64_t vocab, int64_t dim, void* grad_hidden,
+                                       void* grad_weight, void* workspace,
+                                       size_t workspace_bytes, void* stream);
 
 /* ---- layout helpers ---------------------------------------------------- */
 

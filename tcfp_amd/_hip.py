@@ -189,8 +189,8 @@ _SIGNATURES = {
     "tcfp_scale_bf16": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _c_void_p],
     "tcfp_linear_cross_entropy_backward_workspace_bytes": [_i64, _i64, _i64, _i32, _i32],
     "tcfp_linear_cross_entropy_backward": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64,
-                                           _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64,
-                                           _i64, _c_void_p, _c_void_p, _c_void_p,
+                                           _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64,
+                                           _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
                                            ctypes.c_size_t, _c_void_p],
     "tcfp_gemm_set_tile_policy": [_i32],
     "tcfp_dual_quantize_set_candidates": [_i32],

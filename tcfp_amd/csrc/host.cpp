@@ -1334,26 +1334,31 @@ Outs linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tens
 }
 
 Outs linear_cross_entropy_backward(const Tensor& grad_, const Tensor& hidden, const Tensor& weight,
-                                   const Tensor& targets, const Tensor& lse_, const OptT& count,
-                                   int64_t ignore, bool need_h, bool need_w) {
+                                   const Tensor& targets, const Tensor& lse_, const OptT& losses_,
+                                   const OptT& count, int64_t ignore, bool need_h, bool need_w) {
   OnGpu g;
   g.add(grad_);
   g.add(hidden);
   g.add(weight);
   g.add(targets);
   g.add(lse_);
+  g.add(losses_);
   g.add(count);
   const c10::DeviceGuard guard(g.device());
   const HeadIn in = head_inputs(hidden, weight, targets);
   if (lse_.scalar_type() != at::kFloat || lse_.numel() != in.h.rows)
     value_error("lse must hold a float32 for each of the " + std::to_string(in.h.rows) +
                 " tokens");
+  if (losses_ && (losses_->scalar_type() != at::kFloat || losses_->numel() != in.h.rows))
+    value_error("losses must hold a float32 for each of the " + std::to_string(in.h.rows) +
+                " tokens");
   if (grad_.scalar_type() != at::kFloat || (grad_.dim() != 0 && grad_.sizes() != targets.sizes()))
     value_error("grad must be one float32, or hold one for each token");
   if (count && (count->scalar_type() != at::kFloat || count->numel() != 1))
     value_error("count must be one float32");
   const bool each = grad_.dim() != 0;
-  const Tensor grad = grad_.contiguous(), lse = lse_.contiguous();
+  const Tensor grad = grad_.contiguous(), lse = lse_.contiguous(),
+               losses = losses_ ? losses_->contiguous() : Tensor();
   Tensor dh, dw;
   if (need_h) dh = g.empty(hidden.sizes(), at::kBFloat16);
   if (need_w) dw = g.empty(weight.sizes(), at::kBFloat16);
@@ -1362,8 +1367,8 @@ Outs linear_cross_entropy_backward(const Tensor& grad_, const Tensor& hidden, co
   Tensor ws = g.empty({int64_t(std::max<size_t>(nb, 16))}, at::kByte);
   check(tcfp_linear_cross_entropy_backward(
             ptr(in.h.t), in.h.ld, ptr(in.w.t), in.w.ld, ptr<int64_t>(in.targets), ignore, f32(lse),
-            f32(grad), each ? 1 : 0, f32(opt(count)), in.h.rows, in.w.rows, in.h.cols, ptr(dh),
-            ptr(dw), ptr(ws), nb, g.stream()),
+            f32(losses), f32(grad), each ? 1 : 0, f32(opt(count)), in.h.rows, in.w.rows, in.h.cols,
+            ptr(dh), ptr(dw), ptr(ws), nb, g.stream()),
         "linear_cross_entropy_backward");
   return outs(dh, dw);
 }
@@ -1559,7 +1564,9 @@ struct LossNode : torch::autograd::Function<LossNode> {
     }
     Outs o = made ? std::move(*made)
                   : linear_cross_entropy(hidden, weight, targets, ignore, reduce, mean);
-    ctx->save_for_backward({hidden, weight, targets, o.t[1], mean ? o.t[3] : Tensor()});
+    // (every token's loss, where it is the caller's: a copy, as the caller may change it)
+    ctx->save_for_backward({hidden, weight, targets, o.t[1], reduce ? o.t[0] : o.t[0].clone(),
+                            mean ? o.t[3] : Tensor()});
     ctx->saved_data["ignore"] = ignore;
     return reduce ? o.t[2] : o.t[0];
   }
@@ -1587,8 +1594,8 @@ struct LossNode : torch::autograd::Function<LossNode> {
     } else {
       got = in_engine([&] {
         const at::NoGradGuard no_grad;
-        return linear_cross_entropy_backward(grads[0], s[0], s[1], s[2], s[3],
-                                             s[4].defined() ? OptT(s[4]) : OptT(),
+        return linear_cross_entropy_backward(grads[0], s[0], s[1], s[2], s[3], s[4],
+                                             s[5].defined() ? OptT(s[5]) : OptT(),
                                              ctx->saved_data["ignore"].toInt(), need_h, need_w);
       });
     }

@@ -12,6 +12,13 @@
 // reduces every 256 (128) classes of a token to their maximum and sum of
 // exponentials, which a small launch joins; z is not stored.
 //
+// Exponentials are of differences from the maximum, formed before they are scaled to
+// powers of two, and the loss is (maximum - z[target]) + log(sum): right to 2^-23 or so
+// whatever the logits' size, and never below 0.  As lse - z[target], with lse rounded, it
+// would be off by 2^-24 of lse: of 30, by 1.8e-6, as much as a confident token's whole
+// loss.  The gradient of the target's logit, p - 1, is formed from the loss as exp(-loss)
+// - 1; other classes' p = exp(z - lse) are off by lse's rounding in proportion only.
+//
 // Gradients, where they are wanted of the losses' sum or mean and tokens x classes
 // take at most 1 GiB of workspace in 16 bits: with the forward, three products in
 // all.  The first one's epilogue leaves 2^15 exp(z - maximum of its tile) in fp16 (11
@@ -82,16 +89,25 @@ struct Product {
   int64_t ignore;
   int64_t first;     // class of m = 0
   int64_t classes;   // of the whole vocabulary
-  float2* part;      // [tiles_m, n]: maximum in units of log2, sum
+  float2* part;      // [tiles_m, n]: maximum, sum
   float* picked;     // [n]: z of the target
   int* done;         // cleared for the launch that joins the parts
   const float* lse;
+  const float* losses;     // nullptr: the target's p - 1 from lse
   const float* grad;       // nullptr, or one a token, divided by *up
   const float *up, *over;  // unit is *up / *over, nullptr: 1 (bf16 results are times unit)
 };
 TCFP_DEV float unit_of(const float* up, const float* over) {
   const float u = up ? *up : 1.0f, o = over ? *over : 1.0f;
   return o == 0.0f ? 0.0f : u / o;  // (no tokens that count: no gradients)
+}
+
+// exp(-loss) - 1, to 2^-22 of itself: below 0.05 by its series, of which the next term is
+// 5e-8.
+TCFP_DEV float less_one(float loss) {
+  const float x = -loss;
+  return loss < 0.05f ? x * (1.0f + x * (0.5f + x * (1.0f / 6 + x * (1.0f / 24))))
+                      : exp2_fast(x * kLog2e) - 1.0f;
 }
 
 // What the exponentials, 1 at most, are stored times.
@@ -269,7 +285,7 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
   // ---- what the epilogue takes of the wave's 64 tokens (the loss's products): target,
   // lse and gradient, brought into the wave's own LDS with the tile's first stages
   // (loaded in the epilogue, each wait for them would wait for the next tile's copies)
-  constexpr int TAKEN = EPI == kGrad ? 4 : STATS ? 2 : 0;
+  constexpr int TAKEN = EPI == kGrad ? 5 : STATS ? 2 : 0;
   const int mw = wm * S::MB * 32, nw = wn * 64;
   auto take = [&](const Unit& u) {
     if constexpr (MANY && TAKEN > 0) {
@@ -281,12 +297,13 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
       if constexpr (EPI == kGrad) {
         copy4(make_rsrc(g.lse + n, uint32_t(there) * 4), lane4, to + 512);
         copy4(make_rsrc(g.grad + n, g.grad ? uint32_t(there) * 4 : 0u), lane4, to + 768);
+        copy4(make_rsrc(g.losses + n, g.losses ? uint32_t(there) * 4 : 0u), lane4, to + 1024);
       }
     }
   };
   struct Token {
     int64_t target;
-    float lse, grad;
+    float lse, grad, loss;
   };
   auto token_of = [&](const Unit& u, int y, int col) {  // (of a row past the tokens: anything)
     Token t{};
@@ -297,6 +314,7 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
       if constexpr (EPI == kGrad) {
         t.lse = *reinterpret_cast<const float*>(p + 512);
         t.grad = g.grad ? *reinterpret_cast<const float*>(p + 768) : 1.0f;
+        t.loss = *reinterpret_cast<const float*>(p + 1024);
       }
     } else {
       const int64_t n = min(u.n0 + nw + 32 * y + col, g.n - 1);
@@ -304,6 +322,7 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
       if constexpr (EPI == kGrad) {
         t.lse = g.lse[n];
         t.grad = g.grad ? g.grad[n] : 1.0f;
+        t.loss = g.losses ? g.losses[n] : 0.0f;
       }
     }
     return t;
@@ -389,7 +408,9 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
     if constexpr (EPI == kGrad) {
       // (of g and the exponentials whole tiles are written: what lies behind the classes
       // is zero)
-      float off[2], scale[2];
+      // (a target's is its p times `of_p`, plus less[])
+      const float of_p = g.losses ? 0.0f : 1.0f;
+      float off[2], scale[2], less[2];
       int rel[2];
       bool keep[2];
 #pragma unroll
@@ -402,13 +423,15 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
         // gradients)
         if (t.target < 0 || t.target >= g.classes) scale[y] = NAN;
         off[y] = t.lse * kLog2e;
+        less[y] = g.losses ? less_one(t.loss) : -1.0f;
       }
       store_rows(u, u.m0 + T, lane, [&](int x, int y, int q) {
         float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float p = exp2_fast(__builtin_fmaf(acc[x][y][4 * q + r], kLog2e, -off[y]));
-          v[r] = keep[y] ? (p - (rel[y] == 32 * x + 8 * q + r ? 1.0f : 0.0f)) * scale[y] : 0.0f;
+          const float at = rel[y] == 32 * x + 8 * q + r ? __builtin_fmaf(p, of_p, less[y]) : p;
+          v[r] = keep[y] ? at * scale[y] : 0.0f;
         }
         if (u.m0 + T > g.m) {
 #pragma unroll
@@ -469,13 +492,13 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
 #pragma unroll
       for (int y = 0; y < S::NB; ++y) {
         const float top = fmaxf(mine[32 * y + col], other[32 * y + col]);
-        const float off = top == -INFINITY ? 0.0f : top * kLog2e;
+        const float off = top == -INFINITY ? 0.0f : top;
         float sum = 0.0f;
 #pragma unroll
         for (int x = 0; x < S::MB; ++x)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float e = exp2_fast(__builtin_fmaf(acc[x][y][r], kLog2e, -off));
+            const float e = exp2_fast((acc[x][y][r] - off) * kLog2e);
             sum += e;
             if constexpr (EPI == kExps) acc[x][y][r] = e;
           }
@@ -487,7 +510,7 @@ __global__ __launch_bounds__(T == 256 ? 512 : 256, T == 128 && ST == 2 ? 2 : 1) 
       if (wm == 0 && n < g.n) {
         const float top = fmaxf(mine[lane], other[lane]);
         g.part[int64_t(u.m0 / T) * g.n + n] =
-            make_float2(top == -INFINITY ? 0.0f : top * kLog2e, mine[64 + lane] + other[64 + lane]);
+            make_float2(top == -INFINITY ? 0.0f : top, mine[64 + lane] + other[64 + lane]);
       }
       if constexpr (EPI == kExps) {
         sync_lds();
@@ -618,7 +641,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_losses_kernel(
   auto add = [&](const float2& p) {
     if (p.y == 0.0f) return;
     const float next = fmaxf(top, p.x);
-    sum = (sum == 0.0f ? 0.0f : sum * exp2_fast(top - next)) + p.y * exp2_fast(p.x - next);
+    sum = (sum == 0.0f ? 0.0f : sum * exp2_fast((top - next) * kLog2e)) +
+          p.y * exp2_fast((p.x - next) * kLog2e);
     top = next;
   };
   if (t < tokens)
@@ -636,11 +660,12 @@ __global__ __launch_bounds__(kJoinThreads) void join_losses_kernel(
   double loss = 0.0, count = 0.0;
   if (slice == 0 && t < tokens) {
     for (int i = 1; i < 32; ++i) add(s[i][tl]);
-    const float l = (top + log2_fast(sum)) * kLn2;
+    const float rest = log2_fast(sum) * kLn2;
     const int64_t target = targets[t];
     const bool keep = target != ignore;
-    const float each = !keep ? 0.0f : target < 0 || target >= classes ? NAN : l - picked[t];
-    lse[t] = l;
+    const float each = !keep ? 0.0f : target < 0 || target >= classes
+                                     ? NAN : (top - picked[t]) + rest;
+    lse[t] = top + rest;
     losses[t] = each;
     loss = each;
     count = keep ? 1.0 : 0.0;
@@ -684,19 +709,19 @@ __global__ void no_tokens_kernel(int mean, float* total, float* count) {
 template <int T>
 __global__ __launch_bounds__(256) void exps_to_grad_kernel(
     uint16_t* __restrict__ x, int64_t ld, const float2* __restrict__ part,
-    const float* __restrict__ lse, const int64_t* __restrict__ targets, int64_t ignore,
-    int64_t classes, int tokens) {
+    const float* __restrict__ lse, const float* __restrict__ losses,
+    const int64_t* __restrict__ targets, int64_t ignore, int64_t classes, int tokens) {
   const int t = int(blockIdx.y) * 8 + threadIdx.x / 32;
   if (t >= tokens) return;
   const int64_t target = targets[t];
   const bool keep = target != ignore;
   const float c = target < 0 || target >= classes ? NAN : 1.0f;  // (as its loss)
-  const float l = lse[t] * kLog2e;
+  const float l = lse[t], less = less_one(losses[t]);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t v0 = (int64_t(blockIdx.x) * 128 + i * 32 + threadIdx.x % 32) * 8;
     if (v0 >= classes) return;
-    const float f = exp2_fast(part[v0 / T * tokens + t].x - l) * (c / kExpsUp);
+    const float f = exp2_fast((part[v0 / T * tokens + t].x - l) * kLog2e) * (c / kExpsUp);
     uint4* p = reinterpret_cast<uint4*>(x + int64_t(t) * ld + v0);
     typedef _Float16 v8h __attribute__((ext_vector_type(8)));
     const v8h e = __builtin_bit_cast(v8h, *p);
@@ -705,7 +730,7 @@ __global__ __launch_bounds__(256) void exps_to_grad_kernel(
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       // (what lies behind the classes stays zero)
-      const float z = v0 + j < classes ? float(e[j]) * f - (j == at ? c : 0.0f) : 0.0f;
+      const float z = v0 + j < classes ? (j == at ? less : float(e[j]) * f) : 0.0f;
       g[j] = keep ? z : 0.0f;
     }
     *p = make_uint4(pack2(g[0], g[1]), pack2(g[2], g[3]), pack2(g[4], g[5]), pack2(g[6], g[7]));
@@ -1098,11 +1123,11 @@ int tcfp_linear_cross_entropy_train(const void* hidden, int64_t ldh, const void*
   const auto* part = reinterpret_cast<const float2*>(parts);
   const float* each = mean ? count : nullptr;
   if (logits_cut(tokens, vocab, dim).tile == 256)
-    exps_to_grad_kernel<256><<<grid, 256, 0, st>>>(g, l.run, part, lse, targets, ignore, vocab,
-                                                   int(tokens));
+    exps_to_grad_kernel<256><<<grid, 256, 0, st>>>(g, l.run, part, lse, losses, targets, ignore,
+                                                   vocab, int(tokens));
   else
-    exps_to_grad_kernel<128><<<grid, 256, 0, st>>>(g, l.run, part, lse, targets, ignore, vocab,
-                                                   int(tokens));
+    exps_to_grad_kernel<128><<<grid, 256, 0, st>>>(g, l.run, part, lse, losses, targets, ignore,
+                                                   vocab, int(tokens));
   if (launch_status() != TCFP_OK) return TCFP_ERR_HIP;
   done = products_of(head, l, g, 0, vocab, nullptr, each, grad_hidden, grad_weight,
                      reinterpret_cast<float*>(ws + l.g),
@@ -1134,8 +1159,8 @@ size_t tcfp_linear_cross_entropy_backward_workspace_bytes(int64_t tokens, int64_
 
 int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const void* weight,
                                        int64_t ldw, const int64_t* targets, int64_t ignore,
-                                       const float* lse, const float* grad, int64_t grad_step,
-                                       const float* count, int64_t tokens, int64_t vocab,
+                                       const float* lse, const float* losses, const float* grad,
+                                       int64_t grad_step, const float* count, int64_t tokens, int64_t vocab,
                                        int64_t dim, void* grad_hidden, void* grad_weight,
                                        void* workspace, size_t workspace_bytes, void* stream) {
   const int rc = check_sizes(hidden, ldh, weight, ldw, tokens, vocab, dim);
@@ -1174,6 +1199,7 @@ int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const vo
     p.out = g;
     p.ldo = l.run;
     p.lse = lse;
+    p.losses = losses;
     p.grad = grad_step == 1 ? grad : nullptr;
     p.up = up;
     int done = launch_cut<false, false, kGrad>(logits_cut(tokens, classes, dim), p, st);

@@ -72,6 +72,7 @@ def linear_cross_entropy_backward(
     targets: torch.Tensor,
     lse: torch.Tensor,
     *,
+    losses: torch.Tensor | None = None,
     count: torch.Tensor | None = None,
     ignore_index: int = -100,
     need_hidden_grad: bool = True,
@@ -82,8 +83,10 @@ def linear_cross_entropy_backward(
 
     ``grad`` (fp32) is the gradient of every token's loss, or one value for all of
     them, which ``count`` (one fp32 value on the device: the tokens of a mean)
-    divides; ``lse`` is what :func:`linear_cross_entropy_forward` returned.
+    divides; ``lse`` and ``losses`` are what :func:`linear_cross_entropy_forward` returned.
+    Without ``losses`` the gradient of a target's logit comes from ``lse``, whose rounding
+    (2^-24 of it) is then in it: much, where a target's class is almost certain.
     """
-    return _hip.host().linear_cross_entropy_backward(grad, hidden, weight, targets, lse, count,
-                                                     int(ignore_index), bool(need_hidden_grad),
-                                                     bool(need_weight_grad))
+    return _hip.host().linear_cross_entropy_backward(grad, hidden, weight, targets, lse, losses,
+                                                     count, int(ignore_index),
+                                                     bool(need_hidden_grad), bool(need_weight_grad))
