@@ -757,14 +757,19 @@ __global__ __launch_bounds__(256) void scale_kernel(uint16_t* a, int64_t a_eight
   }
 }
 
-// The largest of the tokens' gradients that is finite; 1 if that is 0.
-__global__ __launch_bounds__(1024) void largest_kernel(const float* __restrict__ grad, int tokens,
+// The largest of the tokens' gradients that is finite; 1 if that is 0.  What a token that
+// is left out has does not count: divided by it, the others' could fall below bf16's
+// smallest values.
+__global__ __launch_bounds__(1024) void largest_kernel(const float* __restrict__ grad,
+                                                       const int64_t* __restrict__ targets,
+                                                       int64_t ignore, int64_t classes, int tokens,
                                                        float* unit) {
   __shared__ float s[16];
   float top = 0.0f;
   for (int64_t i = threadIdx.x; i < tokens; i += 1024) {
     const float x = fabsf(grad[i]);
-    if (x < INFINITY) top = fmaxf(top, x);
+    const int64_t target = targets[i];
+    if (x < INFINITY && target != ignore && target >= 0 && target < classes) top = fmaxf(top, x);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -1190,7 +1195,7 @@ int tcfp_linear_cross_entropy_backward(const void* hidden, int64_t ldh, const vo
   const float* up = grad;
   if (grad_step == 1) {
     float* largest = reinterpret_cast<float*>(ws + l.g + l.sum_h + l.sum_w);
-    largest_kernel<<<1, 1024, 0, st>>>(grad, int(tokens), largest);
+    largest_kernel<<<1, 1024, 0, st>>>(grad, targets, ignore, vocab, int(tokens), largest);
     up = largest;
   }
   for (int64_t v0 = 0; v0 < vocab; v0 += l.run) {
