@@ -1297,8 +1297,15 @@ HeadIn head_inputs(const Tensor& hidden, const Tensor& weight, const Tensor& tar
   if (in.h.cols < 8 || in.h.cols % 8 != 0)
     value_error("the hidden dimension must be a multiple of 8, got " + std::to_string(in.h.cols));
   in.w = rows_of(weight, "weight");
-  for (Rows* r : {&in.h, &in.w})  // (a single row's stride means nothing)
+  for (Rows* r : {&in.h, &in.w}) {
+    // (a single row's stride means nothing; rows so far apart that 256 of them pass the
+    // 32-bit offsets of a tile are copied)
     if (r->ld < r->cols || r->rows <= 1) r->ld = r->cols;
+    if (r->ld > r->cols && 512 * r->ld + 2 * r->cols >= (int64_t(1) << 31) - (1 << 20)) {
+      r->t = r->t.clone(at::MemoryFormat::Contiguous);
+      r->ld = r->cols;
+    }
+  }
   if (targets.scalar_type() != at::kLong)
     type_error(std::string("targets must be torch.int64, got ") +
                dtype_str(targets.scalar_type()));

@@ -1,4 +1,4 @@
-"""Cross entropy of a linear head: gradients of tokens that are left out."""
+"""Cross entropy of a linear head: gradients of tokens that are left out, rows far apart."""
 import pytest
 import torch
 
@@ -21,3 +21,20 @@ def test_a_gradient_of_a_token_left_out(dev, huge):
     e = Exact(h, w, t, up, made=False)
     within(dh, e.dh, e.dh_tol, "dh")
     within(dw, e.dw, e.dw_tol, "dw")
+
+
+def test_rows_far_apart(dev):
+    """The last token's hidden state of each long sequence, a weight inside a wide matrix."""
+    h, w, t = inputs(dev, 3, 64, 5, seed=23)
+    far = torch.zeros(3, (1 << 22) + 8, dtype=BF16, device=dev)[:, 8:72]
+    far.copy_(h)
+    wide = torch.zeros(5, 1 << 23, dtype=BF16, device=dev)[:, :64]
+    wide.copy_(w)
+    want = L.linear_cross_entropy(h, w, t, reduction="none")
+    a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+    grads = torch.autograd.grad(L.linear_cross_entropy(a, b, t), (a, b))
+    for x, y in ((far, w), (h, wide), (far, wide)):
+        assert torch.equal(L.linear_cross_entropy(x, y, t, reduction="none"), want)
+        x, y = x.detach().requires_grad_(), y.detach().requires_grad_()
+        got = torch.autograd.grad(L.linear_cross_entropy(x, y, t), (x, y))
+        assert all(torch.equal(p, q) for p, q in zip(got, grads))
