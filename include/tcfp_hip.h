@@ -760,7 +760,9 @@ int tcfp_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, in
  *   h / (heads / kv_heads); dim 64, 128 or 256.
  *   Sequence b has the rows q_starts[b] ... q_starts[b + 1] - 1 of q and
  *   k_starts[b] ... of k and v ([batch + 1] each, not decreasing; the same array
- *   where a sequence attends to itself).
+ *   where a sequence attends to itself).  batch at most 65535, batch * kv_heads (rounded
+ *   up to a multiple of 8) times heads / kv_heads below 2^24, tokens and keys at most
+ *   2^29.
  * Query i of n stands at position p = (the sequence's keys) - n + i and sees the
  * keys j <= p (causal) with j > p - window (window > 0).  A query that sees
  * nothing, and one outside the sequences, gets zeros.

@@ -51,7 +51,8 @@ def packed_attention(
 
     ``q`` [tokens, heads, dim], ``k`` and ``v`` [keys, kv_heads, dim] are bf16 (slices
     of a QKV projection's output are taken as they are), ``dim`` 64, 128 or 256;
-    ``heads`` is a multiple of ``kv_heads``, neighbouring query heads share one.
+    ``heads`` is a multiple of ``kv_heads``, neighbouring query heads share one; sequences
+    times heads stay below 2^24.
     Sequence b has the rows ``seq_start[b]`` to ``seq_start[b + 1]`` (int32
     [sequences + 1], not decreasing) of q, and of k and v too unless ``key_start``
     gives those rows of their own: with more keys than queries the queries are the

@@ -1186,6 +1186,10 @@ PackedIn packed_inputs(OnGpu& g, const Tensor& q, const Tensor& k, const Tensor&
                 ": key_start is needed");
   }
   if (p.batch > 65535) value_error("at most 65535 sequences, got " + std::to_string(p.batch));
+  // (what a launch's grid takes, the first product rounded up to whole rounds of the XCDs)
+  if ((p.batch * kv_heads + 7) / 8 * 8 * (heads / kv_heads) >= 1 << 24)
+    value_error("at most 2^24 sequences times heads, got " + std::to_string(p.batch) +
+                " sequences of " + std::to_string(heads) + " heads");
   if (p.batch == 0 && (p.tokens > 0 || p.keys > 0))
     value_error("there are tokens but no sequences");
   if (max_len < 0 || (max_key_len && *max_key_len < 0))

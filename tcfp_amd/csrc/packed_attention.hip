@@ -706,6 +706,12 @@ int parts_of(int64_t keys, int64_t batch, int64_t max_key_len, int kv_heads, int
   return best;
 }
 
+// (sequence, K/V head)s of a launch: whole rounds of the XCDs, see place().
+int64_t sets_of(int64_t batch, int kv_heads) {
+  const int64_t sets = batch * kv_heads;
+  return sets >= 8 ? (sets + 7) / 8 * 8 : sets;
+}
+
 struct Sizes {
   int64_t tokens, keys, batch, max_len, max_key_len, window;
   int heads, kv_heads, dim;
@@ -715,10 +721,13 @@ int check_sizes(const Sizes& z) {
   if (z.dim != 64 && z.dim != 128 && z.dim != 256) return TCFP_ERR_SHAPE;
   if (z.tokens < 0 || z.keys < 0 || z.tokens > kMostRows || z.keys > kMostRows || z.batch < 0 ||
       z.batch > 65535 || z.heads <= 0 || z.heads > 65535 || z.kv_heads <= 0 ||
-      z.heads % z.kv_heads || z.batch * z.heads > 1 << 30 || z.max_len < 0 || z.max_key_len < 0 ||
+      z.heads % z.kv_heads || z.max_len < 0 || z.max_key_len < 0 ||
       z.window < 0 || !std::isfinite(z.scale))
     return TCFP_ERR_SHAPE;
   if ((z.tokens > 0 || z.keys > 0) && z.batch == 0) return TCFP_ERR_SHAPE;
+  // (a workgroup for each sequence and head at least: what a grid takes)
+  if (!grid_x_fits(sets_of(z.batch, z.kv_heads) * (z.heads / z.kv_heads), 64 * kWaves))
+    return TCFP_ERR_SHAPE;
   return TCFP_OK;
 }
 // Row strides within a descriptor's reach, rows of whole 16-byte vectors.
@@ -745,10 +754,11 @@ Packed arguments(const Sizes& z, bool causal) {
 }
 // Tiles of a sequence and head in a launch with `members` of each set, and its workgroups.
 // A bound far past the lengths (all keys of a batch of many sequences) is cut: a
-// workgroup takes the tiles that are left over, one after another.
+// workgroup takes the tiles that are left over, one after another.  So a launch holds 4
+// million workgroups at most, or one for each set and member where those are more.
 int64_t lay_out(Packed& a, int64_t max_len, int64_t rows, int members) {
-  const int64_t sets = a.sets >= 8 ? (a.sets + 7) / 8 * 8 : a.sets;
-  const int64_t each = sets * members, most = std::max<int64_t>((int64_t(1) << 22) / each, 1);
+  const int64_t each = sets_of(a.batch, a.kv_heads) * members;
+  const int64_t most = std::max<int64_t>((int64_t(1) << 22) / each, 1);
   a.tiles = int(std::clamp<int64_t>(ceil_div(std::min(max_len, rows), 32 * kWaves), 1, most));
   return each * a.tiles;
 }
