@@ -1,14 +1,15 @@
 """Train a small decoder on TCFP-12 layers, then generate from it through the
 8-bit paged K/V cache.
 
-    python examples/generate.py [--steps 600] [--tokens 64] [--rotary]
+    python examples/generate.py [--steps 600] [--tokens 64] [--rotary] [--fp32]
 
 The model is the repository's small transformer (d_model 256, 4 layers, 4 heads,
 FFN 1024, vocab 256) with root-mean-square norms: every norm stands in front of
 a linear layer that reads FP8 codes, so ``TCFPNormLinear`` quantises where it
 normalises.  Positions are a learned table, or with ``--rotary`` turns of the
 queries and keys.  Training attends a batch's sequences packed one after another
-and takes the loss from the hidden states, without the logits.  Serving lays the
+and takes the loss from the hidden states, without the logits, both from bf16; with
+``--fp32`` both are plain products in fp32.  Serving lays the
 weight codes out once; a step of a batch -- whole prompts or one token each -- is,
 per layer,
 
@@ -42,36 +43,48 @@ VOCAB, BLOCK = 256, 64
 
 
 class Layer(nn.Module):
-    def __init__(self, d: int, heads: int, ffn: int) -> None:
+    def __init__(self, d: int, heads: int, ffn: int, fp32: bool = False) -> None:
         super().__init__()
         self.heads = heads
+        self.plain = fp32 or d // heads not in (64, 128, 256)  # (what the kernel has)
         self.qkv = TCFPNormLinear(d, 3 * d, scale_block_size=BLOCK)
         self.proj = TCFPLinear(d, d, use_tensor_cores=True, scale_block_size=BLOCK)
         self.fc1 = TCFPNormLinear(d, ffn, scale_block_size=BLOCK)
         self.fc2 = TCFPLinear(ffn, d, use_tensor_cores=True, scale_block_size=BLOCK)
 
+    def attend(self, qkv, starts, turn):
+        """Every token on itself and those before it in its sequence."""
+        b, t, c = qkv.shape[0], qkv.shape[1], qkv.shape[2] // 3
+        dtype = torch.float32 if self.plain else torch.bfloat16
+        q, k, v = qkv.to(dtype).reshape(b * t, 3, self.heads, -1).unbind(1)
+        if turn is not None:
+            q, k = rotary_embedding(q, k, *turn)
+        if not self.plain:
+            return packed_attention(q, k, v, starts, max_len=t).reshape(b, t, c)
+        q, k, v = (z.reshape(b, t, self.heads, -1).transpose(1, 2).contiguous() for z in (q, k, v))
+        att = torch.matmul(q, k.transpose(-2, -1).contiguous()) / q.shape[-1] ** 0.5
+        mask = torch.triu(torch.ones(t, t, dtype=torch.bool, device=q.device), 1)
+        att = F.softmax(att.masked_fill(mask, float("-inf")), dim=-1)
+        return torch.matmul(att, v).transpose(1, 2).reshape(b, t, c)
+
     def forward(self, x, h, starts, turn):
         """``x``: what the layer before adds to the residual stream ``h``; ``starts``:
         where the batch's sequences begin; ``turn``: positions and frequencies."""
         qkv, h = self.qkv(x, h)
-        b, t, c = h.shape
-        q, k, v = qkv.bfloat16().reshape(b * t, 3, self.heads, -1).unbind(1)
-        if turn is not None:
-            q, k = rotary_embedding(q, k, *turn)
-        y = packed_attention(q, k, v, starts, max_len=t).reshape(b, t, c)
+        y = self.attend(qkv, starts, turn)
         z, h = self.fc1(self.proj(y.to(h.dtype)), h)
         return self.fc2(F.gelu(z)), h
 
 
 class Decoder(nn.Module):
     def __init__(self, d: int = 256, layers: int = 4, heads: int = 4, ffn: int = 1024,
-                 positions: int = 256, rotary: bool = False) -> None:
+                 positions: int = 256, rotary: bool = False, fp32: bool = False) -> None:
         super().__init__()
-        self.tok, self.positions = nn.Embedding(VOCAB, d), positions
+        self.tok, self.positions, self.fp32 = nn.Embedding(VOCAB, d), positions, fp32
         self.pos = None if rotary else nn.Embedding(positions, d)
         self.register_buffer("freqs", rotary_frequencies(d // heads) if rotary else None,
                              persistent=False)
-        self.layers = nn.ModuleList(Layer(d, heads, ffn) for _ in range(layers))
+        self.layers = nn.ModuleList(Layer(d, heads, ffn, fp32) for _ in range(layers))
         self.norm = TCFPRMSNorm(d)
         for m in self.modules():
             if isinstance(m, (nn.Embedding, TCFPLinear)):
@@ -99,7 +112,9 @@ class Decoder(nn.Module):
         return self.hidden(idx).float() @ self.tok.weight.t()
 
     def loss(self, idx, targets):
-        """Mean cross entropy, with the head in bf16 and its logits nowhere."""
+        """Mean cross entropy, with the head in bf16 and its logits nowhere (or in fp32)."""
+        if self.fp32:
+            return F.cross_entropy(self(idx).reshape(-1, VOCAB), targets.reshape(-1))
         return linear_cross_entropy(self.hidden(idx).bfloat16(), self.tok.weight.bfloat16(),
                                     targets)
 
@@ -216,9 +231,10 @@ def main() -> None:
     ap.add_argument("--steps", type=int, default=600)
     ap.add_argument("--tokens", type=int, default=64)
     ap.add_argument("--rotary", action="store_true", help="rotary instead of learned positions")
+    ap.add_argument("--fp32", action="store_true", help="train attention and head in fp32")
     a = ap.parse_args()
     torch.manual_seed(0)
-    model = Decoder(rotary=a.rotary).cuda()
+    model = Decoder(rotary=a.rotary, fp32=a.fp32).cuda()
     losses = train(model, a.steps)
     print(f"loss {losses[0]:.3f} -> {losses[-1]:.3f} in {a.steps} steps", flush=True)
     server = Server(model)
