@@ -850,7 +850,7 @@ int tcfp_scale_bf16(void* a, int64_t a_values, void* b, int64_t b_values, const 
  * [tokens]: the target's softmax(z) - 1 is formed from them, or if NULL from lse, whose
  * rounding is in it then.  z is formed again, for a run of classes at a time whose g,
  * rounded to bf16 before what all its tokens share is multiplied, takes at most 256 MiB
- * of the workspace; sums are f32.  hidden is read for ignored tokens too: a value that
+ * of the workspace (or 512 bytes a token, the shortest run); sums are f32.  hidden is read for ignored tokens too: a value that
  * is not finite there reaches grad_weight. */
 size_t tcfp_linear_cross_entropy_backward_workspace_bytes(int64_t tokens, int64_t vocab,
                                                           int64_t dim, int need_hidden,

@@ -27,8 +27,8 @@
 // operand of dh and dW.  Otherwise (more, or a gradient for every token's
 // loss) the backward forms z again for a run of classes at a time, with g as the
 // epilogue: dh is added up over the runs in fp32, of dW a run has its rows.  g is
-// rounded to bf16 (2^-9 of each value, as the results themselves are); all sums are
-// fp32.
+// rounded to bf16 (2^-8 of each value at most, as the results themselves are); all sums
+// are fp32.
 #include <algorithm>
 #include <cmath>
 #include <utility>
@@ -806,7 +806,7 @@ __global__ __launch_bounds__(256) void round_sum_kernel(const float* __restrict_
 
 constexpr int kCus = 256;
 // g of a run of classes takes at most this much of the workspace, but for runs
-// of 256 classes.
+// of 256 classes, the shortest: 512 bytes a token.
 constexpr int64_t kRunBytes = int64_t(256) << 20;
 // What g of all classes may take where the forward makes the gradients.
 constexpr int64_t kTrainBytes = int64_t(1) << 30;

@@ -34,10 +34,11 @@ namespace {
 
 constexpr int kStep = 64;  // rows of a tile in LDS
 // Where no sequence has more rows than this, dQ and dK take dS as two bf16, its rounding
-// and what that left: 1.7e-3 off, as the results' rounding, instead of 2.4e-3 (32
-// sequences of 128 tokens, 4 heads of 64: a backward pass of 18.5 us instead of 17.7,
-// less than its launches take the host).  For long ones the product more would be a
-// sixth of the pass.
+// and what that left: 1.7e-3 off, as the results' rounding, instead of 2.4e-3 (dV, whose P
+// stays one bf16, is 2.3e-3 off either way).  A backward pass takes, with two and with
+// one: 32 sequences of 128 tokens, 4 heads of 64, 18.2 us and 17.8, less than its launches
+// take the host; 64 of 256, 8 heads of 64, 65 and 61; 256 of 256, 32 / 8 heads of 128, 1490
+// and 1326.  Long sequences take the shorter form.
 constexpr int kShort = 256;
 
 struct Packed {
@@ -685,7 +686,9 @@ constexpr int kWaves = 4;
 // step of 64 queries, heads of 128, 2.6 for a workgroup alone on a CU and 4.2 beside
 // another; the longest chain of steps -- of a causal sequence the first tile of keys has
 // twice the mean's -- against all of them over the card; the parts' writing and joining,
-// 4.5 TB/s.  (32 / 8 heads of 128, the whole backward: one sequence of 8192 4000 us in
+// 4.5 TB/s.  (It counts no window and takes every call for causal: tiles whose chains are
+// alike are shared out as if they were not, 8192 tokens with 1000 seen back in two parts,
+// 539 us the whole backward.)  (32 / 8 heads of 128, the whole backward: one sequence of 8192 4000 us in
 // one part, 1770 in two; four of up to 4096 1310 and 1063; six of up to 1000 198 in two,
 // 199 in four.)
 int parts_of(int64_t keys, int64_t batch, int64_t max_key_len, int kv_heads, int group, int dim) {

@@ -8,9 +8,9 @@
 // Memory bound: every value is read and written once, 16 bytes a lane.  The
 // angles of a token are the same for all its heads, so a workgroup forms them
 // once, in LDS, for the tokens it turns, one thread a pair.  An angle is position
-// * freq / 2 pi in fp64, of which the whole turns are dropped before it is
-// rounded to fp32: at position 2^20 it is still right to 2^-33 turns, where an
-// fp32 product would be off by 2^-8.  Products are fp32, rounded once.
+// * freq / 2 pi in fp64 (at position 2^20 right to 2^-33 turns), of which the whole
+// turns are dropped before the rest, half a turn at most, is rounded to fp32: 2^-26
+// turns, where an fp32 product would be off by 2^-7.  Products are fp32, rounded once.
 #include "mfma_tiles.h"
 
 using namespace tcfp;

@@ -8,7 +8,7 @@ maximum and sum of exponentials.  The gradients of a sum or mean are made in the
 same call, from exponentials in 16 bits that take at most 1 GiB of workspace while it
 runs; where they would take more, and for gradients of every token's loss, the
 backward pass forms the logits again, a run of classes at a time (256 MiB for the
-run's gradients, and fp32 sums of the hidden states').  Memory beside the inputs and
+run's gradients, or 512 bytes a token if that is more, and fp32 sums of the hidden states').  Memory beside the inputs and
 gradients stays bounded either way.
 
 Every op runs on the tensors' GPU and current stream; there is no CPU path.
@@ -41,7 +41,10 @@ def linear_cross_entropy(
     reduction's fp64).
 
     ``reduction`` is ``"mean"``, ``"sum"`` or ``"none"`` (a loss for every token).
-    Differentiable in ``hidden`` and ``weight``, once; gradients are bf16.  The hidden
+    Differentiable in ``hidden`` and ``weight``, once; gradients are bf16.  Those of a sum
+    or mean are multiplied with the loss's own gradient once they are made, which rounds
+    them a second time unless that is a power of two, and leave out classes less than
+    2^-39 as likely as the likeliest of their 128 or 256 neighbours.  The hidden
     states of tokens left out are read all the same: a value there that is not
     finite reaches the weight's gradient.
     """
