@@ -17,7 +17,9 @@
 // whatever the logits' size, and never below 0.  As lse - z[target], with lse rounded, it
 // would be off by 2^-24 of lse: of 30, by 1.8e-6, as much as a confident token's whole
 // loss.  The gradient of the target's logit, p - 1, is formed from the loss as exp(-loss)
-// - 1; other classes' p = exp(z - lse) are off by lse's rounding in proportion only.
+// - 1.  Other classes' p = exp(z - lse) are off in proportion to themselves, by 2^-24 of
+// lse for its rounding and as much for that of its multiple, about what z's own rounding
+// to fp32 is: of 2000, 2e-4.
 //
 // Gradients, where they are wanted of the losses' sum or mean and tokens x classes
 // take at most 1 GiB of workspace in 16 bits: with the forward, three products in
